@@ -1,0 +1,484 @@
+// Products of 8-bit rows with an 8-bit weight on the 5th-generation tensor cores (e4m3 operands, a float32 scale per row and
+// 128 columns of x and per 128 features and 128 columns of W; lb200/fp8.cuh):
+//
+//   y[m, n] = sum_b  sx[m, b] sw[n / 128, b]  sum_{k in block b} qx[m, k] qw[n, k]
+//   plain   : out = round((y + bias) * out_scale)                      bfloat16 or float32
+//   swiglu  : h = silu(act_scale * y_gate) * y_up, then 8-bit rows of h: a scale per row and 128 features
+//
+// The inner sums run on the tensor core, one block of 128 columns at a time into a fresh accumulator in tensor memory; the
+// scales differ from block to block, so each block's accumulator is read back and joined into 32-bit registers, times its
+// scales, while the tensor core works on the next block.
+//
+//   warp 0    one thread issues the TMA loads (128-byte swizzle, zeros outside the matrices) into a ring of stages: a block
+//             of 128 columns of 128 features of W (swiglu: of 128 gate and 128 up features) and of the tile's rows of x
+//   warp 1    allocates tensor memory; one thread issues tcgen05.mma (kind::f8f6f4, K 32: four per block)
+//   warps 2-9 two warpgroups: read a block's accumulator, multiply and add; for swiglu one holds the gate, one the up
+//             features, otherwise each half of the columns
+// Two ways round:
+//   few rows (up to 64, kSwap): 128 features are the M side of the instruction, the rows, padded to 16, 32 or 64, its N side:
+//             bound by reading W once.  A thread is a feature; the scales of the rows lie ready in shared memory.
+//   tiles     128 rows are the M side, 128 features (swiglu: 256) the N side.  A thread is a row.
+// K split: where there are few tiles, up to 8 CTAs of a cluster take a range of blocks each and the sums meet in distributed
+// shared memory: each CTA owns an equal share of the tile's rows, gets every CTA's sums for them by remote stores, and adds
+// them in rank order, so that the result does not depend on timing.  There a warp takes a row, a lane 4 neighbouring features:
+// stores are whole, and the largest magnitude of a row's 128 features takes one reduction.
+//
+// Every wait on an mbarrier is bounded; one that gives up records itself in `error`, all roles run out of their own bounded
+// waits, every thread still meets the cluster barriers, tensor memory is freed and the kernel returns.
+#include "lb200/common.cuh"
+#include "lb200/fp8.cuh"
+#include "lb200/tcgen05.cuh"
+using namespace lb200;
+using namespace lb200::tc;
+
+namespace {
+constexpr int kBK = kFp8Block;                            // columns of a block = bytes of a swizzled row
+constexpr int kFeat = 128;
+constexpr uint32_t kWBytes = kFeat * kBK;
+constexpr int kSumThreads = 256;                          // warps 2-9
+constexpr int kThreads = 64 + kSumThreads;
+constexpr int kMaxStages = 8, kMaxSplit = 8;
+
+struct Args {
+    const float* sx; long sx_row, sx_block;               // scales of x: strides per row and per block
+    const float *sw0, *sw1; long sw_row, sw_block;        // scales of W (swiglu: gate, up): strides per 128 features and per block
+    const float* bias; void* out; long ldo;
+    uint8_t* q; long ldq; float* qs; long qs_row, qs_block;    // swiglu: the 8-bit rows
+    int M, N, K;
+    int split, stages, tiles_n;
+    int early;                                            // W may be read before the kernels in front have ended
+    int out_f32;
+    float out_scale, act_scale;
+    int* error;
+};
+
+__device__ __forceinline__ void report(int* error, int role, int step) {
+    if (error != nullptr) atomicCAS(error, 0, 0x20000000 | (role << 24) | ((blockIdx.x & 0xFFF) << 12) | (step & 0xFFF));
+}
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer_addr(uint32_t local, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, float a) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(a) : "memory");
+}
+__device__ __forceinline__ void store_peer4(uint32_t addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+// e4m3 operands, both K-major, float32 accumulator: formats 0 and 0
+__host__ __device__ constexpr uint32_t f8_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 16 consecutive float32 columns of this thread's lane of tensor memory; complete after tmem_ld_wait()
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// (a0, a1) += (d0, d1) * (s0, s1): both in one instruction
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t d0, uint32_t d1, float s0, float s1) {
+    asm("{\n\t.reg .b64 a, d, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 d, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\t"
+        "fma.rn.f32x2 a, d, s, a;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
+}
+// the product of two scales, finite where both are: a zero sum stays zero
+__device__ __forceinline__ float join(float a, float b) {
+    const float s = a * b;
+    return (magnitude(s) == 0x7f800000u && magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) ? 3.402823466e38f : s;
+}
+
+// kSwap: NR rows on the N side; else 128 rows on the M side (NR = 128).
+template <bool kSwap, int NR, bool kSwiglu>
+struct Form {
+    static constexpr int kXRows = kSwap ? NR : 128;
+    static constexpr uint32_t kXBytes = kXRows * kBK;
+    static constexpr uint32_t kStage = (kSwiglu ? 2 : 1) * kWBytes + kXBytes;
+    static constexpr int kCols = kSwap ? (kSwiglu ? 2 * NR : NR) : (kSwiglu ? 256 : 128);   // accumulator columns of a block
+    static constexpr int kAccs = kSwap && kCols <= 64 ? 4 : 2;                 // accumulators in tensor memory
+    static constexpr uint32_t kTmem = kCols * kAccs < 32 ? 32 : kCols * kAccs;
+    static constexpr int kOutCols = kSwiglu ? 256 : 128;                       // features of a tile, gate and up counted
+    static constexpr int kPitch = kOutCols + 4;                                // floats of a row of sums: rows start in different banks
+    static constexpr int kMine = kSwap ? (kSwiglu ? NR : NR / 2) : (kSwiglu ? 128 : 64);   // sums of a thread
+    static constexpr bool kTwoPerSm = kSwap && kMine <= 64;
+};
+
+template <bool kSwap, int NR, bool kSwiglu>
+__global__ void __launch_bounds__(kThreads, Form<kSwap, NR, kSwiglu>::kTwoPerSm ? 2 : 1)
+fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
+                  const __grid_constant__ CUtensorMap map_x, Args a) {
+    typedef Form<kSwap, NR, kSwiglu> F;
+    constexpr uint32_t kStage = F::kStage;
+    constexpr int kAccs = F::kAccs, kMine = F::kMine;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = a.split, rank = split > 1 ? (int)cluster_rank() : 0;
+    const int tile = blockIdx.x / split, tile_m = tile / a.tiles_n, tile_n = tile - tile_m * a.tiles_n;
+    const int m0 = tile_m * F::kXRows, n0 = tile_n * kFeat, rows = min(F::kXRows, a.M - m0);
+    const int blocks = (a.K + kBK - 1) / kBK;
+    const int kb0 = (int)((long)blocks * rank / split), kbn = (int)((long)blocks * (rank + 1) / split) - kb0;
+    const int stages = a.stages, first = min(stages, kbn);
+    const int share = (rows + split - 1) / split;          // rows of the tile that a CTA of the cluster owns
+    // The sums land here: [source CTA][row of the share][feature].  Few rows: behind the ring, with the table of scales (a
+    // peer may be done while this CTA still loads); tiles: over the ring, once the whole cluster has left it.
+    float* recv = reinterpret_cast<float*>(kSwap ? base + (size_t)stages * kStage : base);
+    float* table = recv + (size_t)(NR + split) * F::kPitch;           // kSwap: [block][gate, up][row]
+    auto load_w = [&](int s, int i) {
+        uint8_t* w = base + (size_t)s * kStage;
+        mbar_expect_tx(full + s, kStage);
+        tma_load_2d(w, &map_w0, full + s, (kb0 + i) * kBK, n0);
+        if (kSwiglu) tma_load_2d(w + kWBytes, &map_w1, full + s, (kb0 + i) * kBK, n0);
+    };
+    auto load_x = [&](int s, int i) {
+        tma_load_2d(base + (size_t)s * kStage + (kSwiglu ? 2 : 1) * kWBytes, &map_x, full + s, (kb0 + i) * kBK, m0);
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+        for (int s = 0; s < kAccs; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, kSumThreads / 32); }
+        failed = 0;
+        mbar_fence_init();
+        if (a.early) for (int i = 0; i < first; ++i) load_w(i, i);     // its own barriers are ready
+    }
+    if (threadIdx.x == 64) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    if (warp == 1) tmem_alloc<F::kTmem>(&tmem_slot);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    pdl_trigger();
+    if (split > 1) cluster_arrive();                       // "this CTA runs": its shared memory may be written to
+    pdl_wait();
+
+    int issued = 0;
+    float sum[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
+    const int group = (warp - 2) >> 2, quarter = warp & 3;             // warpgroup; the lanes of tensor memory a warp may read
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < first; ++i) { if (!a.early) load_w(i, i); load_x(i, i); }
+            issued = first;
+            for (int s = 0, parity = 0; issued < kbn && !failed; ++issued) {
+                if (!mbar_wait(empty + s, parity)) { report(a.error, 1, issued); failed = 1; break; }
+                load_w(s, issued);
+                load_x(s, issued);
+                if (++s == stages) { s = 0; parity ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = kSwap ? f8_idesc(128, NR) : f8_idesc(128, F::kCols);
+            int s = 0, parity = 0;
+            for (int i = 0; i < kbn && !failed; ++i) {
+                const int acc = i % kAccs;
+                if (!mbar_wait(full + s, parity)) { report(a.error, 2, i); failed = 1; break; }
+                if (i >= kAccs && !mbar_wait(acc_empty + acc, (i / kAccs - 1) & 1)) { report(a.error, 3, i); failed = 1; break; }
+                fence_after_sync();
+                const uint64_t wdesc = umma_desc(base + (size_t)s * kStage);
+                const uint64_t xdesc = umma_desc(base + (size_t)s * kStage + (kSwiglu ? 2 : 1) * kWBytes);
+                const uint32_t d = tmem + acc * F::kCols;
+#pragma unroll
+                for (int k = 0; k < kBK / 32; ++k) {       // 32 bytes along K: + 2 in the 16-byte address field
+                    if (kSwap) {
+                        umma_f8(d, wdesc + 2 * k, xdesc + 2 * k, idesc, k != 0);
+                        if (kSwiglu) umma_f8(d + NR, wdesc + (kWBytes >> 4) + 2 * k, xdesc + 2 * k, idesc, k != 0);
+                    } else {
+                        umma_f8(d, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
+                    }
+                }
+                umma_commit(empty + s);
+                umma_commit(acc_full + acc);
+                if (++s == stages) { s = 0; parity ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int t = threadIdx.x - 64;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * kMine;
+        const float* sw = kSwiglu && group ? a.sw1 : a.sw0;
+        const int row = m0 + quarter * 32 + lane;          // tiles: this thread's row
+        const float* sx = a.sx + (long)min(row, a.M - 1) * a.sx_row + kb0 * a.sx_block;
+        sw += (long)tile_n * a.sw_row + kb0 * a.sw_block;
+        float s_next = 0.f;
+        if (kSwap) {
+            for (int e = t; e < kbn * NR; e += kSumThreads) {
+                const int i = e / NR, m = e % NR;
+                const float x = m < rows ? a.sx[(long)(m0 + m) * a.sx_row + (kb0 + i) * a.sx_block] : 0.f;
+                const long at = (long)tile_n * a.sw_row + (kb0 + i) * a.sw_block;
+                if (kSwiglu) {
+                    table[2 * i * NR + m] = join(x, a.sw0[at]);
+                    table[(2 * i + 1) * NR + m] = join(x, a.sw1[at]);
+                } else {
+                    table[i * NR + m] = join(x, a.sw0[at]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        } else if (kbn > 0) {
+            s_next = join(sx[0], sw[0]);
+        }
+        bool ok = true;
+        for (int i = 0; i < kbn; ++i) {
+            const int acc = i % kAccs;
+            const float s = s_next;
+            if (!kSwap && i + 1 < kbn) s_next = join(sx[(i + 1) * a.sx_block], sw[(i + 1) * a.sw_block]);
+            ok = mbar_wait(acc_full + acc, (i / kAccs) & 1);
+            ok = __all_sync(0xffffffffu, ok && !failed);
+            if (!ok) { if (lane == 0 && !failed) { report(a.error, 4, i); failed = 1; } break; }
+            fence_after_sync();
+            const uint32_t at = from + acc * F::kCols;
+            const float* tab = table + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine);
+            if constexpr (kMine < 16) {
+                uint32_t d[8];
+                tmem_ld8(at, d);
+                tmem_ld_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + acc);
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(tab + j);
+                    fma2(sum[j], sum[j + 1], d[j], d[j + 1], f.x, f.y);
+                    fma2(sum[j + 2], sum[j + 3], d[j + 2], d[j + 3], f.z, f.w);
+                }
+            } else {
+                // 16 columns at a time, the next 16 on their way meanwhile
+                uint32_t d[2][16];
+                tmem_ld16(at, d[0]);
+#pragma unroll
+                for (int c = 0; c < kMine; c += 16) {
+                    uint32_t* now = d[(c / 16) & 1];
+                    tmem_ld_wait();
+                    if (c + 16 < kMine) tmem_ld16(at + c + 16, d[(c / 16 + 1) & 1]);
+                    else {
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_empty + acc);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        if (kSwap) {
+                            const float4 f = *reinterpret_cast<const float4*>(tab + c + j);
+                            fma2(sum[c + j], sum[c + j + 1], now[j], now[j + 1], f.x, f.y);
+                            fma2(sum[c + j + 2], sum[c + j + 3], now[j + 2], now[j + 3], f.z, f.w);
+                        } else {
+                            fma2(sum[c + j], sum[c + j + 1], now[j], now[j + 1], s, s);
+                            fma2(sum[c + j + 2], sum[c + j + 3], now[j + 2], now[j + 3], s, s);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // ---- the sums meet at the rows' owners
+    fence_before_sync();
+    if (split > 1) {
+        cluster_wait();
+        if (!kSwap) { cluster_arrive(); cluster_wait(); }  // every CTA of the cluster has left its ring
+    } else if (!kSwap) {
+        __syncthreads();
+    }
+    if (warp >= 2) {
+        const int feat = quarter * 32 + lane;
+        if (kSwap) {
+            const int j0 = kSwiglu ? 0 : group * kMine;
+            int owner = j0 / share, r = j0 - owner * share;
+            const uint32_t mine = smem_u32(recv) + (uint32_t)((rank * share) * F::kPitch + (kSwiglu ? group * 128 : 0) + feat) * 4;
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) {
+                if (j0 + j < rows) {
+                    const uint32_t at = mine + (uint32_t)(r * F::kPitch) * 4;
+                    if (split > 1) store_peer(peer_addr(at, owner), sum[j]);
+                    else recv[r * F::kPitch + (kSwiglu ? group * 128 : 0) + feat] = sum[j];
+                }
+                if (++r == share) { r = 0; ++owner; }
+            }
+        } else if (feat < rows) {
+            const int owner = feat / share, r = feat - owner * share;
+            const uint32_t at = peer_addr(smem_u32(recv) + (uint32_t)((rank * share + r) * F::kPitch + group * kMine) * 4, owner);
+#pragma unroll
+            for (int j = 0; j < kMine; j += 4) store_peer4(at + 4 * j, sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+        }
+    }
+    if (split > 1) { cluster_arrive(); cluster_wait(); }
+    else __syncthreads();
+    if (warp >= 2) {
+        const int col = lane * 4, n = n0 + col;
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!kSwiglu && a.bias != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (n + e < a.N) b[e] = a.bias[n + e];
+        }
+        const int r1 = min(share, rows - rank * share);
+        for (int r = warp - 2; r < r1; r += kSumThreads / 32) {
+            const long m = m0 + rank * share + r;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+            for (int src = 0; src < split; ++src) {
+                const float* p = recv + (size_t)(src * share + r) * F::kPitch + col;
+                const float4 w = *reinterpret_cast<const float4*>(p);
+                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                if (kSwiglu) {
+                    const float4 w1 = *reinterpret_cast<const float4*>(p + 128);
+                    u.x += w1.x; u.y += w1.y; u.z += w1.z; u.w += w1.w;
+                }
+            }
+            if constexpr (kSwiglu) {
+                float h[4] = {silu_f(v.x * a.act_scale) * u.x, silu_f(v.y * a.act_scale) * u.y, silu_f(v.z * a.act_scale) * u.z,
+                              silu_f(v.w * a.act_scale) * u.w};
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { if (n + e >= a.N) h[e] = 0.f; top = max(top, magnitude(h[e])); }
+                const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top)), back = 1.f / scale;
+                // rows are filled up to 16 bytes: four bytes that begin inside the row end inside its storage
+                if (n < a.N) *reinterpret_cast<uint32_t*>(a.q + m * a.ldq + n) = fp8_quad(h[0] * back, h[1] * back, h[2] * back, h[3] * back);
+                if (lane == 0) a.qs[m * a.qs_row + tile_n * a.qs_block] = scale;
+            } else {
+                const float o[4] = {(v.x + b[0]) * a.out_scale, (v.y + b[1]) * a.out_scale, (v.z + b[2]) * a.out_scale, (v.w + b[3]) * a.out_scale};
+                const long at = m * a.ldo + n;
+                if (a.out_f32) {
+                    float* p = (float*)a.out + at;
+                    if (n + 4 <= a.N && ((uintptr_t)p & 15) == 0) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+                    else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = o[e];
+                } else {
+                    __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
+                    if (n + 4 <= a.N && ((uintptr_t)p & 7) == 0) {
+                        uint2 w;
+                        reinterpret_cast<__nv_bfloat162*>(&w)[0] = __floats2bfloat162_rn(o[0], o[1]);
+                        reinterpret_cast<__nv_bfloat162*>(&w)[1] = __floats2bfloat162_rn(o[2], o[3]);
+                        *reinterpret_cast<uint2*>(p) = w;
+                    } else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = __float2bfloat16_rn(o[e]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (failed && threadIdx.x == 0)                        // copies still under way land before the CTA leaves
+        for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(full + i % stages, (i / stages) & 1);
+    if (warp == 1) tmem_free<F::kTmem>(tmem);
+}
+
+// A rows x width matrix of bytes whose rows lie `stride` bytes apart (a multiple of 16; base on a 16-byte boundary); box =
+// box_rows x 128, 128-byte swizzle, zeros outside.  0 or a cudaError.
+int make_byte_map(CUtensorMap* map, const void* ptr, long rows, long width, long stride, int box_rows) {
+    EncodeTiled enc = tensor_map_encoder();
+    if (enc == nullptr) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+struct Operands {
+    const void *x, *w0, *w1;
+    long ldx, ldw;                                        // row strides, bytes
+};
+
+template <bool kSwap, int NR, bool kSwiglu>
+int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
+    typedef Form<kSwap, NR, kSwiglu> F;
+    const int blocks = (a.K + kBK - 1) / kBK, per = (blocks + a.split - 1) / a.split;
+    a.tiles_n = (a.N + kFeat - 1) / kFeat;
+    const long tiles = (long)((a.M + F::kXRows - 1) / F::kXRows) * a.tiles_n;
+    if (tiles * a.split > 0x7fffffffL) return kTooLarge;
+    // Shared memory: a ring as deep as the CTA's share of an SM allows; few rows: beside it the sums that land and the scales
+    const size_t side = kSwap ? ((size_t)(NR + a.split) * F::kPitch + (size_t)per * NR * (kSwiglu ? 2 : 1)) * 4 : 0;
+    const size_t sums = (size_t)(F::kXRows + a.split) * F::kPitch * 4;
+    const size_t budget = (F::kTwoPerSm && tiles * a.split > sms ? 112 : 224) * 1024;
+    if (side + 1024 + F::kStage > budget) return kTooLarge;
+    int stages = (int)((budget - 1024 - side) / F::kStage);
+    stages = stages < per ? stages : per;
+    a.stages = stages < kMaxStages ? stages : kMaxStages;
+    size_t smem = 1024 + a.stages * (size_t)F::kStage + side;
+    if (!kSwap && smem < 1024 + sums) smem = 1024 + sums;
+    CUtensorMap map_w0, map_w1, map_x;
+    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kFeat);
+    if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, kFeat); else map_w1 = map_w0; }
+    if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, F::kXRows);
+    if (rc != 0) return rc;
+    static size_t have = 0;
+    ensure_dynamic_smem(fp8_linear_kernel<kSwap, NR, kSwiglu>, smem, have);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * a.split)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = a.split > 1 ? 2 : 1;
+    rc = (int)cudaLaunchKernelEx(&cfg, fp8_linear_kernel<kSwap, NR, kSwiglu>, map_w0, map_w1, map_x, a);
+    return rc != 0 ? rc : launch_status();
+}
+
+// CTAs that share a tile's blocks of K: doubled as long as the GPU holds them and two blocks are left to each
+int default_split(long tiles, int blocks, int sms, int per_sm) {
+    int split = 1;
+    while (split < kMaxSplit && 2 * tiles * split <= (long)sms * per_sm && blocks / (2 * split) >= 2) split *= 2;
+    return split;
+}
+
+template <bool kSwiglu>
+int launch_any(const Operands& o, Args a, cudaStream_t s) {
+    int device = 0, sms = 148;
+    if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    const int blocks = (a.K + kBK - 1) / kBK;
+    const long tiles_n = (a.N + kFeat - 1) / kFeat;
+    if (a.M <= 64) {
+        a.split = default_split(tiles_n, blocks, sms, 2);
+        const int rc = a.M <= 16 ? launch<true, 16, kSwiglu>(o, a, sms, s) : a.M <= 32 ? launch<true, 32, kSwiglu>(o, a, sms, s)
+                                                                                     : launch<true, 64, kSwiglu>(o, a, sms, s);
+        if (rc != kTooLarge) return rc;                    // a K whose table of scales does not fit goes in tiles
+    }
+    a.split = default_split((a.M + 127) / 128 * tiles_n, blocks, sms, 1);
+    return launch<false, 128, kSwiglu>(o, a, sms, s);
+}
+}  // namespace
+
+// x: [M, K] e4m3 bytes, row stride ldx; w: [N, K], row stride ldw (strides multiples of 16, bases on 16 bytes); sx: float32
+// scales of x with a stride per row and per block of 128 columns, sw: of w with a stride per 128 features and per block.
+// bias: float32 [N] or null.  out: bfloat16 or (out_f32) float32, row stride ldo elements.  early: w and sw are complete and
+// stay as they are, whatever the kernels in front on the stream do.  `error`: a device int that is 0 before the call;
+// non-zero afterwards: a wait gave up.
+extern "C" int lb_linear_fp8(const void* x, long ldx, const float* sx, long sx_row, long sx_block, const void* w, long ldw,
+                             const float* sw, long sw_row, long sw_block, const float* bias, void* out, long ldo, int M, int N,
+                             int K, float out_scale, int out_f32, int early, int* error, void* stream) {
+    if (M <= 0 || N <= 0) return kOk;
+    if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return kBadSize;
+    Args a{};
+    a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sw; a.sw_row = sw_row; a.sw_block = sw_block;
+    a.bias = bias; a.out = out; a.ldo = ldo; a.M = M; a.N = N; a.K = K; a.out_scale = out_scale; a.out_f32 = out_f32;
+    a.early = early; a.error = error;
+    return launch_any<false>(Operands{x, w, nullptr, ldx, ldw}, a, (cudaStream_t)stream);
+}
+
+// gate and up: [N, K] each, the same row stride, their scales with the same strides.  q: [M, N] bytes, row stride ldq (a
+// multiple of 16), qs: its scales with a stride per row and per block.
+extern "C" int lb_linear_swiglu_fp8(const void* x, long ldx, const float* sx, long sx_row, long sx_block, const void* gate,
+                                    const void* up, long ldw, const float* sgate, const float* sup, long sw_row, long sw_block,
+                                    void* q, long ldq, float* qs, long qs_row, long qs_block, int M, int N, int K,
+                                    float act_scale, int early, int* error, void* stream) {
+    if (M <= 0 || N <= 0) return kOk;
+    if (K <= 0 || ldx % 16 || ldw % 16 || ldq % 16 || (((uintptr_t)x | (uintptr_t)gate | (uintptr_t)up | (uintptr_t)q) & 15)) return kBadSize;
+    Args a{};
+    a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sgate; a.sw1 = sup; a.sw_row = sw_row; a.sw_block = sw_block;
+    a.q = (uint8_t*)q; a.ldq = ldq; a.qs = qs; a.qs_row = qs_row; a.qs_block = qs_block; a.M = M; a.N = N; a.K = K;
+    a.act_scale = act_scale; a.early = early; a.error = error;
+    return launch_any<true>(Operands{x, gate, up, ldx, ldw}, a, (cudaStream_t)stream);
+}

@@ -143,6 +143,49 @@ class StreamRows:
         return self.act
 
 
+class Fp8Rows:
+    """Rows in 8-bit floating point: `values` [rows, width] float8_e4m3fn, whose rows lie at multiples of 16 bytes, and `scales`
+    [rows, ceil(width / 128)] float32, one for each row and 128 columns (the last block may be short).  Row m, column k stands for
+    values[m, k] * scales[m, k // 128].  The operators that make such rows lay the scales of one column block side by side
+    (strides (1, rows)); those that read them take any strides."""
+    __slots__ = ("values", "scales")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        self.values, self.scales = values, scales
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def tensor(self, dtype=torch.float32) -> torch.Tensor:
+        """What the rows stand for, as an ordinary tensor (elementary operations: for inspection, not for a step)."""
+        each = self.scales.repeat_interleave(128, 1)[:, :self.values.shape[1]]
+        return (self.values.float() * each).to(dtype)
+
+
+class Fp8Weight:
+    """A weight in 8-bit floating point: `values` [features, width] float8_e4m3fn, whose rows lie at multiples of 16 bytes, and
+    `scales` [ceil(features / 128), ceil(width / 128)] float32, one for each block of 128 x 128 (the last ones may be short).
+
+    `settled`: the values and scales are complete on the device and stay as they are, so that a product may ask for them before
+    the kernels in front of it on its stream have ended.  Set it once whatever wrote them has been waited for (a model does
+    after its weights are loaded); without it every product waits for all that is in front of it."""
+    __slots__ = ("values", "scales", "settled")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, settled: bool = False):
+        self.values, self.scales, self.settled = values, scales, settled
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def tensor(self, dtype=torch.float32) -> torch.Tensor:
+        """What the weight stands for, as an ordinary tensor (elementary operations: for inspection, not for a step)."""
+        rows, width = self.values.shape
+        each = self.scales.repeat_interleave(128, 0)[:rows].repeat_interleave(128, 1)[:, :width]
+        return (self.values.float() * each).to(dtype)
+
+
 @dataclass(frozen=True)
 class StepSizes:
     """Sizes, multipliers and epsilons of a pre-norm layer with attention and a Mamba2 mixer side by side and a gated

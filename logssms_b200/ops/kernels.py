@@ -19,7 +19,7 @@ from ctypes import c_float, c_int, c_long, c_void_p
 import torch
 
 from . import build
-from .fusion import NormedRows, ResidualJoin, ScaledRows, StepSizes, SummedRows      # the fusion protocol (re-exported here)
+from .fusion import Fp8Rows, Fp8Weight, NormedRows, ResidualJoin, ScaledRows, StepSizes, SummedRows      # the fusion protocol (re-exported here)
 from .profiler import PROFILER
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
@@ -2621,3 +2621,143 @@ def stream_pair_rows(x: torch.Tensor, x0: torch.Tensor) -> torch.Tensor:
     f = _fn("stream_layer", "lb_stream_pair_rows", [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(x), _ptr(x0), _ptr(out), x.shape[0], x.shape[1], _code(x0), _stream()), "stream_pair_rows")
     return out
+
+
+# --------------------------------------------------------------------------- 8-bit floating point
+# e4m3 values with a float32 scale per block of 128: max(max |v| / 448, 2^-126); a value is v / scale, rounded once.
+_FP8 = torch.float8_e4m3fn
+
+
+def _fp8_empty(rows: int, width: int, scale_rows: int, device, side_by_side: bool):
+    """(values, scales) to be written: rows at multiples of 16 bytes, the scales of a column block side by side or row by row."""
+    pitch = (width + 15) & -16
+    blocks = (width + 127) >> 7
+    return (torch.empty_strided((rows, width), (pitch, 1), dtype=_FP8, device=device),
+            torch.empty_strided((scale_rows, blocks), (1, scale_rows) if side_by_side else (blocks, 1), dtype=torch.float32, device=device))
+
+
+def _rows_of(t: torch.Tensor, name: str) -> int:
+    """Row stride of a [rows, width] matrix with unit column stride."""
+    _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{name} must be a [rows, width] matrix with unit column stride")
+    return t.stride(0)
+
+
+def _fp8_operand(t, name: str, cls, block_rows: int, device=None):
+    """Checks an `Fp8Rows` or `Fp8Weight`; returns its row stride in bytes."""
+    _need(isinstance(t, cls), f"{name} must be `{cls.__name__}`")
+    v, s = t.values, t.scales
+    if not (v.is_cuda and s.is_cuda):
+        raise KernelError("logssms_b200 kernels run on CUDA tensors only; there is no CPU path")
+    _need(v.dtype == _FP8 and s.dtype == torch.float32, f"{name}: float8_e4m3fn values and float32 scales")
+    _need(v.dim() == 2 and v.shape[1] > 0 and s.shape == (-(-v.shape[0] // block_rows), (v.shape[1] + 127) >> 7),
+          f"{name}: values [rows, width] and one scale for each {'row' if block_rows == 1 else '128 rows'} and 128 columns")
+    _need(v.device == s.device and (device is None or v.device == device), f"{name}: values, scales and operands must be on one device")
+    pitch = v.stride(0) if v.shape[0] > 1 else (v.shape[1] + 15) & -16
+    _need((v.stride(1) == 1 or v.shape[1] == 1) and pitch % 16 == 0 and pitch >= v.shape[1] and v.data_ptr() % 16 == 0,
+          f"{name}: rows of values must lie at multiples of 16 bytes, on a 16-byte boundary (the quantising operators lay them out so)")
+    return pitch
+
+
+def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None, *,
+                    other: torch.Tensor | None = None, in_scales=(1.0, 1.0), out_scale: float = 1.0,
+                    want_residual: bool = True, in_place: bool = True):
+    """(`Fp8Rows`, new residual): r = x * in_scales[0] (+ other * in_scales[1]) (+ residual), the new residual is r rounded to
+    x's dtype, and the rows are r * rsqrt(mean(r^2) + eps) * weight * out_scale in 8 bits, a scale per 128 columns.  All of it is
+    32-bit up to the two roundings.  The new residual is written in place of `residual` when one is given, unless `in_place` is
+    off (then into a new tensor); None without `want_residual`.  Row strides are free."""
+    _cuda(x, weight, residual, other)
+    ldx = _rows_of(x, "x")
+    rows, width = x.shape
+    _need(width > 0, "rows need at least one column")
+    _need(weight.dtype == torch.float32 and weight.shape == (width,) and weight.is_contiguous(),
+          "norm weight must be a contiguous float32 vector of the row width")
+    ldo = ldr = 0
+    if other is not None:
+        ldo = _rows_of(other, "other")
+        _need(other.shape == x.shape and other.dtype == x.dtype, "other must match the input")
+    if residual is not None:
+        ldr = _rows_of(residual, "residual")
+        _need(residual.shape == x.shape and residual.dtype == x.dtype, "residual must match the input")
+    new = None
+    if want_residual:
+        new = residual if residual is not None and in_place else torch.empty((rows, width), dtype=x.dtype, device=x.device)
+    values, scales = _fp8_empty(rows, width, rows, x.device, True)
+    f = _fn("fp8_rows", "lb_add_rmsnorm_fp8",
+            [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_long,
+             c_long, c_int, c_int, c_float, c_float, c_float, c_float, c_int, c_void_p])
+    _check(f(x.data_ptr(), ldx, _ptr(other), ldo, _ptr(residual), ldr, _ptr(new), 0 if new is None else new.stride(0),
+             weight.data_ptr(), values.data_ptr(), values.stride(0), scales.data_ptr(), 1, rows, rows, width, eps, in_scales[0],
+             in_scales[1], out_scale, _code(x), _stream()), "add_rmsnorm_fp8", f"(width {width})")
+    return Fp8Rows(values, scales), new
+
+
+def _quantize(x: torch.Tensor, block_rows: int):
+    _cuda(x)
+    ldx = _rows_of(x, "x")
+    rows, width = x.shape
+    _need(width > 0, "rows need at least one column")
+    side_by_side = block_rows == 1
+    values, scales = _fp8_empty(rows, width, -(-rows // block_rows), x.device, side_by_side)
+    f = _fn("fp8_rows", "lb_quantize_fp8", [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_long, c_int, c_int,
+                                            c_int, c_void_p])
+    _check(f(x.data_ptr(), ldx, values.data_ptr(), values.stride(0), scales.data_ptr(), 1 if side_by_side else scales.shape[1],
+             rows if side_by_side else 1, rows, width, block_rows, _code(x), _stream()),
+           "quantize_rows_fp8" if side_by_side else "quantize_weight_fp8", f"(width {width})")
+    return values, scales
+
+
+def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
+    """[rows, width] bfloat16 or float32 in 8 bits, a scale for each row and 128 columns.  The row stride is free."""
+    return Fp8Rows(*_quantize(x, 1))
+
+
+def quantize_weight_fp8(w: torch.Tensor) -> Fp8Weight:
+    """[features, width] bfloat16 or float32 in 8 bits, a scale for each block of 128 x 128.  The row stride is free."""
+    return Fp8Weight(*_quantize(w, 128))
+
+
+def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, out_scale: float = 1.0,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(x [M, K] @ w[N, K]^T + bias) * out_scale of 8-bit operands: 32-bit sums, rounded once, to `out_dtype` (bfloat16 or
+    float32).  `bias`: float32 [N].  `check_kernel_errors()` reports a kernel whose internal wait gave up."""
+    ldx = _fp8_operand(x, "x", Fp8Rows, 1)
+    device = x.values.device
+    ldw = _fp8_operand(w, "w", Fp8Weight, 128, device)
+    (M, width), (N, wide) = x.values.shape, w.values.shape
+    _need(wide == width, f"weight must be [N, {width}], got [{N}, {wide}]")
+    _need(out_dtype in _DTYPE_CODE, "out_dtype must be bfloat16 or float32")
+    if bias is not None:
+        _cuda(bias)
+        _need(bias.dtype == torch.float32 and bias.shape == (N,) and bias.is_contiguous() and bias.device == device,
+              "bias must be a contiguous float32 vector of the weight's features")
+    out = torch.empty((M, N), dtype=out_dtype, device=device)
+    xs, ws = x.scales, w.scales
+    f = _fn("fp8_linear", "lb_linear_fp8",
+            [c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_long, c_int,
+             c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p])
+    _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), w.values.data_ptr(), ldw, ws.data_ptr(),
+             ws.stride(0), ws.stride(1), _ptr(bias), out.data_ptr(), N, M, N, width, out_scale, int(out_dtype == torch.float32),
+             int(w.settled), error_word(device).data_ptr(), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
+    return out
+
+
+def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: float = 1.0) -> Fp8Rows:
+    """silu((x @ gate^T) * act_scale) * (x @ up^T) of 8-bit operands, in 32 bits up to the result, which is 8-bit rows again (a
+    scale for each row and 128 features): one kernel.  `check_kernel_errors()` reports one whose internal wait gave up."""
+    ldx = _fp8_operand(x, "x", Fp8Rows, 1)
+    device = x.values.device
+    ldg, ldu = _fp8_operand(gate, "gate", Fp8Weight, 128, device), _fp8_operand(up, "up", Fp8Weight, 128, device)
+    (M, width), (N, wide) = x.values.shape, gate.values.shape
+    _need(wide == width and up.values.shape == gate.values.shape, f"gate and up must both be [N, {width}]")
+    gs, us = gate.scales, up.scales
+    _need(ldg == ldu and gs.stride() == us.stride(), "gate and up must be laid out alike")
+    values, scales = _fp8_empty(M, N, M, device, True)
+    f = _fn("fp8_linear", "lb_linear_swiglu_fp8",
+            [c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_long, c_long, c_void_p,
+             c_long, c_void_p, c_long, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+    xs = x.scales
+    _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), gate.values.data_ptr(), up.values.data_ptr(), ldg,
+             gs.data_ptr(), us.data_ptr(), gs.stride(0), gs.stride(1), values.data_ptr(), values.stride(0), scales.data_ptr(), 1, M, M,
+             N, width, act_scale, int(gate.settled and up.settled), error_word(device).data_ptr(), _stream()),
+           "linear_swiglu_fp8", f"([{M}, {width}] x 2 x [{N}, {width}])")
+    return Fp8Rows(values, scales)
