@@ -25,78 +25,17 @@
 //
 // Every wait on an mbarrier is bounded; one that gives up records itself in `error`, all roles run out of their own bounded
 // waits, every thread still meets the cluster barriers, tensor memory is freed and the kernel returns.
-#include "lb200/common.cuh"
-#include "lb200/fp8.cuh"
-#include "lb200/tcgen05.cuh"
+#include "lb200/fp8_linear.cuh"
+#include "lb200/fp8_pair.cuh"
 using namespace lb200;
-using namespace lb200::tc;
+using namespace lb200::fp8;
 
 namespace {
-constexpr int kBK = kFp8Block;                            // columns of a block = bytes of a swizzled row
 constexpr int kFeat = 128;
 constexpr uint32_t kWBytes = kFeat * kBK;
 constexpr int kSumThreads = 256;                          // warps 2-9
 constexpr int kThreads = 64 + kSumThreads;
 constexpr int kMaxStages = 8, kMaxSplit = 8;
-
-struct Args {
-    const float* sx; long sx_row, sx_block;               // scales of x: strides per row and per block
-    const float *sw0, *sw1; long sw_row, sw_block;        // scales of W (swiglu: gate, up): strides per 128 features and per block
-    const float* bias; void* out; long ldo;
-    uint8_t* q; long ldq; float* qs; long qs_row, qs_block;    // swiglu: the 8-bit rows
-    int M, N, K;
-    int split, stages, tiles_n;
-    int early;                                            // W may be read before the kernels in front have ended
-    int out_f32;
-    float out_scale, act_scale;
-    int* error;
-};
-
-__device__ __forceinline__ void report(int* error, int role, int step) {
-    if (error != nullptr) atomicCAS(error, 0, 0x20000000 | (role << 24) | ((blockIdx.x & 0xFFF) << 12) | (step & 0xFFF));
-}
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t peer_addr(uint32_t local, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void store_peer(uint32_t addr, float a) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(a) : "memory");
-}
-__device__ __forceinline__ void store_peer4(uint32_t addr, float a, float b, float c, float d) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
-// e4m3 operands, both K-major, float32 accumulator: formats 0 and 0
-__host__ __device__ constexpr uint32_t f8_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-// 16 consecutive float32 columns of this thread's lane of tensor memory; complete after tmem_ld_wait()
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// (a0, a1) += (d0, d1) * (s0, s1): both in one instruction
-__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t d0, uint32_t d1, float s0, float s1) {
-    asm("{\n\t.reg .b64 a, d, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 d, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\t"
-        "fma.rn.f32x2 a, d, s, a;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
-}
-// the product of two scales, finite where both are: a zero sum stays zero
-__device__ __forceinline__ float join(float a, float b) {
-    const float s = a * b;
-    return (magnitude(s) == 0x7f800000u && magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) ? 3.402823466e38f : s;
-}
 
 // kSwap: NR rows on the N side; else 128 rows on the M side (NR = 128).
 template <bool kSwap, int NR, bool kSwiglu>
@@ -371,21 +310,6 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     if (warp == 1) tmem_free<F::kTmem>(tmem);
 }
 
-// A rows x width matrix of bytes whose rows lie `stride` bytes apart (a multiple of 16; base on a 16-byte boundary); box =
-// box_rows x 128, 128-byte swizzle, zeros outside.  0 or a cudaError.
-int make_byte_map(CUtensorMap* map, const void* ptr, long rows, long width, long stride, int box_rows) {
-    EncodeTiled enc = tensor_map_encoder();
-    if (enc == nullptr) return (int)cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)kBK, (cuuint32_t)box_rows};
-    const cuuint32_t elem[2] = {1, 1};
-    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return rc == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
-}
-
 struct Operands {
     const void *x, *w0, *w1;
     long ldx, ldw;                                        // row strides, bytes
@@ -434,19 +358,54 @@ int default_split(long tiles, int blocks, int sms, int per_sm) {
     return split;
 }
 
+enum : int { kAuto = 0, kRows = 1, kTiles = 2, kPair = 3 };
+
 template <bool kSwiglu>
-int launch_any(const Operands& o, Args a, cudaStream_t s) {
+int launch_pair(const Operands& o, Args a, int sms, cudaStream_t s) {
+    constexpr int feat = kSwiglu ? 128 : 256;
+    const long tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + feat - 1) / feat);
+    if (tiles > 0x3fffffffL) return kTooLarge;
+    const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+    CUtensorMap map_w0, map_w1, map_x;
+    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 64 : 128);
+    if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, 64); else map_w1 = map_w0; }
+    if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, 128);
+    if (rc != 0) return rc;
+    static size_t have = 0;
+    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu>, kPairSmem, have);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = kPairSmem; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu>, map_w0, map_w1, map_x, a);
+    return rc != 0 ? rc : launch_status();
+}
+
+// `form`: kAuto, or the form that is asked for (its low byte) with so many CTAs per tile (the next byte; 0: by the rule)
+template <bool kSwiglu>
+int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
     int device = 0, sms = 148;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     const int blocks = (a.K + kBK - 1) / kBK;
     const long tiles_n = (a.N + kFeat - 1) / kFeat;
-    if (a.M <= 64) {
-        a.split = default_split(tiles_n, blocks, sms, 2);
+    int split = (form >> 8) & 255;
+    if (split > blocks) split = blocks;
+    if (split > kMaxSplit) return kBadSize;
+    form &= 255;
+    if (form == kRows || (form == kAuto && a.M <= 64)) {
+        if (a.M > 64) return kTooLarge;
+        a.split = split ? split : default_split(tiles_n, blocks, sms, 2);
         const int rc = a.M <= 16 ? launch<true, 16, kSwiglu>(o, a, sms, s) : a.M <= 32 ? launch<true, 32, kSwiglu>(o, a, sms, s)
                                                                                      : launch<true, 64, kSwiglu>(o, a, sms, s);
-        if (rc != kTooLarge) return rc;                    // a K whose table of scales does not fit goes in tiles
+        if (rc != kTooLarge || form != kAuto) return rc;   // a K whose table of scales does not fit goes in tiles
     }
-    a.split = default_split((a.M + 127) / 128 * tiles_n, blocks, sms, 1);
+    const long pair_tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + (kSwiglu ? 127 : 255)) / (kSwiglu ? 128 : 256));
+    if (form == kPair || (form == kAuto && pair_tiles >= sms / 4)) return launch_pair<kSwiglu>(o, a, sms, s);
+    a.split = split ? split : default_split((a.M + 127) / 128 * tiles_n, blocks, sms, 1);
     return launch<false, 128, kSwiglu>(o, a, sms, s);
 }
 }  // namespace
@@ -455,17 +414,17 @@ int launch_any(const Operands& o, Args a, cudaStream_t s) {
 // scales of x with a stride per row and per block of 128 columns, sw: of w with a stride per 128 features and per block.
 // bias: float32 [N] or null.  out: bfloat16 or (out_f32) float32, row stride ldo elements.  early: w and sw are complete and
 // stay as they are, whatever the kernels in front on the stream do.  `error`: a device int that is 0 before the call;
-// non-zero afterwards: a wait gave up.
+// non-zero afterwards: a wait gave up.  form: 0, or a form of the kernel (kRows, kTiles, kPair).
 extern "C" int lb_linear_fp8(const void* x, long ldx, const float* sx, long sx_row, long sx_block, const void* w, long ldw,
                              const float* sw, long sw_row, long sw_block, const float* bias, void* out, long ldo, int M, int N,
-                             int K, float out_scale, int out_f32, int early, int* error, void* stream) {
+                             int K, float out_scale, int out_f32, int early, int form, int* error, void* stream) {
     if (M <= 0 || N <= 0) return kOk;
     if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return kBadSize;
     Args a{};
     a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sw; a.sw_row = sw_row; a.sw_block = sw_block;
     a.bias = bias; a.out = out; a.ldo = ldo; a.M = M; a.N = N; a.K = K; a.out_scale = out_scale; a.out_f32 = out_f32;
     a.early = early; a.error = error;
-    return launch_any<false>(Operands{x, w, nullptr, ldx, ldw}, a, (cudaStream_t)stream);
+    return launch_any<false>(Operands{x, w, nullptr, ldx, ldw}, a, form, (cudaStream_t)stream);
 }
 
 // gate and up: [N, K] each, the same row stride, their scales with the same strides.  q: [M, N] bytes, row stride ldq (a
@@ -473,12 +432,12 @@ extern "C" int lb_linear_fp8(const void* x, long ldx, const float* sx, long sx_r
 extern "C" int lb_linear_swiglu_fp8(const void* x, long ldx, const float* sx, long sx_row, long sx_block, const void* gate,
                                     const void* up, long ldw, const float* sgate, const float* sup, long sw_row, long sw_block,
                                     void* q, long ldq, float* qs, long qs_row, long qs_block, int M, int N, int K,
-                                    float act_scale, int early, int* error, void* stream) {
+                                    float act_scale, int early, int form, int* error, void* stream) {
     if (M <= 0 || N <= 0) return kOk;
     if (K <= 0 || ldx % 16 || ldw % 16 || ldq % 16 || (((uintptr_t)x | (uintptr_t)gate | (uintptr_t)up | (uintptr_t)q) & 15)) return kBadSize;
     Args a{};
     a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sgate; a.sw1 = sup; a.sw_row = sw_row; a.sw_block = sw_block;
     a.q = (uint8_t*)q; a.ldq = ldq; a.qs = qs; a.qs_row = qs_row; a.qs_block = qs_block; a.M = M; a.N = N; a.K = K;
     a.act_scale = act_scale; a.early = early; a.error = error;
-    return launch_any<true>(Operands{x, gate, up, ldx, ldw}, a, (cudaStream_t)stream);
+    return launch_any<true>(Operands{x, gate, up, ldx, ldw}, a, form, (cudaStream_t)stream);
 }

@@ -2626,6 +2626,9 @@ def stream_pair_rows(x: torch.Tensor, x0: torch.Tensor) -> torch.Tensor:
 # --------------------------------------------------------------------------- 8-bit floating point
 # e4m3 values with a float32 scale per block of 128: max(max |v| / 448, 2^-126); a value is v / scale, rounded once.
 _FP8 = torch.float8_e4m3fn
+# which form of the products' kernel runs: "auto" (by the sizes), or "rows" (up to 64 rows), "tiles", "pair" for all of them
+FP8_FORM = "auto"
+_FP8_FORMS = {"auto": 0, "rows": 1, "tiles": 2, "pair": 3}
 
 
 def _fp8_empty(rows: int, width: int, scale_rows: int, device, side_by_side: bool):
@@ -2734,10 +2737,10 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, ou
     xs, ws = x.scales, w.scales
     f = _fn("fp8_linear", "lb_linear_fp8",
             [c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_long, c_int,
-             c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p])
+             c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p])
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), w.values.data_ptr(), ldw, ws.data_ptr(),
              ws.stride(0), ws.stride(1), _ptr(bias), out.data_ptr(), N, M, N, width, out_scale, int(out_dtype == torch.float32),
-             int(w.settled), error_word(device).data_ptr(), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
+             int(w.settled), _FP8_FORMS[FP8_FORM], error_word(device).data_ptr(), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
     return out
 
 
@@ -2754,10 +2757,10 @@ def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: flo
     values, scales = _fp8_empty(M, N, M, device, True)
     f = _fn("fp8_linear", "lb_linear_swiglu_fp8",
             [c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_long, c_long, c_void_p,
-             c_long, c_void_p, c_long, c_long, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p])
+             c_long, c_void_p, c_long, c_long, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p])
     xs = x.scales
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), gate.values.data_ptr(), up.values.data_ptr(), ldg,
              gs.data_ptr(), us.data_ptr(), gs.stride(0), gs.stride(1), values.data_ptr(), values.stride(0), scales.data_ptr(), 1, M, M,
-             N, width, act_scale, int(gate.settled and up.settled), error_word(device).data_ptr(), _stream()),
+             N, width, act_scale, int(gate.settled and up.settled), _FP8_FORMS[FP8_FORM], error_word(device).data_ptr(), _stream()),
            "linear_swiglu_fp8", f"([{M}, {width}] x 2 x [{N}, {width}])")
     return Fp8Rows(values, scales)

@@ -12,6 +12,15 @@ def K():
     return kernels
 
 
+@pytest.fixture(params=["auto", "tiles", "pair"])
+def form(request):
+    """The form of the kernel that runs, whatever the rule would choose."""
+    k = K()
+    k.FP8_FORM = request.param
+    yield request.param
+    k.FP8_FORM = "auto"
+
+
 def operands(m, n, k, seed=0, row_major=False):
     g = torch.Generator().manual_seed(1000 * m + n + k + seed)
     kk = K()
@@ -58,7 +67,7 @@ SIZES = [(1, 16), (40, 100), (128, 128), (130, 1), (257, 640), (1003, 1431), (12
 
 @pytest.mark.parametrize("m", ROWS)
 @pytest.mark.parametrize("n,k", SIZES)
-def test_linear(m, n, k):
+def test_linear(m, n, k, form):
     x, w = operands(m, n, k, seed=m % 2, row_major=m % 3 == 0)
     check_linear(x, w)
     check_linear(x, w, torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda(), 0.7)
@@ -66,7 +75,7 @@ def test_linear(m, n, k):
 
 @pytest.mark.parametrize("m", ROWS)
 @pytest.mark.parametrize("n,k", SIZES)
-def test_swiglu(m, n, k):
+def test_swiglu(m, n, k, form):
     x, gate = operands(m, n, k, seed=m % 2, row_major=m % 3 == 0)
     _, up = operands(m, n, k, seed=m % 2 + 2)
     check_swiglu(x, gate, up, 0.9)
@@ -74,14 +83,14 @@ def test_swiglu(m, n, k):
 
 # a K whose scales do not fit beside the ring, long sums, prompts
 @pytest.mark.parametrize("m,n,k", [(64, 70000, 3000), (64, 256, 70000), (16, 128, 140000), (700, 640, 2500), (2100, 1300, 1100)])
-def test_large(m, n, k):
+def test_large(m, n, k, form):
     x, w = operands(m, n, k)
     check_linear(x, w)
     if n * k < 1 << 26:
         check_swiglu(x, w, operands(m, n, k, 2)[1], 1.0)
 
 
-def test_every_block_has_its_own_scales():
+def test_every_block_has_its_own_scales(form):
     """Blocks of very different size: a scale that met a neighbour's block would be off by its factor."""
     k = K()
     g = torch.Generator().manual_seed(5)
@@ -98,7 +107,7 @@ def test_every_block_has_its_own_scales():
         check_swiglu(xq, wq, wq, 1e-3)
 
 
-def test_the_order_of_sums_is_fixed():
+def test_the_order_of_sums_is_fixed(form):
     k = K()
     x, w = operands(24, 640, 4096)
     first = k.linear_fp8(x, w, out_dtype=torch.float32)
