@@ -103,33 +103,44 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     pdl_wait();
 
     int issued = 0;
-    float sum[kMine];
+    uint64_t sum2[kMine / 2];                              // pairs of sums
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
+    for (int j = 0; j < kMine / 2; ++j) sum2[j] = 0;
     const int group = (warp - 2) >> 2, quarter = warp & 3;             // warpgroup; the lanes of tensor memory a warp may read
+    // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait takes
+    // some 200 cycles even when the phase is long over)
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one())
             for (int i = 0; i < first; ++i) { if (!a.early) load_w(i, i); load_x(i, i); }
-            issued = first;
-            for (int s = 0, parity = 0; issued < kbn && !failed; ++issued) {
-                if (!mbar_wait(empty + s, parity)) { report(a.error, 1, issued); failed = 1; break; }
+        issued = first;
+        int s = 0, parity = 0;
+        bool ready = false;
+        for (; issued < kbn; ++issued) {
+            if (!ready) ready = mbar_wait(empty + s, parity);
+            if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, issued); failed = 1; break; }
+            const int s1 = s + 1 == stages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
+            ready = mbar_test(empty + s1, parity1);
+            if (elect_one()) {
                 load_w(s, issued);
                 load_x(s, issued);
-                if (++s == stages) { s = 0; parity ^= 1; }
             }
+            s = s1; parity = parity1;
         }
-        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = kSwap ? f8_idesc(128, NR) : f8_idesc(128, F::kCols);
-            int s = 0, parity = 0;
-            for (int i = 0; i < kbn && !failed; ++i) {
-                const int acc = i % kAccs;
-                if (!mbar_wait(full + s, parity)) { report(a.error, 2, i); failed = 1; break; }
-                if (i >= kAccs && !mbar_wait(acc_empty + acc, (i / kAccs - 1) & 1)) { report(a.error, 3, i); failed = 1; break; }
-                fence_after_sync();
-                const uint64_t wdesc = umma_desc(base + (size_t)s * kStage);
-                const uint64_t xdesc = umma_desc(base + (size_t)s * kStage + (kSwiglu ? 2 : 1) * kWBytes);
+        constexpr uint32_t idesc = kSwap ? f8_idesc(128, NR) : f8_idesc(128, F::kCols);
+        constexpr uint32_t kXAt = ((kSwiglu ? 2 : 1) * kWBytes) >> 4;
+        const uint64_t desc0 = umma_desc(base);
+        int s = 0, parity = 0;
+        bool ready = false, room = true;
+        for (int i = 0; i < kbn; ++i) {
+            const int acc = i % kAccs;
+            if (!ready) ready = mbar_wait(full + s, parity);
+            if (!room) room = mbar_wait(acc_empty + acc, (i / kAccs - 1) & 1);
+            if (!__all_sync(0xffffffffu, ready && room)) { if (lane == 0) report(a.error, ready ? 3 : 2, i); failed = 1; break; }
+            fence_after_sync();
+            const int s1 = s + 1 == stages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
+            if (elect_one()) {
+                const uint64_t wdesc = desc0 + (uint64_t)(s * (kStage >> 4)), xdesc = wdesc + kXAt;
                 const uint32_t d = tmem + acc * F::kCols;
 #pragma unroll
                 for (int k = 0; k < kBK / 32; ++k) {       // 32 bytes along K: + 2 in the 16-byte address field
@@ -142,10 +153,12 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 }
                 umma_commit(empty + s);
                 umma_commit(acc_full + acc);
-                if (++s == stages) { s = 0; parity ^= 1; }
             }
+            __syncwarp();
+            ready = i + 1 < kbn && mbar_test(full + s1, parity1);
+            room = i + 1 < kAccs || (i + 1 < kbn && mbar_test(acc_empty + (i + 1) % kAccs, ((i + 1) / kAccs - 1) & 1));
+            s = s1; parity = parity1;
         }
-        __syncwarp();
     } else {
         const int t = threadIdx.x - 64;
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * kMine;
@@ -173,7 +186,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         bool ok = true;
         for (int i = 0; i < kbn; ++i) {
             const int acc = i % kAccs;
-            const float s = s_next;
+            const uint64_t both = pair_of(s_next, s_next);
             if (!kSwap && i + 1 < kbn) s_next = join(sx[(i + 1) * a.sx_block], sw[(i + 1) * a.sw_block]);
             ok = mbar_wait(acc_full + acc, (i / kAccs) & 1);
             ok = __all_sync(0xffffffffu, ok && !failed);
@@ -191,8 +204,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
 #pragma unroll
                 for (int j = 0; j < 8; j += 4) {
                     const float4 f = *reinterpret_cast<const float4*>(tab + j);
-                    fma2(sum[j], sum[j + 1], d[j], d[j + 1], f.x, f.y);
-                    fma2(sum[j + 2], sum[j + 3], d[j + 2], d[j + 3], f.z, f.w);
+                    fma2(sum2[j / 2], d[j], d[j + 1], pair_of(f.x, f.y));
+                    fma2(sum2[j / 2 + 1], d[j + 2], d[j + 3], pair_of(f.z, f.w));
                 }
             } else {
                 // 16 columns at a time, the next 16 on their way meanwhile
@@ -212,11 +225,11 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                     for (int j = 0; j < 16; j += 4) {
                         if (kSwap) {
                             const float4 f = *reinterpret_cast<const float4*>(tab + c + j);
-                            fma2(sum[c + j], sum[c + j + 1], now[j], now[j + 1], f.x, f.y);
-                            fma2(sum[c + j + 2], sum[c + j + 3], now[j + 2], now[j + 3], f.z, f.w);
+                            fma2(sum2[(c + j) / 2], now[j], now[j + 1], pair_of(f.x, f.y));
+                            fma2(sum2[(c + j) / 2 + 1], now[j + 2], now[j + 3], pair_of(f.z, f.w));
                         } else {
-                            fma2(sum[c + j], sum[c + j + 1], now[j], now[j + 1], s, s);
-                            fma2(sum[c + j + 2], sum[c + j + 3], now[j + 2], now[j + 3], s, s);
+                            fma2(sum2[(c + j) / 2], now[j], now[j + 1], both);
+                            fma2(sum2[(c + j) / 2 + 1], now[j + 2], now[j + 3], both);
                         }
                     }
                 }
@@ -232,6 +245,9 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         __syncthreads();
     }
     if (warp >= 2) {
+        float sum[kMine];
+#pragma unroll
+        for (int j = 0; j < kMine; j += 2) { sum[j] = low_of(sum2[j / 2]); sum[j + 1] = high_of(sum2[j / 2]); }
         const int feat = quarter * 32 + lane;
         if (kSwap) {
             const int j0 = kSwiglu ? 0 : group * kMine;

@@ -58,10 +58,31 @@ __device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t* r) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// (a0, a1) += (d0, d1) * (s0, s1): both in one instruction
-__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t d0, uint32_t d1, float s0, float s1) {
-    asm("{\n\t.reg .b64 a, d, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 d, {%2, %3};\n\tmov.b64 s, {%4, %5};\n\t"
-        "fma.rn.f32x2 a, d, s, a;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "r"(d0), "r"(d1), "f"(s0), "f"(s1));
+// Two float32 sums side by side in 64 bits, so that both are joined in one instruction: acc += (d0, d1) * scale
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t d0, uint32_t d1, uint64_t scale) {
+    asm("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\tfma.rn.f32x2 %0, d, %3, %0;\n\t}" : "+l"(acc) : "r"(d0), "r"(d1), "l"(scale));
+}
+__device__ __forceinline__ float low_of(uint64_t p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float high_of(uint64_t p) { return __uint_as_float((uint32_t)(p >> 32)); }
+// One thread of a whole warp.  The loops that feed the tensor core run on the whole warp, with this around the instructions that
+// one thread issues, so that addresses and descriptors stay in the warp's own registers: as a branch for lane 0, the four
+// products of a block and their two commits took 480 cycles to issue, nearly as long as they run.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+// has the phase with this parity completed?  (No waiting: asked for ahead of the work that precedes its use.)
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
 }
 // the product of two scales, finite where both are: a zero sum stays zero
 __device__ __forceinline__ float join(float a, float b) {

@@ -40,7 +40,9 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
                  ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    // (not a release at cluster scope, which waits for every load of the thread that is under way: 1,900 cycles a block.  What is
+    // handed over is tensor memory, ordered by tcgen05's own wait and fences)
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -98,45 +100,63 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     pdl_trigger();
     pdl_wait();
     int issued = 0;
+    const uint32_t full0 = peer_addr(smem_u32(full), 0);
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 0 && lane == 0) {
-            for (int t = pair, s = 0, parity = 1; t < tiles && !failed; t += pairs) {
+        // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait
+        // takes some 200 cycles even when the phase is long over)
+        if (warp == 0) {
+            int s = 0, parity = 1;
+            bool ready = true, going = true;
+            for (int t = pair; t < tiles && going; t += pairs) {
                 const Tile at = tile_at(t, tiles_m, tiles_n);
                 const int row = at.m * kPairRows + rank * 128, feat = at.n * kFeat;
-                for (int kb = 0; kb < kbn && !failed; ++kb, ++issued) {
-                    if (issued >= kPairStages && !mbar_wait(empty + s, parity)) { report(a.error, 1, kb); failed = 1; break; }
-                    uint8_t* x = base + (size_t)s * kPairStage;
-                    uint8_t* w = x + 128 * kBK;
-                    if (rank == 0) mbar_expect_tx(full + s, 2 * kPairStage);
-                    const uint32_t bar = peer_addr(smem_u32(full + s), 0);
-                    tma_load_2d_pair(x, &map_x, bar, kb * kBK, row);
-                    if (kSwiglu) {                         // gate and up of this CTA's 64 features
-                        tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 64);
-                        tma_load_2d_pair(w + 64 * kBK, &map_w1, bar, kb * kBK, feat + rank * 64);
-                    } else {
-                        tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 128);
+                for (int kb = 0; kb < kbn; ++kb, ++issued) {
+                    if (!ready) ready = mbar_wait(empty + s, parity);
+                    if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, kb); failed = 1; going = false; break; }
+                    const int s1 = s + 1 == kPairStages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
+                    ready = issued + 1 < kPairStages || mbar_test(empty + s1, parity1);
+                    if (elect_one()) {
+                        uint8_t* x = base + (size_t)s * kPairStage;
+                        uint8_t* w = x + 128 * kBK;
+                        if (rank == 0) mbar_expect_tx(full + s, 2 * kPairStage);
+                        const uint32_t bar = full0 + s * 8;
+                        tma_load_2d_pair(x, &map_x, bar, kb * kBK, row);
+                        if (kSwiglu) {                     // gate and up of this CTA's 64 features
+                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 64);
+                            tma_load_2d_pair(w + 64 * kBK, &map_w1, bar, kb * kBK, feat + rank * 64);
+                        } else {
+                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 128);
+                        }
                     }
-                    if (++s == kPairStages) { s = 0; parity ^= 1; }
+                    s = s1; parity = parity1;
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp == 1 && rank == 0) {
             constexpr uint32_t idesc = f8_idesc(256, 256);
-            int s = 0, parity = 0, n = 0;
-            for (int t = pair; t < tiles && !failed; t += pairs)
-                for (int kb = 0; kb < kbn && !failed; ++kb, ++n) {
-                    const int acc = n & 1;
-                    if (!mbar_wait(full + s, parity)) { report(a.error, 2, kb); failed = 1; break; }
-                    if (n >= 2 && !mbar_wait(acc_empty + acc, ((n >> 1) - 1) & 1)) { report(a.error, 3, kb); failed = 1; break; }
-                    fence_after_sync();
-                    const uint64_t xdesc = umma_desc(base + (size_t)s * kPairStage);
-                    const uint64_t wdesc = umma_desc(base + (size_t)s * kPairStage + 128 * kBK);
+            const uint64_t desc0 = umma_desc(base);
+            const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;      // blocks of all tiles of this pair
+            int s = 0, parity = 0;
+            bool ready = false, room = true;
+            for (int n = 0; n < total; ++n) {
+                const int acc = n & 1;
+                if (!ready) ready = mbar_wait(full + s, parity);
+                if (!room) room = mbar_wait(acc_empty + acc, ((n >> 1) - 1) & 1);
+                if (!__all_sync(0xffffffffu, ready && room)) { if (lane == 0) report(a.error, ready ? 3 : 2, n); failed = 1; break; }
+                fence_after_sync();
+                const int s1 = s + 1 == kPairStages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
+                if (elect_one()) {
+                    const uint64_t xdesc = desc0 + (uint64_t)(s * (kPairStage >> 4)), wdesc = xdesc + (128 * kBK >> 4);
 #pragma unroll
                     for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(tmem + acc * 256, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
                     umma_commit_pair(empty + s);
                     umma_commit_pair(acc_full + acc);
-                    if (++s == kPairStages) { s = 0; parity ^= 1; }
                 }
+                __syncwarp();
+                ready = n + 1 < total && mbar_test(full + s1, parity1);
+                room = n == 0 || (n + 1 < total && mbar_test(acc_empty + (acc ^ 1), (((n + 1) >> 1) - 1) & 1));
+                s = s1; parity = parity1;
+            }
         }
         __syncwarp();
     } else {
@@ -147,14 +167,15 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
         const int last_block = (a.N + kBK - 1) / kBK - 1;
         int n = 0;
         bool ok = true;
+        // A block's scales are asked for two blocks ahead, into one of two sets of registers
+        struct Scales { float x, w, u; };
+        Scales even, odd;
         const float *sx = nullptr, *sw = nullptr, *su = nullptr;
-        float x1 = 0.f, w1 = 0.f, u1 = 0.f, x2 = 0.f, w2 = 0.f, u2 = 0.f;        // the scales of the next block and the one after
-        int next = 0;
-        auto fetch = [&]() {
-            const int kb = min(next++, kbn - 1);
-            x1 = x2; w1 = w2; u1 = u2;
-            x2 = sx[kb * a.sx_block]; w2 = sw[kb * a.sw_block];
-            if (kSwiglu) u2 = su[kb * a.sw_block];
+        auto fetch = [&](Scales& f, int kb) {
+            kb = min(kb, kbn - 1);
+            f.x = sx[kb * a.sx_block];
+            f.w = sw[kb * a.sw_block];
+            f.u = kSwiglu ? su[kb * a.sw_block] : 0.f;
         };
         auto open = [&](int t) {                           // the scales' places of a tile, and its first two blocks' on their way
             const Tile at = tile_at(t, tiles_m, tiles_n);
@@ -162,42 +183,62 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             const int block = kSwiglu ? at.n : min(2 * at.n + group, last_block);
             sw = a.sw0 + block * a.sw_row;
             if (kSwiglu) su = a.sw1 + block * a.sw_row;
-            next = 0;
-            fetch();
-            fetch();
+            fetch(even, 0);
+            fetch(odd, 1);
         };
         if (pair < tiles) open(pair);
         for (int t = pair; t < tiles && ok; t += pairs) {
             const Tile at = tile_at(t, tiles_m, tiles_n);
-            float sum[128];
+            uint64_t sum2[64];
 #pragma unroll
-            for (int j = 0; j < 128; ++j) sum[j] = 0.f;
-            for (int kb = 0; kb < kbn; ++kb, ++n) {
-                const int acc = n & 1;
-                const float s = join(x1, w1), v = kSwiglu ? join(x1, u1) : s;
-                fetch();
-                ok = mbar_wait(acc_full + acc, (n >> 1) & 1);
-                ok = __all_sync(0xffffffffu, ok && !failed);
-                if (!ok) { if (lane == 0 && !failed) { report(a.error, 4, kb); failed = 1; } break; }
+            for (int j = 0; j < 64; ++j) sum2[j] = 0;
+            // 32 columns at a time, the next 32 on their way meanwhile, also from one block to the next: the wait for a block's
+            // accumulator is asked for early and its first columns are fetched before the last ones of the block before are added
+            uint32_t d[2][32];
+            auto arrived = [&](int at, bool known) {       // this warp may read accumulator number `at`
+                bool yes = known || mbar_wait(acc_full + (at & 1), (at >> 1) & 1);
+                yes = __all_sync(0xffffffffu, yes && !failed);
+                if (!yes && lane == 0 && !failed) { report(a.error, 4, at); failed = 1; }
                 fence_after_sync();
-                uint32_t d[2][32];
-                tmem_ld32_async(from + acc * 256, d[0]);
+                return yes;
+            };
+            auto block = [&](int kb, Scales& f) {
+                const float s = join(f.x, f.w), v = kSwiglu ? join(f.x, f.u) : s;
+                fetch(f, kb + 2);
+                const uint64_t low = pair_of(s, s), high = pair_of(v, v);
+                const uint32_t at = from + (n & 1) * 256;
+                bool ready = false;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     tmem_ld_wait();
-                    if (c < 3) tmem_ld32_async(from + acc * 256 + 32 * (c + 1), d[(c + 1) & 1]);
-                    else {
+                    if (c < 3) {
+                        tmem_ld32_async(at + 32 * (c + 1), d[(c + 1) & 1]);
+                        if (c == 1) ready = mbar_test(acc_full + ((n + 1) & 1), ((n + 1) >> 1) & 1);
+                    } else {
                         fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_at(release0 + acc * 8);
+                        if (lane == 0) mbar_arrive_at(release0 + (n & 1) * 8);
+                        if (kb + 1 < kbn) {
+                            ok = arrived(n + 1, ready);
+                            if (ok) tmem_ld32_async(from + ((n + 1) & 1) * 256, d[0]);
+                        }
                     }
-                    const float f = c < 2 ? s : v;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) fma2(sum[32 * c + j], sum[32 * c + j + 1], d[c & 1][j], d[c & 1][j + 1], f, f);
+                    for (int j = 0; j < 16; ++j) fma2(sum2[16 * c + j], d[c & 1][2 * j], d[c & 1][2 * j + 1], c < 2 ? low : high);
                 }
+                ++n;
+            };
+            ok = arrived(n, false);
+            if (ok) tmem_ld32_async(from + (n & 1) * 256, d[0]);
+            for (int kb = 0; kb < kbn && ok; kb += 2) {
+                block(kb, even);
+                if (ok && kb + 1 < kbn) block(kb + 1, odd);
             }
             if (!ok) break;
             if (t + pairs < tiles) open(t + pairs);
+            float sum[128];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) { sum[2 * j] = low_of(sum2[j]); sum[2 * j + 1] = high_of(sum2[j]); }
             const long m = (long)at.m * kPairRows + rank * 128 + in_tile;
             if constexpr (kSwiglu) {
                 const int f0 = at.n * 128 + group * 64;    // this thread's features
