@@ -84,10 +84,20 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
                  : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return done != 0;
 }
+// Wait by asking again and again: mbarrier.try_wait takes some 300 cycles even when the phase is long over, a test 50, and the
+// loops here hand an accumulator to and fro every 500.  false: the phase did not complete within about a second.
+__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity) {
+    for (uint32_t spin = 0; spin < (kSpinLimit << 3); ++spin)
+        if (mbar_test(bar, parity)) return true;
+    return false;
+}
 // the product of two scales, finite where both are: a zero sum stays zero
 __device__ __forceinline__ float join(float a, float b) {
-    const float s = a * b;
-    return (magnitude(s) == 0x7f800000u && magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) ? 3.402823466e38f : s;
+    float s = a * b;
+    if (magnitude(s) == 0x7f800000u) {
+        if (magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) s = copysignf(3.402823466e38f, s);
+    }
+    return s;
 }
 
 // A rows x width matrix of bytes whose rows lie `stride` bytes apart (a multiple of 16; base on a 16-byte boundary); box =

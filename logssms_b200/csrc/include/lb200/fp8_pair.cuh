@@ -20,10 +20,17 @@
 namespace lb200 {
 namespace fp8 {
 
-constexpr int kPairThreads = 384, kPairStages = 6;
-constexpr uint32_t kPairStage = 256 * kBK;                // this CTA's 128 rows of x and 128 features of W
 constexpr int kPairRows = 256;
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage;
+// Tiles of 192 features, for SwiGLU of 128 gate and 128 up features: a thread of `kGroups` warpgroups adds 64 columns
+template <bool kSwiglu>
+struct Pair {
+    static constexpr int kGroups = kSwiglu ? 4 : 3, kAdders = 128 * kGroups, kThreads = 128 + kAdders;
+    static constexpr int kCols = 64 * kGroups;            // accumulator columns of a block
+    static constexpr int kFeat = kSwiglu ? 128 : kCols;   // output features of a tile
+    static constexpr uint32_t kStage = (128 + kCols / 2) * kBK;        // a CTA's 128 rows of x and half of the features
+    static constexpr int kStages = kSwiglu ? 6 : 7;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage;
+};
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -44,14 +51,30 @@ __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
     // handed over is tensor memory, ordered by tcgen05's own wait and fences)
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32_async(uint32_t addr, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+// the same where `mine` is set, without a branch
+__device__ __forceinline__ void mbar_arrive_at_if(uint32_t bar, uint32_t mine) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"(mine) : "memory");
+}
+__device__ __forceinline__ bool mbar_test_at(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+// barriers of the CTA among `kCount` threads: some only arrive, the others sleep until all have
+template <int kCount>
+__device__ __forceinline__ void wake(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
+template <int kCount>
+__device__ __forceinline__ void sleep_until_woken(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
+// 64 consecutive float32 columns of this thread's lane of tensor memory; complete after tmem_ld_wait()
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t (&r)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), 
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), 
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), 
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
                  : "r"(addr));
 }
 
@@ -66,14 +89,16 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
 }
 
 template <bool kSwiglu>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(Pair<kSwiglu>::kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                 const __grid_constant__ CUtensorMap map_x, Args a) {
-    constexpr int kFeat = kSwiglu ? 128 : 256;            // output features of a tile
+    typedef Pair<kSwiglu> P;
+    constexpr int kFeat = P::kFeat, kPairStages = P::kStages, kPairGroups = P::kGroups;
+    constexpr uint32_t kPairStage = P::kStage;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
-    __shared__ uint32_t tops[2][128];                     // SwiGLU: a row's largest magnitude in either half of the features
+    __shared__ __align__(16) uint64_t acc_full[2], acc_empty[2], full[kPairStages], empty[kPairStages];
+    __shared__ uint32_t tops[kSwiglu ? kPairGroups : 1][128];       // SwiGLU: a row's largest magnitude among a group's features
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,7 +108,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     const int kbn = (a.K + kBK - 1) / kBK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 16); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * 4 * kPairGroups); }
         failed = 0;
         mbar_fence_init();
     }
@@ -102,7 +127,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     int issued = 0;
     const uint32_t full0 = peer_addr(smem_u32(full), 0);
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if constexpr (kSwiglu) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");       // 640 threads x 96 registers
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");                         // 512 x 128
         // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait
         // takes some 200 cycles even when the phase is long over)
         if (warp == 0) {
@@ -112,7 +138,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 const Tile at = tile_at(t, tiles_m, tiles_n);
                 const int row = at.m * kPairRows + rank * 128, feat = at.n * kFeat;
                 for (int kb = 0; kb < kbn; ++kb, ++issued) {
-                    if (!ready) ready = mbar_wait(empty + s, parity);
+                    if (!ready) ready = mbar_spin(empty + s, parity);
                     if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, kb); failed = 1; going = false; break; }
                     const int s1 = s + 1 == kPairStages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
                     ready = issued + 1 < kPairStages || mbar_test(empty + s1, parity1);
@@ -122,26 +148,29 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                         if (rank == 0) mbar_expect_tx(full + s, 2 * kPairStage);
                         const uint32_t bar = full0 + s * 8;
                         tma_load_2d_pair(x, &map_x, bar, kb * kBK, row);
-                        if (kSwiglu) {                     // gate and up of this CTA's 64 features
-                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 64);
-                            tma_load_2d_pair(w + 64 * kBK, &map_w1, bar, kb * kBK, feat + rank * 64);
+                        if (kSwiglu) {                     // gate and up of two groups' 32 features each
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                tma_load_2d_pair(w + 64 * g * kBK, &map_w0, bar, kb * kBK, feat + rank * 64 + 32 * g);
+                                tma_load_2d_pair(w + (64 * g + 32) * kBK, &map_w1, bar, kb * kBK, feat + rank * 64 + 32 * g);
+                            }
                         } else {
-                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * 128);
+                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * (P::kCols / 2));
                         }
                     }
                     s = s1; parity = parity1;
                 }
             }
         } else if (warp == 1 && rank == 0) {
-            constexpr uint32_t idesc = f8_idesc(256, 256);
+            constexpr uint32_t idesc = f8_idesc(256, P::kCols);
             const uint64_t desc0 = umma_desc(base);
             const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;      // blocks of all tiles of this pair
             int s = 0, parity = 0;
             bool ready = false, room = true;
             for (int n = 0; n < total; ++n) {
                 const int acc = n & 1;
-                if (!ready) ready = mbar_wait(full + s, parity);
-                if (!room) room = mbar_wait(acc_empty + acc, ((n >> 1) - 1) & 1);
+                if (!ready) ready = mbar_spin(full + s, parity);
+                if (!room) room = mbar_spin(acc_empty + acc, ((n >> 1) - 1) & 1);
                 if (!__all_sync(0xffffffffu, ready && room)) { if (lane == 0) report(a.error, ready ? 3 : 2, n); failed = 1; break; }
                 fence_after_sync();
                 const int s1 = s + 1 == kPairStages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
@@ -157,105 +186,110 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 room = n == 0 || (n + 1 < total && mbar_test(acc_empty + (acc ^ 1), (((n + 1) >> 1) - 1) & 1));
                 s = s1; parity = parity1;
             }
+        } else if (warp == 2) {
+            // One warp per CTA watches the accumulators and wakes the warps that add, by a barrier that costs them nothing while they
+            // wait: a dozen warps that ask the same mbarrier make each answer, also the one to the warp that issues the products,
+            // some 300 cycles late.  After a wait that gave up it goes on without waiting: everybody else's loops end by count.
+            const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;
+            bool fine = true;
+            for (int n = 0; n < total; ++n) {
+                if (fine) {
+                    fine = __all_sync(0xffffffffu, mbar_spin(acc_full + (n & 1), (n >> 1) & 1));
+                    if (!fine) { if (lane == 0) report(a.error, 4, n); failed = 1; }
+                }
+                fence_after_sync();
+                fence_before_sync();
+                wake<P::kAdders + 32>(2 + (n & 1));
+            }
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        if constexpr (kSwiglu) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
         const int group = (warp - 4) >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane;
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * 128;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * 64;
         const uint32_t release0 = peer_addr(smem_u32(acc_empty), 0);
         const int last_block = (a.N + kBK - 1) / kBK - 1;
-        int n = 0;
-        bool ok = true;
+        int n = 0;                                         // blocks so far
         // A block's scales are asked for two blocks ahead, into one of two sets of registers
         struct Scales { float x, w, u; };
         Scales even, odd;
-        const float *sx = nullptr, *sw = nullptr, *su = nullptr;
-        auto fetch = [&](Scales& f, int kb) {
-            kb = min(kb, kbn - 1);
-            f.x = sx[kb * a.sx_block];
-            f.w = sw[kb * a.sw_block];
-            f.u = kSwiglu ? su[kb * a.sw_block] : 0.f;
+        const float *sx = nullptr, *sw = nullptr, *su = nullptr;          // of the block that is asked for next
+        auto fetch = [&](Scales& f) {
+            f.x = *sx;
+            f.w = *sw;
+            sx += a.sx_block;
+            sw += a.sw_block;
+            if (kSwiglu) { f.u = *su; su += a.sw_block; }
         };
         auto open = [&](int t) {                           // the scales' places of a tile, and its first two blocks' on their way
             const Tile at = tile_at(t, tiles_m, tiles_n);
             sx = a.sx + (long)min(at.m * kPairRows + rank * 128 + in_tile, a.M - 1) * a.sx_row;
-            const int block = kSwiglu ? at.n : min(2 * at.n + group, last_block);
+            const int block = kSwiglu ? at.n : min((at.n * kFeat + group * 64) / kBK, last_block);
             sw = a.sw0 + block * a.sw_row;
             if (kSwiglu) su = a.sw1 + block * a.sw_row;
-            fetch(even, 0);
-            fetch(odd, 1);
+            fetch(even);
+            if (kbn > 1) fetch(odd);
         };
-        if (pair < tiles) open(pair);
-        for (int t = pair; t < tiles && ok; t += pairs) {
-            const Tile at = tile_at(t, tiles_m, tiles_n);
-            uint64_t sum2[64];
+        open(pair);
+        for (int t = pair; t < tiles; t += pairs) {
+            float sum[64];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) sum2[j] = 0;
-            // 32 columns at a time, the next 32 on their way meanwhile, also from one block to the next: the wait for a block's
-            // accumulator is asked for early and its first columns are fetched before the last ones of the block before are added
-            uint32_t d[2][32];
-            auto arrived = [&](int at, bool known) {       // this warp may read accumulator number `at`
-                bool yes = known || mbar_wait(acc_full + (at & 1), (at >> 1) & 1);
-                yes = __all_sync(0xffffffffu, yes && !failed);
-                if (!yes && lane == 0 && !failed) { report(a.error, 4, at); failed = 1; }
-                fence_after_sync();
-                return yes;
-            };
-            auto block = [&](int kb, Scales& f) {
+            for (int j = 0; j < 64; ++j) sum[j] = 0.f;
+            // one block: its accumulator, times its scales `f`, joins this thread's sums
+            auto block = [&](Scales& f, bool more) {
                 const float s = join(f.x, f.w), v = kSwiglu ? join(f.x, f.u) : s;
-                fetch(f, kb + 2);
-                const uint64_t low = pair_of(s, s), high = pair_of(v, v);
-                const uint32_t at = from + (n & 1) * 256;
-                bool ready = false;
+                if (more) fetch(f);
+                const uint32_t col = from + (n & 1) * 256, release = release0 + (n & 1) * 8;
+                sleep_until_woken<P::kAdders + 32>(2 + (n & 1));
+                fence_after_sync();
+                if constexpr (kSwiglu) {                   // registers for 32 columns at a time
+                    uint32_t d[32];
+                    tmem_ld32(col, d);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                    for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
+                    tmem_ld32(col + 32, d);
+                    fence_before_sync();
+                    mbar_arrive_at_if(release, lane == 0);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
+                } else {                                   // all 64 at once: the accumulator is free again at once
+                    uint32_t d[64];
+                    tmem_ld64(col, d);
                     tmem_ld_wait();
-                    if (c < 3) {
-                        tmem_ld32_async(at + 32 * (c + 1), d[(c + 1) & 1]);
-                        if (c == 1) ready = mbar_test(acc_full + ((n + 1) & 1), ((n + 1) >> 1) & 1);
-                    } else {
-                        fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_at(release0 + (n & 1) * 8);
-                        if (kb + 1 < kbn) {
-                            ok = arrived(n + 1, ready);
-                            if (ok) tmem_ld32_async(from + ((n + 1) & 1) * 256, d[0]);
-                        }
-                    }
+                    fence_before_sync();
+                    mbar_arrive_at_if(release, lane == 0);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fma2(sum2[16 * c + j], d[c & 1][2 * j], d[c & 1][2 * j + 1], c < 2 ? low : high);
+                    for (int j = 0; j < 64; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
                 }
                 ++n;
             };
-            ok = arrived(n, false);
-            if (ok) tmem_ld32_async(from + (n & 1) * 256, d[0]);
-            for (int kb = 0; kb < kbn && ok; kb += 2) {
-                block(kb, even);
-                if (ok && kb + 1 < kbn) block(kb + 1, odd);
+#pragma unroll 1
+            for (int kb = 0; kb < kbn; kb += 2) {
+                block(even, kb + 2 < kbn);
+                if (kb + 1 < kbn) block(odd, kb + 3 < kbn);
             }
-            if (!ok) break;
             if (t + pairs < tiles) open(t + pairs);
-            float sum[128];
-#pragma unroll
-            for (int j = 0; j < 64; ++j) { sum[2 * j] = low_of(sum2[j]); sum[2 * j + 1] = high_of(sum2[j]); }
+            const Tile at = tile_at(t, tiles_m, tiles_n);
             const long m = (long)at.m * kPairRows + rank * 128 + in_tile;
             if constexpr (kSwiglu) {
-                const int f0 = at.n * 128 + group * 64;    // this thread's features
+                const int f0 = at.n * 128 + group * 32;    // this thread's features
                 uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    sum[j] = f0 + j < a.N ? silu_f(sum[j] * a.act_scale) * sum[64 + j] : 0.f;
+                for (int j = 0; j < 32; ++j) {
+                    sum[j] = f0 + j < a.N ? silu_f(sum[j] * a.act_scale) * sum[32 + j] : 0.f;
                     top = max(top, magnitude(sum[j]));
                 }
                 tops[group][in_tile] = top;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                const float scale = fp8_scale(max(top, tops[group ^ 1][in_tile])), back = 1.f / scale;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+#pragma unroll
+                for (int g = 0; g < kPairGroups; ++g) top = max(top, tops[g][in_tile]);
+                const float scale = fp8_scale(top), back = 1.f / scale;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
                 if (m < a.M) {
                     uint8_t* q = a.q + m * a.ldq + f0;
 #pragma unroll
-                    for (int j = 0; j < 64; j += 16) {
+                    for (int j = 0; j < 32; j += 16) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -266,12 +300,12 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     if (group == 0) a.qs[m * a.qs_row + at.n * a.qs_block] = scale;
                 }
             } else if (m < a.M) {
-                const int n0 = at.n * 256 + group * 128;
+                const int n0 = at.n * kFeat + group * 64;
                 const int size = a.out_f32 ? 4 : 2;
                 uint8_t* out = (uint8_t*)a.out + ((size_t)m * a.ldo + n0) * size;
                 const bool whole = ((uintptr_t)out & 15) == 0;
 #pragma unroll
-                for (int j = 0; j < 128; j += 8) {
+                for (int j = 0; j < 64; j += 8) {
                     float o[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
