@@ -292,8 +292,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 }
             }
             if constexpr (kSwiglu) {
-                float h[4] = {silu_f(v.x * a.act_scale) * u.x, silu_f(v.y * a.act_scale) * u.y, silu_f(v.z * a.act_scale) * u.z,
-                              silu_f(v.w * a.act_scale) * u.w};
+                float h[4] = {silu_of(v.x * a.act_scale) * u.x, silu_of(v.y * a.act_scale) * u.y, silu_of(v.z * a.act_scale) * u.z,
+                              silu_of(v.w * a.act_scale) * u.w};
                 uint32_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { if (n + e >= a.N) h[e] = 0.f; top = max(top, magnitude(h[e])); }
@@ -378,20 +378,19 @@ enum : int { kAuto = 0, kRows = 1, kTiles = 2, kPair = 3 };
 
 template <bool kSwiglu>
 int launch_pair(const Operands& o, Args a, int sms, cudaStream_t s) {
-    typedef Pair<kSwiglu> P;
-    constexpr int feat = P::kFeat;
+    constexpr int feat = kSwiglu ? 128 : 256;
     const long tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + feat - 1) / feat);
     if (tiles > 0x3fffffffL) return kTooLarge;
     const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
     CUtensorMap map_w0, map_w1, map_x;
-    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 32 : P::kCols / 2);
+    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 32 : 128);
     if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, 32); else map_w1 = map_w0; }
     if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, 128);
     if (rc != 0) return rc;
     static size_t have = 0;
-    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu>, P::kSmem, have);
+    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu>, kPairSmem, have);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(P::kThreads); cfg.dynamicSmemBytes = P::kSmem; cfg.stream = s;
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = kPairSmem; cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -420,7 +419,7 @@ int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
                                                                                      : launch<true, 64, kSwiglu>(o, a, sms, s);
         if (rc != kTooLarge || form != kAuto) return rc;   // a K whose table of scales does not fit goes in tiles
     }
-    const long pair_tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + Pair<kSwiglu>::kFeat - 1) / Pair<kSwiglu>::kFeat);
+    const long pair_tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + (kSwiglu ? 127 : 255)) / (kSwiglu ? 128 : 256));
     if (form == kPair || (form == kAuto && pair_tiles >= sms / 4)) return launch_pair<kSwiglu>(o, a, sms, s);
     a.split = split ? split : default_split((a.M + 127) / 128 * tiles_n, blocks, sms, 1);
     return launch<false, 128, kSwiglu>(o, a, sms, s);

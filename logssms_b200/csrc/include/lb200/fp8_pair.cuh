@@ -6,6 +6,7 @@
 //   warp 0      one thread issues this CTA's TMA loads; their bytes are counted at the first CTA's barrier
 //   warp 1      first CTA: one thread issues the products for both, into one of two accumulators of 256 columns each; both
 //               CTAs: allocates tensor memory
+//   warps 2, 3  watch the barriers and wake the warps that add and the one that issues (first CTA)
 //   warps 4-11  two warpgroups: a thread is a row of its CTA's 128 and takes 128 columns of the accumulator: it reads a block's
 //               sums, multiplies them by the block's scales and adds them to its 128 sums, while the tensor cores work on the
 //               next block.  Warps 0-3 give up registers for that.
@@ -21,16 +22,11 @@ namespace lb200 {
 namespace fp8 {
 
 constexpr int kPairRows = 256;
-// Tiles of 192 features, for SwiGLU of 128 gate and 128 up features: a thread of `kGroups` warpgroups adds 64 columns
-template <bool kSwiglu>
-struct Pair {
-    static constexpr int kGroups = kSwiglu ? 4 : 3, kAdders = 128 * kGroups, kThreads = 128 + kAdders;
-    static constexpr int kCols = 64 * kGroups;            // accumulator columns of a block
-    static constexpr int kFeat = kSwiglu ? 128 : kCols;   // output features of a tile
-    static constexpr uint32_t kStage = (128 + kCols / 2) * kBK;        // a CTA's 128 rows of x and half of the features
-    static constexpr int kStages = kSwiglu ? 6 : 7;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage;
-};
+constexpr int kPairGroups = 4, kAdders = 128 * kPairGroups, kPairThreads = 128 + kAdders;
+constexpr int kAccs = 2, kAccCols = 64 * kPairGroups;     // accumulators in tensor memory, and their columns
+constexpr uint32_t kPairStage = (128 + kAccCols / 2) * kBK;            // a CTA's 128 rows of x and half of the features
+constexpr int kPairStages = 6;
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage;
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -62,22 +58,11 @@ __device__ __forceinline__ bool mbar_test_at(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 // barriers of the CTA among `kCount` threads: some only arrive, the others sleep until all have
+constexpr int kWakeAdders = 2;                             // one for each accumulator, up to four
 template <int kCount>
 __device__ __forceinline__ void wake(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
 template <int kCount>
 __device__ __forceinline__ void sleep_until_woken(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
-// 64 consecutive float32 columns of this thread's lane of tensor memory; complete after tmem_ld_wait()
-__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t (&r)[64]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), 
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), 
-                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), 
-                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-                 : "r"(addr));
-}
-
 // tile number -> place: bands of 8 tiles of rows, all features of a band before the next, the rows fastest, so that the pairs
 // at work at one time share their rows and their features in L2
 struct Tile { int m, n; };
@@ -89,15 +74,13 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
 }
 
 template <bool kSwiglu>
-__global__ void __launch_bounds__(Pair<kSwiglu>::kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                 const __grid_constant__ CUtensorMap map_x, Args a) {
-    typedef Pair<kSwiglu> P;
-    constexpr int kFeat = P::kFeat, kPairStages = P::kStages, kPairGroups = P::kGroups;
-    constexpr uint32_t kPairStage = P::kStage;
+    constexpr int kFeat = kSwiglu ? 128 : 256;            // output features of a tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(16) uint64_t acc_full[2], acc_empty[2], full[kPairStages], empty[kPairStages];
+    __shared__ __align__(16) uint64_t acc_full[kAccs], acc_empty[kAccs], full[kPairStages], empty[kPairStages];
     __shared__ uint32_t tops[kSwiglu ? kPairGroups : 1][128];       // SwiGLU: a row's largest magnitude among a group's features
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
@@ -108,7 +91,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     const int kbn = (a.K + kBK - 1) / kBK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * 4 * kPairGroups); }
+        for (int s = 0; s < kAccs; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * 4 * kPairGroups); }
         failed = 0;
         mbar_fence_init();
     }
@@ -125,10 +108,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     pdl_trigger();
     pdl_wait();
     int issued = 0;
+    const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;             // blocks of all tiles of this pair
     const uint32_t full0 = peer_addr(smem_u32(full), 0);
     if (warp < 4) {
-        if constexpr (kSwiglu) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");       // 640 threads x 96 registers
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");                         // 512 x 128
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");              // 640 threads x 96 registers at launch: 128 x 32 + 512 x 112
         // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait
         // takes some 200 cycles even when the phase is long over)
         if (warp == 0) {
@@ -136,7 +119,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             bool ready = true, going = true;
             for (int t = pair; t < tiles && going; t += pairs) {
                 const Tile at = tile_at(t, tiles_m, tiles_n);
-                const int row = at.m * kPairRows + rank * 128, feat = at.n * kFeat;
+                const int row = at.m * kPairRows + rank * 128;
+                const int feat = at.n * kFeat + rank * (kFeat / 2);
                 for (int kb = 0; kb < kbn; ++kb, ++issued) {
                     if (!ready) ready = mbar_spin(empty + s, parity);
                     if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, kb); failed = 1; going = false; break; }
@@ -151,65 +135,66 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                         if (kSwiglu) {                     // gate and up of two groups' 32 features each
 #pragma unroll
                             for (int g = 0; g < 2; ++g) {
-                                tma_load_2d_pair(w + 64 * g * kBK, &map_w0, bar, kb * kBK, feat + rank * 64 + 32 * g);
-                                tma_load_2d_pair(w + (64 * g + 32) * kBK, &map_w1, bar, kb * kBK, feat + rank * 64 + 32 * g);
+                                tma_load_2d_pair(w + 64 * g * kBK, &map_w0, bar, kb * kBK, feat + 32 * g);
+                                tma_load_2d_pair(w + (64 * g + 32) * kBK, &map_w1, bar, kb * kBK, feat + 32 * g);
                             }
                         } else {
-                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat + rank * (P::kCols / 2));
+                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat);
                         }
                     }
                     s = s1; parity = parity1;
                 }
             }
-        } else if (warp == 1 && rank == 0) {
-            constexpr uint32_t idesc = f8_idesc(256, P::kCols);
+        } else if (warp != 2 && rank == 0) {
+            // Two warps issue the products, block by block in turn: what a warp has to do for a block besides (two barriers, a fence,
+            // descriptors, the commit) takes it some 400 cycles, longer than the block's products run.
+            constexpr uint32_t idesc = f8_idesc(256, kAccCols);
             const uint64_t desc0 = umma_desc(base);
-            const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;      // blocks of all tiles of this pair
-            int s = 0, parity = 0;
-            bool ready = false, room = true;
-            for (int n = 0; n < total; ++n) {
+#pragma unroll 1
+            for (int n = warp >> 1, s = n, parity = 0, room = 1; n < total; n += 2) {
                 const int acc = n & 1;
-                if (!ready) ready = mbar_spin(full + s, parity);
-                if (!room) room = mbar_spin(acc_empty + acc, ((n >> 1) - 1) & 1);
-                if (!__all_sync(0xffffffffu, ready && room)) { if (lane == 0) report(a.error, ready ? 3 : 2, n); failed = 1; break; }
+                bool fine = mbar_spin(full + s, parity);
+                if (n >= kAccs) fine = mbar_spin(acc_empty + acc, room) && fine;
+                if (!__all_sync(0xffffffffu, fine)) { if (lane == 0) report(a.error, 2, n); failed = 1; break; }
+                const uint64_t xdesc = desc0 + (uint64_t)(s * (kPairStage >> 4)), wdesc = xdesc + (128 * kBK >> 4);
+                const uint32_t d = tmem + acc * kAccCols;
                 fence_after_sync();
-                const int s1 = s + 1 == kPairStages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
                 if (elect_one()) {
-                    const uint64_t xdesc = desc0 + (uint64_t)(s * (kPairStage >> 4)), wdesc = xdesc + (128 * kBK >> 4);
 #pragma unroll
-                    for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(tmem + acc * 256, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
-                    umma_commit_pair(empty + s);
+                    for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(d, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
                     umma_commit_pair(acc_full + acc);
                 }
                 __syncwarp();
-                ready = n + 1 < total && mbar_test(full + s1, parity1);
-                room = n == 0 || (n + 1 < total && mbar_test(acc_empty + (acc ^ 1), (((n + 1) >> 1) - 1) & 1));
-                s = s1; parity = parity1;
+                room ^= 1;
+                s += 2;
+                if (s >= kPairStages) { s -= kPairStages; parity ^= 1; }
             }
         } else if (warp == 2) {
-            // One warp per CTA watches the accumulators and wakes the warps that add, by a barrier that costs them nothing while they
-            // wait: a dozen warps that ask the same mbarrier make each answer, also the one to the warp that issues the products,
-            // some 300 cycles late.  After a wait that gave up it goes on without waiting: everybody else's loops end by count.
-            const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;
+            // Watches the accumulators: hands the block's stage back to the producer of its CTA and wakes the warps that add, by a
+            // barrier that costs them nothing while they wait: a dozen warps that ask the same mbarrier make each answer, also the one
+            // to the warp that issues the products, some 300 cycles late.  (It is never more than
+            // the accumulators ahead of them.)  After a wait that gave up it meets them at that barrier instead, block by block, until
+            // their loops have ended by count.
             bool fine = true;
-            for (int n = 0; n < total; ++n) {
+            for (int n = 0, s = 0, acc = 0, parity = 0; n < total; ++n) {
                 if (fine) {
-                    fine = __all_sync(0xffffffffu, mbar_spin(acc_full + (n & 1), (n >> 1) & 1));
+                    fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, parity));
                     if (!fine) { if (lane == 0) report(a.error, 4, n); failed = 1; }
                 }
                 fence_after_sync();
                 fence_before_sync();
-                wake<P::kAdders + 32>(2 + (n & 1));
+                if (fine) wake<kAdders + 32>(kWakeAdders + acc); else sleep_until_woken<kAdders + 32>(kWakeAdders + acc);
+                if (lane == 0) mbar_arrive(empty + s);
+                s = s + 1 == kPairStages ? 0 : s + 1;
+                if (++acc == kAccs) { acc = 0; parity ^= 1; }
             }
         }
         __syncwarp();
     } else {
-        if constexpr (kSwiglu) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         const int group = (warp - 4) >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane;
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * 64;
         const uint32_t release0 = peer_addr(smem_u32(acc_empty), 0);
-        const int last_block = (a.N + kBK - 1) / kBK - 1;
         int n = 0;                                         // blocks so far
         // A block's scales are asked for two blocks ahead, into one of two sets of registers
         struct Scales { float x, w, u; };
@@ -225,9 +210,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
         auto open = [&](int t) {                           // the scales' places of a tile, and its first two blocks' on their way
             const Tile at = tile_at(t, tiles_m, tiles_n);
             sx = a.sx + (long)min(at.m * kPairRows + rank * 128 + in_tile, a.M - 1) * a.sx_row;
-            const int block = kSwiglu ? at.n : min((at.n * kFeat + group * 64) / kBK, last_block);
-            sw = a.sw0 + block * a.sw_row;
-            if (kSwiglu) su = a.sw1 + block * a.sw_row;
+            sw = a.sw0 + (kSwiglu ? at.n : min(2 * at.n + (group >> 1), (a.N - 1) / kBK)) * a.sw_row;
+            if (kSwiglu) su = a.sw1 + at.n * a.sw_row;
             fetch(even);
             if (kbn > 1) fetch(odd);
         };
@@ -236,32 +220,22 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             float sum[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) sum[j] = 0.f;
-            // one block: its accumulator, times its scales `f`, joins this thread's sums
+            // a block's accumulator, times its scales, joins this thread's sums, 32 columns at a time
             auto block = [&](Scales& f, bool more) {
                 const float s = join(f.x, f.w), v = kSwiglu ? join(f.x, f.u) : s;
                 if (more) fetch(f);
-                const uint32_t col = from + (n & 1) * 256, release = release0 + (n & 1) * 8;
-                sleep_until_woken<P::kAdders + 32>(2 + (n & 1));
+                const uint32_t col = from + (n & 1) * kAccCols;
+                uint32_t d[32];
+                sleep_until_woken<kAdders + 32>(kWakeAdders + (n & 1));
                 fence_after_sync();
-                if constexpr (kSwiglu) {                   // registers for 32 columns at a time
-                    uint32_t d[32];
-                    tmem_ld32(col, d);
+                tmem_ld32(col, d);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
-                    tmem_ld32(col + 32, d);
-                    fence_before_sync();
-                    mbar_arrive_at_if(release, lane == 0);
+                for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
+                tmem_ld32(col + 32, d);
+                fence_before_sync();
+                mbar_arrive_at_if(release0 + (n & 1) * 8, lane == 0);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
-                } else {                                   // all 64 at once: the accumulator is free again at once
-                    uint32_t d[64];
-                    tmem_ld64(col, d);
-                    tmem_ld_wait();
-                    fence_before_sync();
-                    mbar_arrive_at_if(release, lane == 0);
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
-                }
+                for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
                 ++n;
             };
 #pragma unroll 1
@@ -273,11 +247,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             const Tile at = tile_at(t, tiles_m, tiles_n);
             const long m = (long)at.m * kPairRows + rank * 128 + in_tile;
             if constexpr (kSwiglu) {
-                const int f0 = at.n * 128 + group * 32;    // this thread's features
+                const int f0 = at.n * kFeat + group * 32;  // this thread's features
                 uint32_t top = 0;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    sum[j] = f0 + j < a.N ? silu_f(sum[j] * a.act_scale) * sum[32 + j] : 0.f;
+                    sum[j] = f0 + j < a.N ? silu_of(sum[j] * a.act_scale) * sum[32 + j] : 0.f;
                     top = max(top, magnitude(sum[j]));
                 }
                 tops[group][in_tile] = top;
@@ -292,45 +266,42 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     for (int j = 0; j < 32; j += 16) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = fp8_quad(sum[j + 4 * e] * back, sum[j + 4 * e + 1] * back, sum[j + 4 * e + 2] * back, sum[j + 4 * e + 3] * back);
+                        for (int e = 0; e < 4; ++e) w[e] = fp8_quad(sum[j + 4 * e] * back, sum[j + 4 * e + 1] * back, sum[j + 4 * e + 2] * back, sum[j + 4 * e + 3] * back);
                         // rows are filled up to 16 bytes
                         if (f0 + j < a.N) *reinterpret_cast<uint4*>(q + j) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     if (group == 0) a.qs[m * a.qs_row + at.n * a.qs_block] = scale;
                 }
             } else if (m < a.M) {
-                const int n0 = at.n * kFeat + group * 64;
-                const int size = a.out_f32 ? 4 : 2;
-                uint8_t* out = (uint8_t*)a.out + ((size_t)m * a.ldo + n0) * size;
-                const bool whole = ((uintptr_t)out & 15) == 0;
+                const int n0 = at.n * kFeat + group * 64, live = a.N - n0;
+                if (a.bias != nullptr) {
 #pragma unroll
-                for (int j = 0; j < 64; j += 8) {
-                    float o[8];
+                    for (int j = 0; j < 64; ++j) if (j < live) sum[j] += a.bias[n0 + j];
+                }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float b = a.bias != nullptr && n0 + j + e < a.N ? a.bias[n0 + j + e] : 0.f;
-                        o[e] = (sum[j + e] + b) * a.out_scale;
-                    }
-                    if (whole && n0 + j + 8 <= a.N) {
-                        if (a.out_f32) {
-                            reinterpret_cast<float4*>(out + 4 * j)[0] = make_float4(o[0], o[1], o[2], o[3]);
-                            reinterpret_cast<float4*>(out + 4 * j)[1] = make_float4(o[4], o[5], o[6], o[7]);
-                        } else {
-                            uint4 w;
-                            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+                for (int j = 0; j < 64; ++j) sum[j] *= a.out_scale;
+                uint8_t* out = (uint8_t*)a.out + ((size_t)m * a.ldo + n0) * (a.out_f32 ? 4 : 2);
+                if (live >= 64 && ((uintptr_t)out & 15) == 0) {
+                    if (a.out_f32) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(o[2 * e], o[2 * e + 1]);
-                            *reinterpret_cast<uint4*>(out + 2 * j) = w;
-                        }
+                        for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(out + 4 * j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (n0 + j + e < a.N) {
-                                if (a.out_f32) reinterpret_cast<float*>(out)[j + e] = o[e];
-                                else reinterpret_cast<__nv_bfloat16*>(out)[j + e] = __float2bfloat16_rn(o[e]);
-                            }
+                        for (int j = 0; j < 64; j += 8) {
+                            uint4 w;
+                            __nv_bfloat162* b = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) b[e] = __floats2bfloat162_rn(sum[j + 2 * e], sum[j + 2 * e + 1]);
+                            *reinterpret_cast<uint4*>(out + 2 * j) = w;
+                        }
                     }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (j < live) {
+                            if (a.out_f32) reinterpret_cast<float*>(out)[j] = sum[j];
+                            else reinterpret_cast<__nv_bfloat16*>(out)[j] = __float2bfloat16_rn(sum[j]);
+                        }
                 }
             }
         }
