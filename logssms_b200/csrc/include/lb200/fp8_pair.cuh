@@ -63,6 +63,11 @@ template <int kCount>
 __device__ __forceinline__ void wake(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
 template <int kCount>
 __device__ __forceinline__ void sleep_until_woken(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kCount) : "memory"); }
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 // tile number -> place: bands of 8 tiles of rows, all features of a band before the next, the rows fastest, so that the pairs
 // at work at one time share their rows and their features in L2
 struct Tile { int m, n; };
@@ -281,18 +286,24 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 64; ++j) sum[j] *= a.out_scale;
                 uint8_t* out = (uint8_t*)a.out + ((size_t)m * a.ldo + n0) * (a.out_f32 ? 4 : 2);
-                if (live >= 64 && ((uintptr_t)out & 15) == 0) {
+                if (live >= 64 && ((uintptr_t)out & 31) == 0) {
+                    // whole sectors of 32 bytes: a lane is a row, and every store of a warp touches 32 lines
                     if (a.out_f32) {
 #pragma unroll
-                        for (int j = 0; j < 64; j += 4) *reinterpret_cast<float4*>(out + 4 * j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+                        for (int j = 0; j < 64; j += 8) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(sum[j + e]);
+                            store32(out + 4 * j, w);
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 64; j += 8) {
-                            uint4 w;
-                            __nv_bfloat162* b = reinterpret_cast<__nv_bfloat162*>(&w);
+                        for (int j = 0; j < 64; j += 16) {
+                            uint32_t w[8];
+                            __nv_bfloat162* b = reinterpret_cast<__nv_bfloat162*>(w);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) b[e] = __floats2bfloat162_rn(sum[j + 2 * e], sum[j + 2 * e + 1]);
-                            *reinterpret_cast<uint4*>(out + 2 * j) = w;
+                            for (int e = 0; e < 8; ++e) b[e] = __floats2bfloat162_rn(sum[j + 2 * e], sum[j + 2 * e + 1]);
+                            store32(out + 2 * j, w);
                         }
                     }
                 } else {

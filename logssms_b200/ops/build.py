@@ -34,6 +34,11 @@ NVCC_FLAGS = [
 ]
 
 
+def package_bindings() -> tuple[str, ...]:
+    """Names of the package's host sources: Python modules that call the kernels' launchers."""
+    return tuple(sorted(f[:-4] for f in os.listdir(CSRC) if f.endswith(".cpp")))
+
+
 def package_libraries() -> tuple[str, ...]:
     """Names of all kernel sources of the package itself."""
     return tuple(sorted(f[:-3] for f in os.listdir(CSRC) if f.endswith(".cu")))
@@ -51,8 +56,10 @@ def all_libraries() -> tuple[str, ...]:
 
 
 def source_path(name: str) -> str:
-    """The `.cu` file behind a library name: `name` itself if it is a path, else `csrc/<name>.cu`."""
+    """The file behind a library name: `name` itself if it is a path, else `csrc/<name>.cu`, or `csrc/<name>.cpp` of a binding."""
     src = name if (os.sep in name or name.endswith(".cu")) else os.path.join(CSRC, f"{name}.cu")
+    if not os.path.isfile(src) and os.path.isfile(src[:-3] + ".cpp"):
+        src = src[:-3] + ".cpp"
     if not os.path.isfile(src):
         raise KernelBuildError(f"kernel source {src} is missing")
     return os.path.abspath(src)
@@ -112,10 +119,24 @@ def _find_build_dir() -> str:
     raise KernelBuildError(f"no writable folder for built kernels among {candidates}")
 
 
+def _host_command(compiler: str, src: str, out: str) -> list[str]:
+    """How a binding is compiled: against the headers and libraries of the torch that runs (named by its version, so that
+    another torch gets a build of its own)."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    return [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", f"-DLB200_TORCH=\"{torch.__version__}\"",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(root, "include"),
+            "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
+            "-I", sysconfig.get_paths()["include"], "-o", out, src, "-L", os.path.join(root, "lib"),
+            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+
+
 def _digest(name: str) -> str:
     h = hashlib.sha1()
-    h.update(" ".join(NVCC_FLAGS).encode())
     src = source_path(name)
+    h.update(" ".join(_host_command("", src, "")[1:] if src.endswith(".cpp") else NVCC_FLAGS).encode())
     paths = [src]
     for root, _, files in sorted(os.walk(INCLUDE)):
         paths += [os.path.join(root, f) for f in sorted(files)]
@@ -137,10 +158,17 @@ def build(name: str, verbose: bool = True) -> str:
     if os.path.isfile(out):
         return out
     tmp = f"{out}.{os.getpid()}.{threading.get_ident()}.tmp"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", os.path.dirname(src), "-o", tmp, src]
-    name = _stem(name)
+    host = src.endswith(".cpp")
+    if host:
+        compiler = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+        if compiler is None:
+            raise KernelBuildError("no C++ compiler found (looked at $CXX, g++ and c++)")
+        cmd = _host_command(compiler, src, tmp)
+    else:
+        cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", os.path.dirname(src), "-o", tmp, src]
+    name, file = _stem(name), os.path.basename(src)
     if verbose:
-        _log(f"compiling {name}.cu for sm_100a ...")
+        _log(f"compiling {file}{'' if host else ' for sm_100a'} ...")
     start = time.time()
     proc = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True,
                             env={**os.environ, "TMPDIR": os.path.dirname(out)})
@@ -150,11 +178,11 @@ def build(name: str, verbose: bool = True) -> str:
             break
         except subprocess.TimeoutExpired:
             if verbose:
-                _log(f"  still compiling {name}.cu ({time.time() - start:.0f} s)")
+                _log(f"  still compiling {file} ({time.time() - start:.0f} s)")
     if proc.returncode != 0:
         if os.path.exists(tmp):
             os.remove(tmp)
-        raise KernelBuildError(f"nvcc failed on {name}.cu:\n{output}")
+        raise KernelBuildError(f"{'the C++ compiler' if host else 'nvcc'} failed on {file}:\n{output}")
     os.replace(tmp, out)
     # builds of earlier versions of this source are of no use any more
     prefix = f"lb200_{name}-"
@@ -190,3 +218,24 @@ def load(name: str) -> ctypes.CDLL:
             lib = ctypes.CDLL(build(name))
             _loaded[name] = lib
     return lib
+
+
+_bound: dict[str, object] = {}
+
+
+def load_binding(name: str):
+    """The Python module of a host source `csrc/<name>.cpp`, building it first if needed."""
+    module = _bound.get(name)
+    if module is not None:
+        return module
+    with _lock:
+        module = _bound.get(name)
+        if module is None:
+            import importlib.util
+            from importlib.machinery import ExtensionFileLoader
+            import torch  # noqa: F401  (its libraries have to be there first)
+            loader = ExtensionFileLoader(name, build(name))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+            loader.exec_module(module)
+            _bound[name] = module
+    return module

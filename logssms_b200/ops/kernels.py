@@ -2631,6 +2631,33 @@ FP8_FORM = "auto"
 _FP8_FORMS = {"auto": 0, "rows": 1, "tiles": 2, "pair": 3}
 
 
+_fp8_binding = None
+
+
+def _fp8_calls():
+    """The binding that takes a call that is plainly in order straight to its launcher (`csrc/fp8_calls.cpp`): checks, outputs and
+    launch in 5 us where the functions below take 15.  It answers None where anything is out of the ordinary, and they take over."""
+    global _fp8_binding
+    if _fp8_binding is None:
+        binding = build.load_binding("fp8_calls")
+        at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
+        binding.launchers(at("fp8_rows", "lb_add_rmsnorm_fp8"), at("fp8_rows", "lb_quantize_fp8"),
+                          at("fp8_linear", "lb_linear_fp8"), at("fp8_linear", "lb_linear_swiglu_fp8"))
+        for index in range(torch.cuda.device_count()):
+            binding.error_word(index, error_word(torch.device("cuda", index)).data_ptr())
+        _fp8_binding = binding
+    return _fp8_binding
+
+
+def _fp8_done(got, name: str):
+    """What the binding answered: counts a launch, or raises what the launcher said."""
+    global launch_count
+    if type(got) is int:
+        _check(got, name)
+    launch_count += 1
+    return got
+
+
 def _fp8_empty(rows: int, width: int, scale_rows: int, device, side_by_side: bool):
     """(values, scales) to be written: rows at multiples of 16 bytes, the scales of a column block side by side or row by row."""
     pitch = (width + 15) & -16
@@ -2668,6 +2695,12 @@ def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual:
     x's dtype, and the rows are r * rsqrt(mean(r^2) + eps) * weight * out_scale in 8 bits, a scale per 128 columns.  All of it is
     32-bit up to the two roundings.  The new residual is written in place of `residual` when one is given, unless `in_place` is
     off (then into a new tensor); None without `want_residual`.  Row strides are free."""
+    if not PROFILER.enabled:
+        got = (_fp8_binding or _fp8_calls()).norm(x, weight, eps, residual, other, in_scales[0], in_scales[1], out_scale,
+                                                  want_residual, in_place)
+        if got is not None:
+            values, scales, new = _fp8_done(got, "add_rmsnorm_fp8")
+            return Fp8Rows(values, scales), new
     _cuda(x, weight, residual, other)
     ldx = _rows_of(x, "x")
     rows, width = x.shape
@@ -2695,6 +2728,10 @@ def add_rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual:
 
 
 def _quantize(x: torch.Tensor, block_rows: int):
+    if not PROFILER.enabled:
+        got = (_fp8_binding or _fp8_calls()).quantize(x, block_rows)
+        if got is not None:
+            return _fp8_done(got, "quantize_rows_fp8" if block_rows == 1 else "quantize_weight_fp8")
     _cuda(x)
     ldx = _rows_of(x, "x")
     rows, width = x.shape
@@ -2723,6 +2760,11 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, ou
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """(x [M, K] @ w[N, K]^T + bias) * out_scale of 8-bit operands: 32-bit sums, rounded once, to `out_dtype` (bfloat16 or
     float32).  `bias`: float32 [N].  `check_kernel_errors()` reports a kernel whose internal wait gave up."""
+    if not PROFILER.enabled and type(x) is Fp8Rows and type(w) is Fp8Weight and out_dtype in _DTYPE_CODE:
+        got = (_fp8_binding or _fp8_calls()).linear(x.values, x.scales, w.values, w.scales, bias, out_scale,
+                                                    out_dtype is torch.float32, w.settled, _FP8_FORMS[FP8_FORM])
+        if got is not None:
+            return _fp8_done(got, "linear_fp8")
     ldx = _fp8_operand(x, "x", Fp8Rows, 1)
     device = x.values.device
     ldw = _fp8_operand(w, "w", Fp8Weight, 128, device)
@@ -2747,6 +2789,11 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, ou
 def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: float = 1.0) -> Fp8Rows:
     """silu((x @ gate^T) * act_scale) * (x @ up^T) of 8-bit operands, in 32 bits up to the result, which is 8-bit rows again (a
     scale for each row and 128 features): one kernel.  `check_kernel_errors()` reports one whose internal wait gave up."""
+    if not PROFILER.enabled and type(x) is Fp8Rows and type(gate) is Fp8Weight and type(up) is Fp8Weight:
+        got = (_fp8_binding or _fp8_calls()).swiglu(x.values, x.scales, gate.values, gate.scales, up.values, up.scales, act_scale,
+                                                    gate.settled and up.settled, _FP8_FORMS[FP8_FORM])
+        if got is not None:
+            return Fp8Rows(*_fp8_done(got, "linear_swiglu_fp8"))
     ldx = _fp8_operand(x, "x", Fp8Rows, 1)
     device = x.values.device
     ldg, ldu = _fp8_operand(gate, "gate", Fp8Weight, 128, device), _fp8_operand(up, "up", Fp8Weight, 128, device)
