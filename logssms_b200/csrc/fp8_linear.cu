@@ -11,7 +11,8 @@
 //
 //   warp 0    one thread issues the TMA loads (128-byte swizzle, zeros outside the matrices) into a ring of stages: a block
 //             of 128 columns of 128 features of W (swiglu: of 128 gate and 128 up features) and of the tile's rows of x
-//   warp 1    allocates tensor memory; one thread issues tcgen05.mma (kind::f8f6f4, K 32: four per block)
+//   warps 1, 10  issue tcgen05.mma (one thread; kind::f8f6f4, K 32: four per block), block by block in turn, since what a warp has
+//             to do for a block besides takes some 400 cycles; warp 1 allocates tensor memory
 //   warps 2-9 two warpgroups: read a block's accumulator, multiply and add; for swiglu one holds the gate, one the up
 //             features, otherwise each half of the columns
 // Two ways round:
@@ -21,7 +22,7 @@
 // K split: where there are few tiles, up to 8 CTAs of a cluster take a range of blocks each and the sums meet in distributed
 // shared memory: each CTA owns an equal share of the tile's rows, gets every CTA's sums for them by remote stores, and adds
 // them in rank order, so that the result does not depend on timing.  There a warp takes a row, a lane 4 neighbouring features:
-// stores are whole, and the largest magnitude of a row's 128 features takes one reduction.
+// stores are whole, and the largest magnitude of a row's 128 features takes one reduction (few rows without SwiGLU: a thread takes a feature and four rows).
 //
 // Every wait on an mbarrier is bounded; one that gives up records itself in `error`, all roles run out of their own bounded
 // waits, every thread still meets the cluster barriers, tensor memory is freed and the kernel returns.
@@ -34,7 +35,7 @@ namespace {
 constexpr int kFeat = 128;
 constexpr uint32_t kWBytes = kFeat * kBK;
 constexpr int kSumThreads = 256;                          // warps 2-9
-constexpr int kThreads = 64 + kSumThreads;
+constexpr int kThreads = 96 + kSumThreads;
 constexpr int kMaxStages = 8, kMaxSplit = 8;
 
 // kSwap: NR rows on the N side; else 128 rows on the M side (NR = 128).
@@ -44,12 +45,15 @@ struct Form {
     static constexpr uint32_t kXBytes = kXRows * kBK;
     static constexpr uint32_t kStage = (kSwiglu ? 2 : 1) * kWBytes + kXBytes;
     static constexpr int kCols = kSwap ? (kSwiglu ? 2 * NR : NR) : (kSwiglu ? 256 : 128);   // accumulator columns of a block
-    static constexpr int kAccs = kSwap && kCols <= 64 ? 4 : 2;                 // accumulators in tensor memory
+    static constexpr bool kTwoPerSm = kSwap && NR <= 32;   // CTAs on an SM: where 80 registers hold sums, columns and scales
+    static constexpr int kAccs = kCols <= (kTwoPerSm ? 64 : 128) ? 4 : 2;      // accumulators in tensor memory
     static constexpr uint32_t kTmem = kCols * kAccs < 32 ? 32 : kCols * kAccs;
     static constexpr int kOutCols = kSwiglu ? 256 : 128;                       // features of a tile, gate and up counted
-    static constexpr int kPitch = kOutCols + 4;                                // floats of a row of sums: rows start in different banks
+    static constexpr bool kQuads = kSwap && !kSwiglu;                          // the sums of four rows and a feature lie together
+    static constexpr int kPitch = kOutCols + (kQuads ? 0 : 4);                 // floats of a row of sums (else rows start in different banks)
+    static constexpr int kShareOf = kQuads ? 4 : 1;                            // a CTA owns a multiple of so many rows
     static constexpr int kMine = kSwap ? (kSwiglu ? NR : NR / 2) : (kSwiglu ? 128 : 64);   // sums of a thread
-    static constexpr bool kTwoPerSm = kSwap && kMine <= 64;
+    static constexpr bool kOver = !kSwap || (NR == 64 && kSwiglu);             // the sums land over the ring
 };
 
 template <bool kSwap, int NR, bool kSwiglu>
@@ -71,11 +75,13 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     const int blocks = (a.K + kBK - 1) / kBK;
     const int kb0 = (int)((long)blocks * rank / split), kbn = (int)((long)blocks * (rank + 1) / split) - kb0;
     const int stages = a.stages, first = min(stages, kbn);
-    const int share = (rows + split - 1) / split;          // rows of the tile that a CTA of the cluster owns
-    // The sums land here: [source CTA][row of the share][feature].  Few rows: behind the ring, with the table of scales (a
-    // peer may be done while this CTA still loads); tiles: over the ring, once the whole cluster has left it.
-    float* recv = reinterpret_cast<float*>(kSwap ? base + (size_t)stages * kStage : base);
-    float* table = recv + (size_t)(NR + split) * F::kPitch;           // kSwap: [block][gate, up][row]
+    const int share = ((rows + split - 1) / split + F::kShareOf - 1) / F::kShareOf * F::kShareOf;      // rows that a CTA of the cluster owns
+    // The sums land here: [source CTA][row of the share][feature] (kQuads: [source CTA][four rows][feature][row]).  Few sums: behind
+    // the ring (a peer may be done while this CTA still loads); many: over it, once the whole cluster has left it.  Few rows: then the
+    // scales, [block][gate, up][row].
+    float* recv = reinterpret_cast<float*>(F::kOver ? base : base + (size_t)stages * kStage);
+    float* table = reinterpret_cast<float*>(base + (size_t)stages * kStage) + (F::kOver ? 0 : (size_t)split * share * F::kPitch);
+    const uint32_t table_at = smem_u32(table);
     auto load_w = [&](int s, int i) {
         uint8_t* w = base + (size_t)s * kStage;
         mbar_expect_tx(full + s, kStage);
@@ -103,9 +109,9 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     pdl_wait();
 
     int issued = 0;
-    uint64_t sum2[kMine / 2];                              // pairs of sums
+    float sum[kMine];
 #pragma unroll
-    for (int j = 0; j < kMine / 2; ++j) sum2[j] = 0;
+    for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
     const int group = (warp - 2) >> 2, quarter = warp & 3;             // warpgroup; the lanes of tensor memory a warp may read
     // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait takes
     // some 200 cycles even when the phase is long over)
@@ -116,7 +122,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         int s = 0, parity = 0;
         bool ready = false;
         for (; issued < kbn; ++issued) {
-            if (!ready) ready = mbar_wait(empty + s, parity);
+            if (!ready) ready = mbar_spin(empty + s, parity);
             if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, issued); failed = 1; break; }
             const int s1 = s + 1 == stages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
             ready = mbar_test(empty + s1, parity1);
@@ -126,22 +132,22 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
             }
             s = s1; parity = parity1;
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 10) {
         constexpr uint32_t idesc = kSwap ? f8_idesc(128, NR) : f8_idesc(128, F::kCols);
         constexpr uint32_t kXAt = ((kSwiglu ? 2 : 1) * kWBytes) >> 4;
         const uint64_t desc0 = umma_desc(base);
-        int s = 0, parity = 0;
-        bool ready = false, room = true;
-        for (int i = 0; i < kbn; ++i) {
+        int s = warp == 1 ? 0 : 1, parity = 0;             // (see `launch` on the number of stages)
+#pragma unroll 1
+        for (int i = s; i < kbn; i += 2, s += 2) {
+            while (s >= stages) { s -= stages; parity ^= 1; }
             const int acc = i % kAccs;
-            if (!ready) ready = mbar_wait(full + s, parity);
-            if (!room) room = mbar_wait(acc_empty + acc, (i / kAccs - 1) & 1);
-            if (!__all_sync(0xffffffffu, ready && room)) { if (lane == 0) report(a.error, ready ? 3 : 2, i); failed = 1; break; }
+            bool fine = mbar_spin(full + s, parity);
+            if (i >= kAccs) fine = mbar_spin(acc_empty + acc, (i / kAccs - 1) & 1) && fine;
+            if (!__all_sync(0xffffffffu, fine)) { if (lane == 0) report(a.error, 2, i); failed = 1; break; }
+            const uint64_t wdesc = desc0 + (uint64_t)(s * (kStage >> 4)), xdesc = wdesc + kXAt;
+            const uint32_t d = tmem + acc * F::kCols;
             fence_after_sync();
-            const int s1 = s + 1 == stages ? 0 : s + 1, parity1 = s1 == 0 ? parity ^ 1 : parity;
             if (elect_one()) {
-                const uint64_t wdesc = desc0 + (uint64_t)(s * (kStage >> 4)), xdesc = wdesc + kXAt;
-                const uint32_t d = tmem + acc * F::kCols;
 #pragma unroll
                 for (int k = 0; k < kBK / 32; ++k) {       // 32 bytes along K: + 2 in the 16-byte address field
                     if (kSwap) {
@@ -151,13 +157,9 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                         umma_f8(d, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
                     }
                 }
-                umma_commit(empty + s);
                 umma_commit(acc_full + acc);
             }
             __syncwarp();
-            ready = i + 1 < kbn && mbar_test(full + s1, parity1);
-            room = i + 1 < kAccs || (i + 1 < kbn && mbar_test(acc_empty + (i + 1) % kAccs, ((i + 1) / kAccs - 1) & 1));
-            s = s1; parity = parity1;
         }
     } else {
         const int t = threadIdx.x - 64;
@@ -183,54 +185,58 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         } else if (kbn > 0) {
             s_next = join(sx[0], sw[0]);
         }
-        bool ok = true;
+        bool fine = true;
+        int slot = 0;
         for (int i = 0; i < kbn; ++i) {
             const int acc = i % kAccs;
-            const uint64_t both = pair_of(s_next, s_next);
+            const float s = s_next;
             if (!kSwap && i + 1 < kbn) s_next = join(sx[(i + 1) * a.sx_block], sw[(i + 1) * a.sw_block]);
-            ok = mbar_wait(acc_full + acc, (i / kAccs) & 1);
-            ok = __all_sync(0xffffffffu, ok && !failed);
-            if (!ok) { if (lane == 0 && !failed) { report(a.error, 4, i); failed = 1; } break; }
+            // one warp asks for the accumulator, the others sleep at the barrier: eight warps that ask make every answer late
+            if (warp == 2 && fine) {
+                fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, (i / kAccs) & 1));
+                if (!fine) { if (lane == 0) report(a.error, 4, i); failed = 1; }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (threadIdx.x == 64) mbar_arrive(empty + slot);             // the block's products have read its stage
+            slot = slot + 1 == stages ? 0 : slot + 1;
             fence_after_sync();
             const uint32_t at = from + acc * F::kCols;
-            const float* tab = table + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine);
-            if constexpr (kMine < 16) {
-                uint32_t d[8];
-                tmem_ld8(at, d);
-                tmem_ld_wait();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + acc);
+            if constexpr (!kSwap) {
+                constexpr int kStep = kMine > 64 ? 16 : 32;        // what the registers hold beside the sums
 #pragma unroll
-                for (int j = 0; j < 8; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(tab + j);
-                    fma2(sum2[j / 2], d[j], d[j + 1], pair_of(f.x, f.y));
-                    fma2(sum2[j / 2 + 1], d[j + 2], d[j + 3], pair_of(f.z, f.w));
-                }
-            } else {
-                // 16 columns at a time, the next 16 on their way meanwhile
-                uint32_t d[2][16];
-                tmem_ld16(at, d[0]);
-#pragma unroll
-                for (int c = 0; c < kMine; c += 16) {
-                    uint32_t* now = d[(c / 16) & 1];
-                    tmem_ld_wait();
-                    if (c + 16 < kMine) tmem_ld16(at + c + 16, d[(c / 16 + 1) & 1]);
-                    else {
+                for (int c = 0; c < kMine; c += kStep) {
+                    uint32_t d[kStep];
+                    if constexpr (kStep == 32) tmem_ld32(at + c, d);
+                    else { tmem_ld16(at + c, d); tmem_ld_wait(); }
+                    if (c + kStep == kMine) {
                         fence_before_sync();
-                        __syncwarp();
                         if (lane == 0) mbar_arrive(acc_empty + acc);
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        if (kSwap) {
-                            const float4 f = *reinterpret_cast<const float4*>(tab + c + j);
-                            fma2(sum2[(c + j) / 2], now[j], now[j + 1], pair_of(f.x, f.y));
-                            fma2(sum2[(c + j) / 2 + 1], now[j + 2], now[j + 3], pair_of(f.z, f.w));
-                        } else {
-                            fma2(sum2[(c + j) / 2], now[j], now[j + 1], both);
-                            fma2(sum2[(c + j) / 2 + 1], now[j + 2], now[j + 3], both);
-                        }
+                    for (int j = 0; j < kStep; ++j) sum[c + j] = fmaf(__uint_as_float(d[j]), s, sum[c + j]);
+                }
+            } else {                                       // all columns at once: one wait for tensor memory a block
+                uint32_t d[kMine];
+                if constexpr (kMine == 8) tmem_ld8(at, d);
+                else if constexpr (kMine == 16) tmem_ld16(at, d);
+                else if constexpr (kMine == 32) tmem_ld32_async(at, d);
+                else tmem_ld64(at, d);
+                // the rows' scales, where there are registers for them while the columns are on their way
+                const uint32_t tab = table_at + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine) * 4;
+                constexpr int kAhead = kMine <= 16 || !F::kTwoPerSm ? (kMine < 32 ? kMine : 32) : 8;
+                float f[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * j, f + j);
+                tmem_ld_wait();
+                fence_before_sync();
+                if (lane == 0) mbar_arrive(acc_empty + acc);
+#pragma unroll
+                for (int c = 0; c < kMine; c += kAhead) {
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) sum[c + j] = fmaf(__uint_as_float(d[c + j]), f[j], sum[c + j]);
+                    if (c + kAhead < kMine) {
+#pragma unroll
+                        for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * (c + kAhead + j), f + j);
                     }
                 }
             }
@@ -240,27 +246,34 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     fence_before_sync();
     if (split > 1) {
         cluster_wait();
-        if (!kSwap) { cluster_arrive(); cluster_wait(); }  // every CTA of the cluster has left its ring
-    } else if (!kSwap) {
+        if (F::kOver) { cluster_arrive(); cluster_wait(); }    // every CTA of the cluster has left its ring
+    } else if (F::kOver) {
         __syncthreads();
     }
-    if (warp >= 2) {
-        float sum[kMine];
-#pragma unroll
-        for (int j = 0; j < kMine; j += 2) { sum[j] = low_of(sum2[j / 2]); sum[j + 1] = high_of(sum2[j / 2]); }
+    if (warp >= 2 && warp < 10) {
         const int feat = quarter * 32 + lane;
-        if (kSwap) {
-            const int j0 = kSwiglu ? 0 : group * kMine;
-            int owner = j0 / share, r = j0 - owner * share;
-            const uint32_t mine = smem_u32(recv) + (uint32_t)((rank * share) * F::kPitch + (kSwiglu ? group * 128 : 0) + feat) * 4;
+        if constexpr (kSwap && kSwiglu) {
+            int owner = 0, r = 0;
+            const uint32_t mine = smem_u32(recv) + (uint32_t)(rank * share * F::kPitch + group * 128 + feat) * 4;
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
-                if (j0 + j < rows) {
+                if (j < rows) {
                     const uint32_t at = mine + (uint32_t)(r * F::kPitch) * 4;
-                    if (split > 1) store_peer(peer_addr(at, owner), sum[j]);
-                    else recv[r * F::kPitch + (kSwiglu ? group * 128 : 0) + feat] = sum[j];
+                    store_peer(split > 1 ? peer_addr(at, owner) : at, sum[j]);
                 }
                 if (++r == share) { r = 0; ++owner; }
+            }
+        } else if constexpr (kSwap) {
+            const int j0 = group * kMine, col = feat;
+            int owner = j0 / share, r = j0 - owner * share;
+#pragma unroll
+            for (int j = 0; j < kMine; j += 4) {
+                if (j0 + j < rows) {
+                    const uint32_t at = smem_u32(recv) + (uint32_t)((rank * share + r) * F::kPitch + 4 * col) * 4;
+                    store_peer4(split > 1 ? peer_addr(at, owner) : at, sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+                }
+                r += 4;
+                if (r == share) { r = 0; ++owner; }
             }
         } else if (feat < rows) {
             const int owner = feat / share, r = feat - owner * share;
@@ -271,7 +284,32 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     }
     if (split > 1) { cluster_arrive(); cluster_wait(); }
     else __syncthreads();
-    if (warp >= 2) {
+    if (F::kQuads && warp >= 2 && warp < 10) {
+        // a thread takes a feature and four rows: the sums in rank order; a warp's stores lie side by side
+        const int f = (threadIdx.x - 64) & 127, half = (threadIdx.x - 64) >> 7, n = n0 + f, r1 = min(share, rows - rank * share);
+        const float bias = a.bias != nullptr && n < a.N ? a.bias[n] : 0.f;
+        for (int r = 4 * half; r < r1; r += 8) {           // the same for all 128 threads of a half
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int src = 0; src < kMaxSplit; ++src)
+                if (src < split) {
+                    const float4 w = *reinterpret_cast<const float4*>(recv + (size_t)(src * share + r) * F::kPitch + 4 * f);
+                    v[0] += w.x; v[1] += w.y; v[2] += w.z; v[3] += w.w;
+                }
+            const long m = m0 + rank * share + r;
+            const int live = r1 - r;
+            if (n < a.N) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < live) {
+                        const float o = (v[j] + bias) * a.out_scale;
+                        if (a.out_f32) ((float*)a.out)[(m + j) * a.ldo + n] = o;
+                        else ((__nv_bfloat16*)a.out)[(m + j) * a.ldo + n] = __float2bfloat16_rn(o);
+                    }
+            }
+        }
+    }
+    if (!F::kQuads && warp >= 2 && warp < 10) {
         const int col = lane * 4, n = n0 + col;
         float b[4] = {0.f, 0.f, 0.f, 0.f};
         if (!kSwiglu && a.bias != nullptr) {
@@ -339,15 +377,20 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
     const long tiles = (long)((a.M + F::kXRows - 1) / F::kXRows) * a.tiles_n;
     if (tiles * a.split > 0x7fffffffL) return kTooLarge;
     // Shared memory: a ring as deep as the CTA's share of an SM allows; few rows: beside it the sums that land and the scales
-    const size_t side = kSwap ? ((size_t)(NR + a.split) * F::kPitch + (size_t)per * NR * (kSwiglu ? 2 : 1)) * 4 : 0;
-    const size_t sums = (size_t)(F::kXRows + a.split) * F::kPitch * 4;
+    const int rows = kSwap && a.M < NR ? a.M : F::kXRows, share = ((rows + a.split - 1) / a.split + F::kShareOf - 1) / F::kShareOf * F::kShareOf;
+    const size_t side = kSwap ? ((F::kOver ? 0 : (size_t)a.split * share * F::kPitch) + (size_t)per * NR * (kSwiglu ? 2 : 1)) * 4 : 0;
+    const size_t sums = (size_t)a.split * share * F::kPitch * 4;
     const size_t budget = (F::kTwoPerSm && tiles * a.split > sms ? 112 : 224) * 1024;
     if (side + 1024 + F::kStage > budget) return kTooLarge;
     int stages = (int)((budget - 1024 - side) / F::kStage);
-    stages = stages < per ? stages : per;
-    a.stages = stages < kMaxStages ? stages : kMaxStages;
+    stages = stages < kMaxStages ? stages : kMaxStages;
+    // A ring that goes round has an even number of stages: each of the two warps that issue then meets every use of its stages.
+    // (A warp that met every second use only could ask for a phase while the one before is not over: the answer would be yes.)
+    stages = stages >= per ? per : stages & ~1;
+    if (stages < 1) return kTooLarge;
+    a.stages = stages;
     size_t smem = 1024 + a.stages * (size_t)F::kStage + side;
-    if (!kSwap && smem < 1024 + sums) smem = 1024 + sums;
+    if (F::kOver && smem < 1024 + sums + side) smem = 1024 + sums + side;
     CUtensorMap map_w0, map_w1, map_x;
     int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kFeat);
     if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, kFeat); else map_w1 = map_w0; }

@@ -25,7 +25,7 @@ constexpr int kPairRows = 256;
 constexpr int kPairGroups = 4, kAdders = 128 * kPairGroups, kPairThreads = 128 + kAdders;
 constexpr int kAccs = 2, kAccCols = 64 * kPairGroups;     // accumulators in tensor memory, and their columns
 constexpr uint32_t kPairStage = (128 + kAccCols / 2) * kBK;            // a CTA's 128 rows of x and half of the features
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 6;                            // even: each of the two warps that issue meets every use of its stages
 constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStage;
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {

@@ -119,15 +119,20 @@ def _find_build_dir() -> str:
     raise KernelBuildError(f"no writable folder for built kernels among {candidates}")
 
 
+def _host_flags() -> list[str]:
+    """Flags of a binding; the torch that runs is named among them, so that another torch gets a build of its own."""
+    import torch
+    return ["-O2", "-std=c++17", "-fPIC", "-shared", f"-DLB200_TORCH=\"{torch.__version__}\"",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+
+
 def _host_command(compiler: str, src: str, out: str) -> list[str]:
-    """How a binding is compiled: against the headers and libraries of the torch that runs (named by its version, so that
-    another torch gets a build of its own)."""
+    """How a binding is compiled: against the headers and libraries of the torch that runs."""
     import sysconfig
     import torch
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
-    return [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", f"-DLB200_TORCH=\"{torch.__version__}\"",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(root, "include"),
+    return [compiler, *_host_flags(), "-I", os.path.join(root, "include"),
             "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
             "-I", sysconfig.get_paths()["include"], "-o", out, src, "-L", os.path.join(root, "lib"),
             "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
@@ -136,7 +141,7 @@ def _host_command(compiler: str, src: str, out: str) -> list[str]:
 def _digest(name: str) -> str:
     h = hashlib.sha1()
     src = source_path(name)
-    h.update(" ".join(_host_command("", src, "")[1:] if src.endswith(".cpp") else NVCC_FLAGS).encode())
+    h.update(" ".join(_host_flags() if src.endswith(".cpp") else NVCC_FLAGS).encode())
     paths = [src]
     for root, _, files in sorted(os.walk(INCLUDE)):
         paths += [os.path.join(root, f) for f in sorted(files)]

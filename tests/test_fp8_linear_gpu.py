@@ -90,6 +90,27 @@ def test_large(m, n, k, form):
         check_swiglu(x, w, operands(m, n, k, 2)[1], 1.0)
 
 
+@pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("m", [1, 6, 17, 33, 64, 150])
+def test_every_split(m, split):
+    """A tile's blocks over so many CTAs, whatever the rule would choose: few blocks and many each, rings that go round and rings
+    that do not, shares of rows that are empty."""
+    k = K()
+    k._FP8_FORMS["split"] = (1 if m <= 64 else 2) + 256 * split
+    k.FP8_FORM = "split"
+    try:
+        for n, kd in ((200, 128 * 9), (257, 128 * 8 * 3 - 5), (128, 128 * 40), (300, 100)):
+            x, w = operands(m, n, kd)
+            try:
+                check_linear(x, w)
+                check_swiglu(x, w, operands(m, n, kd, 2)[1], 0.8)
+            except k.KernelError as e:
+                assert "beyond the kernel's limit" in str(e)      # a ring that does not fit: the rule takes another form then
+    finally:
+        k.FP8_FORM = "auto"
+        del k._FP8_FORMS["split"]
+
+
 def test_every_block_has_its_own_scales(form):
     """Blocks of very different size: a scale that met a neighbour's block would be off by its factor."""
     k = K()
