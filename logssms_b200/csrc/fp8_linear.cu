@@ -170,15 +170,25 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         sw += (long)tile_n * a.sw_row + kb0 * a.sw_block;
         float s_next = 0.f;
         if (kSwap) {
-            for (int e = t; e < kbn * NR; e += kSumThreads) {
-                const int i = e / NR, m = e % NR;
-                const float x = m < rows ? a.sx[(long)(m0 + m) * a.sx_row + (kb0 + i) * a.sx_block] : 0.f;
-                const long at = (long)tile_n * a.sw_row + (kb0 + i) * a.sw_block;
-                if (kSwiglu) {
-                    table[2 * i * NR + m] = join(x, a.sw0[at]);
-                    table[(2 * i + 1) * NR + m] = join(x, a.sw1[at]);
-                } else {
-                    table[i * NR + m] = join(x, a.sw0[at]);
+            // several entries at a time, all their loads first
+            constexpr int kBatch = NR == 64 ? 8 : NR == 32 ? 4 : 2;
+            for (int e0 = t; e0 < kbn * NR; e0 += kBatch * kSumThreads) {
+                float x[kBatch], w0[kBatch], w1[kBatch];
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) {
+                    const int e = min(e0 + q * kSumThreads, kbn * NR - 1), i = e / NR, m = min(e % NR, rows - 1);
+                    const long at = (long)tile_n * a.sw_row + (kb0 + i) * a.sw_block;
+                    x[q] = a.sx[(long)(m0 + m) * a.sx_row + (kb0 + i) * a.sx_block];
+                    w0[q] = a.sw0[at];
+                    if (kSwiglu) w1[q] = a.sw1[at];
+                }
+#pragma unroll
+                for (int q = 0; q < kBatch; ++q) {
+                    const int e = e0 + q * kSumThreads, i = e / NR, m = e % NR;
+                    if (e < kbn * NR) {
+                        table[(kSwiglu ? 2 : 1) * i * NR + m] = join(x[q], w0[q]);
+                        if (kSwiglu) table[(2 * i + 1) * NR + m] = join(x[q], w1[q]);
+                    }
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -223,7 +233,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 else tmem_ld64(at, d);
                 // the rows' scales, where there are registers for them while the columns are on their way
                 const uint32_t tab = table_at + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine) * 4;
-                constexpr int kAhead = kMine <= 16 || !F::kTwoPerSm ? (kMine < 32 ? kMine : 32) : 8;
+                constexpr int kAhead = kMine <= 16 ? kMine : F::kTwoPerSm ? 8 : kMine == 32 ? 32 : 16;
                 float f[kAhead];
 #pragma unroll
                 for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * j, f + j);
@@ -258,8 +268,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
 #pragma unroll
             for (int j = 0; j < kMine; ++j) {
                 if (j < rows) {
-                    const uint32_t at = mine + (uint32_t)(r * F::kPitch) * 4;
-                    store_peer(split > 1 ? peer_addr(at, owner) : at, sum[j]);
+                    if (split > 1) store_peer(peer_addr(mine + (uint32_t)(r * F::kPitch) * 4, owner), sum[j]);
+                    else recv[j * F::kPitch + group * 128 + feat] = sum[j];
                 }
                 if (++r == share) { r = 0; ++owner; }
             }
@@ -317,43 +327,58 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
             for (int e = 0; e < 4; ++e) if (n + e < a.N) b[e] = a.bias[n + e];
         }
         const int r1 = min(share, rows - rank * share);
-        for (int r = warp - 2; r < r1; r += kSumThreads / 32) {
-            const long m = m0 + rank * share + r;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
-            for (int src = 0; src < split; ++src) {
-                const float* p = recv + (size_t)(src * share + r) * F::kPitch + col;
-                const float4 w = *reinterpret_cast<const float4*>(p);
-                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-                if (kSwiglu) {
-                    const float4 w1 = *reinterpret_cast<const float4*>(p + 128);
-                    u.x += w1.x; u.y += w1.y; u.z += w1.z; u.w += w1.w;
-                }
-            }
-            if constexpr (kSwiglu) {
-                float h[4] = {silu_of(v.x * a.act_scale) * u.x, silu_of(v.y * a.act_scale) * u.y, silu_of(v.z * a.act_scale) * u.z,
-                              silu_of(v.w * a.act_scale) * u.w};
-                uint32_t top = 0;
+        constexpr int kWarps = kSumThreads / 32, kAtOnce = NR >= 64 ? 4 : 1;
+        for (int r0 = warp - 2; r0 < r1; r0 += kWarps * kAtOnce) {
+            float4 vs[kAtOnce], us[kSwiglu ? kAtOnce : 1];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { if (n + e >= a.N) h[e] = 0.f; top = max(top, magnitude(h[e])); }
-                const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top)), back = 1.f / scale;
-                // rows are filled up to 16 bytes: four bytes that begin inside the row end inside its storage
-                if (n < a.N) *reinterpret_cast<uint32_t*>(a.q + m * a.ldq + n) = fp8_quad(h[0] * back, h[1] * back, h[2] * back, h[3] * back);
-                if (lane == 0) a.qs[m * a.qs_row + tile_n * a.qs_block] = scale;
-            } else {
-                const float o[4] = {(v.x + b[0]) * a.out_scale, (v.y + b[1]) * a.out_scale, (v.z + b[2]) * a.out_scale, (v.w + b[3]) * a.out_scale};
-                const long at = m * a.ldo + n;
-                if (a.out_f32) {
-                    float* p = (float*)a.out + at;
-                    if (n + 4 <= a.N && ((uintptr_t)p & 15) == 0) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
-                    else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = o[e];
+            for (int k = 0; k < kAtOnce; ++k) {
+                vs[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (kSwiglu) us[k] = vs[k];
+            }
+            for (int src = 0; src < split; ++src)
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int r = min(r0 + k * kWarps, r1 - 1);
+                    const float* p = recv + (size_t)(src * share + r) * F::kPitch + col;
+                    const float4 w = *reinterpret_cast<const float4*>(p);
+                    vs[k].x += w.x; vs[k].y += w.y; vs[k].z += w.z; vs[k].w += w.w;
+                    if constexpr (kSwiglu) {
+                        const float4 w1 = *reinterpret_cast<const float4*>(p + 128);
+                        us[k].x += w1.x; us[k].y += w1.y; us[k].z += w1.z; us[k].w += w1.w;
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int r = r0 + k * kWarps;
+                if (r >= r1) break;                            // the same for the whole warp
+                const long m = m0 + rank * share + r;
+                const float4 v = vs[k], u = us[kSwiglu ? k : 0];
+                if constexpr (kSwiglu) {
+                    float h[4] = {silu_of(v.x * a.act_scale) * u.x, silu_of(v.y * a.act_scale) * u.y, silu_of(v.z * a.act_scale) * u.z,
+                                  silu_of(v.w * a.act_scale) * u.w};
+                    uint32_t top = 0;
+    #pragma unroll
+                    for (int e = 0; e < 4; ++e) { if (n + e >= a.N) h[e] = 0.f; top = max(top, magnitude(h[e])); }
+                    const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top)), back = 1.f / scale;
+                    // rows are filled up to 16 bytes: four bytes that begin inside the row end inside its storage
+                    if (n < a.N) *reinterpret_cast<uint32_t*>(a.q + m * a.ldq + n) = fp8_quad(h[0] * back, h[1] * back, h[2] * back, h[3] * back);
+                    if (lane == 0) a.qs[m * a.qs_row + tile_n * a.qs_block] = scale;
                 } else {
-                    __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
-                    if (n + 4 <= a.N && ((uintptr_t)p & 7) == 0) {
-                        uint2 w;
-                        reinterpret_cast<__nv_bfloat162*>(&w)[0] = __floats2bfloat162_rn(o[0], o[1]);
-                        reinterpret_cast<__nv_bfloat162*>(&w)[1] = __floats2bfloat162_rn(o[2], o[3]);
-                        *reinterpret_cast<uint2*>(p) = w;
-                    } else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = __float2bfloat16_rn(o[e]);
+                    const float o[4] = {(v.x + b[0]) * a.out_scale, (v.y + b[1]) * a.out_scale, (v.z + b[2]) * a.out_scale, (v.w + b[3]) * a.out_scale};
+                    const long at = m * a.ldo + n;
+                    if (a.out_f32) {
+                        float* p = (float*)a.out + at;
+                        if (n + 4 <= a.N && ((uintptr_t)p & 15) == 0) *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+                        else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = o[e];
+                    } else {
+                        __nv_bfloat16* p = (__nv_bfloat16*)a.out + at;
+                        if (n + 4 <= a.N && ((uintptr_t)p & 7) == 0) {
+                            uint2 w;
+                            reinterpret_cast<__nv_bfloat162*>(&w)[0] = __floats2bfloat162_rn(o[0], o[1]);
+                            reinterpret_cast<__nv_bfloat162*>(&w)[1] = __floats2bfloat162_rn(o[2], o[3]);
+                            *reinterpret_cast<uint2*>(p) = w;
+                        } else for (int e = 0; e < 4; ++e) if (n + e < a.N) p[e] = __float2bfloat16_rn(o[e]);
+                    }
                 }
             }
         }
@@ -410,18 +435,27 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
     return rc != 0 ? rc : launch_status();
 }
 
-// CTAs that share a tile's blocks of K: doubled as long as the GPU holds them and two blocks are left to each
-int default_split(long tiles, int blocks, int sms, int per_sm) {
+// CTAs that share a tile's blocks of K: doubled as long as the GPU holds them at once, `per_sm` on an SM, and `left` blocks remain
+// to each.  Few rows, us for a split of 1 / 2 / 4 / 8: down 3,072 x 12,288 (24 tiles, 96 blocks) at 1 row 22 / 13 / 11 / 10, at 64 rows
+// 33 / 19 / 13 / 19 (one CTA on an SM); gate|up 12,288 x 3,072 (96 tiles, 24 blocks) at 64 rows 22 / 30 / 37 / 81, 3,072 x 1,280 (24
+// tiles, 10 blocks) at 1 row 5.5 / 4.5 / 4.7 / 5.2.  With one CTA on an SM not every SM can be in a larger cluster (tiles of 128 rows,
+// 1,024 x 2,048: 8 tiles x 8 7.8 us, x 4 8.2; 16 tiles x 8 12.6, x 4 8.2; 32 tiles x 4 9.4, x 2 10.1; 64 tiles x 2 11.4, x 1 13.4).
+int default_split(long tiles, int blocks, int sms, int per_sm, int left) {
     int split = 1;
-    while (split < kMaxSplit && 2 * tiles * split <= (long)sms * per_sm && blocks / (2 * split) >= 2) split *= 2;
+    while (split < kMaxSplit && blocks / (2 * split) >= left) {
+        const long held = per_sm > 1 ? (long)sms * per_sm : split == 1 ? sms : split == 2 ? sms * 13 / 15 : sms * 2 / 3;
+        if (2 * tiles * split > held) break;
+        split *= 2;
+    }
     return split;
 }
 
 enum : int { kAuto = 0, kRows = 1, kTiles = 2, kPair = 3 };
 
-template <bool kSwiglu>
-int launch_pair(const Operands& o, Args a, int sms, cudaStream_t s) {
+template <bool kSwiglu, bool kRagged>
+int launch_pair(const Operands& o, const Args& a, int sms, cudaStream_t s) {
     constexpr int feat = kSwiglu ? 128 : 256;
+    constexpr size_t smem = pair_smem(kRagged);
     const long tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + feat - 1) / feat);
     if (tiles > 0x3fffffffL) return kTooLarge;
     const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
@@ -431,16 +465,16 @@ int launch_pair(const Operands& o, Args a, int sms, cudaStream_t s) {
     if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, 128);
     if (rc != 0) return rc;
     static size_t have = 0;
-    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu>, kPairSmem, have);
+    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu, kRagged>, smem, have);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = kPairSmem; cfg.stream = s;
+    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu>, map_w0, map_w1, map_x, a);
+    rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged>, map_w0, map_w1, map_x, a);
     return rc != 0 ? rc : launch_status();
 }
 
@@ -457,14 +491,25 @@ int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
     form &= 255;
     if (form == kRows || (form == kAuto && a.M <= 64)) {
         if (a.M > 64) return kTooLarge;
-        a.split = split ? split : default_split(tiles_n, blocks, sms, 2);
+        a.split = split ? split : default_split(tiles_n, blocks, sms, !kSwiglu && a.M <= 32 ? 2 : 1, kSwiglu ? 4 : 2);
         const int rc = a.M <= 16 ? launch<true, 16, kSwiglu>(o, a, sms, s) : a.M <= 32 ? launch<true, 32, kSwiglu>(o, a, sms, s)
                                                                                      : launch<true, 64, kSwiglu>(o, a, sms, s);
         if (rc != kTooLarge || form != kAuto) return rc;   // a K whose table of scales does not fit goes in tiles
     }
-    const long pair_tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + (kSwiglu ? 127 : 255)) / (kSwiglu ? 128 : 256));
-    if (form == kPair || (form == kAuto && pair_tiles >= sms / 4)) return launch_pair<kSwiglu>(o, a, sms, s);
-    a.split = split ? split : default_split((a.M + 127) / 128 * tiles_n, blocks, sms, 1);
+    // Pairs, us against tiles of 128 rows: 3,072 x 12,288 256 rows (48 tiles) 47 / 33, 512 rows (96) 49 / 65; 1,280 x 3,072 512 rows (40)
+    // 16 / 13, 1,024 rows (80) 16.6 / 17.0, 2,048 rows (160) 18 / 34; 1,024 x 2,048 1,024 rows (64) 14 / 11, 2,048 rows (128) 13.8 / 13.3;
+    // 1,003 x 1,431 2,048 rows (128) 14 / 12; gate|up 12,288 x 3,072 65 rows 32 / 25, 128 rows 33 / 29, 203 rows 33 / 50; 3,072 x 1,280
+    // 65 rows 10.5 / 9.8, 128 rows 10.8 / 12.5.
+    const long tiles = (a.M + 127L) / 128 * tiles_n;
+    if (form == kPair || (form == kAuto && (kSwiglu ? a.M > 96 : tiles > sms || (tiles > sms / 2 && blocks >= 24)))) {
+        if constexpr (kSwiglu) return launch_pair<true, false>(o, a, sms, s);
+        else {
+            const int size = a.out_f32 ? 4 : 2;
+            const bool ragged = ((uintptr_t)a.out & 31) != 0 || a.ldo * size % 32 != 0 || a.N * (long)size % 32 != 0;
+            return ragged ? launch_pair<false, true>(o, a, sms, s) : launch_pair<false, false>(o, a, sms, s);
+        }
+    }
+    a.split = split ? split : default_split(tiles, blocks, sms, 1, 2);
     return launch<false, 128, kSwiglu>(o, a, sms, s);
 }
 }  // namespace

@@ -21,6 +21,17 @@ __device__ __forceinline__ float fp8_scale(uint32_t top) {
     const float s = __uint_as_float(top) / 448.f;
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;      // a NaN stays
 }
+// v / scale, rounded as a division is (up to its last bit, where the quotient is tiny): the product with the reciprocal and one
+// correction by what is left over.  A product alone lies on the wrong side of a rounding boundary where a quotient of bfloat16 values
+// lies on it, which is not rare.
+struct Fp8Divide {
+    float scale, back;
+    __device__ __forceinline__ explicit Fp8Divide(float s) : scale(magnitude(s) == 0x7f800000u ? 0.f : s), back(1.f / s) {}     // x / inf: 0, NaN for inf
+    __device__ __forceinline__ float operator()(float v) const {
+        const float q = v * back;
+        return fmaf(fmaf(-q, scale, v), back, q);
+    }
+};
 // two values, already divided by their scale, as two bytes (the first one in the low byte)
 __device__ __forceinline__ uint32_t fp8_pair(float a, float b) {
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
