@@ -47,6 +47,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--ssm-state-dtype", choices=["float32", "activation"], default="float32",
                    help="dtype in which recurrent states are kept between steps: float32, or the model's dtype (as the "
                         "reference keeps them: half the bytes of a decode step's state update, one rounding per step)")
+    p.add_argument("--feed-forward-weights", choices=["model", "float8"], default="model",
+                   help="weights of the feed-forwards: as they are stored, or in 8-bit floating point with a scale per 128 x 128 "
+                        "(half the bytes of their part of a decode step, about twice the rate of a prompt's; rows go in 8 bits too)")
     p.add_argument("--profile", default=None, metavar="FILE",
                    help="time every kernel with CUDA events and write the sums per kernel class to FILE (JSON) at exit; "
                         "such a run launches every step kernel by kernel")
@@ -188,7 +191,8 @@ def main(argv=None) -> int:
               memory_ratio=args.memory_ratio, max_prefill_tokens=args.max_prefill_tokens, seed=args.seed,
               scheduling_policy=args.scheduling_policy, mixed_prefill_tokens=args.mixed_prefill_tokens,
               use_graphs=not args.no_graph, profile=args.profile is not None, nvtx=args.nvtx,
-              cuda_graph_max_bs=args.cuda_graph_max_bs, ssm_state_dtype=args.ssm_state_dtype)
+              cuda_graph_max_bs=args.cuda_graph_max_bs, ssm_state_dtype=args.ssm_state_dtype,
+              feed_forward_weights=args.feed_forward_weights)
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                             ignore_eos=args.ignore_eos, max_tokens=args.max_tokens)
     def write_profile():

@@ -67,7 +67,8 @@ class Engine:
                  device: str = "cuda:0", poison_on_free: bool = False, max_step_tokens: int = 1 << 30,
                  use_graphs: bool = True, max_graphs: int = 64, max_shape_graphs: int = 8, max_bucket_graphs: int = 32,
                  max_graph_tokens: int = 4096, profile: bool = False, nvtx: bool = False,
-                 cuda_graph_max_bs: int | None = None, ssm_state_dtype: str = "float32"):
+                 cuda_graph_max_bs: int | None = None, ssm_state_dtype: str = "float32",
+                 feed_forward_weights: str = "model"):
         if not torch.cuda.is_available():
             raise RuntimeError("logssms_b200 needs a CUDA device (built for sm_100a); there is no CPU path")
         try:
@@ -83,7 +84,15 @@ class Engine:
         with torch.inference_mode():
             load_weights(self.model, model_dir, self.dtype, self.device)
             # `ssm_state_dtype`: "float32" (the default), or "activation" to keep recurrent states in the model's dtype
-            self.model.setup(Runtime(self.device, self.dtype, max_seq_len, page_size, {"ssm_state_dtype": ssm_state_dtype}))
+            # `feed_forward_weights`: "model" (as they are stored), or "float8": feed-forwards that have such a form run on 8-bit
+            # weights and rows
+            self.model.setup(Runtime(self.device, self.dtype, max_seq_len, page_size,
+                                     {"ssm_state_dtype": ssm_state_dtype, "feed_forward_weights": feed_forward_weights}))
+        if feed_forward_weights not in ("model", "float8"):
+            raise ValueError(f"feed_forward_weights must be model or float8, got {feed_forward_weights!r}")
+        if feed_forward_weights == "float8" and not any(getattr(getattr(b, "feed_forward", None), "takes_fp8_rows", False)
+                                                        for b in self.model.layers):
+            raise ValueError("feed_forward_weights float8: no feed-forward of this model has an 8-bit form")
         needs = self.model.cache_needs()
         if num_pages is None:
             num_pages = self._pages_that_fit(needs, max_requests, memory_ratio)

@@ -77,6 +77,8 @@ class PreNormParallelBlock(Part):
                 or tuple(map(type, parts)) != (Attention, Mamba2, GatedMLP, RMSNorm, RMSNorm)):
             return None
         attn, mamba, ff = self.mixers[0], self.mixers[1], self.feed_forward
+        if ff.fp8 is not None:
+            return None
         a, m = attn.spec, mamba.spec
         table = attn.position.table
         if a.window or m.gated_norm or mamba.in_b is not None or mamba.out_b is not None or table.shape[1] == 0:
@@ -118,6 +120,9 @@ class PreNormParallelBlock(Part):
                                          and all(getattr(m, "takes_normed_rows", False) for m in self.mixers)) else {}
         defer_ff = {"defer": True} if (getattr(self.ff_norm, "can_defer", False)
                                        and getattr(self.feed_forward, "takes_normed_rows", False)) else {}
+        # ... or, to a feed-forward on 8-bit weights, hand over 8-bit rows
+        ff_form = {"fp8": True} if (getattr(self.feed_forward, "takes_fp8_rows", False)
+                                    and getattr(self.ff_norm, "can_fp8", False)) else defer_ff
         ins, residual = self.mixer_norm.forward(x, residual, out_scales=tuple(m.in_scale for m in slots), **defer_mix)
         # Where the norm in front of the feed-forward is deferred anyway, the first mixer's last product may join the
         # residual stream in its epilogue (`joins_residual`): it then returns `SummedRows`, the norm has nothing left to
@@ -160,14 +165,14 @@ class PreNormParallelBlock(Part):
             outs = [first, second]
         next_join = bool(ctx.extras.get("next_norm_takes_summed")) and getattr(self.feed_forward, "joins_residual", False)
         if isinstance(outs[0], K.SummedRows):
-            (h,), residual = self.ff_norm.forward(outs[0], None, **defer_ff)
+            (h,), residual = self.ff_norm.forward(outs[0], None, **ff_form)
         elif len(outs) == 2:
             (h,), residual = self.ff_norm.forward(outs[0], residual, other=outs[1],
-                                                  in_scales=(slots[0].out_scale, slots[1].out_scale), **defer_ff)
+                                                  in_scales=(slots[0].out_scale, slots[1].out_scale), **ff_form)
         else:
             if slots[0].out_scale != 1.0:
                 outs[0] = K.scale(outs[0], slots[0].out_scale)
-            (h,), residual = self.ff_norm.forward(outs[0], residual, **defer_ff)
+            (h,), residual = self.ff_norm.forward(outs[0], residual, **ff_form)
         if next_join and isinstance(h, K.NormedRows):
             # the same at the feed-forward's last product, for the norm of the next layer
             out = self.feed_forward.forward(h, join=K.ResidualJoin(residual))

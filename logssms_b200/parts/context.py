@@ -17,7 +17,8 @@ class Runtime:
     dtype: torch.dtype
     max_seq_len: int
     page_size: int
-    # choices of the engine's user that a part may honour, by name ("ssm_state_dtype": "float32" | "activation")
+    # choices of the engine's user that a part may honour, by name ("ssm_state_dtype": "float32" | "activation";
+    # "feed_forward_weights": "model" | "float8")
     options: Mapping[str, Any] = field(default_factory=dict)
 
 

@@ -17,6 +17,7 @@ class RMSNorm(Part):
     takes_summed_rows = True  # forward() takes `K.SummedRows` as x: the product before has joined the residual already
     takes_scaled_rows = True  # forward() takes `K.ScaledRows` as x: it applies the pending multiplier while it loads x
     takes_stream_rows = True  # forward() takes `K.StreamRows` as x (a 32-bit stream); `post()` is the post-norm form
+    can_fp8 = True            # forward() takes `fp8=`: see there
     norm_kind = "rmsnorm"     # what the kernels of a pre-norm stream call this norm (`K.NORM_KINDS`)
     kernels = ("norm", "linear_skinny", "linear_rows_tc", "stream_norm")
 
@@ -48,10 +49,13 @@ class RMSNorm(Part):
         return K.skip_rmsnorm(stream, y, skip_scale, self.weight, self.eps, extra=extra, row_scale=row_scale)
 
     def forward(self, x, residual=None, *, other=None, in_scales=(1.0, 1.0), out_scales=(1.0,), want_residual=True,
-                defer=False):
-        """With `defer` (the caller's consumers all take `NormedRows`: their first step is a product), and
+                defer=False, fp8=False):
+        """With `fp8` (the caller's consumer takes `K.Fp8Rows`) the one output is 8-bit rows, which the kernel that norms leaves.
+        With `defer` (the caller's consumers all take `NormedRows`: their first step is a product), and
         few enough rows, nothing is launched here: the outputs are `NormedRows` that the consumers' products
         normalise in their prologue, and the new residual is a fresh tensor that the first of them writes."""
+        if fp8:
+            return self._fp8_rows(x, residual, other, in_scales, out_scales, want_residual)
         if isinstance(x, K.StreamRows):
             # a 32-bit stream: normalised in 32-bit, handed on in the activation dtype
             if residual is not None or other is not None:
@@ -78,6 +82,28 @@ class RMSNorm(Part):
             return outs, shared["residual_out"]
         return K.add_rmsnorm(x, self.weight, self.eps, residual, other=other, in_scales=in_scales,
                              out_scales=out_scales, want_residual=want_residual)
+
+
+    def _fp8_rows(self, x, residual, other, in_scales, out_scales, want_residual):
+        if len(out_scales) != 1:
+            raise ValueError("8-bit rows are one output")
+        if isinstance(x, K.ScaledRows):
+            # the multiplier of the product that made x is applied as x is loaded
+            x, in_scales = x.rows, (x.scale * in_scales[0], in_scales[1])
+        if isinstance(x, K.SummedRows):
+            # x has joined its residual already: the float32 sums are normed, the rounded copy is the new residual
+            if residual is not None or other is not None:
+                raise ValueError("summed rows have joined their residual already")
+            rows, _ = K.add_rmsnorm_fp8(x.vsum, self.weight, self.eps, out_scale=out_scales[0], want_residual=False)
+            return (rows,), x.residual
+        if isinstance(x, K.StreamRows):
+            if residual is not None or other is not None:
+                raise ValueError("a 32-bit stream carries its residual itself")
+            rows, _ = K.add_rmsnorm_fp8(x.f32, self.weight, self.eps, out_scale=out_scales[0], want_residual=False)
+            return (rows,), None
+        rows, residual = K.add_rmsnorm_fp8(x, self.weight, self.eps, residual, other=other, in_scales=in_scales,
+                                           out_scale=out_scales[0], want_residual=want_residual)
+        return (rows,), residual
 
 
 @NORMS.register("layernorm")
