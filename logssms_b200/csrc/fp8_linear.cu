@@ -80,7 +80,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     // the ring (a peer may be done while this CTA still loads); many: over it, once the whole cluster has left it.  Few rows: then the
     // scales, [block][gate, up][row].
     float* recv = reinterpret_cast<float*>(F::kOver ? base : base + (size_t)stages * kStage);
-    float* table = reinterpret_cast<float*>(base + (size_t)stages * kStage) + (F::kOver ? 0 : (size_t)split * share * F::kPitch);
+    float* table = reinterpret_cast<float*>(base + (size_t)stages * kStage) + (F::kOver ? 0 : (size_t)(kSwiglu && split == 1 ? NR : split * share) * F::kPitch);
     const uint32_t table_at = smem_u32(table);
     auto load_w = [&](int s, int i) {
         uint8_t* w = base + (size_t)s * kStage;
@@ -170,25 +170,27 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         sw += (long)tile_n * a.sw_row + kb0 * a.sw_block;
         float s_next = 0.f;
         if (kSwap) {
-            // several entries at a time, all their loads first
-            constexpr int kBatch = NR == 64 ? 8 : NR == 32 ? 4 : 2;
-            for (int e0 = t; e0 < kbn * NR; e0 += kBatch * kSumThreads) {
+            // a thread has one row and every kEvery-th block, four at a time, their loads first.  (Short code: what runs once per CTA
+            // comes from memory itself, instruction by instruction.)
+            constexpr int kEvery = kSumThreads / NR, kBatch = 4;
+            const int m = t % NR;
+            const float* px = a.sx + (long)(m0 + min(m, rows - 1)) * a.sx_row;
+            const float *p0 = a.sw0 + (long)tile_n * a.sw_row, *p1 = kSwiglu ? a.sw1 + (long)tile_n * a.sw_row : nullptr;
+#pragma unroll 1
+            for (int i0 = t / NR; i0 < kbn; i0 += kBatch * kEvery) {
                 float x[kBatch], w0[kBatch], w1[kBatch];
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
-                    const int e = min(e0 + q * kSumThreads, kbn * NR - 1), i = e / NR, m = min(e % NR, rows - 1);
-                    const long at = (long)tile_n * a.sw_row + (kb0 + i) * a.sw_block;
-                    x[q] = a.sx[(long)(m0 + m) * a.sx_row + (kb0 + i) * a.sx_block];
-                    w0[q] = a.sw0[at];
-                    if (kSwiglu) w1[q] = a.sw1[at];
+                    const long kb = kb0 + min(i0 + q * kEvery, kbn - 1);
+                    x[q] = px[kb * a.sx_block];
+                    w0[q] = p0[kb * a.sw_block];
+                    if (kSwiglu) w1[q] = p1[kb * a.sw_block];
                 }
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
-                    const int e = e0 + q * kSumThreads, i = e / NR, m = e % NR;
-                    if (e < kbn * NR) {
-                        table[(kSwiglu ? 2 : 1) * i * NR + m] = join(x[q], w0[q]);
-                        if (kSwiglu) table[(2 * i + 1) * NR + m] = join(x[q], w1[q]);
-                    }
+                    const int i = min(i0 + q * kEvery, kbn - 1);           // (the last one may be written several times, alike)
+                    table[(kSwiglu ? 2 : 1) * i * NR + m] = join(x[q], w0[q]);
+                    if (kSwiglu) table[(2 * i + 1) * NR + m] = join(x[q], w1[q]);
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -263,15 +265,19 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     if (warp >= 2 && warp < 10) {
         const int feat = quarter * 32 + lane;
         if constexpr (kSwap && kSwiglu) {
-            int owner = 0, r = 0;
-            const uint32_t mine = smem_u32(recv) + (uint32_t)(rank * share * F::kPitch + group * 128 + feat) * 4;
+            uint32_t at = smem_u32(recv) + (uint32_t)(rank * share * F::kPitch + group * 128 + feat) * 4;
+            if (split == 1) {                              // there is room for all NR rows
 #pragma unroll
-            for (int j = 0; j < kMine; ++j) {
-                if (j < rows) {
-                    if (split > 1) store_peer(peer_addr(mine + (uint32_t)(r * F::kPitch) * 4, owner), sum[j]);
-                    else recv[j * F::kPitch + group * 128 + feat] = sum[j];
+                for (int j = 0; j < kMine; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + j * F::kPitch * 4), "f"(sum[j]) : "memory");
+            } else {
+                int owner = 0, r = 0;
+                uint32_t to = peer_addr(at, 0);
+#pragma unroll
+                for (int j = 0; j < kMine; ++j) {
+                    if (j < rows) store_peer(to, sum[j]);
+                    to += F::kPitch * 4;
+                    if (++r == share) { r = 0; to = peer_addr(at, min(++owner, split - 1)); }
                 }
-                if (++r == share) { r = 0; ++owner; }
             }
         } else if constexpr (kSwap) {
             const int j0 = group * kMine, col = feat;
@@ -298,6 +304,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
         // a thread takes a feature and four rows: the sums in rank order; a warp's stores lie side by side
         const int f = (threadIdx.x - 64) & 127, half = (threadIdx.x - 64) >> 7, n = n0 + f, r1 = min(share, rows - rank * share);
         const float bias = a.bias != nullptr && n < a.N ? a.bias[n] : 0.f;
+#pragma unroll 1
         for (int r = 4 * half; r < r1; r += 8) {           // the same for all 128 threads of a half
             float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -327,7 +334,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
             for (int e = 0; e < 4; ++e) if (n + e < a.N) b[e] = a.bias[n + e];
         }
         const int r1 = min(share, rows - rank * share);
-        constexpr int kWarps = kSumThreads / 32, kAtOnce = NR >= 64 ? 4 : 1;
+        constexpr int kWarps = kSumThreads / 32, kAtOnce = NR >= 64 ? 2 : 1;
+#pragma unroll 1
         for (int r0 = warp - 2; r0 < r1; r0 += kWarps * kAtOnce) {
             float4 vs[kAtOnce], us[kSwiglu ? kAtOnce : 1];
 #pragma unroll
@@ -335,6 +343,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 vs[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (kSwiglu) us[k] = vs[k];
             }
+#pragma unroll 1
             for (int src = 0; src < split; ++src)
 #pragma unroll
                 for (int k = 0; k < kAtOnce; ++k) {
@@ -403,8 +412,8 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
     if (tiles * a.split > 0x7fffffffL) return kTooLarge;
     // Shared memory: a ring as deep as the CTA's share of an SM allows; few rows: beside it the sums that land and the scales
     const int rows = kSwap && a.M < NR ? a.M : F::kXRows, share = ((rows + a.split - 1) / a.split + F::kShareOf - 1) / F::kShareOf * F::kShareOf;
-    const size_t side = kSwap ? ((F::kOver ? 0 : (size_t)a.split * share * F::kPitch) + (size_t)per * NR * (kSwiglu ? 2 : 1)) * 4 : 0;
-    const size_t sums = (size_t)a.split * share * F::kPitch * 4;
+    const size_t side = kSwap ? ((F::kOver ? 0 : (size_t)(kSwiglu && a.split == 1 ? NR : a.split * share) * F::kPitch) + (size_t)per * NR * (kSwiglu ? 2 : 1)) * 4 : 0;
+    const size_t sums = (size_t)(kSwap && kSwiglu && a.split == 1 ? NR : a.split * share) * F::kPitch * 4;
     const size_t budget = (F::kTwoPerSm && tiles * a.split > sms ? 112 : 224) * 1024;
     if (side + 1024 + F::kStage > budget) return kTooLarge;
     int stages = (int)((budget - 1024 - side) / F::kStage);
@@ -460,7 +469,7 @@ int launch_pair(const Operands& o, const Args& a, int sms, cudaStream_t s) {
     if (tiles > 0x3fffffffL) return kTooLarge;
     const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
     CUtensorMap map_w0, map_w1, map_x;
-    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 32 : 128);
+    int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 32 : 64);
     if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, 32); else map_w1 = map_w0; }
     if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, 128);
     if (rc != 0) return rc;

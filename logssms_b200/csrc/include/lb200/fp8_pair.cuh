@@ -3,15 +3,19 @@
 // an SM fetches 32 KB per block of 128 columns where a tile of 128 x 256 of its own would take 48: at the 8-bit rate of the
 // tensor cores (512 cycles a block) that is 64 bytes a cycle and SM instead of 96.  A pair stays and takes tile after tile.
 //
-//   warp 0      one thread issues this CTA's TMA loads; their bytes are counted at the first CTA's barrier
-//   warp 1      first CTA: one thread issues the products for both, into one of two accumulators of 256 columns each; both
-//               CTAs: allocates tensor memory
-//   warps 2, 3  watch the barriers and wake the warps that add and the one that issues (first CTA)
-//   warps 4-11  two warpgroups: a thread is a row of its CTA's 128 and takes 128 columns of the accumulator: it reads a block's
-//               sums, multiplies them by the block's scales and adds them to its 128 sums, while the tensor cores work on the
-//               next block.  Warps 0-3 give up registers for that.
-// SwiGLU: the features are laid out so that a thread has gate and up of the same 64 features (columns 0-63 and 64-127 of its
-// half); only a row's largest magnitude is exchanged between the two warpgroups.
+//   warp 0      issues this CTA's TMA loads; their bytes are counted at the first CTA's barrier
+//   warps 1, 3  first CTA: issue the products for both, one warp for either half of 128 columns; two accumulators of 256 columns.
+//               Warp 1 also allocates tensor memory (both CTAs)
+//   warp 2      watches the accumulators, hands stages back, wakes the warps that add
+//   warps 4-19  four warpgroups: a thread is a row of its CTA's 128 and takes 64 columns of the accumulator: it reads a block's
+//               sums, multiplies them by the block's scales and adds them to its 64 sums, while the tensor cores work on the next
+//               block.  Warps 0-3 give up registers for that.
+// What bounds it: the adding (256 cycles of multiply-adds and two waits for tensor memory per block), the products (512 cycles) and
+// the hand-over of an accumulator between them lie within a quarter of each other; left out one at a time, down 8,192 x 3,072 x 12,288
+// takes 264 us without the multiply-adds, 277 with a quarter of the products, 285 without loads, 314 with all (1.97 PFLOP/s; 356 us in
+// a long row of calls on random data, when the power limit sets the clock).
+// SwiGLU: the features are laid out so that a thread has gate and up of the same 32 features; only a row's largest magnitude is
+// exchanged between the four warpgroups.
 //
 // Every wait on an mbarrier is bounded; one that gives up records itself in `error`, the roles run out of their own bounded
 // waits, both CTAs still meet the last cluster barrier, tensor memory is freed and the kernel returns.
@@ -23,8 +27,9 @@ namespace fp8 {
 
 constexpr int kPairRows = 256;
 constexpr int kPairGroups = 4, kAdders = 128 * kPairGroups, kPairThreads = 128 + kAdders;
-constexpr int kAccs = 2, kAccCols = 64 * kPairGroups;     // accumulators in tensor memory, and their columns
-constexpr uint32_t kPairStage = (128 + kAccCols / 2) * kBK;            // a CTA's 128 rows of x and half of the features
+constexpr int kCols = 64 * kPairGroups, kHalf = kCols / 2;                // accumulator columns of a block, and of one of its halves
+constexpr int kHalfAdders = kAdders / 2;
+constexpr uint32_t kPairStage = (128 + kCols / 2) * kBK;            // a CTA's 128 rows of x and half of the features
 constexpr int kPairStages = 6;                            // even: each of the two warps that issue meets every use of its stages
 constexpr size_t kPairTurn = 4 * kPairGroups * 32 * 16 * 4;            // 32 rows x 16 features for each warp that adds
 constexpr size_t pair_smem(bool ragged) { return 1024 + (size_t)kPairStages * kPairStage + (ragged ? kPairTurn : 0); }
@@ -87,7 +92,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     constexpr int kFeat = kSwiglu ? 128 : 256;            // output features of a tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(16) uint64_t acc_full[kAccs], acc_empty[kAccs], full[kPairStages], empty[kPairStages];
+    __shared__ __align__(16) uint64_t acc_full[4], acc_empty[4], full[kPairStages], empty[kPairStages];
     __shared__ uint32_t tops[kSwiglu ? kPairGroups : 1][128];       // SwiGLU: a row's largest magnitude among a group's features
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
@@ -97,8 +102,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
     const int kbn = (a.K + kBK - 1) / kBK;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPairStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
-        for (int s = 0; s < kAccs; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * 4 * kPairGroups); }
+        for (int s = 0; s < kPairStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 2); }
+        for (int s = 0; s < 4; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * kHalfAdders / 32); }
         failed = 0;
         mbar_fence_init();
     }
@@ -127,7 +132,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             for (int t = pair; t < tiles && going; t += pairs) {
                 const Tile at = tile_at(t, tiles_m, tiles_n);
                 const int row = at.m * kPairRows + rank * 128;
-                const int feat = at.n * kFeat + rank * (kFeat / 2);
+                const int feat = at.n * kFeat + rank * (kSwiglu ? 32 : 64);
                 for (int kb = 0; kb < kbn; ++kb, ++issued) {
                     if (!ready) ready = mbar_spin(empty + s, parity);
                     if (!__all_sync(0xffffffffu, ready)) { if (lane == 0) report(a.error, 1, kb); failed = 1; going = false; break; }
@@ -139,32 +144,34 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                         if (rank == 0) mbar_expect_tx(full + s, 2 * kPairStage);
                         const uint32_t bar = full0 + s * 8;
                         tma_load_2d_pair(x, &map_x, bar, kb * kBK, row);
-                        if (kSwiglu) {                     // gate and up of two groups' 32 features each
 #pragma unroll
-                            for (int g = 0; g < 2; ++g) {
-                                tma_load_2d_pair(w + 64 * g * kBK, &map_w0, bar, kb * kBK, feat + 32 * g);
-                                tma_load_2d_pair(w + (64 * g + 32) * kBK, &map_w1, bar, kb * kBK, feat + 32 * g);
+                        for (int h = 0; h < 2; ++h) {      // the features of this CTA in either half of the columns
+                            if (kSwiglu) {
+                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, kb * kBK, feat + 64 * h);
+                                tma_load_2d_pair(w + (64 * h + 32) * kBK, &map_w1, bar, kb * kBK, feat + 64 * h);
+                            } else {
+                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, kb * kBK, feat + 128 * h);
                             }
-                        } else {
-                            tma_load_2d_pair(w, &map_w0, bar, kb * kBK, feat);
                         }
                     }
                     s = s1; parity = parity1;
                 }
             }
         } else if (warp != 2 && rank == 0) {
-            // Two warps issue the products, block by block in turn: what a warp has to do for a block besides (two barriers, a fence,
-            // descriptors, the commit) takes it some 400 cycles, longer than the block's products run.
-            constexpr uint32_t idesc = f8_idesc(256, kAccCols);
+            // Two warps issue the products, one for either half of the columns: what a warp has to do for a block besides (two barriers,
+            // a fence, descriptors, the commit) takes it some 400 cycles.
+            const int half = warp >> 1;
+            constexpr uint32_t idesc = f8_idesc(256, kHalf);
             const uint64_t desc0 = umma_desc(base);
+            int s = 0, parity = 0;
 #pragma unroll 1
-            for (int n = warp >> 1, s = n, parity = 0, room = 1; n < total; n += 2) {
-                const int acc = n & 1;
+            for (int n = 0; n < total; ++n) {
+                const int acc = (n & 1) * 2 + half;
                 bool fine = mbar_spin(full + s, parity);
-                if (n >= kAccs) fine = mbar_spin(acc_empty + acc, room) && fine;
+                if (n >= 2) fine = mbar_spin(acc_empty + acc, ((n >> 1) - 1) & 1) && fine;
                 if (!__all_sync(0xffffffffu, fine)) { if (lane == 0) report(a.error, 2, n); failed = 1; break; }
-                const uint64_t xdesc = desc0 + (uint64_t)(s * (kPairStage >> 4)), wdesc = xdesc + (128 * kBK >> 4);
-                const uint32_t d = tmem + acc * kAccCols;
+                const uint64_t xdesc = desc0 + (uint64_t)(s * (kPairStage >> 4)), wdesc = xdesc + ((128 + 64 * half) * kBK >> 4);
+                const uint32_t d = tmem + (n & 1) * kCols + half * kHalf;
                 fence_after_sync();
                 if (elect_one()) {
 #pragma unroll
@@ -172,9 +179,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     umma_commit_pair(acc_full + acc);
                 }
                 __syncwarp();
-                room ^= 1;
-                s += 2;
-                if (s >= kPairStages) { s -= kPairStages; parity ^= 1; }
+                if (++s == kPairStages) { s = 0; parity ^= 1; }
             }
         } else if (warp == 2) {
             // Watches the accumulators: hands the block's stage back to the producer of its CTA and wakes the warps that add, by a
@@ -183,17 +188,20 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             // the accumulators ahead of them.)  After a wait that gave up it meets them at that barrier instead, block by block, until
             // their loops have ended by count.
             bool fine = true;
-            for (int n = 0, s = 0, acc = 0, parity = 0; n < total; ++n) {
-                if (fine) {
-                    fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, parity));
-                    if (!fine) { if (lane == 0) report(a.error, 4, n); failed = 1; }
+            for (int n = 0, s = 0; n < total; ++n) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int acc = (n & 1) * 2 + half;
+                    if (fine) {
+                        fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, (n >> 1) & 1));
+                        if (!fine) { if (lane == 0) report(a.error, 4, n); failed = 1; }
+                    }
+                    fence_after_sync();
+                    fence_before_sync();
+                    if (fine) wake<kHalfAdders + 32>(kWakeAdders + acc); else sleep_until_woken<kHalfAdders + 32>(kWakeAdders + acc);
+                    if (lane == 0) mbar_arrive(empty + s);
                 }
-                fence_after_sync();
-                fence_before_sync();
-                if (fine) wake<kAdders + 32>(kWakeAdders + acc); else sleep_until_woken<kAdders + 32>(kWakeAdders + acc);
-                if (lane == 0) mbar_arrive(empty + s);
                 s = s + 1 == kPairStages ? 0 : s + 1;
-                if (++acc == kAccs) { acc = 0; parity ^= 1; }
             }
         }
         __syncwarp();
@@ -201,7 +209,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
         asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         const int group = (warp - 4) >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane;
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * 64;
-        const uint32_t release0 = peer_addr(smem_u32(acc_empty), 0);
+        const uint32_t release0 = peer_addr(smem_u32(acc_empty + (group >> 1)), 0);
         int n = 0;                                         // blocks so far
         // A block's scales are asked for two blocks ahead, into one of two sets of registers
         struct Scales { float x, w, u; };
@@ -231,16 +239,16 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             auto block = [&](Scales& f, bool more) {
                 const float s = join(f.x, f.w), v = kSwiglu ? join(f.x, f.u) : s;
                 if (more) fetch(f);
-                const uint32_t col = from + (n & 1) * kAccCols;
+                const uint32_t col = from + (n & 1) * kCols;
                 uint32_t d[32];
-                sleep_until_woken<kAdders + 32>(kWakeAdders + (n & 1));
+                sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
                 fence_after_sync();
                 tmem_ld32(col, d);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
                 tmem_ld32(col + 32, d);
                 fence_before_sync();
-                mbar_arrive_at_if(release0 + (n & 1) * 8, lane == 0);
+                mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
                 ++n;
