@@ -16,7 +16,7 @@
 //   warps 2-9 two warpgroups: read a block's accumulator, multiply and add; for swiglu one holds the gate, one the up
 //             features, otherwise each half of the columns
 // Two ways round:
-//   few rows (up to 64, kSwap): 128 features are the M side of the instruction, the rows, padded to 16, 32 or 64, its N side:
+//   few rows (kSwap): 128 features are the M side of the instruction, up to 64 rows, padded to 16, 32 or 64, its N side:
 //             bound by reading W once.  A thread is a feature; the scales of the rows lie ready in shared memory.
 //   tiles     128 rows are the M side, 128 features (swiglu: 256) the N side.  A thread is a row.
 // K split: where there are few tiles, up to 8 CTAs of a cluster take a range of blocks each and the sums meet in distributed
@@ -490,19 +490,23 @@ int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
     if (split > blocks) split = blocks;
     if (split > kMaxSplit) return kBadSize;
     form &= 255;
-    if (form == kRows || (form == kAuto && a.M <= 64)) {
-        if (a.M > 64) return kTooLarge;
-        a.split = split ? split : default_split(tiles_n, blocks, sms, !kSwiglu && a.M <= 32 ? 2 : 1, kSwiglu ? 4 : 2);
+    // Few rows, in tiles of 64 where there are more: as long as all of a product's tiles are at work at once.  us against tiles of 128
+    // rows and pairs: 1,024 x 2,048 128 rows (16 tiles) 5.0 / 7.7 / 13, 512 rows (64) 7.9 / 9.6 / 13; 1,280 x 3,072 512 rows (80) 12.0 /
+    // 12.8 / 16; 3,072 x 12,288 128 rows (48) 19.2 / 20.5 / 49, 256 rows (96) 34 / 33 / 49; gate|up 3,072 x 1,280 128 rows (48) 9.2 / 13.2
+    // / 10.2, 256 rows (96) 9.9 / 13.8 / 10.2; 12,288 x 3,072 128 rows (192) 36 / 28 / 32.
+    const long rows_tiles = (a.M + 63L) / 64 * tiles_n;
+    const bool few = a.M <= 64 || (kSwiglu ? rows_tiles <= sms : rows_tiles <= sms / 2 || (rows_tiles <= sms && blocks < 48));
+    if (form == kRows || (form == kAuto && few)) {
+        a.split = split ? split : default_split(rows_tiles, blocks, sms, !kSwiglu && a.M <= 32 ? 2 : 1, kSwiglu ? 4 : 2);
         const int rc = a.M <= 16 ? launch<true, 16, kSwiglu>(o, a, sms, s) : a.M <= 32 ? launch<true, 32, kSwiglu>(o, a, sms, s)
                                                                                      : launch<true, 64, kSwiglu>(o, a, sms, s);
         if (rc != kTooLarge || form != kAuto) return rc;   // a K whose table of scales does not fit goes in tiles
     }
     // Pairs, us against tiles of 128 rows: 3,072 x 12,288 256 rows (48 tiles) 47 / 33, 512 rows (96) 49 / 65; 1,280 x 3,072 512 rows (40)
     // 16 / 13, 1,024 rows (80) 16.6 / 17.0, 2,048 rows (160) 18 / 34; 1,024 x 2,048 1,024 rows (64) 14 / 11, 2,048 rows (128) 13.8 / 13.3;
-    // 1,003 x 1,431 2,048 rows (128) 14 / 12; gate|up 12,288 x 3,072 65 rows 32 / 25, 128 rows 33 / 29, 203 rows 33 / 50; 3,072 x 1,280
-    // 65 rows 10.5 / 9.8, 128 rows 10.8 / 12.5.
+    // 1,003 x 1,431 2,048 rows (128) 14 / 12; gate|up 12,288 x 3,072 65 rows 32 / 25, 128 rows 32 / 28, 203 rows 32 / 48.
     const long tiles = (a.M + 127L) / 128 * tiles_n;
-    if (form == kPair || (form == kAuto && (kSwiglu ? a.M > 96 : tiles > sms || (tiles > sms / 2 && blocks >= 24)))) {
+    if (form == kPair || (form == kAuto && (kSwiglu ? a.M > 128 : tiles > sms || (tiles > sms / 2 && blocks >= 24)))) {
         if constexpr (kSwiglu) return launch_pair<true, false>(o, a, sms, s);
         else {
             const int size = a.out_f32 ? 4 : 2;

@@ -2626,7 +2626,8 @@ def stream_pair_rows(x: torch.Tensor, x0: torch.Tensor) -> torch.Tensor:
 # --------------------------------------------------------------------------- 8-bit floating point
 # e4m3 values with a float32 scale per block of 128: max(max |v| / 448, 2^-126); a value is v / scale, rounded once.
 _FP8 = torch.float8_e4m3fn
-# which form of the products' kernel runs: "auto" (by the sizes), or "rows" (up to 64 rows), "tiles", "pair" for all of them
+# which form of the products' kernel runs: "auto" (by the sizes), or "rows" (tiles of up to 64 rows), "tiles" (of 128), "pair" (of
+# 256, two CTAs each) for all of them
 FP8_FORM = "auto"
 _FP8_FORMS = {"auto": 0, "rows": 1, "tiles": 2, "pair": 3}
 
@@ -2667,8 +2668,10 @@ def _fp8_empty(rows: int, width: int, scale_rows: int, device, side_by_side: boo
 
 
 def _rows_of(t: torch.Tensor, name: str) -> int:
-    """Row stride of a [rows, width] matrix with unit column stride."""
+    """Row stride of a [rows, width] matrix with unit column stride, on the device whose stream is launched on."""
     _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{name} must be a [rows, width] matrix with unit column stride")
+    _need(t.device.index == torch._C._cuda_getDevice(), f"{name} must be on the current device")
+    _need(max(t.shape) < 1 << 31, f"{name}: more rows or columns than 32 bits count")
     return t.stride(0)
 
 
@@ -2682,6 +2685,8 @@ def _fp8_operand(t, name: str, cls, block_rows: int, device=None):
     _need(v.dim() == 2 and v.shape[1] > 0 and s.shape == (-(-v.shape[0] // block_rows), (v.shape[1] + 127) >> 7),
           f"{name}: values [rows, width] and one scale for each {'row' if block_rows == 1 else '128 rows'} and 128 columns")
     _need(v.device == s.device and (device is None or v.device == device), f"{name}: values, scales and operands must be on one device")
+    _need(v.device.index == torch._C._cuda_getDevice(), f"{name} must be on the current device")
+    _need(max(v.shape) < 1 << 31, f"{name}: more rows or columns than 32 bits count")
     pitch = v.stride(0) if v.shape[0] > 1 else (v.shape[1] + 15) & -16
     _need((v.stride(1) == 1 or v.shape[1] == 1) and pitch % 16 == 0 and pitch >= v.shape[1] and v.data_ptr() % 16 == 0,
           f"{name}: rows of values must lie at multiples of 16 bytes, on a 16-byte boundary (the quantising operators lay them out so)")

@@ -12,7 +12,7 @@ def K():
     return kernels
 
 
-@pytest.fixture(params=["auto", "tiles", "pair"])
+@pytest.fixture(params=["auto", "rows", "tiles", "pair"])
 def form(request):
     """The form of the kernel that runs, whatever the rule would choose."""
     k = K()
@@ -84,6 +84,8 @@ def test_swiglu(m, n, k, form):
 # a K whose scales do not fit beside the ring, long sums, prompts
 @pytest.mark.parametrize("m,n,k", [(64, 70000, 3000), (64, 256, 70000), (16, 128, 140000), (700, 640, 2500), (2100, 1300, 1100)])
 def test_large(m, n, k, form):
+    if form == "rows" and k > 60000:
+        pytest.skip("the scales of so many columns do not fit beside the ring; the rule takes another form")
     x, w = operands(m, n, k)
     check_linear(x, w)
     if n * k < 1 << 26:
