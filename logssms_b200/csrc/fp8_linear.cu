@@ -443,10 +443,13 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
 // 1,024 x 2,048: 8 tiles x 8 7.8 us, x 4 8.2; 16 tiles x 8 12.6, x 4 8.2; 32 tiles x 4 9.4, x 2 10.1; 64 tiles x 2 11.4, x 1 13.4).
 int default_split(long tiles, int blocks, int sms, int per_sm, int left) {
     int split = 1;
-    while (split < kMaxSplit && blocks / (2 * split) >= left) {
-        const long held = per_sm > 1 ? (long)sms * per_sm : split == 1 ? sms : split == 2 ? sms * 13 / 15 : sms * 2 / 3;
-        if (2 * tiles * split > held) break;
-        split *= 2;
+    while (split < kMaxSplit) {
+        // with one CTA on an SM five follow four: three clusters of five in a GPC of 16 to 20 SMs, two of eight (down 3,072 x 12,288,
+        // 64 rows: 4 12.9, 5 12.1, 8 18.0; 1,280 x 3,072: 4 5.5, 5 5.2, 8 5.6)
+        const int next = per_sm == 1 && split == 4 ? 5 : 2 * split;
+        const long held = per_sm > 1 ? (long)sms * per_sm : split == 1 ? sms : split == 2 ? sms * 13 / 15 : sms * 5 / 6;
+        if (blocks / next < left || tiles * next > held || split == 5) break;
+        split = next;
     }
     return split;
 }
