@@ -456,65 +456,124 @@ int default_split(long tiles, int blocks, int sms, int per_sm, int left) {
 
 enum : int { kAuto = 0, kRows = 1, kTiles = 2, kPair = 3 };
 
+template <bool kSwiglu, bool kRagged, int kParts>
+struct PairLaunch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2] = {};
+    PairLaunch(int pairs, cudaStream_t s) {
+        constexpr size_t smem = pair_smem(kRagged);
+        static size_t have = 0;
+        ensure_dynamic_smem(fp8_pair_kernel<kSwiglu, kRagged, kParts>, smem, have);
+        cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = 2 * kParts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 2;
+    }
+    // (one pair for a tile: tile0 is 0)
+    int run(const CUtensorMap& map_w0, const CUtensorMap& map_w1, const CUtensorMap& map_x, Args a, int tile0, int tiles) {
+        a.tile0 = tile0; a.tiles = tiles;
+        const int rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged, kParts>, map_w0, map_w1, map_x, a);
+        return rc != 0 ? rc : launch_status();
+    }
+    // clusters that are at work at one time (a group of neighbouring SMs holds whole clusters only: 15 of eight CTAs, 33 of four)
+    static int at_once() {
+        static const int n = [] {
+            PairLaunch l(kParts, nullptr);
+            int n = 0;
+            l.cfg.attrs = l.attr + 1; l.cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel<kSwiglu, kRagged, kParts>, &l.cfg) == cudaSuccess) return n;
+            (void)cudaGetLastError();
+            return 0;
+        }();
+        return n;
+    }
+};
+
+// Tiles left over from whole rounds of all pairs (all tiles, where there are fewer) go to clusters of four or of two pairs, whichever
+// are all at work at once, and where enough of a tile's blocks are saved: behind whole rounds the second launch and the sums that
+// change places cost what 16 blocks take, on their own some 6.  us with one pair / two / four for a tile: 3,072 x 12,288 256 rows (12
+// tiles) 48.8 / 30.5 / 21.2, 512 rows (24) 48.9 / 31.2 / 41.7, 2,048 rows (22 left) 97 / 83 / 93; 2,048 x 8,192 5,000 rows (12 left)
+// 101 / 96 / 90; 1,280 x 3,072 512 rows (10) 16.4 / 12.7 / 11.8, 4,096 rows (6 left) 30.6 / 30.8 / 29.7; 1,024 x 2,048 5,000 rows (6
+// left) 24.1 / 26.0 / 25.7; 8,192 x 1,024 200 rows (32) 10.1 / 10.5 / 29.  A SwiGLU's tiles are not shared: a row's largest magnitude
+// would cross the cluster once more, and gate | up have the most tiles.
 template <bool kSwiglu, bool kRagged>
-int launch_pair(const Operands& o, const Args& a, int sms, cudaStream_t s) {
-    constexpr int feat = kSwiglu ? 128 : 256;
-    constexpr size_t smem = pair_smem(kRagged);
-    const long tiles = (long)((a.M + kPairRows - 1) / kPairRows) * ((a.N + feat - 1) / feat);
-    if (tiles > 0x3fffffffL) return kTooLarge;
-    const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+int launch_pair(const Operands& o, const Args& a, int parts, int sms, cudaStream_t s) {
+    const long all = (a.M + kPairRows - 1L) / kPairRows * ((a.N + (kSwiglu ? 127L : 255L)) / (kSwiglu ? 128 : 256));
+    if (all > 0x3fffffffL) return kTooLarge;
     CUtensorMap map_w0, map_w1, map_x;
     int rc = make_byte_map(&map_w0, o.w0, a.N, a.K, o.ldw, kSwiglu ? 32 : 64);
     if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, 32); else map_w1 = map_w0; }
     if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, 128);
     if (rc != 0) return rc;
-    static size_t have = 0;
-    ensure_dynamic_smem(fp8_pair_kernel<kSwiglu, kRagged>, smem, have);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged>, map_w0, map_w1, map_x, a);
-    return rc != 0 ? rc : launch_status();
+    const int tiles = (int)all, pairs = sms / 2, left = tiles % pairs;
+    if constexpr (!kSwiglu) {
+        typedef PairLaunch<false, kRagged, 2> Two;
+        typedef PairLaunch<false, kRagged, 4> Four;
+        const int blocks = (a.K + kBK - 1) / kBK;
+        if (left == 0) parts = 1;
+        else if (parts == 0) {
+            parts = left <= Four::at_once() ? 4 : left <= Two::at_once() ? 2 : 1;
+            if (blocks * (parts - 1) / parts < (tiles > pairs ? 16 : 6)) parts = 1;
+        }
+        if (parts > 1) {
+            if (tiles > left) rc = PairLaunch<false, kRagged, 1>(pairs, s).run(map_w0, map_w1, map_x, a, 0, tiles - left);
+            if (rc != 0) return rc;
+            return parts == 4 ? Four(left * 4, s).run(map_w0, map_w1, map_x, a, tiles - left, tiles)
+                              : Two(left * 2, s).run(map_w0, map_w1, map_x, a, tiles - left, tiles);
+        }
+    }
+    return PairLaunch<kSwiglu, kRagged, 1>(tiles < pairs ? tiles : pairs, s).run(map_w0, map_w1, map_x, a, 0, tiles);
 }
 
-// `form`: kAuto, or the form that is asked for (its low byte) with so many CTAs per tile (the next byte; 0: by the rule)
-template <bool kSwiglu>
-int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
+// Few rows, in tiles of 64 where there are more: as long as all of a product's tiles are at work at once.  us against tiles of 128
+// rows and pairs: 1,024 x 2,048 512 rows (64 tiles) 8.0 / 9.7 / 10.7, 1,024 rows (128) 10.0 / 11.4 / 11.2; 1,280 x 3,072 400 rows (70)
+// 9.1 / 12.1 / 11.7, 640 rows (100) 12.2 / 13.1 / 12.4; 4,096 x 4,096 256 rows (128) 14.7 / 15.8 / 15.6; 1,280 x 5,120 400 rows (70)
+// 11.3 / 16.3 / 13.8, 512 rows (80) 16.9 / 17.0 / 13.8; 3,072 x 12,288 128 rows (48) 19.2 / 19.1 / 21.1, 256 rows (96) 34 / 33 / 21;
+// gate|up 3,072 x 1,280 128 rows (48) 9.2 / 13.2 / 10.2, 256 rows (96) 9.9 / 13.8 / 10.2; 12,288 x 3,072 128 rows (192) 36 / 28 / 32.
+bool in_rows(long M, long tiles_n, int blocks, bool swiglu, int sms) {
+    const long tiles = (M + 63) / 64 * tiles_n;
+    return M <= 64 || (swiglu ? tiles <= sms : tiles <= sms / 2 || (tiles <= sms && blocks <= 32));
+}
+// Pairs, us against tiles of 128 rows: 3,072 x 12,288 200 rows (48 tiles) 21 / 32, 512 rows (96) 31 / 67; 1,280 x 3,072 1,024 rows
+// (80) 13.6 / 17.5, 2,048 rows (160) 18 / 34; 1,024 x 2,048 1,536 rows (96) 11.8 / 13.3; 12,288 x 3,072 128 rows (96) 18.5 / 18.3, 256
+// rows (192) 19 / 36; 1,003 x 1,431 1,536 rows (96) 12.3 / 11.6; 8,192 x 1,024 256 rows (128) 10.1 / 9.6, 400 rows (256) 11 / 18;
+// gate|up 12,288 x 3,072 65 rows 32 / 25, 128 rows 32 / 28, 203 rows 32 / 48.
+bool in_pairs(long M, long tiles_n, int blocks, bool swiglu, int sms) {
+    if (in_rows(M, tiles_n, blocks, swiglu, sms)) return false;
+    const long tiles = (M + 127) / 128 * tiles_n;
+    return swiglu ? M > 128 : tiles > sms || blocks >= 16;
+}
+int sm_count() {
     int device = 0, sms = 148;
     if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const int blocks = (a.K + kBK - 1) / kBK;
+    return sms;
+}
+
+// `form`: kAuto, or the form that is asked for (its low byte) with so many CTAs per tile (pairs: so many pairs; the next byte; 0: by the rule)
+template <bool kSwiglu>
+int launch_any(const Operands& o, Args a, int form, cudaStream_t s) {
+    const int sms = sm_count(), blocks = (a.K + kBK - 1) / kBK;
     const long tiles_n = (a.N + kFeat - 1) / kFeat;
     int split = (form >> 8) & 255;
     if (split > blocks) split = blocks;
     if (split > kMaxSplit) return kBadSize;
     form &= 255;
-    // Few rows, in tiles of 64 where there are more: as long as all of a product's tiles are at work at once.  us against tiles of 128
-    // rows and pairs: 1,024 x 2,048 128 rows (16 tiles) 5.0 / 7.7 / 13, 512 rows (64) 7.9 / 9.6 / 13; 1,280 x 3,072 512 rows (80) 12.0 /
-    // 12.8 / 16; 3,072 x 12,288 128 rows (48) 19.2 / 20.5 / 49, 256 rows (96) 34 / 33 / 49; gate|up 3,072 x 1,280 128 rows (48) 9.2 / 13.2
-    // / 10.2, 256 rows (96) 9.9 / 13.8 / 10.2; 12,288 x 3,072 128 rows (192) 36 / 28 / 32.
     const long rows_tiles = (a.M + 63L) / 64 * tiles_n;
-    const bool few = a.M <= 64 || (kSwiglu ? rows_tiles <= sms : rows_tiles <= sms / 2 || (rows_tiles <= sms && blocks < 48));
-    if (form == kRows || (form == kAuto && few)) {
+    if (form == kRows || (form == kAuto && in_rows(a.M, tiles_n, blocks, kSwiglu, sms))) {
         a.split = split ? split : default_split(rows_tiles, blocks, sms, !kSwiglu && a.M <= 32 ? 2 : 1, kSwiglu ? 4 : 2);
         const int rc = a.M <= 16 ? launch<true, 16, kSwiglu>(o, a, sms, s) : a.M <= 32 ? launch<true, 32, kSwiglu>(o, a, sms, s)
                                                                                      : launch<true, 64, kSwiglu>(o, a, sms, s);
         if (rc != kTooLarge || form != kAuto) return rc;   // a K whose table of scales does not fit goes in tiles
     }
-    // Pairs, us against tiles of 128 rows: 3,072 x 12,288 256 rows (48 tiles) 47 / 33, 512 rows (96) 49 / 65; 1,280 x 3,072 512 rows (40)
-    // 16 / 13, 1,024 rows (80) 16.6 / 17.0, 2,048 rows (160) 18 / 34; 1,024 x 2,048 1,024 rows (64) 14 / 11, 2,048 rows (128) 13.8 / 13.3;
-    // 1,003 x 1,431 2,048 rows (128) 14 / 12; gate|up 12,288 x 3,072 65 rows 32 / 25, 128 rows 32 / 28, 203 rows 32 / 48.
     const long tiles = (a.M + 127L) / 128 * tiles_n;
-    if (form == kPair || (form == kAuto && (kSwiglu ? a.M > 128 : tiles > sms || (tiles > sms / 2 && blocks >= 24)))) {
-        if constexpr (kSwiglu) return launch_pair<true, false>(o, a, sms, s);
+    if (form == kPair || (form == kAuto && in_pairs(a.M, tiles_n, blocks, kSwiglu, sms))) {
+        if constexpr (kSwiglu) return launch_pair<true, false>(o, a, 1, sms, s);
         else {
-            const int size = a.out_f32 ? 4 : 2;
+            const int size = a.out_f32 ? 4 : 2, parts = split;
             const bool ragged = ((uintptr_t)a.out & 31) != 0 || a.ldo * size % 32 != 0 || a.N * (long)size % 32 != 0;
-            return ragged ? launch_pair<false, true>(o, a, sms, s) : launch_pair<false, false>(o, a, sms, s);
+            return ragged ? launch_pair<false, true>(o, a, parts, sms, s) : launch_pair<false, false>(o, a, parts, sms, s);
         }
     }
     a.split = split ? split : default_split(tiles, blocks, sms, 1, 2);

@@ -20,6 +20,7 @@ struct Args {
     int early;                                            // W may be read before the kernels in front have ended
     int out_f32;
     float out_scale, act_scale;
+    int tile0, tiles;                                      // pairs: the tiles of this launch are tile0 up to here
     int* error;
 };
 

@@ -12,10 +12,13 @@
 //               block.  Warps 0-3 give up registers for that.
 // What bounds it: the adding (256 cycles of multiply-adds and two waits for tensor memory per block), the products (512 cycles) and
 // the hand-over of an accumulator between them lie within a quarter of each other; left out one at a time, down 8,192 x 3,072 x 12,288
-// takes 264 us without the multiply-adds, 277 with a quarter of the products, 285 without loads, 314 with all (1.97 PFLOP/s; 356 us in
-// a long row of calls on random data, when the power limit sets the clock).
+// takes 264 us without the multiply-adds, 277 with a quarter of the products, 285 without loads, 314 with all (1.97 PFLOP/s; 353 us in
+// a long row of calls on random data, when the power limit sets the clock, 329 with the last round's tiles shared).
 // SwiGLU: the features are laid out so that a thread has gate and up of the same 32 features; only a row's largest magnitude is
 // exchanged between the four warpgroups.
+//
+// Fewer tiles than pairs, and those left over from whole rounds: a cluster of two or four pairs shares a tile's blocks (kParts; see
+// `launch_pair` for what it brings).
 //
 // Every wait on an mbarrier is bounded; one that gives up records itself in `error`, the roles run out of their own bounded
 // waits, both CTAs still meet the last cluster barrier, tensor memory is freed and the kernel returns.
@@ -44,9 +47,9 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t adesc, ui
                  ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 // the barrier of both CTAs gets one arrival when every product issued by this thread so far has completed
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar, int ctas) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
+                 ::"r"(smem_u32(bar)), "h"((unsigned short)ctas) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
     // (not a release at cluster scope, which waits for every load of the thread that is under way: 1,900 cycles a block.  What is
@@ -85,11 +88,16 @@ __device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
 }
 
 // kRagged: rows of `out` that do not lie on 32 bytes, or features that do not fill 32 bytes
-template <bool kSwiglu, bool kRagged>
+// kParts > 1: a cluster of so many pairs shares the blocks of a tile; for tiles that do not fill a round of all pairs.  Once every
+// pair's ring is empty, each thread hands the other pairs their share of its 64 sums, over the ring, and finishes its own share: the
+// sums of all pairs are added in the order of their blocks.
+template <bool kSwiglu, bool kRagged, int kParts>
 __global__ void __launch_bounds__(kPairThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constant__ CUtensorMap map_w1,
                 const __grid_constant__ CUtensorMap map_x, Args a) {
     constexpr int kFeat = kSwiglu ? 128 : 256;            // output features of a tile
+    constexpr int kMine = 64 / kParts;                    // columns that a thread finishes
+    static_assert(!kSwiglu || kParts == 1, "a row's largest magnitude is taken in one CTA");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(16) uint64_t acc_full[4], acc_empty[4], full[kPairStages], empty[kPairStages];
@@ -97,10 +105,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)cluster_rank();
-    const int tiles_m = (a.M + kPairRows - 1) / kPairRows, tiles_n = (a.N + kFeat - 1) / kFeat, tiles = tiles_m * tiles_n;
+    const int in_cluster = (int)cluster_rank(), rank = kParts > 1 ? in_cluster & 1 : in_cluster;
+    const int leader = kParts > 1 ? in_cluster & ~1 : 0, part = kParts > 1 ? in_cluster >> 1 : 0;
+    const int tiles_m = (a.M + kPairRows - 1) / kPairRows, tiles_n = (a.N + kFeat - 1) / kFeat;
     const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
-    const int kbn = (a.K + kBK - 1) / kBK;
+    // this pair's tiles, and the blocks of K that it takes of each
+    const int first = kParts > 1 ? a.tile0 + pair / kParts : pair, end = kParts > 1 ? first + 1 : a.tiles;
+    const int all = (a.K + kBK - 1) / kBK;
+    const int kb0 = kParts > 1 ? all * part / kParts : 0, kbn = kParts > 1 ? all * (part + 1) / kParts - kb0 : all;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 2); }
         for (int s = 0; s < 4; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, 2 * kHalfAdders / 32); }
@@ -120,8 +132,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
     pdl_trigger();
     pdl_wait();
     int issued = 0;
-    const int total = ((tiles - pair + pairs - 1) / pairs) * kbn;             // blocks of all tiles of this pair
-    const uint32_t full0 = peer_addr(smem_u32(full), 0);
+    const int total = (kParts > 1 ? 1 : (end - first + pairs - 1) / pairs) * kbn;       // blocks of all tiles of this pair
+    const uint32_t full0 = peer_addr(smem_u32(full), leader);
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");              // 640 threads x 96 registers at launch: 128 x 32 + 512 x 112
         // (whole warps: see elect_one; the next block's barrier is asked for before the current block is worked on, since a wait
@@ -129,7 +141,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
         if (warp == 0) {
             int s = 0, parity = 1;
             bool ready = true, going = true;
-            for (int t = pair; t < tiles && going; t += pairs) {
+            for (int t = first; t < end && going; t += pairs) {
                 const Tile at = tile_at(t, tiles_m, tiles_n);
                 const int row = at.m * kPairRows + rank * 128;
                 const int feat = at.n * kFeat + rank * (kSwiglu ? 32 : 64);
@@ -143,14 +155,15 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                         uint8_t* w = x + 128 * kBK;
                         if (rank == 0) mbar_expect_tx(full + s, 2 * kPairStage);
                         const uint32_t bar = full0 + s * 8;
-                        tma_load_2d_pair(x, &map_x, bar, kb * kBK, row);
+                        const int k = (kb0 + kb) * kBK;
+                        tma_load_2d_pair(x, &map_x, bar, k, row);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {      // the features of this CTA in either half of the columns
                             if (kSwiglu) {
-                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, kb * kBK, feat + 64 * h);
-                                tma_load_2d_pair(w + (64 * h + 32) * kBK, &map_w1, bar, kb * kBK, feat + 64 * h);
+                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, k, feat + 64 * h);
+                                tma_load_2d_pair(w + (64 * h + 32) * kBK, &map_w1, bar, k, feat + 64 * h);
                             } else {
-                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, kb * kBK, feat + 128 * h);
+                                tma_load_2d_pair(w + 64 * h * kBK, &map_w0, bar, k, feat + 128 * h);
                             }
                         }
                     }
@@ -176,7 +189,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kBK / 32; ++k) umma_f8_pair(d, xdesc + 2 * k, wdesc + 2 * k, idesc, k != 0);
-                    umma_commit_pair(acc_full + acc);
+                    umma_commit_pair(acc_full + acc, 3 << leader);
                 }
                 __syncwarp();
                 if (++s == kPairStages) { s = 0; parity ^= 1; }
@@ -205,11 +218,12 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             }
         }
         __syncwarp();
+        if constexpr (kParts > 1) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }      // as the warps that add
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         const int group = (warp - 4) >> 2, quarter = warp & 3, in_tile = quarter * 32 + lane;
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + group * 64;
-        const uint32_t release0 = peer_addr(smem_u32(acc_empty + (group >> 1)), 0);
+        const uint32_t release0 = peer_addr(smem_u32(acc_empty + (group >> 1)), leader);
         int n = 0;                                         // blocks so far
         // A block's scales are asked for two blocks ahead, into one of two sets of registers
         struct Scales { float x, w, u; };
@@ -224,14 +238,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
         };
         auto open = [&](int t) {                           // the scales' places of a tile, and its first two blocks' on their way
             const Tile at = tile_at(t, tiles_m, tiles_n);
-            sx = a.sx + (long)min(at.m * kPairRows + rank * 128 + in_tile, a.M - 1) * a.sx_row;
-            sw = a.sw0 + (kSwiglu ? at.n : min(2 * at.n + (group >> 1), (a.N - 1) / kBK)) * a.sw_row;
-            if (kSwiglu) su = a.sw1 + at.n * a.sw_row;
+            sx = a.sx + (long)min(at.m * kPairRows + rank * 128 + in_tile, a.M - 1) * a.sx_row + kb0 * a.sx_block;
+            sw = a.sw0 + (kSwiglu ? at.n : min(2 * at.n + (group >> 1), (a.N - 1) / kBK)) * a.sw_row + kb0 * a.sw_block;
+            if (kSwiglu) su = a.sw1 + at.n * a.sw_row + kb0 * a.sw_block;
             fetch(even);
             if (kbn > 1) fetch(odd);
         };
-        open(pair);
-        for (int t = pair; t < tiles; t += pairs) {
+        open(first);
+        for (int t = first; t < end; t += pairs) {
             float sum[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) sum[j] = 0.f;
@@ -258,7 +272,32 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 block(even, kb + 2 < kbn);
                 if (kb + 1 < kbn) block(odd, kb + 3 < kbn);
             }
-            if (t + pairs < tiles) open(t + pairs);
+            if (t + pairs < end) open(t + pairs);
+            if constexpr (kParts > 1) {
+                cluster_arrive();                          // everybody's products are done
+                cluster_wait();
+                const uint32_t mine = smem_u32(base) + (threadIdx.x - 128) * 16;
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const uint32_t to = peer_addr(mine, 2 * p + rank) + part * (kMine / 4 * kAdders * 16);
+#pragma unroll
+                    for (int j = 0; j < kMine; j += 4)
+                        store_peer4(to + j * (kAdders * 4), sum[p * kMine + j], sum[p * kMine + j + 1], sum[p * kMine + j + 2], sum[p * kMine + j + 3]);
+                }
+                cluster_arrive();                          // everybody's sums are here
+                cluster_wait();
+#pragma unroll
+                for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
+#pragma unroll
+                for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                    for (int j = 0; j < kMine; j += 4) {
+                        float v[4];
+                        load_shared4(mine + (p * kMine + j) * (kAdders * 4), v);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum[j + e] += v[e];
+                    }
+            }
             const Tile at = tile_at(t, tiles_m, tiles_n);
             const long m = (long)at.m * kPairRows + rank * 128 + in_tile;
             if constexpr (kSwiglu) {
@@ -289,14 +328,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     if (group == 0) a.qs[m * a.qs_row + at.n * a.qs_block] = scale;
                 }
             } else {
-                const int n0 = at.n * kFeat + group * 64, live = a.N - n0;
+                const int n0 = at.n * kFeat + group * 64 + (kParts > 1 ? part * kMine : 0), live = a.N - n0;
                 if (a.bias != nullptr) {
                     const float* bias = a.bias + n0;
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) sum[j] += bias[min(j, live - 1)];
+                    for (int j = 0; j < kMine; ++j) sum[j] += bias[min(j, live - 1)];
                 }
 #pragma unroll
-                for (int j = 0; j < 64; ++j) sum[j] *= a.out_scale;
+                for (int j = 0; j < kMine; ++j) sum[j] *= a.out_scale;
                 const int size = a.out_f32 ? 4 : 2;
                 uint8_t* out = (uint8_t*)a.out + ((size_t)m * a.ldo + n0) * size;
                 if constexpr (!kRagged) {
@@ -304,7 +343,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     if (m < a.M) {
                         if (a.out_f32) {
 #pragma unroll
-                            for (int j = 0; j < 64; j += 8) {
+                            for (int j = 0; j < kMine; j += 8) {
                                 uint32_t w[8];
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(sum[j + e]);
@@ -312,7 +351,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                             }
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 64; j += 16) {
+                            for (int j = 0; j < kMine; j += 16) {
                                 uint32_t w[8];
                                 __nv_bfloat162* b = reinterpret_cast<__nv_bfloat162*>(w);
 #pragma unroll
@@ -327,7 +366,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     float* turn = reinterpret_cast<float*>(base + (size_t)kPairStages * kPairStage) + (warp - 4) * 512;
                     const int j = lane & 15, first = lane >> 4, rows = (int)min(32L, a.M - (m - lane));
 #pragma unroll
-                    for (int c = 0; c < 64; c += 16) {
+                    for (int c = 0; c < kMine; c += 16) {
                         __syncwarp();
 #pragma unroll
                         for (int e = 0; e < 16; ++e) turn[lane * 16 + (e ^ j)] = sum[c + e];

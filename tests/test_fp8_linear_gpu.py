@@ -113,6 +113,27 @@ def test_every_split(m, split):
         del k._FP8_FORMS["split"]
 
 
+@pytest.mark.parametrize("parts", [2, 4])
+@pytest.mark.parametrize("m,n,k", [(1, 256, 128), (300, 200, 100), (129, 257, 128 * 3), (256, 256, 128 * 4 + 5), (700, 640, 128 * 33),
+                                   (257, 1003, 5001), (513, 130, 128 * 60), (4900, 1000, 128 * 9), (18900, 64, 1100)])
+def test_pairs_share_a_tile(m, n, k, parts):
+    """A tile's blocks over so many pairs: fewer blocks than pairs, uneven ranges, rings that go round, whole rounds of tiles in
+    front, ragged rows and features."""
+    kk = K()
+    kk._FP8_FORMS["parts"] = 3 + 256 * parts
+    kk.FP8_FORM = "parts"
+    try:
+        x, w = operands(m, n, k, seed=m % 2)
+        check_linear(x, w)
+        check_linear(x, w, torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda(), 0.7)
+        first = kk.linear_fp8(x, w, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(kk.linear_fp8(x, w, out_dtype=torch.float32), first)
+    finally:
+        kk.FP8_FORM = "auto"
+        del kk._FP8_FORMS["parts"]
+
+
 def test_every_block_has_its_own_scales(form):
     """Blocks of very different size: a scale that met a neighbour's block would be off by its factor."""
     k = K()
