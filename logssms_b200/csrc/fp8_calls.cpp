@@ -52,8 +52,13 @@ bool operand(Fp8& f, PyObject* values, PyObject* scales, int block_rows, int dev
     f.pitch = rows > 1 ? f.v->stride(0) : (width + 15) / 16 * 16;
     return f.pitch % 16 == 0 && f.pitch >= width && ((uintptr_t)f.v->data_ptr() & 15) == 0 && fits(rows) && fits(width);
 }
+// whole rows of the pitch, the last one too: kernels write what fills up a row
 at::Tensor values_for(int64_t rows, int64_t width, at::Device device) {
-    return at::detail::empty_strided_cuda({rows, width}, {(width + 15) / 16 * 16, 1}, at::kFloat8_e4m3fn, device);
+    const int64_t pitch = (width + 15) / 16 * 16;
+    at::Tensor t = at::detail::empty_strided_cuda({rows, pitch}, {pitch, 1}, at::kFloat8_e4m3fn, device);
+    const int64_t sizes[2] = {rows, width}, strides[2] = {pitch, 1};
+    if (pitch != width) t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes), at::IntArrayRef(strides));
+    return t;
 }
 at::Tensor scales_for(int64_t rows, int64_t width, at::Device device, bool side_by_side) {
     const int64_t blocks = (width + 127) / 128;

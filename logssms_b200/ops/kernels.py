@@ -2660,10 +2660,11 @@ def _fp8_done(got, name: str):
 
 
 def _fp8_empty(rows: int, width: int, scale_rows: int, device, side_by_side: bool):
-    """(values, scales) to be written: rows at multiples of 16 bytes, the scales of a column block side by side or row by row."""
+    """(values, scales) to be written: rows at multiples of 16 bytes, the last one with what fills it up (kernels write it), the
+    scales of a column block side by side or row by row."""
     pitch = (width + 15) & -16
     blocks = (width + 127) >> 7
-    return (torch.empty_strided((rows, width), (pitch, 1), dtype=_FP8, device=device),
+    return (torch.empty((rows, pitch), dtype=_FP8, device=device)[:, :width],
             torch.empty_strided((scale_rows, blocks), (1, scale_rows) if side_by_side else (blocks, 1), dtype=torch.float32, device=device))
 
 
