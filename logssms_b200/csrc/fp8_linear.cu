@@ -67,7 +67,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
     __shared__ uint32_t tmem_slot;
-    __shared__ volatile int failed;
+    __shared__ volatile int failed, lifted;               // lifted: some of this CTA's pairs of scales have no normal product
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = a.split, rank = split > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / split, tile_m = tile / a.tiles_n, tile_n = tile - tile_m * a.tiles_n;
@@ -94,7 +94,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
         for (int s = 0; s < kAccs; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, kSumThreads / 32); }
-        failed = 0;
+        failed = lifted = 0;
         mbar_fence_init();
         if (a.early) for (int i = 0; i < first; ++i) load_w(i, i);     // its own barriers are ready
     }
@@ -189,70 +189,96 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
                     const int i = min(i0 + q * kEvery, kbn - 1);           // (the last one may be written several times, alike)
-                    table[(kSwiglu ? 2 : 1) * i * NR + m] = join(x[q], w0[q]);
-                    if (kSwiglu) table[(2 * i + 1) * NR + m] = join(x[q], w1[q]);
+                    const float p0 = x[q] * w0[q], p1 = kSwiglu ? x[q] * w1[q] : 1.f;
+                    if (!plain(p0) || !plain(p1)) lifted = 1;
+                    table[(kSwiglu ? 2 : 1) * i * NR + m] = p0;
+                    if (kSwiglu) table[(2 * i + 1) * NR + m] = p1;
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
         } else if (kbn > 0) {
-            s_next = join(sx[0], sw[0]);
+            s_next = sx[0] * sw[0];
         }
-        bool fine = true;
-        int slot = 0;
-        for (int i = 0; i < kbn; ++i) {
-            const int acc = i % kAccs;
-            const float s = s_next;
-            if (!kSwap && i + 1 < kbn) s_next = join(sx[(i + 1) * a.sx_block], sw[(i + 1) * a.sw_block]);
-            // one warp asks for the accumulator, the others sleep at the barrier: eight warps that ask make every answer late
-            if (warp == 2 && fine) {
-                fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, (i / kAccs) & 1));
-                if (!fine) { if (lane == 0) report(a.error, 4, i); failed = 1; }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (threadIdx.x == 64) mbar_arrive(empty + slot);             // the block's products have read its stage
-            slot = slot + 1 == stages ? 0 : slot + 1;
-            fence_after_sync();
-            const uint32_t at = from + acc * F::kCols;
-            if constexpr (!kSwap) {
-                constexpr int kStep = kMine > 64 ? 16 : 32;        // what the registers hold beside the sums
-#pragma unroll
-                for (int c = 0; c < kMine; c += kStep) {
-                    uint32_t d[kStep];
-                    if constexpr (kStep == 32) tmem_ld32(at + c, d);
-                    else { tmem_ld16(at + c, d); tmem_ld_wait(); }
-                    if (c + kStep == kMine) {
-                        fence_before_sync();
-                        if (lane == 0) mbar_arrive(acc_empty + acc);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kStep; ++j) sum[c + j] = fmaf(__uint_as_float(d[j]), s, sum[c + j]);
+        // (a loop of its own where scales have to be lifted: in one loop the rare part costs the other one registers)
+        auto add_blocks = [&](auto lift_rows) {
+            bool fine = true;
+            int slot = 0;
+            for (int i = 0; i < kbn; ++i) {
+                const int acc = i % kAccs;
+                [[maybe_unused]] const float s = s_next;
+                if (!kSwap && i + 1 < kbn) s_next = sx[(i + 1) * a.sx_block] * sw[(i + 1) * a.sw_block];
+                // one warp asks for the accumulator, the others sleep at the barrier: eight warps that ask make every answer late
+                if (warp == 2 && fine) {
+                    fine = __all_sync(0xffffffffu, mbar_spin(acc_full + acc, (i / kAccs) & 1));
+                    if (!fine) { if (lane == 0) report(a.error, 4, i); failed = 1; }
                 }
-            } else {                                       // all columns at once: one wait for tensor memory a block
-                uint32_t d[kMine];
-                if constexpr (kMine == 8) tmem_ld8(at, d);
-                else if constexpr (kMine == 16) tmem_ld16(at, d);
-                else if constexpr (kMine == 32) tmem_ld32_async(at, d);
-                else tmem_ld64(at, d);
-                // the rows' scales, where there are registers for them while the columns are on their way
-                const uint32_t tab = table_at + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine) * 4;
-                constexpr int kAhead = kMine <= 16 ? kMine : F::kTwoPerSm ? 8 : kMine == 32 ? 32 : 16;
-                float f[kAhead];
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (threadIdx.x == 64) mbar_arrive(empty + slot);             // the block's products have read its stage
+                slot = slot + 1 == stages ? 0 : slot + 1;
+                fence_after_sync();
+                const uint32_t at = from + acc * F::kCols;
+                if constexpr (!kSwap) {
+                    constexpr int kStep = kMine > 64 ? 16 : 32;        // what the registers hold beside the sums
+                    auto add = [&](float times, auto plain_scales) {
+                        [[maybe_unused]] const float lift = plain_scales.value ? 1.f : lift_of(sx[i * a.sx_block], sw[i * a.sw_block]);
 #pragma unroll
-                for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * j, f + j);
-                tmem_ld_wait();
-                fence_before_sync();
-                if (lane == 0) mbar_arrive(acc_empty + acc);
+                        for (int c = 0; c < kMine; c += kStep) {
+                            uint32_t d[kStep];
+                            if constexpr (kStep == 32) tmem_ld32(at + c, d);
+                            else { tmem_ld16(at + c, d); tmem_ld_wait(); }
+                            if (c + kStep == kMine) {
+                                fence_before_sync();
+                                if (lane == 0) mbar_arrive(acc_empty + acc);
+                            }
 #pragma unroll
-                for (int c = 0; c < kMine; c += kAhead) {
+                            for (int j = 0; j < kStep; ++j) {
+                                const float v = plain_scales.value ? __uint_as_float(d[j]) : __uint_as_float(d[j]) * lift;
+                                sum[c + j] = fmaf(v, times, sum[c + j]);
+                            }
+                        }
+                    };
+                    if (__builtin_expect(__all_sync(0xffffffffu, plain(s)), 1)) add(s, std::true_type{});
+                    else add(join(sx[i * a.sx_block], sw[i * a.sw_block]), std::false_type{});
+                } else {                                       // all columns at once: one wait for tensor memory a block
+                    uint32_t d[kMine];
+                    if constexpr (kMine == 8) tmem_ld8(at, d);
+                    else if constexpr (kMine == 16) tmem_ld16(at, d);
+                    else if constexpr (kMine == 32) tmem_ld32_async(at, d);
+                    else tmem_ld64(at, d);
+                    // the rows' scales, where there are registers for them while the columns are on their way
+                    const uint32_t tab = table_at + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine) * 4;
+                    constexpr int kAhead = kMine <= 16 ? kMine : F::kTwoPerSm ? 8 : kMine == 32 ? 32 : 16;
+                    float f[kAhead];
 #pragma unroll
-                    for (int j = 0; j < kAhead; ++j) sum[c + j] = fmaf(__uint_as_float(d[c + j]), f[j], sum[c + j]);
-                    if (c + kAhead < kMine) {
+                    for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * j, f + j);
+                    tmem_ld_wait();
+                    fence_before_sync();
+                    if (lane == 0) mbar_arrive(acc_empty + acc);
+                    if constexpr (lift_rows.value) {           // (the table has no place for it: the scales are read once more)
+                        const int r0 = kSwiglu ? 0 : group * kMine;
+                        const volatile float* px = a.sx + (long)(m0 + min(r0, rows - 1)) * a.sx_row + (kb0 + i) * a.sx_block;
+                        const float w = sw[i * a.sw_block];
 #pragma unroll
-                        for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * (c + kAhead + j), f + j);
+                        for (int j = 0; j < kMine; ++j) {
+                            const float x = *px;
+                            sum[j] = fmaf(__uint_as_float(d[j]) * lift_of(x, w), join(x, w), sum[j]);
+                            if (r0 + j + 1 < rows) px += a.sx_row;
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < kMine; c += kAhead) {
+#pragma unroll
+                            for (int j = 0; j < kAhead; ++j) sum[c + j] = fmaf(__uint_as_float(d[c + j]), f[j], sum[c + j]);
+                            if (c + kAhead < kMine) {
+#pragma unroll
+                                for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * (c + kAhead + j), f + j);
+                            }
+                        }
                     }
                 }
             }
-        }
+        };
+        if (kSwap && __builtin_expect(lifted, 0)) add_blocks(std::true_type{}); else add_blocks(std::false_type{});
     }
     // ---- the sums meet at the rows' owners
     fence_before_sync();

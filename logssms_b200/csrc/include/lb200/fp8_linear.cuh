@@ -112,11 +112,25 @@ __device__ __forceinline__ float silu_of(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
     return v * r;
 }
-// the product of two scales, finite where both are: a zero sum stays zero
+// Two scales of a block, joined: its sums are multiplied by their product where that is `plain`, a normal number.  Beyond 2^128 or
+// below 2^-126 the product would be infinite or lose its bits, although its multiple of the block's sums (0, or 2^-18 to 2^25) may well
+// be a number: there the sums are multiplied by `lift_of` (2^64 or 2^-64) first and by `join` then.  An infinite or NaN scale stays
+// what it is; a zero sum stays zero under any two finite scales.  That part of the code is rare and stands on its own: a block of
+// zeros has the smallest scale.
+__device__ __forceinline__ bool plain(float product) { return magnitude(product) - 0x00800000u < 0x7f000000u; }
+__device__ __forceinline__ float lift_of(float a, float b) {
+    const uint32_t m = magnitude(a * b);
+    return m >= 0x7f800000u ? 1.84467441e19f : m < 0x00800000u ? 5.42101086e-20f : 1.f;      // 2^64, 2^-64
+}
 __device__ __forceinline__ float join(float a, float b) {
     float s = a * b;
-    if (magnitude(s) == 0x7f800000u) {
-        if (magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) s = copysignf(3.402823466e38f, s);
+    if (!plain(s)) {
+        if (magnitude(s) >= 0x7f800000u) {
+            s = a * 5.42101086e-20f * b;
+            if (magnitude(s) == 0x7f800000u && magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) s = copysignf(3.402823466e38f, s);
+        } else if (a != 0.f && b != 0.f) {
+            s = a * 1.84467441e19f * b;
+        }
     }
     return s;
 }

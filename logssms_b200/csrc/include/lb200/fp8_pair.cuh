@@ -24,6 +24,7 @@
 // waits, both CTAs still meet the last cluster barrier, tensor memory is freed and the kernel returns.
 #pragma once
 #include "lb200/fp8_linear.cuh"
+#include <type_traits>
 
 namespace lb200 {
 namespace fp8 {
@@ -250,22 +251,41 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
 #pragma unroll
             for (int j = 0; j < 64; ++j) sum[j] = 0.f;
             // a block's accumulator, times its scales, joins this thread's sums, 32 columns at a time
-            auto block = [&](Scales& f, bool more) {
-                const float s = join(f.x, f.w), v = kSwiglu ? join(f.x, f.u) : s;
-                if (more) fetch(f);
+            auto add = [&](Scales& f, bool more, auto plain_scales) {
                 const uint32_t col = from + (n & 1) * kCols;
                 uint32_t d[32];
-                sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
-                fence_after_sync();
-                tmem_ld32(col, d);
+                if constexpr (plain_scales.value) {
+                    const float s = f.x * f.w, v = kSwiglu ? f.x * f.u : s;
+                    if (more) fetch(f);
+                    sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
+                    fence_after_sync();
+                    tmem_ld32(col, d);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
-                tmem_ld32(col + 32, d);
-                fence_before_sync();
-                mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);
+                    for (int j = 0; j < 32; ++j) sum[j] = fmaf(__uint_as_float(d[j]), s, sum[j]);
+                    tmem_ld32(col + 32, d);
+                    fence_before_sync();
+                    mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
+                    for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
+                } else {                                   // the same, lifted; what it keeps costs the other form no registers
+                    sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
+                    fence_after_sync();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float w = kSwiglu && h ? f.u : f.w, l = lift_of(f.x, w), s = join(f.x, w);
+                        tmem_ld32(col + 32 * h, d);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[32 * h + j] = fmaf(__uint_as_float(d[j]) * l, s, sum[32 * h + j]);
+                    }
+                    fence_before_sync();
+                    mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);
+                    if (more) fetch(f);
+                }
                 ++n;
+            };
+            auto block = [&](Scales& f, bool more) {
+                if (__builtin_expect(__all_sync(0xffffffffu, plain(f.x * f.w) && (!kSwiglu || plain(f.x * f.u))), 1)) add(f, more, std::true_type{});
+                else add(f, more, std::false_type{});
             };
 #pragma unroll 1
             for (int kb = 0; kb < kbn; kb += 2) {
