@@ -383,7 +383,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 uint32_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[e] = n + e < a.N ? silu_of(v[e] * a.act_scale) * u[e] : 0.f;
+                    v[e] = n + e < a.N ? silu_of(v[e], 0.125f * a.act_scale) * u[e] : 0.f;
                     top = max(top, magnitude(v[e]));
                 }
                 const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top)), back = 1.f / scale;

@@ -105,12 +105,16 @@ __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity) {
         if (mbar_test(bar, parity)) return true;
     return false;
 }
-// v / (1 + e^-v) by the special-function unit's exponential and reciprocal: off by (|v| + 6) 2^-24 of itself at most.  The
-// accurate division and exponential made the end of a tile half as long as its products.
-__device__ __forceinline__ float silu_of(float v) {
-    float e = ex2_approx(-1.44269504f * v), r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return v * r;
+// v / (1 + e^-v) of v = sum * act_scale, by the special-function unit's exponential and reciprocal; `eighth`: act_scale / 8 (exact from
+// 2^-123 up).  Off by (1.25 |v| + 8) 2^-24 of itself at most, and by what the sum and v are: the exponent's constant and its rounding
+// (1.25 |v|), the exponential (4), the denominator (1), the reciprocal (2), the product (1).  v and the denominator are scaled by an
+// eighth, else the reciprocal would be flushed to zero from -87.3 down; from -88.7 down e^-v is infinite and the result zero, as in
+// any 32-bit form.  The accurate division and exponential made the end of a tile half as long as its products.
+__device__ __forceinline__ float silu_of(float sum, float eighth) {
+    const float v8 = sum * eighth, e = ex2_approx(-8.f * 1.44269504f * v8);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.125f, 0.125f)));
+    return v8 * r;
 }
 // Two scales of a block, joined: its sums are multiplied by their product where that is `plain`, a normal number.  Beyond 2^128 or
 // below 2^-126 the product would be infinite or lose its bits, although its multiple of the block's sums (0, or 2^-18 to 2^25) may well

@@ -325,7 +325,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 uint32_t top = 0;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    sum[j] = f0 + j < a.N ? silu_of(sum[j] * a.act_scale) * sum[32 + j] : 0.f;
+                    sum[j] = f0 + j < a.N ? silu_of(sum[j], 0.125f * a.act_scale) * sum[32 + j] : 0.f;
                     top = max(top, magnitude(sum[j]));
                 }
                 tops[group][in_tile] = top;

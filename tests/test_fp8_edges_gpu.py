@@ -1,7 +1,9 @@
-"""8-bit operators where their 32-bit numbers end: scales whose product leaves 32 bits, whatever form of the kernel runs."""
+"""8-bit operators where their 32-bit numbers end, whatever form of the kernel runs: scales whose product leaves 32 bits, SiLU far
+below zero."""
 import pytest
 import torch
 
+from fp8_util import holds
 from test_fp8_linear_gpu import check_linear, check_swiglu
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +65,52 @@ def test_scales_whose_product_leaves_32_bits(m, case, form):
     check_linear(x, w)
     check_swiglu(x, plain, w, 1.0)                         # as the up half of a gated product
     check_swiglu(x, w, plain, act_scale)                   # as the gate half
+
+
+def one_column(rows, width, columns):
+    """e4m3 rows that are zero but for the given {column: values}, on 16 bytes."""
+    held = torch.zeros(rows, (width + 15) // 16 * 16, dtype=torch.float8_e4m3fn)
+    for c, v in columns.items():
+        held[:, c] = torch.as_tensor(v, dtype=torch.float32).to(torch.float8_e4m3fn)
+    return held.cuda()[:, :width]
+
+
+@pytest.mark.parametrize("m", [3, 70, 260])
+def test_silu_far_below_zero(m, form):
+    """Gates from -80 down to -92 under up values that keep the product a number: SiLU's own size is 1e-33 to 1e-38."""
+    k = K()
+    width = 520
+    gates = torch.arange(80.0, 92.0, 0.25).float() / 448           # a scale for each 128 features
+    blocks = len(gates)
+    n = 128 * blocks
+    g = torch.Generator().manual_seed(m)
+    x = k.Fp8Rows(one_column(m, width, {0: 1.0}), torch.ones(m, 5).cuda())
+    gate = k.Fp8Weight(one_column(n, width, {0: -448.0}), gates.cuda()[:, None].repeat(1, 5))
+    ups = torch.randint(1, 0x7F, (n,), generator=g).to(torch.uint8).view(torch.float8_e4m3fn).float()
+    up = k.Fp8Weight(one_column(n, width, {0: ups}), torch.full((blocks, 5), 1e30).cuda())
+    a = (-448 * gates.double()).repeat_interleave(128)
+    h = (a * torch.sigmoid(a) * ups.double() * float(torch.tensor(1e30))).cuda().expand(m, n)
+    # the exponent's constant and its rounding: 1.25 |a|; exponential 4, denominator 1, reciprocal 2, products 5, all 2^-24 of h.
+    # Where e^-a is beyond 32 bits (a below -88.7) the denominator is infinite, as in any 32-bit form of it, and SiLU 0.
+    error = h.abs() * torch.where(a < -88.7, 1.0, (1.25 * a.abs() + 12) * 2.0 ** -24).cuda()
+    got = k.linear_swiglu_fp8(x, gate, up)
+    holds(got.values, got.scales, h, error)
+    assert bool((got.scales[:, :32] > 2.0 ** -126).all())          # gates down to -87.75: nothing is lost
+    k.check_kernel_errors()
+
+
+@pytest.mark.parametrize("m", [3, 70, 260])
+def test_silu_of_large_gates(m, form):
+    """Gates up to the largest numbers are their own SiLU, down to the largest negative ones nothing is left of them."""
+    k = K()
+    width = 520
+    sizes = torch.tensor([1e2, 1e10, 1e30, 1e36, 3e38])
+    n = 128 * len(sizes)
+    sign = torch.where(torch.arange(n) % 2 == 0, 1.0, -1.0)
+    x = k.Fp8Rows(one_column(m, width, {0: 1.0}), torch.ones(m, 5).cuda())
+    gate = k.Fp8Weight(one_column(n, width, {0: 64 * sign}), (sizes / 64).cuda()[:, None].repeat(1, 5))
+    up = k.Fp8Weight(one_column(n, width, {0: torch.full((n,), 0.5)}), torch.full((len(sizes), 5), 0.25).cuda())
+    h = torch.where(sign > 0, (64.0 * (sizes / 64)).double().repeat_interleave(128) / 8, 0.0).cuda().expand(m, n)
+    got = k.linear_swiglu_fp8(x, gate, up)
+    holds(got.values, got.scales, h, h * 2.0 ** -22)
+    k.check_kernel_errors()
