@@ -67,7 +67,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[kAccs], acc_empty[kAccs];
     __shared__ uint32_t tmem_slot;
-    __shared__ volatile int failed, lifted;               // lifted: some of this CTA's pairs of scales have no normal product
+    __shared__ volatile int failed, odd;                  // odd: some of this CTA's pairs of scales have no normal product
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = a.split, rank = split > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / split, tile_m = tile / a.tiles_n, tile_n = tile - tile_m * a.tiles_n;
@@ -94,7 +94,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
         for (int s = 0; s < kAccs; ++s) { mbar_init(acc_full + s, 1); mbar_init(acc_empty + s, kSumThreads / 32); }
-        failed = lifted = 0;
+        failed = odd = 0;
         mbar_fence_init();
         if (a.early) for (int i = 0; i < first; ++i) load_w(i, i);     // its own barriers are ready
     }
@@ -189,18 +189,18 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
                     const int i = min(i0 + q * kEvery, kbn - 1);           // (the last one may be written several times, alike)
-                    const float p0 = x[q] * w0[q], p1 = kSwiglu ? x[q] * w1[q] : 1.f;
-                    if (!plain(p0) || !plain(p1)) lifted = 1;
-                    table[(kSwiglu ? 2 : 1) * i * NR + m] = p0;
-                    if (kSwiglu) table[(2 * i + 1) * NR + m] = p1;
+                    const float v0 = x[q] * w0[q], v1 = kSwiglu ? x[q] * w1[q] : 1.f;
+                    if (!plain(v0) || !plain(v1)) odd = 1;
+                    table[(kSwiglu ? 2 : 1) * i * NR + m] = v0;
+                    if (kSwiglu) table[(2 * i + 1) * NR + m] = v1;
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
         } else if (kbn > 0) {
             s_next = sx[0] * sw[0];
         }
-        // (a loop of its own where scales have to be lifted: in one loop the rare part costs the other one registers)
-        auto add_blocks = [&](auto lift_rows) {
+        // (a loop of its own where some scales have no normal product: in one loop the rare part costs the other one registers)
+        auto add_blocks = [&](auto rows_odd) {
             bool fine = true;
             int slot = 0;
             for (int i = 0; i < kbn; ++i) {
@@ -219,8 +219,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                 const uint32_t at = from + acc * F::kCols;
                 if constexpr (!kSwap) {
                     constexpr int kStep = kMine > 64 ? 16 : 32;        // what the registers hold beside the sums
-                    auto add = [&](float times, auto plain_scales) {
-                        [[maybe_unused]] const float lift = plain_scales.value ? 1.f : lift_of(sx[i * a.sx_block], sw[i * a.sw_block]);
+                    auto add = [&](auto to) {              // `to`: a sum and a block's share of it -> the new sum
 #pragma unroll
                         for (int c = 0; c < kMine; c += kStep) {
                             uint32_t d[kStep];
@@ -231,15 +230,52 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                                 if (lane == 0) mbar_arrive(acc_empty + acc);
                             }
 #pragma unroll
-                            for (int j = 0; j < kStep; ++j) {
-                                const float v = plain_scales.value ? __uint_as_float(d[j]) : __uint_as_float(d[j]) * lift;
-                                sum[c + j] = fmaf(v, times, sum[c + j]);
-                            }
+                            for (int j = 0; j < kStep; ++j) sum[c + j] = to(d[j], sum[c + j]);
                         }
                     };
-                    if (__builtin_expect(__all_sync(0xffffffffu, plain(s)), 1)) add(s, std::true_type{});
-                    else add(join(sx[i * a.sx_block], sw[i * a.sw_block]), std::false_type{});
-                } else {                                       // all columns at once: one wait for tensor memory a block
+                    if (__builtin_expect(__all_sync(0xffffffffu, plain(s)), 1)) {
+                        add([&](uint32_t d, float sum) { return fmaf(__uint_as_float(d), s, sum); });
+                    } else {
+                        float factor, then;
+                        Apart(sw[i * a.sw_block]).of(sx[i * a.sx_block], factor, then);
+                        add([&](uint32_t d, float sum) { return fmaf(__uint_as_float(d) * factor, then, sum); });
+                    }
+                } else if constexpr (rows_odd.value) {
+                    const uint32_t tab = table_at + (kSwiglu ? (2 * i + group) * NR : i * NR + group * kMine) * 4;
+                    const int r0 = m0 + (kSwiglu ? 0 : group * kMine);
+#pragma unroll
+                    for (int c = 0; c < kMine; c += 8) {
+                        uint32_t d[8];
+                        float f[8];
+                        tmem_ld8(at + c, d);
+                        load_shared4(tab + 4 * c, f);
+                        load_shared4(tab + 4 * c + 16, f + 4);
+                        tmem_ld_wait();
+                        bool joined = true;                // (the same for the whole warp)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) joined = joined && plain(f[j]);
+                        if (!joined) {                     // (sums of a block of zeros are zero, whatever the scales)
+                            bool zero = true;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) zero = zero && (plain(f[j]) || (d[j] << 1 == 0 && magnitude(f[j]) < 0x7f800000u));
+                            joined = __all_sync(0xffffffffu, zero);
+                        }
+                        if (joined) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sum[c + j] = fmaf(__uint_as_float(d[j]), f[j], sum[c + j]);
+                        } else {
+                            const Apart by(sw[i * a.sw_block]);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                float factor;
+                                by.of(a.sx[(long)min(r0 + c + j, a.M - 1) * a.sx_row + (kb0 + i) * a.sx_block], factor, f[j]);
+                                sum[c + j] = fmaf(__uint_as_float(d[j]) * factor, f[j], sum[c + j]);
+                            }
+                        }
+                    }
+                    fence_before_sync();
+                    if (lane == 0) mbar_arrive(acc_empty + acc);
+                } else {                                   // all columns at once: one wait for tensor memory a block
                     uint32_t d[kMine];
                     if constexpr (kMine == 8) tmem_ld8(at, d);
                     else if constexpr (kMine == 16) tmem_ld16(at, d);
@@ -254,31 +290,19 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                     tmem_ld_wait();
                     fence_before_sync();
                     if (lane == 0) mbar_arrive(acc_empty + acc);
-                    if constexpr (lift_rows.value) {           // (the table has no place for it: the scales are read once more)
-                        const int r0 = kSwiglu ? 0 : group * kMine;
-                        const volatile float* px = a.sx + (long)(m0 + min(r0, rows - 1)) * a.sx_row + (kb0 + i) * a.sx_block;
-                        const float w = sw[i * a.sw_block];
 #pragma unroll
-                        for (int j = 0; j < kMine; ++j) {
-                            const float x = *px;
-                            sum[j] = fmaf(__uint_as_float(d[j]) * lift_of(x, w), join(x, w), sum[j]);
-                            if (r0 + j + 1 < rows) px += a.sx_row;
-                        }
-                    } else {
+                    for (int c = 0; c < kMine; c += kAhead) {
 #pragma unroll
-                        for (int c = 0; c < kMine; c += kAhead) {
+                        for (int j = 0; j < kAhead; ++j) sum[c + j] = fmaf(__uint_as_float(d[c + j]), f[j], sum[c + j]);
+                        if (c + kAhead < kMine) {
 #pragma unroll
-                            for (int j = 0; j < kAhead; ++j) sum[c + j] = fmaf(__uint_as_float(d[c + j]), f[j], sum[c + j]);
-                            if (c + kAhead < kMine) {
-#pragma unroll
-                                for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * (c + kAhead + j), f + j);
-                            }
+                            for (int j = 0; j < kAhead; j += 4) load_shared4(tab + 4 * (c + kAhead + j), f + j);
                         }
                     }
                 }
             }
         };
-        if (kSwap && __builtin_expect(lifted, 0)) add_blocks(std::true_type{}); else add_blocks(std::false_type{});
+        if (kSwap && __builtin_expect(odd, 0)) add_blocks(std::true_type{}); else add_blocks(std::false_type{});
     }
     // ---- the sums meet at the rows' owners
     fence_before_sync();

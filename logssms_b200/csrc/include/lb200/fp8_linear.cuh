@@ -116,28 +116,34 @@ __device__ __forceinline__ float silu_of(float sum, float eighth) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.125f, 0.125f)));
     return v8 * r;
 }
-// Two scales of a block, joined: its sums are multiplied by their product where that is `plain`, a normal number.  Beyond 2^128 or
-// below 2^-126 the product would be infinite or lose its bits, although its multiple of the block's sums (0, or 2^-18 to 2^25) may well
-// be a number: there the sums are multiplied by `lift_of` (2^64 or 2^-64) first and by `join` then.  An infinite or NaN scale stays
-// what it is; a zero sum stays zero under any two finite scales.  That part of the code is rare and stands on its own: a block of
-// zeros has the smallest scale.
+// A block's sums d (0, or 2^-18 to 2^25 in size) are multiplied by the product of its two scales where that is `plain`, a normal
+// number.  Below 2^-126 or beyond 2^128 the product would lose its bits or be infinite, although its multiple of d may well be a number:
+// there d is multiplied by one scale first, then by the other.  With `w` between 2^-100 and 2^100, d w is a normal number and the second
+// product is rounded in its sum only; a `w` outside goes 2^64 nearer to 1 and x as far the other way: what x loses there lies below
+// 2^-160, and past the largest number the result is infinite anyhow.  An infinite or NaN scale stays what it is; a zero sum stays zero
+// under any two finite scales.  A row's sums do not hang on its neighbours' scales.  Blocks of zeros come here too, since they have the
+// smallest scale.  us without / with a block of zeros in x / with a row of zeros (the weight in L2): 3,072 x 12,288 1 row 7.4 / 8.8 /
+// 11.8, 64 rows 11.4 / 20.0 / 21.6, 512 rows 29.8 / 29.8 / 35.1, 8,192 rows 291 / 307 / 336.
 __device__ __forceinline__ bool plain(float product) { return magnitude(product) - 0x00800000u < 0x7f000000u; }
-__device__ __forceinline__ float lift_of(float a, float b) {
-    const uint32_t m = magnitude(a * b);
-    return m >= 0x7f800000u ? 1.84467441e19f : m < 0x00800000u ? 5.42101086e-20f : 1.f;      // 2^64, 2^-64
-}
-__device__ __forceinline__ float join(float a, float b) {
-    float s = a * b;
-    if (!plain(s)) {
-        if (magnitude(s) >= 0x7f800000u) {
-            s = a * 5.42101086e-20f * b;
-            if (magnitude(s) == 0x7f800000u && magnitude(a) < 0x7f800000u && magnitude(b) < 0x7f800000u) s = copysignf(3.402823466e38f, s);
-        } else if (a != 0.f && b != 0.f) {
-            s = a * 1.84467441e19f * b;
-        }
+constexpr float k2p64 = 18446744073709551616.f, k2m64 = 1.f / k2p64;
+struct Apart {
+    float w, first, more;                                  // the weight's scale; what d is multiplied by first, x's share besides
+    __device__ __forceinline__ explicit Apart(float w_) : w(w_) {
+        const uint32_t m = magnitude(w);
+        const bool high = m > 0x71800000u && m < 0x7f800000u, low = m < 0x0d800000u && m != 0;
+        first = w * (high ? k2m64 : low ? k2p64 : 1.f);
+        more = high ? k2p64 : low ? k2m64 : 1.f;
     }
-    return s;
-}
+    // sum + d x w = (d * factor) * then + sum
+    __device__ __forceinline__ void of(float x, float& factor, float& then) const {
+        const float p = x * w;
+        const bool joined = plain(p);
+        then = x * more;
+        if (more > 1.f && magnitude(then) == 0x7f800000u && magnitude(x) < 0x7f800000u) then = copysignf(3.402823466e38f, x);
+        then = joined ? p : then;
+        factor = joined ? 1.f : first;
+    }
+};
 
 // A rows x width matrix of bytes whose rows lie `stride` bytes apart (a multiple of 16; base on a 16-byte boundary); box =
 // box_rows x 128, 128-byte swizzle, zeros outside.  0 or a cudaError.

@@ -253,8 +253,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
             // a block's accumulator, times its scales, joins this thread's sums, 32 columns at a time
             auto add = [&](Scales& f, bool more, auto plain_scales) {
                 const uint32_t col = from + (n & 1) * kCols;
-                uint32_t d[32];
                 if constexpr (plain_scales.value) {
+                    uint32_t d[32];
                     const float s = f.x * f.w, v = kSwiglu ? f.x * f.u : s;
                     if (more) fetch(f);
                     sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
@@ -267,15 +267,19 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                     mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sum[32 + j] = fmaf(__uint_as_float(d[j]), v, sum[32 + j]);
-                } else {                                   // the same, lifted; what it keeps costs the other form no registers
+                } else {                                   // one scale after the other, so many columns at a time as cost the other form no registers
+                    constexpr int kStep = kSwiglu ? 8 : 32;
                     sleep_until_woken<kHalfAdders + 32>(kWakeAdders + (n & 1) * 2 + (group >> 1));
                     fence_after_sync();
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float w = kSwiglu && h ? f.u : f.w, l = lift_of(f.x, w), s = join(f.x, w);
-                        tmem_ld32(col + 32 * h, d);
+                    for (int c = 0; c < 64; c += kStep) {
+                        float factor, then;
+                        Apart(kSwiglu && c >= 32 ? f.u : f.w).of(f.x, factor, then);
+                        uint32_t d[kStep];
+                        if constexpr (kStep == 32) tmem_ld32(col + c, d);
+                        else { tmem_ld8(col + c, d); tmem_ld_wait(); }
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[32 * h + j] = fmaf(__uint_as_float(d[j]) * l, s, sum[32 * h + j]);
+                        for (int j = 0; j < kStep; ++j) sum[c + j] = fmaf(__uint_as_float(d[j]) * factor, then, sum[c + j]);
                     }
                     fence_before_sync();
                     mbar_arrive_at_if(release0 + (n & 1) * 16, lane == 0);

@@ -114,3 +114,24 @@ def test_silu_of_large_gates(m, form):
     got = k.linear_swiglu_fp8(x, gate, up)
     holds(got.values, got.scales, h, h * 2.0 ** -22)
     k.check_kernel_errors()
+
+
+@pytest.mark.parametrize("m", [4, 20, 60, 200, 300])
+def test_a_row_does_not_hang_on_its_neighbours(m, form):
+    """Rows of zeros, NaN, extreme scales beside ordinary ones: the ordinary ones' results keep their bits."""
+    k = K()
+    g = torch.Generator().manual_seed(m)
+    n, width = 200, 400
+    w, u = (k.Fp8Weight(codes(n, width, 0x10, 0x50, g), 0.01 * torch.rand(2, 4, generator=g).cuda()) for _ in range(2))
+    x = codes(m, width, 0x10, 0x50, g)
+    scales = torch.rand(m, 4, generator=g).cuda()
+    plain, gated = k.linear_fp8(k.Fp8Rows(x, scales), w, out_dtype=torch.float32), k.linear_swiglu_fp8(k.Fp8Rows(x, scales), w, u)
+    other = scales.clone()
+    other[0, 0], other[1, 1], other[2], other[-1, 3] = 2.0 ** -126, float("nan"), 1e-38, 3e38
+    rows = k.Fp8Rows(x, other)
+    got, rest = k.linear_fp8(rows, w, out_dtype=torch.float32), slice(3, m - 1)
+    assert torch.equal(got[rest], plain[rest])
+    again = k.linear_swiglu_fp8(rows, w, u)
+    assert torch.equal(again.scales[rest], gated.scales[rest])
+    assert torch.equal(again.values.view(torch.uint8)[rest], gated.values.view(torch.uint8)[rest])
+    k.check_kernel_errors()
