@@ -410,9 +410,10 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_const
                     v[e] = n + e < a.N ? silu_of(v[e], 0.125f * a.act_scale) * u[e] : 0.f;
                     top = max(top, magnitude(v[e]));
                 }
-                const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top)), back = 1.f / scale;
+                const float scale = fp8_scale(__reduce_max_sync(0xffffffffu, top));
+                const Fp8Divide by(scale);
                 // rows are filled up to 16 bytes: four bytes that begin inside the row end inside its storage
-                if (n < a.N) *reinterpret_cast<uint32_t*>(a.q + m * a.ldq + n) = fp8_quad(v[0] * back, v[1] * back, v[2] * back, v[3] * back);
+                if (n < a.N) *reinterpret_cast<uint32_t*>(a.q + m * a.ldq + n) = fp8_quad(by(v[0]), by(v[1]), by(v[2]), by(v[3]));
                 if (lane == 0) a.qs[m * a.qs_row + tile_n * a.qs_block] = scale;
             } else {
 #pragma unroll

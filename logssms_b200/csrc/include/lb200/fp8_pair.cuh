@@ -336,13 +336,14 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w0, const __grid_constan
                 asm volatile("bar.sync 1, 512;" ::: "memory");
 #pragma unroll
                 for (int g = 0; g < kPairGroups; ++g) top = max(top, tops[g][in_tile]);
-                const float scale = fp8_scale(top), back = 1.f / scale;
+                const float scale = fp8_scale(top);
+                const Fp8Divide by(scale);
                 asm volatile("bar.sync 1, 512;" ::: "memory");
                 if (m < a.M) {
                     uint8_t* q = a.q + m * a.ldq + f0;
                     uint32_t w[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = fp8_quad(sum[4 * e] * back, sum[4 * e + 1] * back, sum[4 * e + 2] * back, sum[4 * e + 3] * back);
+                    for (int e = 0; e < 8; ++e) w[e] = fp8_quad(by(sum[4 * e]), by(sum[4 * e + 1]), by(sum[4 * e + 2]), by(sum[4 * e + 3]));
                     if (f0 + 32 <= a.N && ((uintptr_t)q & 31) == 0) {
                         store32(q, w);
                     } else {                               // rows are filled up to 16 bytes

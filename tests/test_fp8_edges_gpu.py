@@ -1,5 +1,5 @@
 """8-bit operators where their 32-bit numbers end, whatever form of the kernel runs: scales whose product leaves 32 bits, SiLU far
-below zero."""
+below zero, quotients beside the boundary between two 8-bit values."""
 import pytest
 import torch
 
@@ -134,4 +134,27 @@ def test_a_row_does_not_hang_on_its_neighbours(m, form):
     again = k.linear_swiglu_fp8(rows, w, u)
     assert torch.equal(again.scales[rest], gated.scales[rest])
     assert torch.equal(again.values.view(torch.uint8)[rest], gated.values.view(torch.uint8)[rest])
+    k.check_kernel_errors()
+
+
+@pytest.mark.parametrize("m", [3, 70, 260])
+def test_gated_rows_are_divided_by_their_scale(m, form):
+    """A gate of 64 is its own SiLU, and sums of two products are exact: the 8-bit values are the float32 quotients by the scale,
+    rounded once, also where a quotient lies on the boundary between two of them or beside it."""
+    k = K()
+    width, blocks = 520, 60
+    n = 128 * blocks
+    g = torch.Generator().manual_seed(7)
+    first = torch.tensor([256, 288, 320, 352, 384, 416, 128, 144, 160, 176, 192, 208, 224, 240] * 9 + [448, 448]).float().repeat(blocks)
+    second = torch.tensor([256, 240, 256, 288, 256, 256, 128, 128, 120, 128, 144, 128, 128, 128] * 9 + [0, 0]).float().repeat(blocks)
+    up_scales = torch.exp(4 * torch.randn(blocks, generator=g))
+    x = k.Fp8Rows(one_column(m, width, {0: 1.0, 1: 0.0625}), torch.ones(m, 5).cuda())
+    gate = k.Fp8Weight(one_column(n, width, {0: 64.0}), torch.ones(blocks, 5).cuda())
+    up = k.Fp8Weight(one_column(n, width, {0: first, 1: second}), up_scales[:, None].repeat(1, 5).cuda())
+    got = k.linear_swiglu_fp8(x, gate, up)
+    h = 64 * ((first + second / 16).view(blocks, 128) * up_scales[:, None])          # float32 on the CPU, one rounding
+    scales = (h.amax(1).double() / 448).float()
+    want = (h / scales[:, None]).to(torch.float8_e4m3fn).view(torch.uint8).view(-1)
+    assert torch.equal(got.scales.cpu(), scales.expand(m, blocks))
+    assert torch.equal(got.values.view(torch.uint8).cpu(), want.expand(m, n))
     k.check_kernel_errors()
