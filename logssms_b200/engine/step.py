@@ -140,7 +140,10 @@ class Engine:
     def _pages_that_fit(self, needs, max_requests: int, memory_ratio: float) -> int:
         """Pages for `memory_ratio` of the device after weights and state slots, capped at what
         `max_requests` full-length requests could ever use (the reference plans the same way,
-        python/logssms/cache/naive/manager.py:352-399)."""
+        python/logssms/cache/naive/manager.py:352-399).  Blocks that loading and setup gave up (16-bit weights behind 8-bit
+        ones, the parts of joined matrices) go back to the device first: the allocator keeps them otherwise, and they would
+        count as taken."""
+        torch.cuda.empty_cache()
         free, total = torch.cuda.mem_get_info(self.device)
         budget = free - (1.0 - memory_ratio) * total - max_requests * CacheManager.bytes_per_request_state(needs, self.dtype)
         per_page = max(CacheManager.bytes_per_page(needs, self.page_size, self.dtype), 1)
