@@ -2644,10 +2644,18 @@ def _fp8_calls():
         at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
         binding.launchers(at("fp8_rows", "lb_add_rmsnorm_fp8"), at("fp8_rows", "lb_quantize_fp8"),
                           at("fp8_linear", "lb_linear_fp8"), at("fp8_linear", "lb_linear_swiglu_fp8"))
-        for index in range(torch.cuda.device_count()):
-            binding.error_word(index, error_word(torch.device("cuda", index)).data_ptr())
         _fp8_binding = binding
     return _fp8_binding
+
+
+def _fp8_error_word(device: torch.device) -> int:
+    """Address of the device's error word, which the binding has from then on (until then it takes no product there)."""
+    if device not in _gemm_error:
+        # (made inside, it would lie in the graph's memory, and every replay would clear what was reported before)
+        _need(not torch.cuda.is_current_stream_capturing(), "the first 8-bit product on a device must come before a capture")
+    address = error_word(device).data_ptr()
+    _fp8_calls().error_word(device.index, address)
+    return address
 
 
 def _fp8_done(got, name: str):
@@ -2788,7 +2796,7 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, ou
              c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p])
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), w.values.data_ptr(), ldw, ws.data_ptr(),
              ws.stride(0), ws.stride(1), _ptr(bias), out.data_ptr(), N, M, N, width, out_scale, int(out_dtype == torch.float32),
-             int(w.settled), _FP8_FORMS[FP8_FORM], error_word(device).data_ptr(), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
+             int(w.settled), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
     return out
 
 
@@ -2814,6 +2822,6 @@ def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: flo
     xs = x.scales
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), gate.values.data_ptr(), up.values.data_ptr(), ldg,
              gs.data_ptr(), us.data_ptr(), gs.stride(0), gs.stride(1), values.data_ptr(), values.stride(0), scales.data_ptr(), 1, M, M,
-             N, width, act_scale, int(gate.settled and up.settled), _FP8_FORMS[FP8_FORM], error_word(device).data_ptr(), _stream()),
+             N, width, act_scale, int(gate.settled and up.settled), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()),
            "linear_swiglu_fp8", f"([{M}, {width}] x 2 x [{N}, {width}])")
     return Fp8Rows(values, scales)

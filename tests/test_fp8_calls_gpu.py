@@ -45,3 +45,62 @@ def test_whole_rows_are_allocated(width, past_the_binding):
             pitch = (width + 15) // 16 * 16
             assert got.values.shape == (3, width) and got.values.stride() == (pitch, 1)
             assert got.values.untyped_storage().nbytes() >= 3 * pitch
+
+
+@pytest.fixture
+def no_words(monkeypatch):
+    """As before the first product of the process: no device has an error word, and the binding knows of none."""
+    k = K()
+    here = torch.cuda.current_device()
+    k._fp8_calls().error_word(here, 0)
+    with monkeypatch.context() as m:
+        m.setattr(k, "_gemm_error", {})
+        yield here
+    k._fp8_calls().error_word(here, k.error_word(torch.device("cuda", here)).data_ptr())
+
+
+def test_only_the_device_in_use_gets_an_error_word(no_words, monkeypatch):
+    k = K()
+    asked, make = [], k.error_word
+
+    def spy(device):
+        asked.append(torch.device(device).index)
+        assert asked[-1] == no_words, "a device that the caller does not use"
+        return make(device)
+    monkeypatch.setattr(k, "error_word", spy)
+    monkeypatch.setattr(k, "_fp8_binding", None)
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 3)
+    x = torch.randn(4, 256, device="cuda")
+    rows = k.quantize_rows_fp8(x)
+    k.add_rmsnorm_fp8(x, torch.ones(256, device="cuda"), 1e-5)
+    assert asked == []                                     # nothing of these waits
+    w = k.quantize_weight_fp8(x)
+    first = k.linear_fp8(rows, w)
+    assert set(asked) == {no_words} and list(k._gemm_error) == [torch.device("cuda", no_words)]
+    count = len(asked)
+    assert torch.equal(k.linear_fp8(rows, w), first) and k.linear_swiglu_fp8(rows, w, w).shape == (4, 4)
+    assert len(asked) == count                             # from then on the binding has it
+    k.check_kernel_errors()
+
+
+def test_a_first_product_inside_a_capture_is_refused(no_words):
+    """Its error word would be cleared by every replay."""
+    k = K()
+    x = torch.randn(4, 256, device="cuda")
+    rows, w = k.quantize_rows_fp8(x), k.quantize_weight_fp8(x)
+    torch.cuda.synchronize()
+    kept = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept.add_(1)
+        for call in (lambda: k.linear_fp8(rows, w), lambda: k.linear_swiglu_fp8(rows, w, w)):
+            with pytest.raises(k.KernelError, match="before a capture"):
+                call()
+    assert k._gemm_error == {}
+    want = k.linear_fp8(rows, w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = k.linear_fp8(rows, w)
+    graph.replay()
+    assert torch.equal(got, want)
+    k.check_kernel_errors()
