@@ -473,8 +473,9 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
     if (rc == 0) { if (kSwiglu) rc = make_byte_map(&map_w1, o.w1, a.N, a.K, o.ldw, kFeat); else map_w1 = map_w0; }
     if (rc == 0) rc = make_byte_map(&map_x, o.x, a.M, a.K, o.ldx, F::kXRows);
     if (rc != 0) return rc;
-    static size_t have = 0;
-    ensure_dynamic_smem(fp8_linear_kernel<kSwap, NR, kSwiglu>, smem, have);
+    static SharedLimits limits;
+    rc = ensure_dynamic_smem(fp8_linear_kernel<kSwap, NR, kSwiglu>, smem, limits);
+    if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * a.split)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -511,10 +512,11 @@ template <bool kSwiglu, bool kRagged, int kParts>
 struct PairLaunch {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2] = {};
+    int rc;
     PairLaunch(int pairs, cudaStream_t s) {
         constexpr size_t smem = pair_smem(kRagged);
-        static size_t have = 0;
-        ensure_dynamic_smem(fp8_pair_kernel<kSwiglu, kRagged, kParts>, smem, have);
+        static SharedLimits limits;
+        rc = ensure_dynamic_smem(fp8_pair_kernel<kSwiglu, kRagged, kParts>, smem, limits);
         cfg.gridDim = dim3((unsigned)(2 * pairs)); cfg.blockDim = dim3(kPairThreads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -525,20 +527,22 @@ struct PairLaunch {
     // (one pair for a tile: tile0 is 0)
     int run(const CUtensorMap& map_w0, const CUtensorMap& map_w1, const CUtensorMap& map_x, Args a, int tile0, int tiles) {
         a.tile0 = tile0; a.tiles = tiles;
-        const int rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged, kParts>, map_w0, map_w1, map_x, a);
+        if (rc == 0) rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged, kParts>, map_w0, map_w1, map_x, a);
         return rc != 0 ? rc : launch_status();
     }
     // clusters that are at work at one time (a group of neighbouring SMs holds whole clusters only: 15 of eight CTAs, 33 of four)
     static int at_once() {
-        static const int n = [] {
+        static AskedOnce asked;
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess) device = -1;
+        return asked.get(device, [] {
             PairLaunch l(kParts, nullptr);
             int n = 0;
             l.cfg.attrs = l.attr + 1; l.cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel<kSwiglu, kRagged, kParts>, &l.cfg) == cudaSuccess) return n;
+            if (l.rc == 0 && cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel<kSwiglu, kRagged, kParts>, &l.cfg) == cudaSuccess) return n;
             (void)cudaGetLastError();
             return 0;
-        }();
-        return n;
+        });
     }
 };
 

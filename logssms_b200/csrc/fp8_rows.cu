@@ -359,9 +359,9 @@ extern "C" int lb_add_rmsnorm_fp8(const void* x, long ldx, const void* other, lo
         const size_t smem = (size_t)width * 4;
         if (smem > 200 * 1024) return kTooLarge;
         LB_DISPATCH_DTYPE(dtype, {
-            static size_t have = 0;
-            ensure_dynamic_smem(add_rmsnorm_fp8_any_kernel<T>, smem, have);
-            const int rc = launch_pdl(add_rmsnorm_fp8_any_kernel<T>, dim3(rows), dim3(256), smem, s, a);
+            static SharedLimits limits;
+            int rc = ensure_dynamic_smem(add_rmsnorm_fp8_any_kernel<T>, smem, limits);
+            if (rc == 0) rc = launch_pdl(add_rmsnorm_fp8_any_kernel<T>, dim3(rows), dim3(256), smem, s, a);
             if (rc != 0) return rc;
         })
     }

@@ -11,6 +11,7 @@
 #include <stdint.h>
 #include <stdlib.h>
 #include <utility>
+#include "lb200/per_device.h"
 
 namespace lb200 {
 
@@ -85,6 +86,16 @@ inline void ensure_dynamic_smem(Kernel kernel, size_t smem, size_t& have) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         have = smem;
     }
+}
+
+// The same for launchers that serve every device of the process; returns a cudaError, after which nothing is remembered.
+template <typename Kernel>
+inline int ensure_dynamic_smem(Kernel kernel, size_t smem, SharedLimits& limits) {
+    int device = 0;
+    int rc = (int)cudaGetDevice(&device);
+    if (rc == 0) rc = limits.raise(device, smem, [&](size_t n) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)n); });
+    if (rc != 0) (void)cudaGetLastError();
+    return rc;
 }
 
 // `allow` false: plain stream order for this launch.
