@@ -80,6 +80,15 @@ bool numbers(double* to, PyObject* const* from, int n) {
     }
     return true;
 }
+// what Python's `if` would say of each; false where that raises (the ordinary way then raises it)
+bool truths(bool* to, PyObject* const* from, int n) {
+    for (int i = 0; i < n; ++i) {
+        const int yes = PyObject_IsTrue(from[i]);
+        if (yes < 0) { PyErr_Clear(); return false; }
+        to[i] = yes != 0;
+    }
+    return true;
+}
 // no C++ exception reaches the interpreter: what throws here (an allocation that fails) goes the ordinary way and says so there
 template <typename F> PyObject* guarded(F f) {
     try {
@@ -96,7 +105,8 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const int device = (int)c10::cuda::current_device();
         double num[4];
-        if (n != 10 || norm_fn == nullptr || !numbers(num, args + 2, 1) || !numbers(num + 1, args + 5, 3)) return none();
+        bool flags[2];
+        if (n != 10 || norm_fn == nullptr || !numbers(num, args + 2, 1) || !numbers(num + 1, args + 5, 3) || !truths(flags, args + 8, 2)) return none();
         const at::Tensor *x = tensor(args[0]), *w = tensor(args[1]), *res = nullptr, *other = nullptr;
         if (x == nullptr || w == nullptr || !matrix(*x, device) || dtype_code(*x) < 0) return none();
         const int64_t rows = x->size(0), width = x->size(1);
@@ -108,7 +118,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
             (i == 0 ? res : other) = t;
         }
         at::Tensor fresh;
-        const bool want = args[8] == Py_True, in_place = args[9] == Py_True;
+        const bool want = flags[0], in_place = flags[1];
         const at::Tensor* to = nullptr;
         if (want && res != nullptr && in_place) to = res;
         else if (want) {
@@ -156,17 +166,19 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int device = (int)c10::cuda::current_device();
         Fp8 x, w;
         double out_scale;
+        bool flags[2];
         if (n != 9 || linear_fn == nullptr || device >= kDevices || error_words[device] == nullptr || !numbers(&out_scale, args + 5, 1)
+            || !truths(flags, args + 6, 2)
             || !operand(x, args[0], args[1], 1, device) || !operand(w, args[2], args[3], 128, device) || x.v->size(1) != w.v->size(1)) return none();
         const int64_t M = x.v->size(0), N = w.v->size(0), K = x.v->size(1);
         const at::Tensor* bias = nullptr;
         if (args[4] != Py_None && ((bias = tensor(args[4])) == nullptr || !vector(*bias, device, N))) return none();
-        const bool f32 = args[6] == Py_True;
+        const bool f32 = flags[0];
         const at::Tensor out = at::detail::empty_strided_cuda({M, N}, {N, 1}, f32 ? at::kFloat : at::kBFloat16, x.v->device());
         const int code = linear_fn(x.v->data_ptr(), x.pitch, (const float*)x.s->data_ptr(), x.s->stride(0), x.s->stride(1), w.v->data_ptr(),
                                    w.pitch, (const float*)w.s->data_ptr(), w.s->stride(0), w.s->stride(1),
                                    bias ? (const float*)bias->data_ptr() : nullptr, out.data_ptr(), N, (int)M, (int)N, (int)K,
-                                   (float)out_scale, f32, args[7] == Py_True, (int)PyLong_AsLong(args[8]), error_words[device], stream_of(device));
+                                   (float)out_scale, f32, flags[1], (int)PyLong_AsLong(args[8]), error_words[device], stream_of(device));
         return code != 0 ? PyLong_FromLong(code) : THPVariable_Wrap(out);
     });
 }
@@ -177,7 +189,9 @@ PyObject* swiglu(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int device = (int)c10::cuda::current_device();
         Fp8 x, g, u;
         double act_scale;
+        bool settled;
         if (n != 9 || swiglu_fn == nullptr || device >= kDevices || error_words[device] == nullptr || !numbers(&act_scale, args + 6, 1)
+            || !truths(&settled, args + 7, 1)
             || !operand(x, args[0], args[1], 1, device) || !operand(g, args[2], args[3], 128, device)
             || !operand(u, args[4], args[5], 128, device) || x.v->size(1) != g.v->size(1) || g.v->sizes() != u.v->sizes()
             || g.pitch != u.pitch || g.s->strides() != u.s->strides()) return none();
@@ -186,7 +200,7 @@ PyObject* swiglu(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int code = swiglu_fn(x.v->data_ptr(), x.pitch, (const float*)x.s->data_ptr(), x.s->stride(0), x.s->stride(1), g.v->data_ptr(),
                                    u.v->data_ptr(), g.pitch, (const float*)g.s->data_ptr(), (const float*)u.s->data_ptr(), g.s->stride(0),
                                    g.s->stride(1), q.data_ptr(), q.stride(0), (float*)s.data_ptr(), 1, M, (int)M, (int)N, (int)K,
-                                   (float)act_scale, args[7] == Py_True, (int)PyLong_AsLong(args[8]), error_words[device], stream_of(device));
+                                   (float)act_scale, settled, (int)PyLong_AsLong(args[8]), error_words[device], stream_of(device));
         return code != 0 ? PyLong_FromLong(code) : two(q, s);
     });
 }

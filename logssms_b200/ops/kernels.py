@@ -2796,7 +2796,7 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, *, ou
              c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p])
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), w.values.data_ptr(), ldw, ws.data_ptr(),
              ws.stride(0), ws.stride(1), _ptr(bias), out.data_ptr(), N, M, N, width, out_scale, int(out_dtype == torch.float32),
-             int(w.settled), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
+             int(bool(w.settled)), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()), "linear_fp8", f"([{M}, {width}] x [{N}, {width}])")
     return out
 
 
@@ -2822,6 +2822,6 @@ def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: flo
     xs = x.scales
     _check(f(x.values.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), gate.values.data_ptr(), up.values.data_ptr(), ldg,
              gs.data_ptr(), us.data_ptr(), gs.stride(0), gs.stride(1), values.data_ptr(), values.stride(0), scales.data_ptr(), 1, M, M,
-             N, width, act_scale, int(gate.settled and up.settled), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()),
+             N, width, act_scale, int(bool(gate.settled and up.settled)), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()),
            "linear_swiglu_fp8", f"([{M}, {width}] x 2 x [{N}, {width}])")
     return Fp8Rows(values, scales)

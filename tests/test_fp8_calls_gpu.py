@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from fp8_util import make_rows, make_weight
+from test_fp8_linear_gpu import check_linear, check_swiglu
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +105,26 @@ def test_a_first_product_inside_a_capture_is_refused(no_words):
     graph.replay()
     assert torch.equal(got, want)
     k.check_kernel_errors()
+
+
+@pytest.mark.parametrize("yes,no", [(1, 0), ("yes", ""), ([0], None)])
+def test_what_is_true_counts_as_true(yes, no, past_the_binding):
+    """Flags of any type, through the binding as past it."""
+    k = K()
+    x, r = torch.randn(4, 64, device="cuda"), torch.randn(4, 64, device="cuda")
+    weight = torch.ones(64, device="cuda")
+    xq, w, u = operands(4, 64, 256)
+    for way in range(2):
+        if way:
+            past_the_binding()
+        kept = r.clone()
+        assert k.add_rmsnorm_fp8(x, weight, 1e-5, kept, want_residual=yes, in_place=yes)[1] is kept
+        assert torch.equal(kept, r + x)
+        kept = r.clone()
+        new = k.add_rmsnorm_fp8(x, weight, 1e-5, kept, want_residual=yes, in_place=no)[1]
+        assert new is not kept and torch.equal(kept, r) and torch.equal(new, r + x)
+        assert k.add_rmsnorm_fp8(x, weight, 1e-5, kept, want_residual=no)[1] is None and torch.equal(kept, r)
+        for settled in (yes, no):
+            a, b = k.Fp8Weight(w.values, w.scales, settled), k.Fp8Weight(u.values, u.scales, settled)
+            check_linear(xq, a)
+            check_swiglu(xq, a, b, 1.0)
