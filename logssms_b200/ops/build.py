@@ -141,7 +141,9 @@ def _host_command(compiler: str, src: str, out: str) -> list[str]:
 def _digest(name: str) -> str:
     h = hashlib.sha1()
     src = source_path(name)
-    h.update(" ".join(_host_flags() if src.endswith(".cpp") else NVCC_FLAGS).encode())
+    # (a compiler that is asked for is part of a binding's build; whichever is found is not, so that a built file also serves where
+    # there is none)
+    h.update(" ".join([os.environ.get("CXX", ""), *_host_flags()] if src.endswith(".cpp") else NVCC_FLAGS).encode())
     paths = [src]
     for root, _, files in sorted(os.walk(INCLUDE)):
         paths += [os.path.join(root, f) for f in sorted(files)]
@@ -152,8 +154,17 @@ def _digest(name: str) -> str:
     return h.hexdigest()[:12]
 
 
+def _file_stem(name: str) -> str:
+    """The name of a library's file up to its hash.  A binding's names the Python whose headers it is compiled against: interpreters
+    that share a folder have a build each."""
+    if source_path(name).endswith(".cpp"):
+        import sysconfig
+        return f"lb200_{_stem(name)}.{sysconfig.get_config_var('SOABI')}"
+    return f"lb200_{_stem(name)}"
+
+
 def library_path(name: str) -> str:
-    return os.path.join(_build_dir(), f"lb200_{_stem(name)}-{_digest(name)}.so")
+    return os.path.join(_build_dir(), f"{_file_stem(name)}-{_digest(name)}.so")
 
 
 def build(name: str, verbose: bool = True) -> str:
@@ -171,7 +182,7 @@ def build(name: str, verbose: bool = True) -> str:
         cmd = _host_command(compiler, src, tmp)
     else:
         cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", os.path.dirname(src), "-o", tmp, src]
-    name, file = _stem(name), os.path.basename(src)
+    prefix, file = f"{_file_stem(name)}-", os.path.basename(src)
     if verbose:
         _log(f"compiling {file}{'' if host else ' for sm_100a'} ...")
     start = time.time()
@@ -190,7 +201,6 @@ def build(name: str, verbose: bool = True) -> str:
         raise KernelBuildError(f"{'the C++ compiler' if host else 'nvcc'} failed on {file}:\n{output}")
     os.replace(tmp, out)
     # builds of earlier versions of this source are of no use any more
-    prefix = f"lb200_{name}-"
     for f in os.listdir(os.path.dirname(out)):
         if f.startswith(prefix) and f.endswith(".so") and f != os.path.basename(out):
             try:
