@@ -646,6 +646,7 @@ extern "C" int lb_linear_fp8(const void* x, long ldx, const float* sx, long sx_r
                              int K, float out_scale, int out_f32, int early, int form, int* error, void* stream) {
     if (M <= 0 || N <= 0) return kOk;
     if (K <= 0 || ldx % 16 || ldw % 16 || (((uintptr_t)x | (uintptr_t)w) & 15)) return kBadSize;
+    if (M > kFp8Most || N > kFp8Most || K > kFp8Most) return kTooLarge;
     Args a{};
     a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sw; a.sw_row = sw_row; a.sw_block = sw_block;
     a.bias = bias; a.out = out; a.ldo = ldo; a.M = M; a.N = N; a.K = K; a.out_scale = out_scale; a.out_f32 = out_f32;
@@ -661,6 +662,7 @@ extern "C" int lb_linear_swiglu_fp8(const void* x, long ldx, const float* sx, lo
                                     float act_scale, int early, int form, int* error, void* stream) {
     if (M <= 0 || N <= 0) return kOk;
     if (K <= 0 || ldx % 16 || ldw % 16 || ldq % 16 || (((uintptr_t)x | (uintptr_t)gate | (uintptr_t)up | (uintptr_t)q) & 15)) return kBadSize;
+    if (M > kFp8Most || N > kFp8Most || K > kFp8Most) return kTooLarge;
     Args a{};
     a.sx = sx; a.sx_row = sx_row; a.sx_block = sx_block; a.sw0 = sgate; a.sw1 = sup; a.sw_row = sw_row; a.sw_block = sw_block;
     a.q = (uint8_t*)q; a.ldq = ldq; a.qs = qs; a.qs_row = qs_row; a.qs_block = qs_block; a.M = M; a.N = N; a.K = K;

@@ -338,6 +338,7 @@ extern "C" int lb_add_rmsnorm_fp8(const void* x, long ldx, const void* other, lo
     if (dtype != kF32 && dtype != kBF16) return kBadDType;
     if (rows <= 0) return kOk;
     if (width <= 0 || ldq % 8 || ((uintptr_t)q & 7)) return kBadSize;
+    if (width > kFp8Most) return kTooLarge;
     const int size = dtype == kF32 ? 4 : 2;
     NormArgs a{x, other, residual, residual_out, weight, (uint8_t*)q, scales, ldx, ldo, ldr, ldres, ldq, scale_row, scale_block,
                rows, width, eps, in0, in1, out_scale};
@@ -374,6 +375,7 @@ extern "C" int lb_quantize_fp8(const void* x, long ldx, void* q, long ldq, float
     if (dtype != kF32 && dtype != kBF16) return kBadDType;
     if (rows <= 0) return kOk;
     if (width <= 0 || ldq % 8 || ((uintptr_t)q & 7) || (block_rows != 1 && block_rows != kFp8Block)) return kBadSize;
+    if (width > kFp8Most) return kTooLarge;
     const int size = dtype == kF32 ? 4 : 2, blocks = (width + kFp8Block - 1) / kFp8Block;
     QuantArgs a{x, (uint8_t*)q, scales, ldx, ldq, scale_row, scale_block, rows, width, blocks};
     cudaStream_t s = (cudaStream_t)stream;

@@ -13,6 +13,7 @@
 namespace lb200 {
 
 constexpr int kFp8Block = 128;
+constexpr int kFp8Most = 0x7fff0000;                      // rows, features and columns at most: sums of a place and a tile's size stay whole numbers of 32 bits
 
 // |v| as bits: their order as whole numbers is the order of magnitudes, infinity above every number and NaN above infinity
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }

@@ -1,4 +1,6 @@
-"""How the 8-bit operators are called: through the binding and past it, and what they allocate."""
+"""How the 8-bit operators are called: through the binding and past it, what they allocate and
+what they refuse."""
+from ctypes import c_float, c_int, c_long, c_void_p
 from types import SimpleNamespace
 
 import pytest
@@ -128,3 +130,26 @@ def test_what_is_true_counts_as_true(yes, no, past_the_binding):
             a, b = k.Fp8Weight(w.values, w.scales, settled), k.Fp8Weight(u.values, u.scales, settled)
             check_linear(xq, a)
             check_swiglu(xq, a, b, 1.0)
+
+
+def test_sizes_near_the_end_of_32_bits_are_refused():
+    """By the launchers, before anything is launched: within 2^16 of 2^31 the kernels' own places would leave 32 bits."""
+    from logssms_b200.ops import build
+    p, l, i, f = c_void_p, c_long, c_int, c_float                     # noqa: E741
+    at, big, pitch = 1 << 20, (1 << 31) - 100, (1 << 31) - (1 << 16)
+    linear = build.load("fp8_linear").lb_linear_fp8
+    linear.argtypes = [p, l, p, l, l, p, l, p, l, l, p, p, l, i, i, i, f, i, i, i, p, p]
+    swiglu = build.load("fp8_linear").lb_linear_swiglu_fp8
+    swiglu.argtypes = [p, l, p, l, l, p, p, l, p, p, l, l, p, l, p, l, l, i, i, i, f, i, i, p, p]
+    for sizes in ((big, 16, 16), (16, big, 16), (16, 16, big)):
+        for form in range(4):
+            assert linear(at, pitch, at, 1, 1, at, pitch, at, 1, 1, None, at, 16, *sizes, 1.0, 0, 0, form, None, None) == -3
+            assert swiglu(at, pitch, at, 1, 1, at, at, pitch, at, at, 1, 1, at, pitch, at, 1, 1, *sizes, 1.0, 0, form, None, None) == -3
+    quantize = build.load("fp8_rows").lb_quantize_fp8
+    quantize.argtypes = [p, l, p, l, p, l, l, l, i, i, i, p]
+    for block_rows in (1, 128):
+        for width in (big, big + 4):                       # by values, by pieces of 8
+            assert quantize(at, 1 << 31, at, 1 << 31, at, 1, 1, 1, width, block_rows, 0, None) == -3
+    norm = build.load("fp8_rows").lb_add_rmsnorm_fp8
+    norm.argtypes = [p, l, p, l, p, l, p, l, p, p, l, p, l, l, i, i, f, f, f, f, i, p]
+    assert norm(at, 1 << 31, None, 0, None, 0, None, 0, at, at, 1 << 31, at, 1, 1, 1, big, 1e-5, 1.0, 1.0, 1.0, 0, None) == -3
