@@ -8,6 +8,7 @@ import torch
 
 from fp8_util import make_rows, make_weight
 from test_fp8_linear_gpu import check_linear, check_swiglu
+from tiny import TINY, make_model_dir
 
 pytestmark = pytest.mark.gpu
 
@@ -21,6 +22,11 @@ def operands(m, n, k, seed=0):
     g = torch.Generator().manual_seed(1000 * m + n + k + seed)
     kk = K()
     return kk.Fp8Rows(*make_rows(m, k, g)), kk.Fp8Weight(*make_weight(n, k, g), settled=True), kk.Fp8Weight(*make_weight(n, k, g), settled=True)
+
+
+def same(a, b):
+    return a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype and torch.equal(
+        a.view(torch.uint8) if a.dtype == torch.float8_e4m3fn else a, b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b)
 
 
 @pytest.fixture
@@ -153,3 +159,70 @@ def test_sizes_near_the_end_of_32_bits_are_refused():
     norm = build.load("fp8_rows").lb_add_rmsnorm_fp8
     norm.argtypes = [p, l, p, l, p, l, p, l, p, p, l, p, l, l, i, i, f, f, f, f, i, p]
     assert norm(at, 1 << 31, None, 0, None, 0, None, 0, at, at, 1 << 31, at, 1, 1, 1, big, 1e-5, 1.0, 1.0, 1.0, 0, None) == -3
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(1, 40), (5, 301), (130, 1024)])
+def test_both_ways_give_the_same_bytes(rows, width, dtype, past_the_binding):
+    k = K()
+    g = torch.Generator().manual_seed(rows)
+    x, o, r = (torch.randn(rows, width, generator=g).to(dtype).cuda() for _ in range(3))
+    weight = torch.rand(width, generator=g).cuda()
+    xq, w, u = operands(rows, 200, width)
+    bias = torch.randn(200, generator=g).cuda()
+
+    def everything():
+        outs = []
+        for kw in ({}, {"other": o, "in_scales": (0.5, 0.25)}, {"other": o, "want_residual": False}, {"in_place": False, "out_scale": 2.0}):
+            kept = r.clone()
+            made, new = k.add_rmsnorm_fp8(x, weight, 1e-5, kept, **kw)
+            outs += [made.values, made.scales, kept, kept if new is None else new]
+        made, new = k.add_rmsnorm_fp8(x, weight, 1e-5)
+        outs += [made.values, made.scales, new]
+        for made in (k.quantize_rows_fp8(x), k.quantize_weight_fp8(x), k.linear_swiglu_fp8(xq, w, u, 0.9)):
+            outs += [made.values, made.scales]
+        return outs + [k.linear_fp8(xq, w), k.linear_fp8(xq, w, bias, out_scale=1.5, out_dtype=torch.float32)]
+    first = everything()
+    past_the_binding()
+    before = k.launch_count
+    second = everything()
+    assert k.launch_count - before == 10
+    assert all(same(a, b) for a, b in zip(first, second, strict=True))
+    k.check_kernel_errors()
+
+
+def test_a_profiled_engine_gives_the_same_logits(tmp_path):
+    from logssms_b200.engine import Engine, StepEntry
+    from logssms_b200.ops.profiler import PROFILER
+    model_dir = make_model_dir(tmp_path / "m", TINY["A"], seed=4, dtype=torch.bfloat16)
+    ids = torch.randint(0, 256, (60,), generator=torch.Generator().manual_seed(1)).tolist()
+    got = []
+    try:
+        for profile in (False, True):
+            engine = Engine(model_dir, "bfloat16", max_requests=2, max_seq_len=64, num_pages=4, use_graphs=False, profile=profile,
+                            feed_forward_weights="float8")
+            r = engine.new_request()
+            got.append([engine.step([StepEntry(r, part, list(range(len(part))))]).clone() for part in (ids[:59], ids[59:])])
+            if profile:
+                names = " ".join(PROFILER.report()["kernels"])
+                assert "lb_add_rmsnorm_fp8" in names and "lb_linear_fp8" in names and "lb_linear_swiglu_fp8" in names
+    finally:
+        PROFILER.disable()
+    assert all(torch.equal(a, b) for a, b in zip(*got, strict=True))
+
+
+@pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("m", [1, 6, 17, 33, 64, 150])
+def test_no_split_is_refused(m, split):
+    """All of these fit an SM's shared memory, the plain product and the gated one."""
+    k = K()
+    k._FP8_FORMS["split"] = (1 if m <= 64 else 2) + 256 * split
+    k.FP8_FORM = "split"
+    try:
+        for n, kd in ((200, 128 * 9), (257, 128 * 8 * 3 - 5), (128, 128 * 40), (300, 100)):
+            x, w, u = operands(m, n, kd)
+            check_linear(x, w)
+            check_swiglu(x, w, u, 0.8)
+    finally:
+        k.FP8_FORM = "auto"
+        del k._FP8_FORMS["split"]
