@@ -17,6 +17,8 @@ def test_8_bit_weights_leave_more_pages(tmp_path):
     raw = {**TINY["A"], "intermediate_size": inter}
     model_dir = make_model_dir(tmp_path / "m", raw, seed=1, dtype=torch.bfloat16)
     held = 3 * raw["num_hidden_layers"] * inter * hidden * 2
+    gc.collect()
+    torch.cuda.empty_cache()                               # (what tests before this one have left behind)
     free, total = torch.cuda.mem_get_info()
     ratio = 1 - (free - (1 << 30)) / total                 # about 1 GB for the engine, whatever the device holds besides
     pages = {}
