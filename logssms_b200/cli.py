@@ -49,7 +49,8 @@ def build_parser() -> argparse.ArgumentParser:
                         "reference keeps them: half the bytes of a decode step's state update, one rounding per step)")
     p.add_argument("--feed-forward-weights", choices=["model", "float8"], default="model",
                    help="weights of the feed-forwards: as they are stored, or in 8-bit floating point with a scale per 128 x 128 "
-                        "(half the bytes of their part of a decode step, about twice the rate of a prompt's; rows go in 8 bits too)")
+                        "(half the bytes of their part of a decode step, products of a prompt about 1.2 times as fast; rows go in 8 bits "
+                        "too).  For layers of a few thousand columns: small models decode most batch sizes slower with it")
     p.add_argument("--profile", default=None, metavar="FILE",
                    help="time every kernel with CUDA events and write the sums per kernel class to FILE (JSON) at exit; "
                         "such a run launches every step kernel by kernel")

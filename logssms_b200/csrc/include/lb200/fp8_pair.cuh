@@ -12,8 +12,8 @@
 //               block.  Warps 0-3 give up registers for that.
 // What bounds it: the adding (256 cycles of multiply-adds and two waits for tensor memory per block), the products (512 cycles) and
 // the hand-over of an accumulator between them lie within a quarter of each other; left out one at a time, down 8,192 x 3,072 x 12,288
-// takes 264 us without the multiply-adds, 277 with a quarter of the products, 285 without loads, 314 with all (1.97 PFLOP/s; 353 us in
-// a long row of calls on random data, when the power limit sets the clock, 329 with the last round's tiles shared).
+// took 264 us without the multiply-adds, 277 with a quarter of the products, 285 without loads, 314 with all.  Now it takes 303 us in
+// bursts (2.04 PFLOP/s), 347 in a long row of calls on random data, when the power limit sets the clock (1,447 MHz), and 249 on zeros.
 // SwiGLU: the features are laid out so that a thread has gate and up of the same 32 features; only a row's largest magnitude is
 // exchanged between the four warpgroups.
 //
