@@ -2,7 +2,8 @@
 // quantisation of rows (a scale per row and 128 columns) and of a weight (a scale per 128 rows and 128 columns).
 //
 // All three read their input once, in 16-byte pieces that stay in registers between the passes over them, and are bound by
-// those bytes and by their instructions (8,192 x 3,072 bfloat16: issue slots 75 % busy in the norm, 78 % in the rows' quantisation).  16 neighbouring threads hold the 8 values each of a block of 128, so a block's maximum takes four shuffles.
+// those bytes and by their instructions (8,192 x 3,072 bfloat16: issue slots 75 % busy in the norm, 78 % in the rows'
+// quantisation).  16 neighbouring threads hold the 8 values each of a block of 128, so a block's maximum takes four shuffles.
 // Widths that are no multiple of 8, and rows that do not lie on 16 bytes, go value by value (`*_any_kernel`).
 #include "lb200/common.cuh"
 #include "lb200/fp8.cuh"
