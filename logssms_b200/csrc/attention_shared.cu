@@ -1,0 +1,229 @@
+// Attention of a batch whose requests begin with the same tokens: the keys of the shared prefix are read once for all of them.
+//
+// The tokens of the batch lie in groups.  A group's queries (its tokens times the query heads of a key/value head) are the rows
+// of one product with the prefix's keys, 8 to 128 rows a tile instead of the heads of one token; what is a request's own (the
+// keys behind the prefix) is read token by token.  Both leave (maximum, sum, weighted values) per range of keys, in float32, and
+// a third kernel puts the ranges of a row together:
+//   m = max m_s,  out = sum o_s 2^(m_s - m) / sum l_s 2^(m_s - m)
+//
+// This file: the general form, for float32, any page size and head sizes in steps of 8 up to 256, and the merge.
+#include "lb200/common.cuh"
+#include "lb200/attention_shared.h"
+using namespace lb200;
+
+namespace {
+constexpr int kThreads = 128, kRows = 16, kKeys = 32;
+
+struct Items { int head_tiles; long prefix_tiles; };
+
+// One CTA: 16 rows (token, query head of one key/value head) x a range of keys.
+//   prefix: grid (tiles of the groups' rows, kv heads, ranges); own: grid (tokens x tiles of a token's heads, kv heads, ranges)
+template <typename T, bool PREFIX>
+__global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, int head_tiles) {
+    pdl_wait();
+    extern __shared__ float smem[];
+    const int hd = a.hd, ld = hd + 4, tid = threadIdx.x;
+    float* q_s = smem;                                   // [kRows][ld]
+    float* k_s = q_s + kRows * ld;                       // [kKeys][ld]
+    float* v_s = k_s + kKeys * ld;
+    float* p_s = v_s + kKeys * ld;                       // [kRows][kKeys + 1]
+    const int G = a.Hq / a.Hkv, kvh = blockIdx.y, split = blockIdx.z;
+    int first, rows, request, begin, end;                // the rows: token first + (row0 + r) / G, head kvh * G + (row0 + r) % G
+    long row0;
+    if (PREFIX) {
+        int g, n;
+        if (!find_tile(a, blockIdx.x, G, kRows, &g, &row0, &first, &n)) return;
+        rows = (int)min((long)kRows, (long)n * G - row0);
+        request = a.token_req[first];
+        begin = 0;
+        end = a.prefix_lens[g];
+    } else {
+        first = blockIdx.x / head_tiles;
+        row0 = (long)(blockIdx.x % head_tiles) * kRows;
+        rows = (int)min((long)kRows, (long)G - row0);
+        const int g = group_of(a, first);
+        if (g < 0) return;
+        request = a.token_req[first];
+        begin = max(a.prefix_lens[g], 0);
+        end = a.positions[first] + 1;
+    }
+    const bool known = request >= 0 && request < a.requests;
+    end = known ? (int)min((long)end, (long)a.bt_cols * a.page_size) : begin;
+    const int splits = PREFIX ? a.prefix_splits : a.own_splits;
+    const int per = end > begin ? (((end - begin + splits - 1) / splits) + kKeys - 1) / kKeys * kKeys : 0;
+    const int from = (int)min((long)begin + (long)split * per, (long)max(end, begin)), to = (int)min((long)from + per, (long)max(end, begin));
+    const int* bt = a.block_table + (long)(known ? request : 0) * a.bt_stride;
+
+    const T* q = (const T*)a.q;
+    for (int i = tid; i < kRows * hd; i += kThreads) {
+        const int r = i / hd, d = i % hd;
+        float v = 0.f;
+        if (r < rows) {
+            const long at = row0 + r;
+            v = to_f32(q[(first + at / G) * a.q_stride + (kvh * G + at % G) * hd + d]) * a.scale_log2;
+        }
+        q_s[r * ld + d] = v;
+    }
+    const int r = tid >> 3, c = tid & 7;                 // this thread's row; its keys c + 8 i, its columns 4 c + 32 i
+    const long at = row0 + r;
+    const int token = r < rows ? (int)(first + at / G) : first;
+    const int limit = r < rows ? a.positions[token] + 1 : 0;
+    float m = -INFINITY, l = 0.f;
+    float4 acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const T* kc = (const T*)a.k_cache;
+    const T* vc = (const T*)a.v_cache;
+    for (int j0 = from; j0 < to; j0 += kKeys) {
+        const int n = min(kKeys, to - j0);
+        __syncthreads();
+        // a page outside of the pool has no keys: its scores are left out below (p_s takes the mark in its last column)
+        for (int i = tid; i < kKeys * (hd >> 2); i += kThreads) {
+            const int key = i / (hd >> 2), d = (i % (hd >> 2)) * 4;
+            float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
+            bool there = key < n;
+            if (there) {
+                const int j = j0 + key;
+                const long page = bt[j / a.page_size];
+                there = page >= 0 && page < a.pages;
+                if (there) {
+                    const size_t base = (((size_t)page * a.page_size + j % a.page_size) * a.Hkv + kvh) * hd + d;
+                    kv = make_float4(to_f32(kc[base]), to_f32(kc[base + 1]), to_f32(kc[base + 2]), to_f32(kc[base + 3]));
+                    vv = make_float4(to_f32(vc[base]), to_f32(vc[base + 1]), to_f32(vc[base + 2]), to_f32(vc[base + 3]));
+                }
+            }
+            if (d == 0) k_s[key * ld + hd] = there ? 1.f : 0.f;
+            *reinterpret_cast<float4*>(k_s + key * ld + d) = kv;
+            *reinterpret_cast<float4*>(v_s + key * ld + d) = vv;
+        }
+        __syncthreads();
+        float s[4] = {};
+#pragma unroll 4
+        for (int d = 0; d < hd; d += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(q_s + r * ld + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 w = *reinterpret_cast<const float4*>(k_s + (c + 8 * i) * ld + d);
+                s[i] = fmaf(u.x, w.x, fmaf(u.y, w.y, fmaf(u.z, w.z, fmaf(u.w, w.w, s[i]))));
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool there = c + 8 * i < n && j0 + c + 8 * i < limit && k_s[(c + 8 * i) * ld + hd] != 0.f;
+            if (!there) s[i] = -INFINITY;
+            mx = fmaxf(mx, s[i]);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float ref = mx == -INFINITY ? 0.f : mx;    // nothing seen yet: every weight is 2^-inf = 0
+        const float factor = exp2f(m - ref);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = exp2f(s[i] - ref);
+            p_s[r * (kKeys + 1) + c + 8 * i] = p;
+            sum += p;
+        }
+        l = l * factor + sum;
+        m = mx;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { acc[i].x *= factor; acc[i].y *= factor; acc[i].z *= factor; acc[i].w *= factor; }
+        for (int key = 0; key < n; ++key) {
+            const float p = p_s[r * (kKeys + 1) + key];
+            if (p == 0.f) continue;                      // (a masked key's value may be anything)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = 4 * c + 32 * i;
+                if (d < hd) {
+                    const float4 w = *reinterpret_cast<const float4*>(v_s + key * ld + d);
+                    acc[i].x = fmaf(p, w.x, acc[i].x); acc[i].y = fmaf(p, w.y, acc[i].y);
+                    acc[i].z = fmaf(p, w.z, acc[i].z); acc[i].w = fmaf(p, w.w, acc[i].w);
+                }
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (r >= rows) return;
+    if (l != l) m = 0.f;                                 // (a NaN among the scores: the range counts, and makes the row NaN)
+    const size_t slot = ((size_t)token * a.Hq + kvh * G + at % G) * (a.prefix_splits + a.own_splits) + (PREFIX ? split : a.prefix_splits + split);
+    if (c == 0) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = 4 * c + 32 * i;
+        if (d < hd) *reinterpret_cast<float4*>(a.part_o + slot * hd + d) = acc[i];
+    }
+}
+
+// One warp per (token, head).
+template <typename T>
+__global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
+    pdl_wait();
+    const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (item >= (long)a.tokens * a.Hq) return;
+    const int t = (int)(item / a.Hq);
+    const int g = group_of(a, t);
+    if (g < 0) return;                                   // rows behind the last group are left as they are
+    const int splits = a.prefix_splits + a.own_splits;
+    const int s0 = a.prefix_lens[g] > 0 ? 0 : a.prefix_splits;      // without a prefix nobody wrote its ranges
+    const float* ml = a.part_ml + (size_t)item * splits * 2;
+    float m = -INFINITY;
+    for (int s = s0 + lane; s < splits; s += 32) m = fmaxf(m, ml[2 * s]);
+    m = warp_max(m);
+    float l = 0.f;
+    for (int s = s0 + lane; s < splits; s += 32) if (ml[2 * s] != -INFINITY) l += ml[2 * s + 1] * exp2f(ml[2 * s] - m);
+    l = warp_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f; // a row that saw no key: zeros
+    for (int d = lane; d < a.hd; d += 32) {
+        float o = 0.f;
+        for (int s = s0; s < splits; ++s) {
+            const float ms = ml[2 * s];
+            if (ms != -INFINITY) o = fmaf(a.part_o[((size_t)item * splits + s) * a.hd + d], exp2f(ms - m), o);
+        }
+        ((T*)a.out)[(size_t)item * a.hd + d] = from_f32<T>(o * inv);
+    }
+}
+
+template <typename T>
+int launch_general(const SharedArgs& a, long prefix_tiles, cudaStream_t stream) {
+    static SharedLimits limits[2];
+    const int G = a.Hq / a.Hkv, head_tiles = (G + kRows - 1) / kRows, ld = a.hd + 4;
+    const size_t smem = (size_t)((kRows + 2 * kKeys) * ld + kRows * (kKeys + 1)) * sizeof(float);
+    int rc = ensure_dynamic_smem(shared_general_kernel<T, true>, smem, limits[0]);
+    if (rc == 0) rc = ensure_dynamic_smem(shared_general_kernel<T, false>, smem, limits[1]);
+    if (rc == 0 && prefix_tiles > 0)
+        rc = launch_pdl(shared_general_kernel<T, true>, dim3((unsigned)prefix_tiles, a.Hkv, a.prefix_splits), dim3(kThreads), smem, stream, a, head_tiles);
+    if (rc == 0)
+        rc = launch_pdl(shared_general_kernel<T, false>, dim3((unsigned)a.tokens * head_tiles, a.Hkv, a.own_splits), dim3(kThreads), smem, stream, a, head_tiles);
+    return rc;
+}
+}  // namespace
+
+// q: [tokens, Hq, hd], rows q_stride elements apart; caches [pages, page_size, Hkv, hd]; block_table [requests, bt_cols].
+// part_o: float32 [tokens * Hq * (prefix_splits + own_splits) * hd], part_ml [.. * 2].  Key j of a token: page block_table[its
+// request][j / page_size]; keys below its group's prefix_len through the table of the group's first token.
+extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_cache, const void* v_cache, void* out,
+                                   const int* block_table, long bt_stride, int bt_cols, int requests, const int* token_req,
+                                   const int* positions, const int* group_start, const int* prefix_lens, int groups, float* part_o,
+                                   float* part_ml, long pages, int tokens, int Hq, int Hkv, int hd, int page_size, int prefix_splits,
+                                   int own_splits, float scale, int* error, int dtype, void* stream) {
+    if (tokens <= 0 || groups <= 0) return kOk;
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || hd <= 0 || hd % 8 != 0 || hd > 256 || page_size <= 0 || prefix_splits < 1 || own_splits < 1) return kBadSize;
+    if (Hkv > 65535 || prefix_splits > 65535 || own_splits > 65535) return kTooLarge;
+    SharedArgs a{q, q_stride, k_cache, v_cache, out, block_table, bt_stride, bt_cols, requests, token_req, positions, group_start,
+                 prefix_lens, groups, part_o, part_ml, pages, tokens, Hq, Hkv, hd, page_size, prefix_splits, own_splits,
+                 scale * 1.4426950408889634f, error};
+    const int G = Hq / Hkv;
+    // a group's last tile may be part full: at most one more tile per group, and no group without a token has one
+    const long tiles = (long)tokens * G / kRows + (groups < tokens ? groups : tokens);
+    if ((long)tokens * ((G + kRows - 1) / kRows) > 0x7fffffffL || tiles > 0x7fffffffL) return kTooLarge;
+    const cudaStream_t s = (cudaStream_t)stream;
+    int rc = kBadDType;
+    LB_DISPATCH_DTYPE(dtype, rc = launch_general<T>(a, tiles, s);
+                      if (rc == 0) rc = launch_pdl(shared_merge_kernel<T>, dim3((unsigned)(((long)tokens * Hq + 7) / 8)), dim3(256), 0, s, a));
+    return rc != 0 ? rc : launch_status();
+}

@@ -450,6 +450,72 @@ def attention_decode_listed(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     return out
 
 
+def shared_splits(tokens: int, num_heads: int, num_kv_heads: int, max_prefix: int, max_own: int) -> tuple[int, int]:
+    """(ranges of the prefix's keys, ranges of a token's own keys) for `attention_decode_shared`."""
+    group = num_heads // num_kv_heads
+    tiles = max(1, -(-tokens * group // 16) * num_kv_heads)
+    items = max(1, tokens * -(-group // 16) * num_kv_heads)
+    cut = lambda n, keys: max(1, min(_SPLIT_TARGET_CTAS // n, -(-keys // 64), 64))       # noqa: E731
+    return cut(tiles, max_prefix), cut(items, max_own)
+
+
+def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                            token_req: torch.Tensor, positions: torch.Tensor, group_start: torch.Tensor, prefix_lens: torch.Tensor,
+                            scale: float, *, max_prefix: int, max_context: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`attention_decode` for tokens whose requests begin with the same keys, which are read once for all of them.  The same q
+    [tokens, Hq, hd] (rotated queries; the row stride is free), caches [pages, page_size, Hkv, hd] (every key and value, the tokens'
+    own included, is there already), block_table [requests, columns], token_req and positions (int32 per token), and the same result:
+    a token sees the keys 0 .. its position of its request.
+
+    `group_start` (int32 [groups + 1], ascending) and `prefix_lens` (int32 [groups]): tokens group_start[g] .. group_start[g + 1] - 1
+    are of requests whose first prefix_lens[g] keys are the same (0: nothing in common); these are read through the table row of the
+    group's first token, and what lies behind them through each token's own.  A request's row may name the same pages or copies of
+    them.  A group's tokens may stand inside of the prefix, belong to any requests and be several of one request.  Rows of no group
+    are left as they are (in `out`; otherwise unwritten).  A row without keys (position -1; a request or pages that are not there)
+    becomes zeros.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right too.
+
+    bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits."""
+    _cuda(q, k_cache, v_cache, block_table, token_req, positions, group_start, prefix_lens, out)
+    _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
+    tokens, Hq, hd = q.shape
+    _need(q.stride(2) == 1 and (q.stride(1) == hd or Hq == 1), "a token's queries must lie side by side")
+    _need(k_cache.dim() == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape
+          and k_cache.dtype == q.dtype == v_cache.dtype and k_cache.shape[3] == hd,
+          "caches must be contiguous [pages, page_size, kv_heads, head_dim] of q's dtype")
+    pages, page_size, Hkv = k_cache.shape[:3]
+    code = _code(q)
+    _need(hd % 8 == 0 and 0 < hd <= 256, f"attention takes head sizes in steps of 8 up to 256, got {hd}")
+    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
+    _need(page_size > 0, "pages must hold a key at least")
+    _need(block_table.dim() == 2 and block_table.dtype == torch.int32 and (block_table.stride(1) == 1 or block_table.shape[1] <= 1),
+          "block table must be a row-major int32 matrix")
+    _need(q.device.index == torch._C._cuda_getDevice(), "q must be on the current device")
+    for t, n in ((token_req, "token_req"), (positions, "positions"), (group_start, "group_start"), (prefix_lens, "prefix_lens")):
+        _i32(t, n)
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache"), (block_table, "block_table"), (token_req, "token_req"), (positions, "positions"),
+                 (group_start, "group_start"), (prefix_lens, "prefix_lens"), (out, "out")):
+        _need(t is None or t.device == q.device, f"{n} must be on q's device")
+    _need(token_req.shape == (tokens,) == positions.shape, "one entry of token_req and positions per token")
+    _need(prefix_lens.dim() == 1 and group_start.shape == (prefix_lens.numel() + 1,), "group_start must have one entry more than prefix_lens")
+    if out is None:
+        out = torch.empty((tokens, Hq, hd), dtype=q.dtype, device=q.device)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out must be a contiguous tensor like q")
+    groups = prefix_lens.numel()
+    if tokens == 0 or groups == 0:
+        return out
+    sp, so = shared_splits(tokens, Hq, Hkv, int(max_prefix), max(1, int(max_context) - int(max_prefix)))
+    part_o = torch.empty(tokens * Hq * (sp + so) * hd, dtype=torch.float32, device=q.device)
+    part_ml = torch.empty(tokens * Hq * (sp + so) * 2, dtype=torch.float32, device=q.device)
+    f = _fn("attention_shared", "lb_attention_shared",
+            [c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+             c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p])
+    _check(f(_ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(block_table), block_table.stride(0),
+             block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(prefix_lens), groups,
+             _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, scale, _ptr(error_word(q.device)), code,
+             _stream()), "attention_decode_shared", launches=3)
+    return out
+
+
 def attention_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                       cu_seqlens: torch.Tensor, start_pos: torch.Tensor, tiles: torch.Tensor, num_tiles: int,
                       scale: float, window: int = 0, *, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -2825,3 +2891,72 @@ def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: flo
              N, width, act_scale, int(bool(gate.settled and up.settled)), _FP8_FORMS[FP8_FORM], _fp8_error_word(device), _stream()),
            "linear_swiglu_fp8", f"([{M}, {width}] x 2 x [{N}, {width}])")
     return Fp8Rows(values, scales)
+
+
+# --------------------------------------------------------------------------- requests that share one thing and own another
+def _same_place(a: torch.Tensor, b: torch.Tensor, name: str) -> None:
+    """`a` (an output) and `b` are one and the same, or share no memory."""
+    if a.data_ptr() == b.data_ptr() and a.stride() == b.stride():
+        return
+    ends = [t.data_ptr() + (sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
+    _need(ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr(), f"{name}: an output may be its input, or share no memory with it")
+
+
+def _rows_out(t: torch.Tensor, name: str) -> int:
+    """Row stride of an output matrix, whose rows must not overlap."""
+    ld = _rows_of(t, name)
+    _need(t.shape[0] <= 1 or ld >= t.shape[1], f"{name}: its rows must not overlap")
+    return ld
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
+                 scales: torch.Tensor | None = None, *, ranks: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """y + scales[i] * (x @ a[i]^T) @ b[i]^T, i = index[row]: what each row's low-rank adapter adds to `y` [rows, features], the
+    product of `x` [rows, width] with a weight that all rows share (`linear`, `linear_fp8`, a part of a wider product's columns).
+    A new tensor, or `out` (which may be `y`); rounded once, to y's dtype, sums in 32 bits.
+
+    `a` [adapters, rank, width] and `b` [adapters, features, rank], of y's dtype (bfloat16 or float32), columns side by side, other
+    strides free.  `index`: int32, one per row, in any order; a row whose index names no adapter (-1) keeps its y, whatever its x.
+    `scales`: float32, one per adapter (none: 1).  `ranks`: int32, one per adapter: how many of the `rank` rows of a[i] and columns of
+    b[i] are its own (none: all of them); the others are not read as values."""
+    _cuda(y, x, a, b, index, scales, ranks, out)
+    ldy, ldx = _rows_of(y, "y"), _rows_of(x, "x")
+    rows, features = y.shape
+    _need(a.dim() == 3 and b.dim() == 3, "a must be [adapters, rank, width] and b [adapters, features, rank]")
+    n, rank, width = a.shape
+    _need(x.shape == (rows, width), f"x must be [{rows}, {width}]")
+    _need(b.shape == (n, features, rank), f"b must be [{n}, {features}, {rank}]")
+    _need(x.dtype == y.dtype == a.dtype == b.dtype, "x, y, a and b must have one dtype")
+    code = _code(y)
+    _need((a.stride(2) == 1 or width <= 1) and (b.stride(2) == 1 or rank <= 1), "columns of a and b must lie side by side")
+    _need(max(n, rank, width, features) < 1 << 30, "more adapters, ranks or columns than the kernel counts")
+    here = y.device
+    for t, name in ((x, "x"), (a, "a"), (b, "b"), (index, "index"), (scales, "scales"), (ranks, "ranks"), (out, "out")):
+        if t is not None:
+            _need(t.device == here, f"{name} must be on y's device")
+    _i32(index, "index")
+    _need(index.shape == (rows,), "one index per row")
+    if scales is not None:
+        _need(scales.dtype == torch.float32 and scales.shape == (n,) and scales.is_contiguous(), "scales must be a contiguous float32 vector, one per adapter")
+    if ranks is not None:
+        _i32(ranks, "ranks")
+        _need(ranks.shape == (n,), "one rank per adapter")
+    if out is None:
+        out = torch.empty((rows, features), dtype=y.dtype, device=here)
+    else:
+        _need(out.shape == y.shape and out.dtype == y.dtype, "out must match y")
+        _same_place(out, y, "out")
+    ldo = _rows_out(out, "out")
+    if rows == 0 or features == 0:
+        return out
+    parts = _fn("adapters", "lb_adapter_parts", [c_long, c_int, c_int])
+    parts = parts(rows, width, rank)
+    h = torch.empty(max(1, parts * rows * rank), dtype=torch.float32, device=here)
+    f = _fn("adapters", "lb_add_adapters",
+            [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
+             c_long, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
+    _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
+             _ptr(ranks), _ptr(out), ldo, _ptr(h), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
+           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=2)
+    return out
