@@ -9,6 +9,8 @@
 // This file: the general form, for float32, any page size and head sizes in steps of 8 up to 256, and the merge.
 #include "lb200/common.cuh"
 #include "lb200/attention_shared.h"
+#include "lb200/attention_shared_own.cuh"
+#include "lb200/attention_shared_tc.cuh"
 using namespace lb200;
 
 namespace {
@@ -188,6 +190,23 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
     }
 }
 
+// Do the tensor-core forms take the call?  (Else: the general form.)
+bool tc_ok(const SharedArgs& a, int dtype) {
+    return dtype == kBF16 && (a.hd == 64 || a.hd == 128) && a.page_size % 64 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
+           (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
+}
+// 256 rows to a tile where the groups have so many on average: a tile of keys is fetched once for all of them
+bool two_ok(long tokens, int G, int groups) { return tokens * G >= 192L * groups; }
+
+int launch_tc(const SharedArgs& a, cudaStream_t stream) {
+    const bool two = two_ok(a.tokens, a.Hq / a.Hkv, a.groups);
+    int rc;
+    if (a.hd == 64) rc = two ? shared_tc::launch_prefix<64, true>(a, stream) : shared_tc::launch_prefix<64, false>(a, stream);
+    else rc = two ? shared_tc::launch_prefix<128, true>(a, stream) : shared_tc::launch_prefix<128, false>(a, stream);
+    if (rc == 0) rc = a.hd == 64 ? shared_own::launch_own<64>(a, stream) : shared_own::launch_own<128>(a, stream);
+    return rc;
+}
+
 template <typename T>
 int launch_general(const SharedArgs& a, long prefix_tiles, cudaStream_t stream) {
     static SharedLimits limits[2];
@@ -202,6 +221,23 @@ int launch_general(const SharedArgs& a, long prefix_tiles, cudaStream_t stream) 
     return rc;
 }
 }  // namespace
+
+// (ranges of the prefix's keys) << 16 | ranges of a token's own keys: so many that the grids fill the SMs, each with some keys left.
+extern "C" int lb_attention_shared_splits(const void* q, long q_stride, const void* k_cache, const void* v_cache, long pages, int tokens,
+                                          int Hq, int Hkv, int hd, int page_size, int groups, long max_prefix, long max_own, int dtype) {
+    if (tokens <= 0 || groups <= 0 || Hkv <= 0 || Hq < Hkv) return 1 << 16 | 1;
+    SharedArgs a{};
+    a.q = q; a.q_stride = q_stride; a.k_cache = k_cache; a.v_cache = v_cache; a.pages = pages; a.hd = hd; a.page_size = page_size;
+    const int G = Hq / Hkv;
+    const bool tc = tc_ok(a, dtype);
+    const long tile = !tc ? kRows : two_ok(tokens, G, groups) ? 256 : 128;
+    const long tiles = (((long)tokens * G + tile - 1) / tile + (groups - 1) / 2) * Hkv, items = (long)tokens * ((G + 15) / 16) * Hkv;
+    auto cut = [](long ctas, long n, long keys, long least) {
+        const long most = keys / least < 1 ? 1 : keys / least, want = ctas / n < 1 ? 1 : ctas / n;
+        return (int)(want > most ? (most > 64 ? 64 : most) : want > 64 ? 64 : want);
+    };
+    return cut(tc ? 148 : 592, tiles, max_prefix, tc ? 128 : 64) << 16 | cut(tc ? 296 : 592, items, max_own, tc ? 128 : 64);
+}
 
 // q: [tokens, Hq, hd], rows q_stride elements apart; caches [pages, page_size, Hkv, hd]; block_table [requests, bt_cols].
 // part_o: float32 [tokens * Hq * (prefix_splits + own_splits) * hd], part_ml [.. * 2].  Key j of a token: page block_table[its
@@ -223,7 +259,7 @@ extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_c
     if ((long)tokens * ((G + kRows - 1) / kRows) > 0x7fffffffL || tiles > 0x7fffffffL) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     int rc = kBadDType;
-    LB_DISPATCH_DTYPE(dtype, rc = launch_general<T>(a, tiles, s);
+    LB_DISPATCH_DTYPE(dtype, rc = tc_ok(a, dtype) ? launch_tc(a, s) : launch_general<T>(a, tiles, s);
                       if (rc == 0) rc = launch_pdl(shared_merge_kernel<T>, dim3((unsigned)(((long)tokens * Hq + 7) / 8)), dim3(256), 0, s, a));
     return rc != 0 ? rc : launch_status();
 }

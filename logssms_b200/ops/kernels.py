@@ -450,15 +450,6 @@ def attention_decode_listed(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     return out
 
 
-def shared_splits(tokens: int, num_heads: int, num_kv_heads: int, max_prefix: int, max_own: int) -> tuple[int, int]:
-    """(ranges of the prefix's keys, ranges of a token's own keys) for `attention_decode_shared`."""
-    group = num_heads // num_kv_heads
-    tiles = max(1, -(-tokens * group // 16) * num_kv_heads)
-    items = max(1, tokens * -(-group // 16) * num_kv_heads)
-    cut = lambda n, keys: max(1, min(_SPLIT_TARGET_CTAS // n, -(-keys // 64), 64))       # noqa: E731
-    return cut(tiles, max_prefix), cut(items, max_own)
-
-
 def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                             token_req: torch.Tensor, positions: torch.Tensor, group_start: torch.Tensor, prefix_lens: torch.Tensor,
                             scale: float, *, max_prefix: int, max_context: int, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -503,7 +494,11 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     groups = prefix_lens.numel()
     if tokens == 0 or groups == 0:
         return out
-    sp, so = shared_splits(tokens, Hq, Hkv, int(max_prefix), max(1, int(max_context) - int(max_prefix)))
+    f = _fn("attention_shared", "lb_attention_shared_splits",
+            [c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_int])
+    splits = f(_ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), pages, tokens, Hq, Hkv, hd, page_size, groups, int(max_prefix),
+               int(max_context) - int(max_prefix), code)
+    sp, so = splits >> 16, splits & 0xffff
     part_o = torch.empty(tokens * Hq * (sp + so) * hd, dtype=torch.float32, device=q.device)
     part_ml = torch.empty(tokens * Hq * (sp + so) * 2, dtype=torch.float32, device=q.device)
     f = _fn("attention_shared", "lb_attention_shared",
