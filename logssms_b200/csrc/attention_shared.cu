@@ -33,20 +33,17 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     int first, rows, request, begin, end;                // the rows: token first + (row0 + r) / G, head kvh * G + (row0 + r) % G
     long row0;
     if (PREFIX) {
-        int g, n;
-        if (!find_tile(a, blockIdx.x, G, kRows, &g, &row0, &first, &n)) return;
+        int n;
+        if (!find_tile(a, blockIdx.x, G, kRows, &end, &row0, &first, &n)) return;
         rows = (int)min((long)kRows, (long)n * G - row0);
         request = a.token_req[first];
         begin = 0;
-        end = a.prefix_lens[g];
     } else {
         first = blockIdx.x / head_tiles;
         row0 = (long)(blockIdx.x % head_tiles) * kRows;
         rows = (int)min((long)kRows, (long)G - row0);
-        const int g = group_of(a, first);
-        if (g < 0) return;
+        if (!prefix_of(a, first, &begin)) return;
         request = a.token_req[first];
-        begin = max(a.prefix_lens[g], 0);
         end = a.positions[first] + 1;
     }
     const bool known = request >= 0 && request < a.requests;
@@ -160,34 +157,62 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     }
 }
 
-// One warp per (token, head).
+// One warp per (token, head): the ranges' weights first, a lane each, then their rows, 16 bytes a lane and several on their way.
+template <typename T> __device__ __forceinline__ void store4(T* p, const float4& v);
+template <> __device__ __forceinline__ void store4<float>(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
+template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16* p, const float4& v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
     pdl_wait();
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (item >= (long)a.tokens * a.Hq) return;
-    const int t = (int)(item / a.Hq);
-    const int g = group_of(a, t);
-    if (g < 0) return;                                   // rows behind the last group are left as they are
+    int prefix;
+    if (!prefix_of(a, (int)(item / a.Hq), &prefix)) return;         // rows of no group are left as they are
     const int splits = a.prefix_splits + a.own_splits;
-    const int s0 = a.prefix_lens[g] > 0 ? 0 : a.prefix_splits;      // without a prefix nobody wrote its ranges
-    const float* ml = a.part_ml + (size_t)item * splits * 2;
-    float m = -INFINITY;
-    for (int s = s0 + lane; s < splits; s += 32) m = fmaxf(m, ml[2 * s]);
-    m = warp_max(m);
-    float l = 0.f;
-    for (int s = s0 + lane; s < splits; s += 32) if (ml[2 * s] != -INFINITY) l += ml[2 * s + 1] * exp2f(ml[2 * s] - m);
-    l = warp_sum(l);
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f; // a row that saw no key: zeros
-    for (int d = lane; d < a.hd; d += 32) {
-        float o = 0.f;
-        for (int s = s0; s < splits; ++s) {
-            const float ms = ml[2 * s];
-            if (ms != -INFINITY) o = fmaf(a.part_o[((size_t)item * splits + s) * a.hd + d], exp2f(ms - m), o);
+    const int s0 = prefix > 0 ? 0 : a.prefix_splits;     // without a prefix nobody wrote its ranges
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)item * splits;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) + (size_t)item * splits * (a.hd >> 2);
+    float m = -INFINITY, l = 0.f;                        // 32 ranges at a time; what is there already is scaled to a new maximum
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    const int pieces = a.hd >> 2;
+    for (int base = s0; base < splits; base += 32) {
+        const float2 mine = base + lane < splits ? ml[base + lane] : make_float2(-INFINITY, 0.f);
+        const float top = fmaxf(m, warp_max(mine.x)), ref = top == -INFINITY ? 0.f : top;
+        const float before = exp2f(m - ref), w = exp2f(mine.x - ref);
+        l = l * before + warp_sum(mine.y * w);
+        m = top;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) { o[h].x *= before; o[h].y *= before; o[h].z *= before; o[h].w *= before; }
+        const int n = min(32, splits - base);
+        for (int s = 0; s < n; s += 4) {
+            float4 v[4][2];
+            float f[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f[u] = s + u < n ? __shfl_sync(0xffffffffu, w, (s + u) & 31) : 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)              // (a range without keys left nothing to read)
+                    v[u][h] = f[u] != 0.f && lane + 32 * h < pieces ? po[(size_t)(base + s + u) * pieces + lane + 32 * h] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    o[h].x = fmaf(v[u][h].x, f[u], o[h].x); o[h].y = fmaf(v[u][h].y, f[u], o[h].y);
+                    o[h].z = fmaf(v[u][h].z, f[u], o[h].z); o[h].w = fmaf(v[u][h].w, f[u], o[h].w);
+                }
         }
-        ((T*)a.out)[(size_t)item * a.hd + d] = from_f32<T>(o * inv);
     }
+    const float inv = l != 0.f ? 1.f / l : 0.f;          // a row that saw no key: zeros
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (lane + 32 * h < pieces)
+            store4((T*)a.out + (size_t)item * a.hd + 4 * (lane + 32 * h), make_float4(o[h].x * inv, o[h].y * inv, o[h].z * inv, o[h].w * inv));
 }
 
 // Do the tensor-core forms take the call?  (Else: the general form.)
@@ -195,14 +220,35 @@ bool tc_ok(const SharedArgs& a, int dtype) {
     return dtype == kBF16 && (a.hd == 64 || a.hd == 128) && a.page_size % 64 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
            (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
 }
-// 256 rows to a tile where the groups have so many on average: a tile of keys is fetched once for all of them
-bool two_ok(long tokens, int G, int groups) { return tokens * G >= 192L * groups; }
+// How the prefix's work is laid out on the tensor cores: rows of a tile, CTAs of a cluster, clusters for a tile's keys.
+struct Layout { bool two; int ranks, clusters; };
+Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_prefix) {
+    // us: a tile of 64 keys takes 0.85 with 256 rows and 0.6 where the groups share the tiles out; a CTA's beginning and end
+    // 5; a row of partial results is written and read at 4 TB/s.  As many CTAs at once as the GPU holds in clusters of that size.
+    const long kt = max_prefix > 0 ? (max_prefix + 63) / 64 : 1;
+    Layout best{false, 1, 1};
+    double least = 1e30;
+    for (int two = 0; two < 2; ++two) {
+        const long rows = two ? 256 : 128, tiles = ((tokens * G + rows - 1) / rows + (groups - 1) / 2) * Hkv;
+        for (int k = 0; k < 4; ++k) {
+            const int ranks = 1 << k;
+            const long room = k == 0 ? 148 : k == 1 ? 148 : k == 2 ? 132 : 120;
+            long clusters = room / (tiles * ranks);
+            if (clusters > (kt + ranks - 1) / ranks) clusters = (kt + ranks - 1) / ranks;
+            if (clusters < 1) clusters = 1;
+            if (clusters > 64) clusters = 64;
+            const long per = (kt + clusters * ranks - 1) / (clusters * ranks), waves = (tiles * ranks * clusters + room - 1) / room;
+            const double us = waves * (5.0 + per * (two ? 0.85 : 0.6)) + clusters * tokens * G * Hkv * hd * 8e-6 / 4.0 + 0.2 * k;
+            if (us < least) { least = us; best = {two != 0, ranks, (int)clusters}; }
+        }
+    }
+    return best;
+}
 
-int launch_tc(const SharedArgs& a, cudaStream_t stream) {
-    const bool two = two_ok(a.tokens, a.Hq / a.Hkv, a.groups);
+int launch_tc(const SharedArgs& a, const Layout& y, cudaStream_t stream) {
     int rc;
-    if (a.hd == 64) rc = two ? shared_tc::launch_prefix<64, true>(a, stream) : shared_tc::launch_prefix<64, false>(a, stream);
-    else rc = two ? shared_tc::launch_prefix<128, true>(a, stream) : shared_tc::launch_prefix<128, false>(a, stream);
+    if (a.hd == 64) rc = y.two ? shared_tc::launch_prefix<64, true>(a, y.ranks, stream) : shared_tc::launch_prefix<64, false>(a, y.ranks, stream);
+    else rc = y.two ? shared_tc::launch_prefix<128, true>(a, y.ranks, stream) : shared_tc::launch_prefix<128, false>(a, y.ranks, stream);
     if (rc == 0) rc = a.hd == 64 ? shared_own::launch_own<64>(a, stream) : shared_own::launch_own<128>(a, stream);
     return rc;
 }
@@ -222,7 +268,8 @@ int launch_general(const SharedArgs& a, long prefix_tiles, cudaStream_t stream) 
 }
 }  // namespace
 
-// (ranges of the prefix's keys) << 16 | ranges of a token's own keys: so many that the grids fill the SMs, each with some keys left.
+// How many partial results a row has: (of the prefix) << 16 | (of its own keys); so many that the grids fill the SMs, each with some
+// keys left.
 extern "C" int lb_attention_shared_splits(const void* q, long q_stride, const void* k_cache, const void* v_cache, long pages, int tokens,
                                           int Hq, int Hkv, int hd, int page_size, int groups, long max_prefix, long max_own, int dtype) {
     if (tokens <= 0 || groups <= 0 || Hkv <= 0 || Hq < Hkv) return 1 << 16 | 1;
@@ -230,13 +277,13 @@ extern "C" int lb_attention_shared_splits(const void* q, long q_stride, const vo
     a.q = q; a.q_stride = q_stride; a.k_cache = k_cache; a.v_cache = v_cache; a.pages = pages; a.hd = hd; a.page_size = page_size;
     const int G = Hq / Hkv;
     const bool tc = tc_ok(a, dtype);
-    const long tile = !tc ? kRows : two_ok(tokens, G, groups) ? 256 : 128;
-    const long tiles = (((long)tokens * G + tile - 1) / tile + (groups - 1) / 2) * Hkv, items = (long)tokens * ((G + 15) / 16) * Hkv;
+    const long tiles = (((long)tokens * G + kRows - 1) / kRows + (groups - 1) / 2) * Hkv, items = (long)tokens * ((G + 15) / 16) * Hkv;
     auto cut = [](long ctas, long n, long keys, long least) {
-        const long most = keys / least < 1 ? 1 : keys / least, want = ctas / n < 1 ? 1 : ctas / n;
+        const long most = keys / least < 1 ? 1 : keys / least, want = (ctas + n - 1) / n;
         return (int)(want > most ? (most > 64 ? 64 : most) : want > 64 ? 64 : want);
     };
-    return cut(tc ? 148 : 592, tiles, max_prefix, tc ? 128 : 64) << 16 | cut(tc ? 296 : 592, items, max_own, tc ? 128 : 64);
+    const int prefix = tc ? layout_for(tokens, G, Hkv, hd, groups, max_prefix).clusters : cut(592, tiles, max_prefix, 64);
+    return prefix << 16 | cut(tc ? 2368 : 592, items, max_own, tc ? 256 : 64);
 }
 
 // q: [tokens, Hq, hd], rows q_stride elements apart; caches [pages, page_size, Hkv, hd]; block_table [requests, bt_cols].
@@ -246,7 +293,8 @@ extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_c
                                    const int* block_table, long bt_stride, int bt_cols, int requests, const int* token_req,
                                    const int* positions, const int* group_start, const int* prefix_lens, int groups, float* part_o,
                                    float* part_ml, long pages, int tokens, int Hq, int Hkv, int hd, int page_size, int prefix_splits,
-                                   int own_splits, float scale, int* error, int dtype, void* stream) {
+                                   int own_splits, long max_prefix, float scale, int* error, int dtype,
+                                   void* stream) {
     if (tokens <= 0 || groups <= 0) return kOk;
     if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || hd <= 0 || hd % 8 != 0 || hd > 256 || page_size <= 0 || prefix_splits < 1 || own_splits < 1) return kBadSize;
     if (Hkv > 65535 || prefix_splits > 65535 || own_splits > 65535) return kTooLarge;
@@ -254,12 +302,12 @@ extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_c
                  prefix_lens, groups, part_o, part_ml, pages, tokens, Hq, Hkv, hd, page_size, prefix_splits, own_splits,
                  scale * 1.4426950408889634f, error};
     const int G = Hq / Hkv;
-    // a group's last tile may be part full: at most one more tile per group, and no group without a token has one
-    const long tiles = (long)tokens * G / kRows + (groups < tokens ? groups : tokens);
+    const long tiles = most_tiles((long)tokens * G, groups < tokens ? groups : tokens, kRows);
     if ((long)tokens * ((G + kRows - 1) / kRows) > 0x7fffffffL || tiles > 0x7fffffffL) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     int rc = kBadDType;
-    LB_DISPATCH_DTYPE(dtype, rc = tc_ok(a, dtype) ? launch_tc(a, s) : launch_general<T>(a, tiles, s);
+    Layout y = layout_for(tokens, G, Hkv, hd, groups, max_prefix);
+    LB_DISPATCH_DTYPE(dtype, rc = tc_ok(a, dtype) ? launch_tc(a, y, s) : launch_general<T>(a, tiles, s);
                       if (rc == 0) rc = launch_pdl(shared_merge_kernel<T>, dim3((unsigned)(((long)tokens * Hq + 7) / 8)), dim3(256), 0, s, a));
     return rc != 0 ? rc : launch_status();
 }

@@ -1,6 +1,7 @@
 // Operands of the kernels for attention over a shared prefix (attention_shared.cu), and who belongs to which group.
 #pragma once
 #include <cuda_runtime.h>
+#include "lb200/per_device.h"
 
 namespace lb200 {
 
@@ -19,19 +20,35 @@ struct SharedArgs {
     int* error;
 };
 
-// The tile `target` of the tiles of `per_tile` (token, head) rows that each group's tokens make, group by group: its group, its
-// first row within the group, the group's tokens.  Called by whole warps; false: there is no such tile.
-__device__ __forceinline__ bool find_tile(const SharedArgs& a, long target, int rows_per_token, int per_tile, int* group, long* row0,
+// An SM on which the kernel runs has all of its shared memory as such (and CTAs of another kernel find room beside it), on each
+// device by itself.
+template <typename Kernel>
+inline int whole_carveout(Kernel kernel) {
+    static AskedOnce done;
+    int device = 0;
+    const int rc = (int)cudaGetDevice(&device);
+    if (rc != 0) return rc;
+    return done.get(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
+}
+
+// At most so many tiles of `per_tile` rows hold `rows` rows of `groups` groups, none of them empty.  (No more: a CTA that finds no tile
+// to do still has to find room on an SM before the kernel behind may start.)
+inline long most_tiles(long rows, long groups, long per_tile) { return (rows + groups * (per_tile - 1)) / per_tile; }
+
+// The tile `target` of the tiles of `per_tile` (token, head) rows that each group's tokens make, group by group: its group's prefix
+// and tokens, its first row within the group.  Called by whole warps; false: there is no such tile.
+__device__ __forceinline__ bool find_tile(const SharedArgs& a, long target, int rows_per_token, int per_tile, int* prefix, long* row0,
                                           int* first, int* tokens) {
     const int lane = threadIdx.x & 31;
     long before = 0;
     for (int base = 0; base < a.groups; base += 32) {
         const int g = base + lane;
-        int t0 = 0, n = 0;
+        int t0 = 0, n = 0, p = 0;
         if (g < a.groups) {
+            p = a.prefix_lens[g];
             t0 = min(max(a.group_start[g], 0), a.tokens);
             n = max(min(max(a.group_start[g + 1], 0), a.tokens) - t0, 0);
-            if (a.prefix_lens[g] <= 0) n = 0;
+            if (p <= 0) n = 0;
         }
         const long mine = ((long)n * rows_per_token + per_tile - 1) / per_tile;
         long upto = mine;
@@ -43,7 +60,7 @@ __device__ __forceinline__ bool find_tile(const SharedArgs& a, long target, int 
         const unsigned hit = __ballot_sync(0xffffffffu, before + upto > target);
         if (hit != 0) {
             const int who = __ffs(hit) - 1;
-            *group = base + who;
+            *prefix = __shfl_sync(0xffffffffu, p, who);
             *row0 = (target - before - __shfl_sync(0xffffffffu, upto - mine, who)) * per_tile;
             *first = __shfl_sync(0xffffffffu, t0, who);
             *tokens = __shfl_sync(0xffffffffu, n, who);
@@ -54,14 +71,26 @@ __device__ __forceinline__ bool find_tile(const SharedArgs& a, long target, int 
     return false;
 }
 
-// The group of a token, or -1.
-__device__ __forceinline__ int group_of(const SharedArgs& a, int t) {
+// The shared prefix of a token's group; false: the token is of no group.  Called by whole warps: up to 32 groups are looked through
+// at once, more by halves.
+__device__ __forceinline__ bool prefix_of(const SharedArgs& a, int t, int* prefix) {
+    if (a.groups <= 32) {
+        const int lane = threadIdx.x & 31;
+        int from = 0, to = 0, p = 0;
+        if (lane < a.groups) { from = a.group_start[lane]; to = a.group_start[lane + 1]; p = a.prefix_lens[lane]; }
+        const unsigned hit = __ballot_sync(0xffffffffu, t >= from && t < to);
+        if (hit == 0) return false;
+        *prefix = max(__shfl_sync(0xffffffffu, p, __ffs(hit) - 1), 0);
+        return true;
+    }
     int lo = 0, hi = a.groups;                           // the last group that starts at or in front of t
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (a.group_start[mid] <= t) lo = mid + 1; else hi = mid;
     }
-    return lo > 0 && t < a.group_start[lo] ? lo - 1 : -1;
+    if (lo == 0 || t >= a.group_start[lo]) return false;
+    *prefix = max(a.prefix_lens[lo - 1], 0);
+    return true;
 }
 
 }  // namespace lb200
