@@ -2,26 +2,18 @@
 //   out[t] = y[t] + scale_a * (x[t] A_a^T) B_a^T,   a = index[t]   (rows without an adapter: out[t] = y[t])
 // x [T, K], y and out [T, N], A [adapters, R, K], B [adapters, N, R], an adapter's rank up to R.
 //
-// The general form, for every type, size and stride: tiles of 32 rows, one pass for each adapter that a tile's rows name (a
-// tile of a prompt names one or two), products in float32 registers.  `shrink` leaves h = x A^T per part of K in float32,
-// `expand` adds the parts up in their order, multiplies by the scale and adds to y: one rounding, of the output.
+// bfloat16: adapters_rows.cuh (decoding rows, any order of adapters) and adapters_tiles.cuh (prompts).  This file: the float32
+// form (and that of ranks over 256), and the choice between them.  Tiles of 32 rows, one pass for each adapter that a tile's rows name, products in float32
+// registers.  `shrink` leaves h = x A^T per part of K, `expand` adds the parts up in their order, multiplies by the scale and
+// adds to y: one rounding, of the output.
 #include "lb200/common.cuh"
 #include "lb200/adapters.cuh"
+#include "lb200/adapters_rows.cuh"
 using namespace lb200;
 
 namespace {
 constexpr int kRows = 32, kCols = 64, kChunk = 32;      // rows, ranks or features of a tile; values of K or R at a time
 constexpr int kThreads = 128;                           // 8 groups of 4 rows x 16 groups of 4 columns
-
-// The smallest adapter behind `prev` that any of the warp's rows names (INT_MAX: none).
-__device__ __forceinline__ int next_adapter(int mine, int prev) { return __reduce_min_sync(0xffffffffu, mine > prev ? mine : 0x7fffffff); }
-
-__device__ __forceinline__ int adapter_of(const AdapterArgs& a, long t) {
-    if (t >= a.T) return -1;
-    const int i = a.index[t];
-    return i >= 0 && i < a.adapters ? i : -1;
-}
-__device__ __forceinline__ int rank_of(const AdapterArgs& a, int i) { return a.ranks ? min(max(a.ranks[i], 0), a.R) : a.R; }
 
 // acc[4][4] += rows of `p` (kRows from its first, ld elements apart) times rows of `q` (kCols), over `depth` values
 struct Tiles { float p[kChunk][kRows + 4]; float q[kChunk][kCols + 4]; };
@@ -58,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) adapter_shrink_kernel(AdapterArgs a)
     const int mine = adapter_of(a, t0 + (tid & 31));
     const int r4 = (tid >> 4) * 4, c4 = (tid & 15) * 4;
     const T* x = (const T*)a.x;
-    for (int i = next_adapter(mine, -1); i != 0x7fffffff; i = next_adapter(mine, i)) {
+    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i)) {
         const int rank = rank_of(a, i);
         if (j0 >= rank) continue;
         const T* A = (const T*)a.A + (size_t)i * a.a_adapter;
@@ -87,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) adapter_expand_kernel(AdapterArgs a)
     const int mine = adapter_of(a, t0 + (tid & 31));
     const int r4 = (tid >> 4) * 4, c4 = (tid & 15) * 4;
     float sum[4][4] = {};
-    for (int i = next_adapter(mine, -1); i != 0x7fffffff; i = next_adapter(mine, i)) {
+    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i)) {
         const int rank = rank_of(a, i);
         const T* B = (const T*)a.B + (size_t)i * a.b_adapter;
         const float scale = a.scales ? a.scales[i] : 1.f;
@@ -137,6 +129,7 @@ extern "C" int lb_adapter_parts(long T, int K, int R) {
 }
 
 // h: float32 scratch [parts, T, R].  Strides in elements; columns lie side by side.  out may be y.
+// (h: float32 only.)
 extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row,
                                const void* B, long b_adapter, long b_row, const int* index, const float* scales, const int* ranks,
                                void* out, long ldo, float* h, int parts, long T, int K, int N, int R, int adapters, int dtype,
@@ -148,6 +141,7 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
                   parts, (K + parts - 1) / parts};
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
-    LB_DISPATCH_DTYPE(dtype, return launch_general<T>(a, s))
-    return kBadDType;
+    if (dtype == kF32) return launch_general<float>(a, s);
+    if (dtype != kBF16) return kBadDType;
+    return R <= adapter_rows::kMostRanks ? adapter_rows::launch(a, s) : launch_general<__nv_bfloat16>(a, s);
 }

@@ -1,5 +1,6 @@
 // Operands of the adapters' kernels (adapters.cu).
 #pragma once
+#include <cuda_runtime.h>
 
 namespace lb200 {
 
@@ -15,5 +16,16 @@ struct AdapterArgs {
     long T;
     int K, N, R, adapters, parts, part_k;
 };
+
+// The smallest adapter behind `prev` that any of the warp's rows names (INT_MAX: none).
+constexpr int kNoAdapter = 0x7fffffff;
+__device__ __forceinline__ int next_adapter(int mine, int prev) { return __reduce_min_sync(0xffffffffu, mine > prev ? mine : kNoAdapter); }
+
+__device__ __forceinline__ int adapter_of(const AdapterArgs& a, long t) {
+    if (t >= a.T) return -1;
+    const int i = a.index[t];
+    return i >= 0 && i < a.adapters ? i : -1;
+}
+__device__ __forceinline__ int rank_of(const AdapterArgs& a, int i) { return a.ranks ? min(max(a.ranks[i], 0), a.R) : a.R; }
 
 }  // namespace lb200

@@ -2889,12 +2889,15 @@ def linear_swiglu_fp8(x: Fp8Rows, gate: Fp8Weight, up: Fp8Weight, act_scale: flo
 
 
 # --------------------------------------------------------------------------- requests that share one thing and own another
+def _apart(a: torch.Tensor, b: torch.Tensor, name: str) -> None:
+    ends = [t.data_ptr() + (sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
+    _need(a.numel() == 0 or b.numel() == 0 or ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr(), f"{name} must not share memory")
+
+
 def _same_place(a: torch.Tensor, b: torch.Tensor, name: str) -> None:
     """`a` (an output) and `b` are one and the same, or share no memory."""
-    if a.data_ptr() == b.data_ptr() and a.stride() == b.stride():
-        return
-    ends = [t.data_ptr() + (sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() for t in (a, b)]
-    _need(ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr(), f"{name}: an output may be its input, or share no memory with it")
+    if a.data_ptr() != b.data_ptr() or a.stride() != b.stride():
+        _apart(a, b, f"{name} and its input, unless they are the same,")
 
 
 def _rows_out(t: torch.Tensor, name: str) -> int:
@@ -2943,15 +2946,17 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
         _need(out.shape == y.shape and out.dtype == y.dtype, "out must match y")
         _same_place(out, y, "out")
     ldo = _rows_out(out, "out")
+    _apart(out, x, "out and x")
     if rows == 0 or features == 0:
         return out
-    parts = _fn("adapters", "lb_adapter_parts", [c_long, c_int, c_int])
-    parts = parts(rows, width, rank)
-    h = torch.empty(max(1, parts * rows * rank), dtype=torch.float32, device=here)
+    parts, h = 1, None
+    if y.dtype == torch.float32 or rank > 256:             # two kernels, with the short sums between them
+        parts = _fn("adapters", "lb_adapter_parts", [c_long, c_int, c_int])(rows, width, rank)
+        h = torch.empty(max(1, parts * rows * rank), dtype=torch.float32, device=here)
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
              c_long, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
              _ptr(ranks), _ptr(out), ldo, _ptr(h), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
-           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=2)
+           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None else 2)
     return out
