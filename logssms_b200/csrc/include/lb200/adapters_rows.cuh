@@ -1,8 +1,9 @@
-// Adapters of decoding rows, bfloat16: one launch, a cluster of 8 CTAs for 1 to 8 rows.
+// Adapters of decoding rows, bfloat16: one launch, a cluster of 4 or 8 CTAs for 1 to 8 rows.
 //
 // Bound by reading the adapters (a row's rank x (K + N) numbers) and by the chain of a call's steps.  So both products are in one
-// kernel: a CTA multiplies its eighth of K, the eight sums meet in distributed shared memory (added in the CTAs' order), and every
-// CTA adds its eighth of the features to y.  Rows are columns of m16n8k16 products whose rows are ranks (A) or features (B): the
+// kernel: a CTA multiplies its part of K, hands its sums to all CTAs of the cluster (which add them up in the CTAs' order), and adds
+// its part of the features to y.  What does not hang on something before it is asked for early: the first features of B and y are on
+// their way while the sums are handed over.  Rows are columns of m16n8k16 products whose rows are ranks (A) or features (B): the
 // adapters are read as they lie in memory, 16 or 8 bytes a lane (the lanes' pieces are what the product takes as its k, in an order
 // that both operands share).  Rows of a cluster that name the same adapter share its reading.  The warps share out the adapters that
 // the cluster's rows name, and then the parts of K or the features, so that all of them are read at the same time; a warp's products
@@ -17,7 +18,7 @@
 namespace lb200 {
 namespace adapter_rows {
 typedef __nv_bfloat16 bf16;
-constexpr int kCluster = 8, kWarps = 8, kThreads = 32 * kWarps, kRows = 8;
+constexpr int kMostParts = 8, kWarps = 8, kThreads = 32 * kWarps, kRows = 8;
 constexpr int kMostRanks = 256;
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -45,10 +46,8 @@ __device__ __forceinline__ void load(uint32_t (&r)[N / 2], const bf16* row, int 
     }
 }
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ float remote(uint32_t at, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %1, %2;\n\tld.shared::cluster.f32 %0, [p];\n\t}" : "=f"(v) : "r"(at), "r"(rank) : "memory");
-    return v;
+__device__ __forceinline__ void hand(uint32_t at, uint32_t rank, float v) {
+    asm volatile("{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %0, %1;\n\tst.shared::cluster.f32 [p], %2;\n\t}" ::"r"(at), "r"(rank), "f"(v) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -56,26 +55,25 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // grid: clusters, each with rows_per rows.  MT: 16 MT ranks at a time.  XV: rows of x and A lie on 16 bytes and K is a multiple of 8;
 // BV: rows of B on 8 bytes, R a multiple of 4.
 template <int MT, bool XV, bool BV>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) __cluster_dims__(kCluster, 1, 1)
-adapter_rows_kernel(AdapterArgs a, int rows_per) {
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel(AdapterArgs a, int rows_per, int parts) {
     constexpr int kRanks = 16 * MT;
     constexpr int kUnits = MT == 4 ? 1 : 2;                // units of K, or of features, on their way (twice as many features)
     pdl_wait();
     __shared__ float part[kWarps][kRanks][kRows];         // the warps' sums of some ranks
-    __shared__ float mine[kMostRanks][kRows];             // this CTA's
-    __shared__ __align__(16) uint32_t high[kRows][kMostRanks / 2 + 4], low[kRows][kMostRanks / 2 + 4];      // all CTAs', times the scale
+    __shared__ __align__(16) uint32_t high[kRows][kMostRanks / 2 + 4], low[kRows][kMostRanks / 2 + 4];      // the sums times the scale
+    extern __shared__ float handed[];                     // [parts][ranks][kRows]: the CTAs' sums
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
-    const uint32_t rank = blockIdx.x % kCluster;
-    const long t0 = (long)(blockIdx.x / kCluster) * rows_per;
+    const int rank = (int)(blockIdx.x % (unsigned)parts), padded = (a.R + 15) / 16 * 16;
+    const long t0 = (long)(blockIdx.x / (unsigned)parts) * rows_per;
     const int rows = (int)min((long)rows_per, a.T - t0);
     const bf16* x = (const bf16*)a.x + (t0 + min(n, rows - 1)) * a.ldx;          // row n of the columns
     const bf16* y = (const bf16*)a.y;
     bf16* out = (bf16*)a.out;
     // this CTA's part of K, in units of 32, and of the features, in units of 16
-    const int k_units = (a.K + 31) / 32, k_per = (k_units + kCluster - 1) / kCluster;
-    const int k_from = min((int)rank * k_per, k_units), k_to = min(k_from + k_per, k_units);
-    const int n_units = (a.N + 15) / 16, n_per = (n_units + kCluster - 1) / kCluster;
-    const int n_from = min((int)rank * n_per, n_units), n_to = min(n_from + n_per, n_units);
+    const int k_units = (a.K + 31) / 32, k_per = (k_units + parts - 1) / parts;
+    const int k_from = min(rank * k_per, k_units), k_to = min(k_from + k_per, k_units);
+    const int n_units = (a.N + 15) / 16, n_per = (n_units + parts - 1) / parts;
+    const int n_from = min(rank * n_per, n_units), n_to = min(n_from + n_per, n_units);
     // the adapters that the rows name, in ascending order, and each row's place among them (0 for a row without one)
     const int own = lane < rows ? adapter_of(a, t0 + lane) : -1;                 // of row `lane`
     int adapters = 0, place = 0;
@@ -85,6 +83,7 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
             for (int r = 0; r < rows; ++r) out[(t0 + r) * a.ldo + i] = y[(t0 + r) * a.ldy + i];
         return;
     }
+    cluster_arrive();                                      // this CTA is there
     // warps take turns at them: 8 / shares warps for each
     const int shares = adapters > 4 ? 8 : adapters > 2 ? 4 : adapters, ours = warp & (shares - 1), team = warp / shares, teams = kWarps / shares;
     const unsigned named = __ballot_sync(0xffffffffu, own >= 0 && place == ours);
@@ -94,10 +93,11 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
     const bool ours_n = i >= 0 && __shfl_sync(0xffffffffu, own, n) == i;
 
     // ------------------------------------------------------------ ranks x rows: this warp's units of K
+    // (all of A's ranks: each has a sum of its own, and those behind the adapter's own are left out later)
     for (int j0 = 0; j0 < a.R; j0 += kRanks) {
         const int tiles = min((a.R - j0 + 15) / 16, MT);   // of 16 ranks
         float sum[MT][4] = {};
-        if (j0 < ranks) {
+        if (i >= 0) {
             const bf16* A = (const bf16*)a.A + (size_t)i * a.a_adapter + (size_t)j0 * a.a_row;
             for (int u = k_from + team; u < k_to; u += kUnits * teams) {
                 uint32_t xv[kUnits][4], av[kUnits][MT][2][4];
@@ -108,8 +108,8 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         const int r = 16 * m + n;
-                        load<XV, 8>(av[h][m][0], A + (size_t)r * a.a_row, k, j0 + r < ranks ? end : 0);
-                        load<XV, 8>(av[h][m][1], A + (size_t)(r + 8) * a.a_row, k, j0 + r + 8 < ranks ? end : 0);
+                        load<XV, 8>(av[h][m][0], A + (size_t)r * a.a_row, k, j0 + r < a.R ? end : 0);
+                        load<XV, 8>(av[h][m][1], A + (size_t)(r + 8) * a.a_row, k, j0 + r + 8 < a.R ? end : 0);
                     }
                 }
 #pragma unroll
@@ -128,18 +128,26 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
             *reinterpret_cast<float2*>(&part[warp][16 * m + n + 8][2 * c]) = make_float2(sum[m][2], sum[m][3]);
         }
         __syncthreads();
+        if (j0 == 0) cluster_wait();                       // every CTA is there
         for (int e = threadIdx.x; e < 16 * tiles * kRows; e += kThreads) {       // (a thread's row is lane % 8)
+            if ((lane & 7) >= rows) continue;
             float v = 0.f;
             for (int w = place_n; w < kWarps; w += shares) v += part[w][e / kRows][e % kRows];
-            mine[j0 + e / kRows][e % kRows] = v;
+            const uint32_t at = smem_at(handed + (rank * padded + j0) * kRows + e);
+            for (int p = 0; p < parts; ++p) hand(at, p, v);
         }
     }
-    // ------------------------------------------------------------ the first features are on their way while the CTAs' sums meet
+    if (a.R <= 0) cluster_wait();
+    cluster_arrive();                                      // the sums are handed over
+    // ------------------------------------------------------------ the first features and y's are on their way in the meantime
+    // The rows that are this warp's to write: those of its adapter, and the first adapter's warps write rows without one.
     constexpr int kAhead = 2 * kUnits;
+    const int own0 = __shfl_sync(0xffffffffu, own, 2 * c), own1 = __shfl_sync(0xffffffffu, own, 2 * c + 1);
+    const bool write0 = 2 * c < rows && (own0 >= 0 ? own0 == i : ours == 0), write1 = 2 * c + 1 < rows && (own1 >= 0 ? own1 == i : ours == 0);
     const bf16* B = (const bf16*)a.B + (size_t)max(i, 0) * a.b_adapter;
     uint32_t bv[kAhead][MT][2][2];
     auto features = [&](int u, int j0) {                   // ranks j0 .. of the features of units u, u + teams, ...
-        const int here = min(ranks - j0, kRanks), end = BV ? (here + 3) & ~3 : here;
+        const int end = min(a.R - j0, kRanks);
 #pragma unroll
         for (int h = 0; h < kAhead; ++h)
 #pragma unroll
@@ -148,38 +156,40 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
                 const bool there = u + h * teams < n_to;
                 load<BV, 4>(bv[h][m][0], B + (size_t)f * a.b_row + j0, j, there && f < a.N ? end : 0);
                 load<BV, 4>(bv[h][m][1], B + (size_t)(f + 8) * a.b_row + j0, j, there && f + 8 < a.N ? end : 0);
-                if (BV && j + 4 > here) {                  // (columns behind the adapter's rank may hold anything)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint32_t keep = (j + 2 * q < here ? 0xffffu : 0u) | (j + 2 * q + 1 < here ? 0xffff0000u : 0u);
-                        bv[h][m][0][q] &= keep;
-                        bv[h][m][1][q] &= keep;
-                    }
-                }
             }
     };
-    features(n_from + team, 0);
-    cluster_arrive();
+    bf16 yv[kAhead][4];
+    auto outputs = [&](int u) {
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
+                if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N) yv[h][e] = y[(t0 + 2 * c + (e & 1)) * a.ldy + f];
+            }
+    };
+    const int u0 = n_from + team;
+    if (i >= 0) { features(u0, 0); outputs(u0); }
+    const int who = lane < 8 ? own : -1;                   // (a thread's row in the next loop is lane % 8 again)
+    const int its = __shfl_sync(0xffffffffu, who >= 0 ? rank_of(a, who) : 0, lane & 7);
+    const float scale = __shfl_sync(0xffffffffu, who >= 0 && a.scales ? a.scales[who] : 1.f, lane & 7);
     cluster_wait();
-    const int padded = (a.R + 15) / 16 * 16;
     for (int e = threadIdx.x; e < padded / 2 * kRows; e += kThreads) {           // two ranks of a row each
         const int r = e % kRows, j = 2 * (e / kRows);
-        const int who = r < rows ? adapter_of(a, t0 + r) : -1;
         float v[2] = {0.f, 0.f};
-        if (who >= 0) {
-            float got[2][kCluster];
+        if (j < its) {                                     // (nothing for a row without an adapter)
+            float got[2][kMostParts];
 #pragma unroll
-            for (int p = 0; p < kCluster; ++p) {
-                got[0][p] = remote(smem_at(&mine[j][r]), p);
-                got[1][p] = remote(smem_at(&mine[j + 1][r]), p);
-            }
-            const float scale = a.scales ? a.scales[who] : 1.f;
-            const int its = rank_of(a, who);
+            for (int p = 0; p < kMostParts; ++p)
+                if (p < parts) {
+                    got[0][p] = handed[(p * padded + j) * kRows + r];
+                    got[1][p] = handed[(p * padded + j + 1) * kRows + r];
+                }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 float total = 0.f;
 #pragma unroll
-                for (int p = 0; p < kCluster; ++p) total += got[q][p];
+                for (int p = 0; p < kMostParts; ++p) if (p < parts) total += got[q][p];
                 v[q] = j + q < its ? total * scale : 0.f;
             }
         }
@@ -189,70 +199,82 @@ adapter_rows_kernel(AdapterArgs a, int rows_per) {
         high[r][j / 2] = *reinterpret_cast<const uint32_t*>(&h);
         low[r][j / 2] = *reinterpret_cast<const uint32_t*>(&l);
     }
-    cluster_arrive();                                      // this CTA has read the others' sums
     __syncthreads();
     // ------------------------------------------------------------ features x rows, 16 features to a product
-    // The rows that are this warp's to write: those of its adapter, and the first adapter's warps write rows without one.
-    const int own0 = __shfl_sync(0xffffffffu, own, 2 * c), own1 = __shfl_sync(0xffffffffu, own, 2 * c + 1);
-    const bool write0 = 2 * c < rows && (own0 >= 0 ? own0 == i : ours == 0), write1 = 2 * c + 1 < rows && (own1 >= 0 ? own1 == i : ours == 0);
-    if (i >= 0) {
-        for (int u = n_from + team; u < n_to; u += kAhead * teams) {
-            bf16 yv[kAhead][4];
+    if (i < 0) return;
+    for (int u = u0; u < n_to; u += kAhead * teams) {
+        if (u != u0) outputs(u);
+        float sum[kAhead][4] = {};
+        for (int j0 = 0; j0 < ranks; j0 += kRanks) {
+            if (u != u0 || j0 > 0) features(u, j0);
+            if (ranks - j0 < kRanks && ranks < a.R) {      // columns behind the adapter's rank may hold anything
 #pragma unroll
-            for (int h = 0; h < kAhead; ++h)
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
-                    if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N) yv[h][e] = y[(t0 + 2 * c + (e & 1)) * a.ldy + f];
-                }
-            float sum[kAhead][4] = {};
-            for (int j0 = 0; j0 < ranks; j0 += kRanks) {
-                if (u != n_from + team || j0 > 0) features(u, j0);
+                    for (int q = 0; q < 2; ++q) {
+                        const int j = j0 + 16 * m + 4 * c + 2 * q;
+                        const uint32_t keep = (j < ranks ? 0xffffu : 0u) | (j + 1 < ranks ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int at = j0 / 2 + 8 * m + 2 * c;
-                    if (16 * m < ranks - j0) {             // (behind the rank nothing was written)
-                        const uint2 h = ours_n ? *reinterpret_cast<const uint2*>(&high[n][at]) : make_uint2(0u, 0u);
-                        const uint2 l = ours_n ? *reinterpret_cast<const uint2*>(&low[n][at]) : make_uint2(0u, 0u);
+                        for (int h = 0; h < kAhead; ++h) { bv[h][m][0][q] &= keep; bv[h][m][1][q] &= keep; }
+                    }
+            }
 #pragma unroll
-                        for (int w = 0; w < kAhead; ++w) {
-                            mma(sum[w], bv[w][m][0][0], bv[w][m][1][0], bv[w][m][0][1], bv[w][m][1][1], h.x, h.y);
-                            mma(sum[w], bv[w][m][0][0], bv[w][m][1][0], bv[w][m][0][1], bv[w][m][1][1], l.x, l.y);
-                        }
+            for (int m = 0; m < MT; ++m) {
+                const int at = j0 / 2 + 8 * m + 2 * c;
+                if (16 * m < ranks - j0) {                 // (behind the rank nothing was written)
+                    const uint2 h = ours_n ? *reinterpret_cast<const uint2*>(&high[n][at]) : make_uint2(0u, 0u);
+                    const uint2 l = ours_n ? *reinterpret_cast<const uint2*>(&low[n][at]) : make_uint2(0u, 0u);
+#pragma unroll
+                    for (int w = 0; w < kAhead; ++w) {
+                        mma(sum[w], bv[w][m][0][0], bv[w][m][1][0], bv[w][m][0][1], bv[w][m][1][1], h.x, h.y);
+                        mma(sum[w], bv[w][m][0][0], bv[w][m][1][0], bv[w][m][0][1], bv[w][m][1][1], l.x, l.y);
                     }
                 }
             }
-#pragma unroll
-            for (int h = 0; h < kAhead; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
-                    if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N)
-                        out[(t0 + 2 * c + (e & 1)) * a.ldo + f] = (e & 1 ? own1 : own0) >= 0 ? __float2bfloat16_rn(__bfloat162float(yv[h][e]) + sum[h][e]) : yv[h][e];
-                }
         }
+#pragma unroll
+        for (int h = 0; h < kAhead; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
+                if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N)
+                    out[(t0 + 2 * c + (e & 1)) * a.ldo + f] = (e & 1 ? own1 : own0) >= 0 ? __float2bfloat16_rn(__bfloat162float(yv[h][e]) + sum[h][e]) : yv[h][e];
+            }
     }
-    cluster_wait();                                        // nobody leaves while another CTA reads its sums
 }
 
-template <bool XV, bool BV>
-inline int launch_as(const AdapterArgs& a, dim3 grid, int rows_per, cudaStream_t stream) {
-    if (a.R <= 16) return launch_pdl(adapter_rows_kernel<1, XV, BV>, grid, dim3(kThreads), 0, stream, a, rows_per);
-    if (a.R <= 32) return launch_pdl(adapter_rows_kernel<2, XV, BV>, grid, dim3(kThreads), 0, stream, a, rows_per);
-    return launch_pdl(adapter_rows_kernel<4, XV, BV>, grid, dim3(kThreads), 0, stream, a, rows_per);
-}
-
-inline int launch(const AdapterArgs& a, cudaStream_t stream) {
-    // about 64 clusters, which are all at work at once, while there are rows for them
+template <int MT, bool XV, bool BV>
+inline int launch_as(const AdapterArgs& a, cudaStream_t stream) {
+    // About 64 clusters while there are rows for them; of 8 CTAs where all of them are on an SM at once, else of 4.
     int rows_per = 1;
     while (rows_per < kRows && a.T > 64 * rows_per) rows_per *= 2;
     const long clusters = (a.T + rows_per - 1) / rows_per;
-    if (clusters * kCluster > 0x7fffffffL) return kTooLarge;
-    const dim3 grid((unsigned)(clusters * kCluster));
+    const int parts = clusters <= 40 ? 8 : 4;
+    if (clusters * parts > 0x7fffffffL) return kTooLarge;
+    const size_t smem = (size_t)parts * ((a.R + 15) / 16 * 16) * kRows * sizeof(float);
+    static SharedLimits limits;
+    int rc = ensure_dynamic_smem(adapter_rows_kernel<MT, XV, BV>, smem + 25 * 1024, limits);        // (with what it has besides)
+    if (rc != 0) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV>, a, rows_per, parts);
+}
+template <bool XV, bool BV>
+inline int launch_loads(const AdapterArgs& a, cudaStream_t stream) {
+    return a.R <= 16 ? launch_as<1, XV, BV>(a, stream) : a.R <= 32 ? launch_as<2, XV, BV>(a, stream) : launch_as<4, XV, BV>(a, stream);
+}
+
+inline int launch(const AdapterArgs& a, cudaStream_t stream) {
     const bool xv = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.A & 15) == 0 && a.ldx % 8 == 0 && a.a_row % 8 == 0 && a.a_adapter % 8 == 0 && a.K % 8 == 0;
     const bool bv = ((uintptr_t)a.B & 7) == 0 && a.b_row % 4 == 0 && a.b_adapter % 4 == 0 && a.R % 4 == 0;
-    const int rc = xv ? bv ? launch_as<true, true>(a, grid, rows_per, stream) : launch_as<true, false>(a, grid, rows_per, stream)
-                      : bv ? launch_as<false, true>(a, grid, rows_per, stream) : launch_as<false, false>(a, grid, rows_per, stream);
+    const int rc = xv ? bv ? launch_loads<true, true>(a, stream) : launch_loads<true, false>(a, stream)
+                      : bv ? launch_loads<false, true>(a, stream) : launch_loads<false, false>(a, stream);
     return rc != 0 ? rc : launch_status();
 }
 
