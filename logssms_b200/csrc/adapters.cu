@@ -9,6 +9,7 @@
 #include "lb200/common.cuh"
 #include "lb200/adapters.cuh"
 #include "lb200/adapters_rows.cuh"
+#include "lb200/adapters_tiles.cuh"
 using namespace lb200;
 
 namespace {
@@ -128,11 +129,14 @@ extern "C" int lb_adapter_parts(long T, int K, int R) {
     return (int)(want < 1 ? 1 : want > most ? most : want > 32 ? 32 : want);
 }
 
+// From so many rows on a call goes to the tiles' kernel.
+constexpr long kTileRows = 384;
+
 // h: float32 scratch [parts, T, R].  Strides in elements; columns lie side by side.  out may be y.
-// (h: float32 only.)
+// (h: float32, or ranks over 256.)  marks: int32 scratch, one per 128 rows; error: the device's error word.
 extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row,
                                const void* B, long b_adapter, long b_row, const int* index, const float* scales, const int* ranks,
-                               void* out, long ldo, float* h, int parts, long T, int K, int N, int R, int adapters, int dtype,
+                               void* out, long ldo, float* h, int* marks, int* error, int parts, long T, int K, int N, int R, int adapters, int dtype,
                                void* stream) {
     if (T <= 0 || N <= 0) return kOk;
     if (K < 0 || R < 0 || adapters < 0 || parts < 1) return kBadSize;
@@ -143,5 +147,8 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == kF32) return launch_general<float>(a, s);
     if (dtype != kBF16) return kBadDType;
-    return R <= adapter_rows::kMostRanks ? adapter_rows::launch(a, s) : launch_general<__nv_bfloat16>(a, s);
+    if (R > adapter_rows::kMostRanks) return launch_general<__nv_bfloat16>(a, s);
+    if (T < kTileRows || marks == nullptr || !adapter_tiles::takes(a)) return adapter_rows::launch(a, nullptr, s);
+    const int rc = adapter_tiles::launch(a, marks, error, s);
+    return rc != 0 ? rc : adapter_rows::launch(a, marks, s);       // what was left to it, if anything
 }

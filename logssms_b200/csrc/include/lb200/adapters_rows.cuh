@@ -52,19 +52,17 @@ __device__ __forceinline__ void hand(uint32_t at, uint32_t rank, float v) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// grid: clusters, each with rows_per rows.  MT: 16 MT ranks at a time.  XV: rows of x and A lie on 16 bytes and K is a multiple of 8;
+// The rows t0 .. t0 + rows_per - 1.  MT: 16 MT ranks at a time.  XV: rows of x and A lie on 16 bytes and K is a multiple of 8;
 // BV: rows of B on 8 bytes, R a multiple of 4.
 template <int MT, bool XV, bool BV>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel(AdapterArgs a, int rows_per, int parts) {
+__device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int rows_per, int parts) {
     constexpr int kRanks = 16 * MT;
     constexpr int kUnits = MT == 4 ? 1 : 2;                // units of K, or of features, on their way (twice as many features)
-    pdl_wait();
     __shared__ float part[kWarps][kRanks][kRows];         // the warps' sums of some ranks
     __shared__ __align__(16) uint32_t high[kRows][kMostRanks / 2 + 4], low[kRows][kMostRanks / 2 + 4];      // the sums times the scale
     extern __shared__ float handed[];                     // [parts][ranks][kRows]: the CTAs' sums
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
     const int rank = (int)(blockIdx.x % (unsigned)parts), padded = (a.R + 15) / 16 * 16;
-    const long t0 = (long)(blockIdx.x / (unsigned)parts) * rows_per;
     const int rows = (int)min((long)rows_per, a.T - t0);
     const bf16* x = (const bf16*)a.x + (t0 + min(n, rows - 1)) * a.ldx;          // row n of the columns
     const bf16* y = (const bf16*)a.y;
@@ -243,17 +241,41 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel
     }
 }
 
-template <int MT, bool XV, bool BV>
-inline int launch_as(const AdapterArgs& a, cudaStream_t stream) {
+// grid: clusters, each with rows_per rows; or (MARKED) which go through the blocks of rows_per rows of the marked tiles of 128.
+// (A CTA is past the first barrier of a block only when all are done with the one before.)
+template <int MT, bool XV, bool BV, bool MARKED>
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel(AdapterArgs a, int rows_per, int parts, const int* marks, int tiles) {
+    pdl_wait();
+    const int cluster = (int)(blockIdx.x / (unsigned)parts), clusters = (int)(gridDim.x / (unsigned)parts);
+    if constexpr (!MARKED) {
+        block_of_rows<MT, XV, BV>(a, (long)cluster * rows_per, rows_per, parts);
+        return;
+    }
+    const int lane = threadIdx.x & 31, blocks = 128 / rows_per;
+    int turn = cluster;                                    // of the blocks of all marked tiles, this cluster's are cluster, + clusters, ...
+    for (int base = 0; base < tiles; base += 32) {
+        unsigned marked = __ballot_sync(0xffffffffu, base + lane < tiles && marks[base + lane] != 0);
+        for (; marked != 0; marked &= marked - 1, turn -= blocks) {
+            const long first = (long)(base + __ffs(marked) - 1) * 128;
+            for (; turn < blocks; turn += clusters) {
+                const long t0 = first + (long)turn * rows_per;
+                if (t0 < a.T) block_of_rows<MT, XV, BV>(a, t0, rows_per, parts);
+            }
+        }
+    }
+}
+
+template <int MT, bool XV, bool BV, bool MARKED>
+inline int launch_as(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
     // About 64 clusters while there are rows for them; of 8 CTAs where all of them are on an SM at once, else of 4.
     int rows_per = 1;
     while (rows_per < kRows && a.T > 64 * rows_per) rows_per *= 2;
-    const long clusters = (a.T + rows_per - 1) / rows_per;
-    const int parts = clusters <= 40 ? 8 : 4;
+    const long clusters = MARKED ? 64 : (a.T + rows_per - 1) / rows_per;
+    const int parts = clusters <= 40 ? 8 : 4, tiles = MARKED ? (int)((a.T + 127) / 128) : 0;
     if (clusters * parts > 0x7fffffffL) return kTooLarge;
     const size_t smem = (size_t)parts * ((a.R + 15) / 16 * 16) * kRows * sizeof(float);
     static SharedLimits limits;
-    int rc = ensure_dynamic_smem(adapter_rows_kernel<MT, XV, BV>, smem + 25 * 1024, limits);        // (with what it has besides)
+    int rc = ensure_dynamic_smem(adapter_rows_kernel<MT, XV, BV, MARKED>, smem + 25 * 1024, limits);        // (with what it has besides)
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
@@ -263,18 +285,24 @@ inline int launch_as(const AdapterArgs& a, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV>, a, rows_per, parts);
+    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV, MARKED>, a, rows_per, parts, marks, tiles);
+}
+template <bool XV, bool BV, bool MARKED>
+inline int launch_ranks(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
+    return a.R <= 16 ? launch_as<1, XV, BV, MARKED>(a, marks, stream) : a.R <= 32 ? launch_as<2, XV, BV, MARKED>(a, marks, stream)
+                                                                                  : launch_as<4, XV, BV, MARKED>(a, marks, stream);
 }
 template <bool XV, bool BV>
-inline int launch_loads(const AdapterArgs& a, cudaStream_t stream) {
-    return a.R <= 16 ? launch_as<1, XV, BV>(a, stream) : a.R <= 32 ? launch_as<2, XV, BV>(a, stream) : launch_as<4, XV, BV>(a, stream);
+inline int launch_loads(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
+    return marks != nullptr ? launch_ranks<XV, BV, true>(a, marks, stream) : launch_ranks<XV, BV, false>(a, marks, stream);
 }
 
-inline int launch(const AdapterArgs& a, cudaStream_t stream) {
+// `marks` (null: all rows): which tiles of 128 rows are meant.
+inline int launch(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
     const bool xv = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.A & 15) == 0 && a.ldx % 8 == 0 && a.a_row % 8 == 0 && a.a_adapter % 8 == 0 && a.K % 8 == 0;
     const bool bv = ((uintptr_t)a.B & 7) == 0 && a.b_row % 4 == 0 && a.b_adapter % 4 == 0 && a.R % 4 == 0;
-    const int rc = xv ? bv ? launch_loads<true, true>(a, stream) : launch_loads<true, false>(a, stream)
-                      : bv ? launch_loads<false, true>(a, stream) : launch_loads<false, false>(a, stream);
+    const int rc = xv ? bv ? launch_loads<true, true>(a, marks, stream) : launch_loads<true, false>(a, marks, stream)
+                      : bv ? launch_loads<false, true>(a, marks, stream) : launch_loads<false, false>(a, marks, stream);
     return rc != 0 ? rc : launch_status();
 }
 

@@ -1,0 +1,462 @@
+// Adapters of prompts, bfloat16, on the 5th-generation tensor cores: tiles of 128 rows, one launch.
+//
+// Bound by reading x and y and writing the output once: the products are a tenth of that.  A cluster of 1 to 8 CTAs (as many as make
+// about as many CTAs as there are SMs) has a tile.  Each CTA multiplies its part of K (x and A by TMA, 64 columns a stage, one product
+// for each adapter that the tile's rows name, at most four: their A tiles lie side by side as one B operand); the CTAs' sums meet in
+// distributed shared memory, each CTA adding up a part of the rows and handing them, times the scale and as two bfloat16 numbers
+// (value and remainder), to all; then each CTA goes through its part of the features, 128 at a time: y by TMA into shared memory, the
+// product of the short sums with B beside it, and the rows of y that name the adapter get its product added in place, from where TMA
+// stores them.  Rows of one adapter never see another's product: it is made for all 128 rows and kept by those that name it.
+//
+// 12 warps: TMA loads, products, one that clears what lies behind an adapter's rank in B (0 x NaN would be NaN), TMA stores, and two
+// groups of 128 threads, a thread per row, which take the tiles of features in turn.
+//
+// A tile whose rows name more adapters than that (decoding rows in front of a prompt) is marked, and left to the rows' kernel.
+#pragma once
+#include "lb200/adapters.cuh"
+#include "lb200/common.cuh"
+#include "lb200/tcgen05.cuh"
+
+namespace lb200 {
+namespace adapter_tiles {
+using namespace tc;
+typedef __nv_bfloat16 bf16;
+constexpr int kRows = 128, kCols = 128, kMost = 4;        // rows and features of a tile, adapters
+constexpr int kFirstAdder = 4, kThreads = 32 * (kFirstAdder + 8);
+constexpr uint32_t kXTile = kRows * 128, kYTile = 2 * kRows * 128;
+
+// RB: blocks of 64 ranks
+template <int RB> struct Shape {
+    static constexpr int kY = RB == 1 ? 3 : 2, kB = RB == 1 ? 3 : 2;             // tiles of y and B on their way or at work
+    static constexpr uint32_t kBTile = RB * kCols * 128, kH = RB * kRows * 128;  // bytes; of the short sums' values (remainders the same)
+    static constexpr uint32_t kSums = kRows * (RB * 64 + 4) * 4;                 // this CTA's sums, float32
+    static constexpr uint32_t kRings = kY * kYTile + kB * kBTile;
+    // short sums | y ring | B ring, and this CTA's sums behind them or (two blocks) over the rings, which are filled afterwards then
+    static constexpr bool kOver = RB == 2;
+    static constexpr uint32_t kWork = 2 * kH + (kOver ? (kRings > kSums ? kRings : kSums) : kRings + kSums);
+    static constexpr uint32_t kSmem = kWork + 1024;
+    static constexpr int kMostStages = 8;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+struct TileArgs {
+    AdapterArgs a;
+    int* marks;                                           // per tile: 1, left to the rows' kernel
+    int parts, padded;                                    // CTAs of a cluster; ranks, filled up to a multiple of 16
+    int* error;
+};
+
+__device__ __forceinline__ void report(int* error, int role, int step) { atomicCAS(error, 0, (role << 24) | ((blockIdx.x & 0xFFF) << 12) | (step & 0xFFF) | 0x40000000); }
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 remote4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void hand2(uint32_t addr, uint32_t x, uint32_t y) {
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_u32(src)) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// grid: tiles x parts; a cluster: a tile's parts
+template <int RB>
+__global__ void __launch_bounds__(kThreads)
+adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, TileArgs ta) {
+    pdl_wait();
+    typedef Shape<RB> Sh;
+    const AdapterArgs& a = ta.a;
+    extern __shared__ __align__(1024) uint8_t base[];      // (the swizzle goes by the address)
+    uint8_t* h_s = base;                                  // values: blocks of 64 ranks, [128][128 B]; then remainders
+    uint8_t* y_s = h_s + 2 * Sh::kH;
+    uint8_t* b_s = y_s + Sh::kY * kYTile;
+    float* sums = reinterpret_cast<float*>(Sh::kOver ? y_s : b_s + Sh::kB * Sh::kBTile);
+    uint8_t* ring = y_s;                                  // the first product's: x tile, then the adapters' A tiles
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base + Sh::kWork);
+    uint64_t* x_full = bars;                              // [kMostStages]
+    uint64_t* x_empty = x_full + Sh::kMostStages;
+    uint64_t* low_ready = x_empty + Sh::kMostStages;      // the first product is done
+    uint64_t* b_full = low_ready + 1;
+    uint64_t* b_clear = b_full + Sh::kB;                  // ... and has nothing behind its adapter's rank
+    uint64_t* b_empty = b_clear + Sh::kB;
+    uint64_t* y_full = b_empty + Sh::kB;
+    uint64_t* y_empty = y_full + Sh::kY;
+    uint64_t* y_done = y_empty + Sh::kY;                  // the sums are in y's place (128 arrivals)
+    uint64_t* d_full = y_done + Sh::kY;                   // [4]: per group of adders two accumulators
+    uint64_t* d_empty = d_full + 4;
+    int* list = reinterpret_cast<int*>(d_empty + 4);      // the adapters, their ranks
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(list + 2 * kMost);
+    volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)(blockIdx.x % (unsigned)ta.parts), tile = (int)(blockIdx.x / (unsigned)ta.parts);
+    const long t0 = (long)tile * kRows;
+
+    // ------------------------------------------------------------ who is in the tile (all warps alike)
+    int count = 0, who[kMost] = {};
+    {
+        int own[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) own[q] = adapter_of(a, t0 + 32 * q + lane);
+        int prev = -1;
+        while (true) {
+            int best = kNoAdapter;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) if (own[q] > prev) best = min(best, own[q]);
+            best = __reduce_min_sync(0xffffffffu, best);
+            if (best == kNoAdapter) break;
+#pragma unroll
+            for (int q = 0; q < kMost; ++q) if (q == count) who[q] = best;
+            prev = best;
+            if (++count > kMost) break;
+        }
+    }
+    if (count > kMost || count * ta.padded > 256) {        // (the whole cluster)
+        if (rank == 0 && threadIdx.x == 0) ta.marks[tile] = 1;
+        return;
+    }
+    if (rank == 0 && threadIdx.x == 0) ta.marks[tile] = 0;
+    const int n_tiles = (a.N + kCols - 1) / kCols, mine = n_tiles > rank ? (n_tiles - rank + ta.parts - 1) / ta.parts : 0;      // tiles rank, rank + parts, ...
+    const int k_tiles = count > 0 ? (a.K + 63) / 64 : 0, k_per = (k_tiles + ta.parts - 1) / ta.parts;
+    const int k_from = min(rank * k_per, k_tiles), k_n = min(k_per, k_tiles - k_from);
+    const uint32_t a_tile = ta.padded * 128, stage = kXTile + count * a_tile;    // (A tiles: multiples of 2,048 bytes)
+    const int stages = min((int)((Sh::kWork - 2 * Sh::kH) / stage), Sh::kMostStages);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Sh::kMostStages; ++s) { mbar_init(x_full + s, 1); mbar_init(x_empty + s, 1); }
+        mbar_init(low_ready, 1);
+        for (int s = 0; s < Sh::kB; ++s) { mbar_init(b_full + s, 1); mbar_init(b_clear + s, 1); mbar_init(b_empty + s, 1); }
+        for (int s = 0; s < Sh::kY; ++s) { mbar_init(y_full + s, 1); mbar_init(y_empty + s, 1); mbar_init(y_done + s, 128); }
+        for (int s = 0; s < 4; ++s) { mbar_init(d_full + s, 1); mbar_init(d_empty + s, 128); }
+        for (int q = 0; q < kMost; ++q) { list[q] = who[q]; list[kMost + q] = q < count ? rank_of(a, who[q]) : 0; }
+        *failed = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc<512>(tmem_slot);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    // a wait of a whole warp
+    auto wait = [&](uint64_t* bar, uint32_t parity, int role, int step) -> bool {
+        const bool ok = __all_sync(0xffffffffu, (mbar_test(bar, parity) || mbar_wait(bar, parity)) && !*failed);
+        if (!ok) { if (lane == 0 && !*failed) report(ta.error, role, step); *failed = 1; }
+        return ok;
+    };
+
+    // ------------------------------------------------------------ short sums: this CTA's part of K
+    int issued = 0;
+    if (warp == 0) {
+        for (int i = 0; i < k_n; ++i) {
+            const int s = i % stages;
+            if (i >= stages && !wait(x_empty + s, ((i / stages) - 1) & 1, 1, i)) break;
+            if (elect_one()) {
+                uint8_t* at = ring + s * stage;
+                mbar_expect_tx(x_full + s, stage);
+                tma_load_2d(at, &map_x, x_full + s, (k_from + i) * 64, (int)t0);
+                for (int q = 0; q < count; ++q) tma_load_3d(at + kXTile + q * a_tile, &map_a, x_full + s, (k_from + i) * 64, 0, list[q]);
+            }
+            __syncwarp();
+            issued = i + 1;
+        }
+        if (*failed) for (int i = max(0, issued - stages); i < issued; ++i) mbar_wait(x_full + i % stages, (i / stages) & 1);
+    } else if (warp == 1 && k_n > 0) {
+        const uint32_t idesc = umma_idesc(kRows, ta.padded);
+        const uint64_t desc0 = umma_desc(ring);
+        bool ok = true;
+        for (int i = 0; i < k_n && ok; ++i) {
+            const int s = i % stages;
+            ok = wait(x_full + s, (i / stages) & 1, 2, i);
+            if (!ok) break;
+            fence_after_sync();
+            if (elect_one()) {
+                const uint64_t xd = desc0 + (uint64_t)(s * (stage >> 4));
+                for (int q = 0; q < count; ++q) {
+                    const uint64_t ad = xd + ((kXTile + q * a_tile) >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_bf16(tmem + q * ta.padded, xd + 2 * k, ad + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                }
+                umma_commit(x_empty + s);
+                if (i + 1 == k_n) umma_commit(low_ready);
+            }
+            __syncwarp();
+        }
+    }
+    const int group = (warp - kFirstAdder) >> 2, r = (warp & 3) * 32 + lane;     // of an adder: its row is its lane of tensor memory
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int own = warp >= kFirstAdder ? adapter_of(a, t0 + r) : -1;
+    int place = -1;
+    if (own >= 0)
+        for (int q = 0; q < count; ++q) if (list[q] == own) place = q;
+    if (warp >= kFirstAdder && group == 0 && count > 0) {
+        float* to = sums + r * (RB * 64 + 4);
+        const bool ok = k_n <= 0 || wait(low_ready, 0, 5, 0);
+        fence_after_sync();
+        for (int j = 0; j < ta.padded; j += 16) {
+            float keep[16] = {};
+            if (ok && k_n > 0)
+                for (int q = 0; q < count; ++q) {
+                    uint32_t v[16];
+                    tmem_get16(lane_addr + q * ta.padded + j, v);
+                    if (place == q) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) keep[e] = __uint_as_float(v[e]);
+                    }
+                }
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(to + j + e) = make_float4(keep[e], keep[e + 1], keep[e + 2], keep[e + 3]);
+        }
+        fence_before_sync();
+    }
+    __syncthreads();
+    if (ta.parts > 1) cluster_meet();
+    // ------------------------------------------------------------ this CTA's part of the rows: all CTAs' sums, handed to all
+    if (warp >= kFirstAdder && count > 0) {
+        const int pieces = ta.padded / 4;                  // four ranks
+        const uint32_t from = smem_u32(sums), to = smem_u32(h_s);
+        for (int i = threadIdx.x - 32 * kFirstAdder; i < kRows / ta.parts * pieces; i += 256) {
+            const int row = rank * (kRows / ta.parts) + i / pieces, j = 4 * (i % pieces);
+            const int its = adapter_of(a, t0 + row);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (its >= 0) {
+                const uint32_t at = from + 4 * (row * (RB * 64 + 4) + j);
+                float4 got[8];
+#pragma unroll
+                for (int p = 0; p < 8; ++p) if (p < ta.parts) got[p] = remote4(ta.parts > 1 ? at_rank(at, p) : at);
+#pragma unroll
+                for (int p = 0; p < 8; ++p) if (p < ta.parts) { v.x += got[p].x; v.y += got[p].y; v.z += got[p].z; v.w += got[p].w; }
+                const float scale = a.scales ? a.scales[its] : 1.f;
+                const int ranks = rank_of(a, its);
+                v.x = j < ranks ? v.x * scale : 0.f;
+                v.y = j + 1 < ranks ? v.y * scale : 0.f;
+                v.z = j + 2 < ranks ? v.z * scale : 0.f;
+                v.w = j + 3 < ranks ? v.w * scale : 0.f;
+            }
+            const __nv_bfloat162 h0 = __floats2bfloat162_rn(v.x, v.y), h1 = __floats2bfloat162_rn(v.z, v.w);
+            const float2 b0 = __bfloat1622float2(h0), b1 = __bfloat1622float2(h1);         // (an infinity has no remainder)
+            const __nv_bfloat162 l0 = __floats2bfloat162_rn(isinf(b0.x) ? 0.f : v.x - b0.x, isinf(b0.y) ? 0.f : v.y - b0.y);
+            const __nv_bfloat162 l1 = __floats2bfloat162_rn(isinf(b1.x) ? 0.f : v.z - b1.x, isinf(b1.y) ? 0.f : v.w - b1.y);
+            // rank j of a row: block j / 64, piece (j % 64) / 8 at (that) ^ (row & 7)
+            const uint32_t at = to + (j >> 6) * (kRows * 128) + row * 128 + ((((j & 63) >> 3) ^ (row & 7)) << 4) + (j & 7) * 2;
+            for (int p = 0; p < ta.parts; ++p) {
+                const uint32_t there = ta.parts > 1 ? at_rank(at, p) : at;
+                hand2(there, *reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                hand2(there + Sh::kH, *reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+            }
+        }
+        fence_async_all();
+    }
+    __syncthreads();
+    if (ta.parts > 1) cluster_meet();
+    fence_async_all();
+
+    // ------------------------------------------------------------ this CTA's tiles of features
+    const int steps = mine * max(count, 1);                // (tile, adapter) by (tile, adapter)
+    if (warp == 0) {
+        int y_done = 0, b_done = 0;
+        for (int i = 0; i < mine && !*failed; ++i) {
+            const int n0 = (rank + i * ta.parts) * kCols, s = i % Sh::kY;
+            if (i >= Sh::kY && !wait(y_empty + s, ((i / Sh::kY) - 1) & 1, 6, i)) break;
+            if (elect_one()) {
+                mbar_expect_tx(y_full + s, kYTile);
+                tma_load_2d(y_s + s * kYTile, &map_y, y_full + s, n0, (int)t0);
+                tma_load_2d(y_s + s * kYTile + kRows * 128, &map_y, y_full + s, n0 + 64, (int)t0);
+            }
+            __syncwarp();
+            y_done = i + 1;
+            for (int q = 0; q < count; ++q) {
+                const int u = i * count + q, sb = u % Sh::kB;
+                if (u >= Sh::kB && !wait(b_empty + sb, ((u / Sh::kB) - 1) & 1, 7, u)) break;
+                if (elect_one()) {
+                    mbar_expect_tx(b_full + sb, Sh::kBTile);
+#pragma unroll
+                    for (int blk = 0; blk < RB; ++blk) tma_load_3d(b_s + sb * Sh::kBTile + blk * (kCols * 128), &map_b, b_full + sb, blk * 64, n0, list[q]);
+                }
+                __syncwarp();
+                b_done = u + 1;
+            }
+        }
+        if (*failed) {                                     // let the copies already under way land before the CTA leaves
+            for (int i = max(0, y_done - Sh::kY); i < y_done; ++i) mbar_wait(y_full + i % Sh::kY, (i / Sh::kY) & 1);
+            for (int u = max(0, b_done - Sh::kB); u < b_done; ++u) mbar_wait(b_full + u % Sh::kB, (u / Sh::kB) & 1);
+        }
+    } else if (warp == 1 && count > 0) {
+        constexpr uint32_t idesc = umma_idesc(kRows, kCols);
+        const uint64_t hd = umma_desc(h_s), bd0 = umma_desc(b_s);
+        for (int u = 0; u < steps; ++u) {
+            const int i = u / count, q = u - i * count, sb = u % Sh::kB, grp = i & 1;
+            const int v = (i >> 1) * count + q, d = 2 * grp + (v & 1);           // the group's step, its accumulator
+            if (!wait(b_clear + sb, (u / Sh::kB) & 1, 8, u)) break;
+            if (v >= 2 && !wait(d_empty + d, ((v >> 1) - 1) & 1, 9, u)) break;
+            fence_after_sync();
+            const int k_steps = (list[kMost + q] + 15) / 16;
+            if (elect_one()) {
+                const uint64_t bd = bd0 + (uint64_t)(sb * (Sh::kBTile >> 4));
+                const uint32_t to = tmem + d * kCols;
+                for (int k = 0; k < k_steps; ++k) {
+                    const uint64_t off = (uint64_t)((k >> 2) * (kRows * 128 >> 4) + 2 * (k & 3));
+                    umma_bf16(to, hd + off, bd + off, idesc, k > 0 ? 1u : 0u);
+                    umma_bf16(to, hd + (Sh::kH >> 4) + off, bd + off, idesc, 1u);
+                }
+                umma_commit(b_empty + sb);
+                umma_commit(d_full + d);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 2 && count > 0) {
+        for (int u = 0; u < steps; ++u) {
+            const int q = u % count, sb = u % Sh::kB, ranks = list[kMost + q], end = (ranks + 15) / 16 * 16;
+            if (!wait(b_full + sb, (u / Sh::kB) & 1, 10, u)) break;
+            if (ranks < a.R && ranks < end) {              // (columns behind R are zeros already)
+                uint8_t* b = b_s + sb * Sh::kBTile + (ranks >> 6) * (kCols * 128);
+                for (int f = lane; f < kCols; f += 32)
+                    for (int j = ranks; j < end; ++j)
+                        *reinterpret_cast<unsigned short*>(b + f * 128 + ((((j & 63) >> 3) ^ (f & 7)) << 4) + (j & 7) * 2) = 0;
+                fence_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_clear + sb);
+        }
+    } else if (warp == 3) {
+        // One store may still be reading its tile while the next one's sums are made; with two tiles in all it is waited for at once.
+        constexpr int kBehind = Sh::kY > 2 ? 1 : 0;
+        for (int i = 0; i < mine; ++i) {
+            const int s = i % Sh::kY, n0 = (rank + i * ta.parts) * kCols;
+            if (!wait(y_done + s, (i / Sh::kY) & 1, 13, i)) break;
+            if (lane == 0) {                               // (the same thread every time: it waits for its own stores)
+                tma_store_2d(&map_out, y_s + s * kYTile, n0, (int)t0);
+                if (n0 + 64 < a.N) tma_store_2d(&map_out, y_s + s * kYTile + kRows * 128, n0 + 64, (int)t0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBehind) : "memory");
+                if (i >= kBehind) mbar_arrive(y_empty + (i - kBehind) % Sh::kY);
+            }
+            __syncwarp();
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else if (warp >= kFirstAdder) {
+        bool ok = true;
+        for (int i = group; i < mine && ok; i += 2) {
+            const int s = i % Sh::kY;
+            ok = wait(y_full + s, (i / Sh::kY) & 1, 11, i);
+            if (!ok) break;
+            uint8_t* row = y_s + s * kYTile + r * 128;
+            for (int q = 0; q < count && ok; ++q) {
+                const int v = (i >> 1) * count + q, d = 2 * group + (v & 1);
+                ok = wait(d_full + d, (v >> 1) & 1, 12, i);
+                if (!ok) break;
+                fence_after_sync();
+                const bool any = __any_sync(0xffffffffu, place == q) && list[kMost + q] > 0;
+#pragma unroll
+                for (int piece = 0; piece < kCols / 32; ++piece) {
+                    if (!any) break;
+                    uint32_t acc[32];
+                    tmem_ld32(lane_addr + d * kCols + piece * 32, acc);
+                    if (place == q) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint4* at = reinterpret_cast<uint4*>(row + (piece >> 1) * (kRows * 128) + ((((piece & 1) * 4 + c) ^ (r & 7)) << 4));
+                            uint4 w = *at;
+                            uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float lo = __uint_as_float(e[k] << 16) + __uint_as_float(acc[8 * c + 2 * k]);
+                                const float hi = __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(acc[8 * c + 2 * k + 1]);
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+                                e[k] = *reinterpret_cast<const uint32_t*>(&b);
+                            }
+                            *at = w;
+                        }
+                    }
+                }
+                fence_before_sync();
+                mbar_arrive(d_empty + d);
+            }
+            fence_async_smem();
+            if (ok) mbar_arrive(y_done + s);
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 1) tmem_free<512>(tmem);
+}
+
+// [layers][rows][width] bfloat16 with free strides (multiples of 8 elements, base on 16 bytes): boxes of 64 x box_rows x 1, 128-byte
+// swizzle, zeros outside.
+inline int make_tile_map_3d(CUtensorMap* map, const void* ptr, long layers, long rows, long width, long layer_stride, long row_stride, int box_rows) {
+    thread_local KeyedCache<CUtensorMap, 7, 64, 8> kept;   // (weights come back step after step)
+    const KeyedCache<CUtensorMap, 7, 64, 8>::Key key = {(int64_t)(uintptr_t)ptr, layers, rows, width, layer_stride, row_stride, box_rows};
+    if (const CUtensorMap* known = kept.find(key)) {
+        *map = *known;
+        return 0;
+    }
+    EncodeTiled enc = tensor_map_encoder();
+    if (enc == nullptr) return (int)cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)layers};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)layer_stride * 2};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, 1u};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return (int)cudaErrorInvalidValue;
+    kept.put(key, *map);
+    return 0;
+}
+
+// Does the kernel take the call (apart from its number of rows)?
+inline bool takes(const AdapterArgs& a) {
+    auto lies = [](const void* p, long stride) { return ((uintptr_t)p & 15) == 0 && stride % 8 == 0; };
+    return a.R > 0 && a.R <= 128 && a.K > 0 && a.adapters > 0 && lies(a.x, a.ldx) && lies(a.y, a.ldy) && lies(a.out, a.ldo) && lies(a.A, a.a_row) &&
+           a.a_adapter % 8 == 0 && lies(a.B, a.b_row) && a.b_adapter % 8 == 0 && a.ldx >= a.K && a.ldy >= a.N && a.ldo >= a.N && a.a_row >= a.K &&
+           a.b_row >= a.R && (a.adapters == 1 || (a.a_adapter > 0 && a.b_adapter > 0));
+}
+
+template <int RB>
+inline int launch_as(const TileArgs& ta, int tiles, cudaStream_t stream) {
+    const AdapterArgs& a = ta.a;
+    CUtensorMap map_x, map_a, map_b, map_y, map_out;
+    int rc = make_tile_map(&map_x, a.x, a.T, a.K, a.ldx, kRows);
+    if (rc == 0) rc = make_tile_map_3d(&map_a, a.A, a.adapters, a.R, a.K, a.adapters > 1 ? a.a_adapter : a.a_row * a.R, a.a_row, ta.padded);
+    if (rc == 0) rc = make_tile_map_3d(&map_b, a.B, a.adapters, a.N, a.R, a.adapters > 1 ? a.b_adapter : a.b_row * a.N, a.b_row, kCols);
+    if (rc == 0) rc = make_tile_map(&map_y, a.y, a.T, a.N, a.ldy, kRows);
+    if (rc == 0) rc = make_tile_map(&map_out, a.out, a.T, a.N, a.ldo, kRows);
+    static SharedLimits limits;
+    if (rc == 0) rc = ensure_dynamic_smem(adapter_tiles_kernel<RB>, Shape<RB>::kSmem, limits);
+    if (rc != 0) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * ta.parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Shape<RB>::kSmem; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ta.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB>, map_x, map_a, map_b, map_y, map_out, ta);
+}
+
+inline int launch(const AdapterArgs& a, int* marks, int* error, cudaStream_t stream) {
+    const long tiles = (a.T + kRows - 1) / kRows;
+    const int parts = tiles <= 18 ? 8 : tiles <= 37 ? 4 : tiles <= 74 ? 2 : 1;
+    if (tiles * parts > 0x7fffffffL) return kTooLarge;
+    const TileArgs ta{a, marks, parts, (a.R + 15) / 16 * 16, error};
+    const int rc = a.R <= 64 ? launch_as<1>(ta, (int)tiles, stream) : launch_as<2>(ta, (int)tiles, stream);
+    return rc != 0 ? rc : launch_status();
+}
+
+}  // namespace adapter_tiles
+}  // namespace lb200

@@ -2949,14 +2949,16 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     _apart(out, x, "out and x")
     if rows == 0 or features == 0:
         return out
-    parts, h = 1, None
+    parts, h, marks = 1, None, None
     if y.dtype == torch.float32 or rank > 256:             # two kernels, with the short sums between them
         parts = _fn("adapters", "lb_adapter_parts", [c_long, c_int, c_int])(rows, width, rank)
         h = torch.empty(max(1, parts * rows * rank), dtype=torch.float32, device=here)
+    elif rows >= 384:                                      # tiles of 128 rows, and what they leave to the rows' kernel
+        marks = torch.empty((rows + 127) // 128, dtype=torch.int32, device=here)
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_long, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
+             c_long, c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
-             _ptr(ranks), _ptr(out), ldo, _ptr(h), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
-           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None else 2)
+             _ptr(ranks), _ptr(out), ldo, _ptr(h), _ptr(marks), _ptr(error_word(here)), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
+           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None and marks is None else 2)
     return out
