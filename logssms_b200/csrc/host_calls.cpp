@@ -1,9 +1,10 @@
-// The calls of the 8-bit operators from Python to their launchers, without a detour: what `kernels.py` checks, allocates and
-// converts in a dozen microseconds per call takes two here, which is what a single token outside a captured graph waits for.
+// The calls of some operators from Python to their launchers, without a detour: the 8-bit operators and the serving operators
+// (attention over a shared prefix, adapters, rules on logits).  What `kernels.py` checks, allocates and converts in a dozen
+// microseconds or two per call takes a few here, which is what a single token outside a captured graph waits for.
 //
-// Only what is plainly in order is taken: every function returns the new tensors, or None, whereupon the caller goes the
-// ordinary way and says what is wrong with the arguments (or finds that all is well), or a launcher's error code.  Nothing is
-// kept between calls but the addresses of the launchers and of each device's error word, which `kernels.py` hands over.
+// Only what is plainly in order is taken: every function returns the new tensors, or None, whereupon the caller goes the ordinary
+// way and says what is wrong with the arguments (or finds that all is well), or a launcher's error code.  Nothing is kept between
+// calls but the addresses of the launchers and of each device's error word, which `kernels.py` hands over.
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -205,6 +206,177 @@ PyObject* swiglu(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ------------------------------------------------------------ serving operators
+namespace serving {
+typedef int (*SplitsFn)(const void*, long, const void*, const void*, long, int, int, int, int, int, int, long, long, int);
+typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, const int*, long, int, int, const int*, const int*, const int*,
+                           const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, float, int*, int, void*);
+typedef int (*PartsFn)(long, int, int);
+typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
+                          const int*, void*, long, float*, int*, int*, int, long, int, int, int, int, int, void*);
+typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
+                       const float*, const float*, const int*, const int*, const float*, int, const int*, long, int, const int*, void*);
+SplitsFn splits_fn;
+AttentionFn attention_fn;
+PartsFn parts_fn;
+AdaptersFn adapters_fn;
+RulesFn rules_fn;
+
+
+// the argument's tensor on the current device, or null
+const at::Tensor* tensor(PyObject* o, int device) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.is_cuda() && t.get_device() == device ? &t : nullptr;
+}
+int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : -1; }
+constexpr int64_t kFits = 0x3fffffff;
+// [rows, columns], columns side by side, rows that do not overlap
+bool matrix(const at::Tensor& t) {
+    return t.dim() == 2 && t.size(0) > 0 && t.size(1) > 0 && t.size(0) <= kFits && t.size(1) <= kFits && t.stride(1) == 1 && t.stride(0) >= t.size(1);
+}
+bool ints(const at::Tensor* t, int64_t n) { return t != nullptr && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->is_contiguous(); }
+bool floats(const at::Tensor* t, int64_t n) { return t != nullptr && t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == n && t->is_contiguous(); }
+template <typename T> const T* data(const at::Tensor* t) { return t == nullptr ? nullptr : (const T*)t->data_ptr(); }
+bool number(double* to, PyObject* from) {
+    *to = PyFloat_AsDouble(from);
+    if (*to == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+bool whole(long* to, PyObject* from) {
+    if (!PyLong_CheckExact(from)) return false;
+    *to = PyLong_AsLong(from);
+    if (*to == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+
+// (q, k_cache, v_cache, block_table, token_req, positions, group_start, prefix_lens, scale, max_prefix, max_context) -> out
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const int device = (int)c10::cuda::current_device();
+        if (n != 11 || attention_fn == nullptr || device >= kDevices || error_words[device] == nullptr) return none();
+        const at::Tensor* t[8];
+        for (int i = 0; i < 8; ++i)
+            if ((t[i] = tensor(args[i], device)) == nullptr) return none();
+        double scale;
+        long max_prefix, max_context;
+        if (!number(&scale, args[8]) || !whole(&max_prefix, args[9]) || !whole(&max_context, args[10])) return none();
+        const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &bt = *t[3];
+        if (q.dim() != 3 || k.dim() != 4 || dtype_code(q) < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return none();
+        const int64_t tokens = q.size(0), Hq = q.size(1), hd = q.size(2), pages = k.size(0), page = k.size(1), Hkv = k.size(2), groups = t[7]->numel();
+        if (tokens < 1 || groups < 1 || hd < 8 || hd > 256 || hd % 8 != 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || pages < 1 || page < 1 || tokens > kFits || Hq > 65535
+            || page > kFits || groups > kFits || q.stride(2) != 1 || (Hq > 1 && q.stride(1) != hd) || k.size(3) != hd || !k.is_contiguous() || !v.is_contiguous() || v.sizes() != k.sizes()
+            || !matrix(bt) || bt.scalar_type() != at::kInt || !ints(t[4], tokens) || !ints(t[5], tokens) || !ints(t[6], groups + 1) || !ints(t[7], groups)) return none();
+        const int code = dtype_code(q);
+        const int splits = splits_fn(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), pages, (int)tokens, (int)Hq, (int)Hkv, (int)hd, (int)page,
+                                     (int)groups, max_prefix, max_context - max_prefix, code);
+        const int sp = splits >> 16, so = splits & 0xffff;
+        const int64_t rows = tokens * Hq * (sp + so);
+        const at::Tensor out = at::detail::empty_strided_cuda({tokens, Hq, hd}, {Hq * hd, hd, 1}, q.scalar_type(), q.device());
+        const at::Tensor parts = at::detail::empty_strided_cuda({rows * (hd + 2)}, {1}, at::kFloat, q.device());
+        float* part_o = (float*)parts.data_ptr();
+        const int rc = attention_fn(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), out.data_ptr(), (const int*)bt.data_ptr(), bt.stride(0),
+                                    (int)bt.size(1), (int)bt.size(0), data<int>(t[4]), data<int>(t[5]), data<int>(t[6]), data<int>(t[7]), (int)groups,
+                                    part_o, part_o + rows * hd, pages, (int)tokens, (int)Hq, (int)Hkv, (int)hd, (int)page, sp, so, max_prefix,
+                                    (float)scale, error_words[device], code, stream_of(device));
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// (y, x, a, b, index, scales | None, ranks | None) -> (out, kernels)
+PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const int device = (int)c10::cuda::current_device();
+        if (n != 7 || adapters_fn == nullptr || device >= kDevices || error_words[device] == nullptr) return none();
+        const at::Tensor *y = tensor(args[0], device), *x = tensor(args[1], device), *a = tensor(args[2], device), *b = tensor(args[3], device);
+        const at::Tensor *index = tensor(args[4], device), *scales = nullptr, *ranks = nullptr;
+        if (y == nullptr || x == nullptr || a == nullptr || b == nullptr || !matrix(*y) || !matrix(*x) || a->dim() != 3 || b->dim() != 3) return none();
+        const int64_t rows = y->size(0), features = y->size(1), width = x->size(1), count = a->size(0), rank = a->size(1);
+        if (x->size(0) != rows || a->size(2) != width || b->size(0) != count || b->size(1) != features || b->size(2) != rank || count < 1 || rank < 1
+            || count > kFits || rank > kFits || a->stride(2) != 1 || b->stride(2) != 1 || dtype_code(*y) < 0 || x->scalar_type() != y->scalar_type()
+            || a->scalar_type() != y->scalar_type() || b->scalar_type() != y->scalar_type() || !ints(index, rows)) return none();
+        if (args[5] != Py_None && !floats(scales = tensor(args[5], device), count)) return none();
+        if (args[6] != Py_None && !ints(ranks = tensor(args[6], device), count)) return none();
+        const int code = dtype_code(*y);
+        const at::Tensor out = at::detail::empty_strided_cuda({rows, features}, {features, 1}, y->scalar_type(), y->device());
+        at::Tensor scratch;
+        int parts = 1;
+        float* h = nullptr;
+        int* marks = nullptr;
+        if (code == 0 || rank > 256) {
+            parts = parts_fn(rows, (int)width, (int)rank);
+            scratch = at::detail::empty_strided_cuda({parts * rows * rank}, {1}, at::kFloat, y->device());
+            h = (float*)scratch.data_ptr();
+        } else if (rows >= 384) {
+            scratch = at::detail::empty_strided_cuda({(rows + 127) / 128}, {1}, at::kInt, y->device());
+            marks = (int*)scratch.data_ptr();
+        }
+        const int rc = adapters_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
+                                   b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features, h, marks,
+                                   error_words[device], parts, rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// (logits, history, lengths, prompt_lengths, slots, repetition, frequency, presence, bias_start, bias_ids, bias_values, allowed,
+//  allowed_row, each but the first may be None) -> edited
+PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const int device = (int)c10::cuda::current_device();
+        if (n != 13 || rules_fn == nullptr) return none();
+        const at::Tensor* t[13] = {};
+        for (int i = 0; i < 13; ++i)
+            if (args[i] != Py_None && (t[i] = tensor(args[i], device)) == nullptr) return none();
+        const at::Tensor *logits = t[0], *history = t[1], *biases = t[8], *allowed = t[11];
+        if (logits == nullptr || !matrix(*logits) || logits->scalar_type() != at::kFloat) return none();
+        const int64_t rows = logits->size(0), V = logits->size(1);
+        int64_t slots = 0, capacity = 0, words = 0, masks = 0, n_biases = 0;
+        if (history != nullptr) {
+            if (!matrix(*history) || history->scalar_type() != at::kInt || t[2] == nullptr) return none();
+            slots = history->size(0);
+            capacity = history->size(1);
+            if (t[4] == nullptr && slots < rows) return none();
+        } else {
+            for (int i = 2; i < 8; ++i) if (t[i] != nullptr) return none();
+        }
+        for (int i : {2, 3, 4, 12}) if (t[i] != nullptr && !ints(t[i], rows)) return none();
+        for (int i : {5, 6, 7}) if (t[i] != nullptr && !floats(t[i], rows)) return none();
+        if (biases != nullptr) {
+            if (t[9] == nullptr || !ints(biases, rows + 1)) return none();
+            n_biases = t[9]->numel();
+            if (n_biases > kFits || !ints(t[9], n_biases) || !floats(t[10], n_biases)) return none();
+        } else if (t[9] != nullptr || t[10] != nullptr) {
+            return none();
+        }
+        if (allowed != nullptr) {
+            if (!matrix(*allowed) || allowed->scalar_type() != at::kInt) return none();
+            masks = allowed->size(0);
+            words = allowed->stride(0);
+            if (allowed->size(1) * 32 < V || (t[12] == nullptr && masks < rows)) return none();
+        } else if (t[12] != nullptr) {
+            return none();
+        }
+        const at::Tensor out = at::detail::empty_strided_cuda({rows, V}, {V, 1}, at::kFloat, logits->device());
+        const int rc = rules_fn(data<float>(logits), logits->stride(0), (float*)out.data_ptr(), V, (int)rows, (int)V, data<int>(history),
+                                history != nullptr ? history->stride(0) : 0, (int)capacity, (int)slots, data<int>(t[4]), data<int>(t[2]), data<int>(t[3]),
+                                data<float>(t[5]), data<float>(t[6]), data<float>(t[7]), data<int>(biases), data<int>(t[9]), data<float>(t[10]), (int)n_biases,
+                                data<int>(allowed), words, (int)masks, data<int>(t[12]), stream_of(device));
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// the launchers' addresses
+PyObject* launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 5) { PyErr_SetString(PyExc_TypeError, "five addresses"); return nullptr; }
+    splits_fn = (SplitsFn)PyLong_AsVoidPtr(args[0]);
+    attention_fn = (AttentionFn)PyLong_AsVoidPtr(args[1]);
+    parts_fn = (PartsFn)PyLong_AsVoidPtr(args[2]);
+    adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[3]);
+    rules_fn = (RulesFn)PyLong_AsVoidPtr(args[4]);
+    return none();
+}
+}  // namespace serving
+
 // the launchers' addresses
 PyObject* launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 4) { PyErr_SetString(PyExc_TypeError, "four addresses"); return nullptr; }
@@ -225,9 +397,11 @@ PyObject* error_word(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"norm", (PyCFunction)(void*)norm, METH_FASTCALL, nullptr},         {"quantize", (PyCFunction)(void*)quantize, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},     {"swiglu", (PyCFunction)(void*)swiglu, METH_FASTCALL, nullptr},
+    {"attention", (PyCFunction)(void*)serving::attention, METH_FASTCALL, nullptr}, {"adapters", (PyCFunction)(void*)serving::adapters, METH_FASTCALL, nullptr},
+    {"rules", (PyCFunction)(void*)serving::rules, METH_FASTCALL, nullptr}, {"serving_launchers", (PyCFunction)(void*)serving::launchers, METH_FASTCALL, nullptr},
     {"launchers", (PyCFunction)(void*)launchers, METH_FASTCALL, nullptr}, {"error_word", (PyCFunction)(void*)error_word, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "fp8_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fp8_calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_host_calls(void) { return PyModule_Create(&module); }

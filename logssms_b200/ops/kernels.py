@@ -450,6 +450,41 @@ def attention_decode_listed(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     return out
 
 
+_serving_binding = None
+
+
+def _serving_calls():
+    """The binding that takes a call of the serving operators that is plainly in order straight to its launcher
+    (`csrc/host_calls.cpp`); it answers None to anything else, and the functions in Python take over."""
+    global _serving_binding
+    if _serving_binding is None:
+        binding = build.load_binding("host_calls")
+        at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
+        binding.serving_launchers(at("attention_shared", "lb_attention_shared_splits"), at("attention_shared", "lb_attention_shared"),
+                                  at("adapters", "lb_adapter_parts"), at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"))
+        _serving_binding = binding
+    return _serving_binding
+
+
+def _serving_error_word(device: torch.device, name: str) -> int:
+    """Address of the device's error word, which the binding has from then on (until then it takes no call that needs it there)."""
+    if device not in _gemm_error:
+        # (made inside, it would lie in the graph's memory, and every replay would clear what was reported before)
+        _need(not torch.cuda.is_current_stream_capturing(), f"the first {name} on a device must come before a capture")
+    address = error_word(device).data_ptr()
+    _serving_calls().error_word(device.index, address)
+    return address
+
+
+def _serving_done(got, name: str, launches: int):
+    """What the binding answered: counts launches, or raises what the launcher said."""
+    global launch_count
+    if type(got) is int:
+        _check(got, name)
+    launch_count += launches
+    return got
+
+
 def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                             token_req: torch.Tensor, positions: torch.Tensor, group_start: torch.Tensor, prefix_lens: torch.Tensor,
                             scale: float, *, max_prefix: int, max_context: int, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -465,7 +500,13 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     are left as they are (in `out`; otherwise unwritten).  A row without keys (position -1; a request or pages that are not there)
     becomes zeros.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right too.
 
-    bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits."""
+    bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits.  `check_kernel_errors()`
+    reports a kernel whose internal wait gave up."""
+    if out is None and not PROFILER.enabled:
+        got = (_serving_binding or _serving_calls()).attention(q, k_cache, v_cache, block_table, token_req, positions, group_start,
+                                                               prefix_lens, scale, max_prefix, max_context)
+        if got is not None:
+            return _serving_done(got, "attention_decode_shared", 3)
     _cuda(q, k_cache, v_cache, block_table, token_req, positions, group_start, prefix_lens, out)
     _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
     tokens, Hq, hd = q.shape
@@ -506,8 +547,8 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
              c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_float, c_void_p, c_int, c_void_p])
     _check(f(_ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(block_table), block_table.stride(0),
              block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(prefix_lens), groups,
-             _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, int(max_prefix), scale, _ptr(error_word(q.device)), code,
-             _stream()), "attention_decode_shared", launches=3)
+             _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, int(max_prefix), scale,
+             _serving_error_word(q.device, "attention_decode_shared"), code, _stream()), "attention_decode_shared", launches=3)
     return out
 
 
@@ -2697,11 +2738,11 @@ _fp8_binding = None
 
 
 def _fp8_calls():
-    """The binding that takes a call that is plainly in order straight to its launcher (`csrc/fp8_calls.cpp`): checks, outputs and
+    """The binding that takes a call that is plainly in order straight to its launcher (`csrc/host_calls.cpp`): checks, outputs and
     launch in 5 us where the functions below take 15.  It answers None where anything is out of the ordinary, and they take over."""
     global _fp8_binding
     if _fp8_binding is None:
-        binding = build.load_binding("fp8_calls")
+        binding = build.load_binding("host_calls")
         at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
         binding.launchers(at("fp8_rows", "lb_add_rmsnorm_fp8"), at("fp8_rows", "lb_quantize_fp8"),
                           at("fp8_linear", "lb_linear_fp8"), at("fp8_linear", "lb_linear_swiglu_fp8"))
@@ -2917,7 +2958,12 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     `a` [adapters, rank, width] and `b` [adapters, features, rank], of y's dtype (bfloat16 or float32), columns side by side, other
     strides free.  `index`: int32, one per row, in any order; a row whose index names no adapter (-1) keeps its y, whatever its x.
     `scales`: float32, one per adapter (none: 1).  `ranks`: int32, one per adapter: how many of the `rank` rows of a[i] and columns of
-    b[i] are its own (none: all of them); the others are not read as values."""
+    b[i] are its own (none: all of them); the others are not read as values.  `check_kernel_errors()` reports a kernel whose internal
+    wait gave up."""
+    if out is None and not PROFILER.enabled:
+        got = (_serving_binding or _serving_calls()).adapters(y, x, a, b, index, scales, ranks)
+        if got is not None:
+            return _serving_done(got, "add_adapters", 2 if y.shape[0] >= 384 or y.dtype is torch.float32 else 1)
     _cuda(y, x, a, b, index, scales, ranks, out)
     ldy, ldx = _rows_of(y, "y"), _rows_of(x, "x")
     rows, features = y.shape
@@ -2959,6 +3005,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
              c_long, c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
-             _ptr(ranks), _ptr(out), ldo, _ptr(h), _ptr(marks), _ptr(error_word(here)), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
+             _ptr(ranks), _ptr(out), ldo, _ptr(h), _ptr(marks),
+             _serving_error_word(here, "add_adapters"), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
            f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None and marks is None else 2)
     return out

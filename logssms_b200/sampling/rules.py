@@ -41,6 +41,11 @@ def edit_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, le
     `allowed`: int32 [masks, at least ceil(vocab / 32)], token t is bit t % 32 of word t // 32, set: allowed.  `allowed_row` (int32)
     names each row's mask; without, row i's is i; a row whose mask is none of these (-1) allows every token.  A mask that allows
     nothing leaves a row of -inf.  Row strides of `logits`, `history`, `allowed` and `out` are free."""
+    if out is None and not K.PROFILER.enabled:
+        got = (K._serving_binding or K._serving_calls()).rules(logits, history, lengths, prompt_lengths, slots, repetition, frequency, presence,
+                                                               bias_start, bias_ids, bias_values, allowed, allowed_row)
+        if got is not None:
+            return K._serving_done(got, "edit_logits", 1)
     K._cuda(logits, history, lengths, prompt_lengths, slots, repetition, frequency, presence, bias_start, bias_ids, bias_values,
             allowed, allowed_row, out)
     K._need(logits.dtype == torch.float32, "logits must be float32")
