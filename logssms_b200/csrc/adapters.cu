@@ -3,9 +3,10 @@
 // x [T, K], y and out [T, N], A [adapters, R, K], B [adapters, N, R], an adapter's rank up to R.
 //
 // bfloat16: adapters_rows.cuh (decoding rows, any order of adapters) and adapters_tiles.cuh (prompts).  This file: the float32
-// form (and that of ranks over 256), and the choice between them.  Tiles of 32 rows, one pass for each adapter that a tile's rows name, products in float32
-// registers.  `shrink` leaves h = x A^T per part of K, `expand` adds the parts up in their order, multiplies by the scale and
-// adds to y: one rounding, of the output.
+// form (and that of ranks over 256), and the choice between them.  Tiles of 32 rows, products in float32 registers; the adapters that
+// a tile's rows name are shared out to some CTAs ("slots"), each of which makes a pass for each of its own.  In `shrink` the
+// CTAs of a cluster have a part of K each and add their sums up in their order; `expand` multiplies by the scale and adds to y: one
+// rounding, of the output.
 #include "lb200/common.cuh"
 #include "lb200/adapters.cuh"
 #include "lb200/adapters_rows.cuh"
@@ -16,99 +17,184 @@ namespace {
 constexpr int kRows = 32, kCols = 64, kChunk = 32;      // rows, ranks or features of a tile; values of K or R at a time
 constexpr int kThreads = 128;                           // 8 groups of 4 rows x 16 groups of 4 columns
 
-// acc[4][4] += rows of `p` (kRows from its first, ld elements apart) times rows of `q` (kCols), over `depth` values
-struct Tiles { float p[kChunk][kRows + 4]; float q[kChunk][kCols + 4]; };
-
-template <typename FP, typename FQ>
-__device__ __forceinline__ void multiply(Tiles& s, float (&acc)[4][4], int depth, FP p_at, FQ q_at) {
-    const int tid = threadIdx.x, r4 = (tid >> 4) * 4, c4 = (tid & 15) * 4;
-    for (int k0 = 0; k0 < depth; k0 += kChunk) {
-        __syncthreads();
-        const int k = tid & 31;
-        for (int r = tid >> 5; r < kRows; r += kThreads / 32) s.p[k][r] = k0 + k < depth ? p_at(r, k0 + k) : 0.f;
-        for (int c = tid >> 5; c < kCols; c += kThreads / 32) s.q[k][c] = k0 + k < depth ? q_at(c, k0 + k) : 0.f;
-        __syncthreads();
+constexpr int kMostParts = 8;
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float remote(uint32_t at, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %1, %2;\n\tld.shared::cluster.f32 %0, [p];\n\t}" : "=f"(v) : "r"(at), "r"(rank) : "memory");
+    return v;
+}
+// Chunks of 32 values of both operands, row by row (rows 36 numbers apart: eight rows' pieces of 16 bytes are in different banks),
+// three of them in turn: two on their way by asynchronous copies while one is multiplied.  At the end a CTA's sums.
+constexpr int kStages = 3, kLd = kChunk + 4;
+union Work {
+    struct { float p[kRows][kLd], q[kCols][kLd]; } stage[kStages];
+    float sums[kRows][kCols];
+};
+template <typename T> struct Operand {
+    const T* at; long ld;                                 // row r at `at + r * ld`
+    bool wide;                                            // 16 bytes at a time: rows lie so, and the depth is a multiple of 4
+};
+__device__ __forceinline__ void put(float* to, const float* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void put4(float* to, const float* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void put(float* to, const __nv_bfloat16* from, bool there) { *to = there ? __bfloat162float(*from) : 0.f; }
+__device__ __forceinline__ void put4(float* to, const __nv_bfloat16* from, bool there) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put(to + i, from + i, there);
+}
+template <typename T, int ROWS, typename F>
+__device__ __forceinline__ void fill(float (&to)[ROWS][kLd], const Operand<T>& o, int k0, int depth, F there) {
+    if (o.wide) {
+#pragma unroll
+        for (int n = 0; n < ROWS * kChunk / 4 / kThreads; ++n) {
+            const int i = threadIdx.x + n * kThreads, r = i / (kChunk / 4), k = i % (kChunk / 4) * 4;
+            const bool ok = there(r) && k0 + k < depth;
+            put4(&to[r][k], o.at + (ok ? (long)r * o.ld + k0 + k : 0), ok);
+        }
+    } else {
 #pragma unroll 8
-        for (int kk = 0; kk < kChunk; ++kk) {
-            const float4 u = *reinterpret_cast<const float4*>(&s.p[kk][r4]), v = *reinterpret_cast<const float4*>(&s.q[kk][c4]);
-            const float pu[4] = {u.x, u.y, u.z, u.w}, pv[4] = {v.x, v.y, v.z, v.w};
+        for (int n = 0; n < ROWS * kChunk / kThreads; ++n) {
+            const int i = threadIdx.x + n * kThreads, r = i / kChunk, k = i % kChunk;
+            const bool ok = there(r) && k0 + k < depth;
+            put(&to[r][k], o.at + (ok ? (long)r * o.ld + k0 + k : 0), ok);
+        }
+    }
+}
+// acc[i][j] += row r4 + i of P times row c + 16 j of Q, over `depth` values; rows that are not there are zeros
+template <typename TP, typename TQ, typename FP, typename FQ>
+__device__ __forceinline__ void multiply(Work& w, float (&acc)[4][4], int depth, const Operand<TP>& p, FP p_there, const Operand<TQ>& q, FQ q_there) {
+    const int r4 = (threadIdx.x >> 4) * 4, c = threadIdx.x & 15, chunks = (depth + kChunk - 1) / kChunk;
+    auto fetch = [&](int n) {
+        if (n < chunks) {
+            fill(w.stage[n % kStages].p, p, n * kChunk, depth, p_there);
+            fill(w.stage[n % kStages].q, q, n * kChunk, depth, q_there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();                                       // (what was there has been read)
+    for (int n = 0; n < kStages - 1; ++n) fetch(n);
+    for (int n = 0; n < chunks; ++n) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncthreads();
+        fetch(n + kStages - 1);
+        const auto& s = w.stage[n % kStages];
+#pragma unroll
+        for (int k = 0; k < kChunk; k += 4) {
+            float4 u[4], v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const float4*>(&s.p[r4 + i][k]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(&s.q[c + 16 * j][k]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(pu[i], pv[j], acc[i][j]);
+                for (int j = 0; j < 4; ++j)
+                    acc[i][j] = fmaf(u[i].x, v[j].x, fmaf(u[i].y, v[j].y, fmaf(u[i].z, v[j].z, fmaf(u[i].w, v[j].w, acc[i][j]))));
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+}
+template <typename T> __device__ __forceinline__ bool lies_wide(const T* p, long ld, int depth) {
+    return sizeof(T) == 4 && ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && depth % 4 == 0;
 }
 
-// grid: (row tiles, parts of K, rank tiles)
+// grid: (row tiles, parts of K, rank tiles x slots); a cluster: the parts
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adapter_shrink_kernel(AdapterArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs a) {
     pdl_wait();
-    __shared__ Tiles s;
+    __shared__ __align__(16) Work w;
     const long t0 = (long)blockIdx.x * kRows;
-    const int part = blockIdx.y, j0 = blockIdx.z * kCols, tid = threadIdx.x;
-    const int k_begin = part * a.part_k, k_end = min(k_begin + a.part_k, a.K);
+    const int part = blockIdx.y, j0 = (int)(blockIdx.z / a.slots) * kCols, slot = blockIdx.z % a.slots, tid = threadIdx.x;
+    const int k_begin = min(part * a.part_k, a.K), depth = min(a.part_k, a.K - k_begin);
     const int mine = adapter_of(a, t0 + (tid & 31));
-    const int r4 = (tid >> 4) * 4, c4 = (tid & 15) * 4;
-    const T* x = (const T*)a.x;
-    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i)) {
+    const int r4 = (tid >> 4) * 4, c = tid & 15;
+    Operand<T> x{(const T*)a.x + t0 * a.ldx + k_begin, a.ldx, false};
+    x.wide = lies_wide(x.at, a.ldx, depth);
+    int turn = 0;
+    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i), ++turn) {
+        if (turn % a.slots != slot) continue;
         const int rank = rank_of(a, i);
         if (j0 >= rank) continue;
-        const T* A = (const T*)a.A + (size_t)i * a.a_adapter;
+        const unsigned named = __ballot_sync(0xffffffffu, mine == i);            // (bit r: row r)
+        Operand<T> A{(const T*)a.A + (size_t)i * a.a_adapter + (size_t)j0 * a.a_row + k_begin, a.a_row, false};
+        A.wide = lies_wide(A.at, a.a_row, depth);
         float acc[4][4] = {};
-        multiply(s, acc, k_end - k_begin,
-                 [&](int r, int k) { return t0 + r < a.T ? to_f32(x[(t0 + r) * a.ldx + k_begin + k]) : 0.f; },
-                 [&](int c, int k) { return j0 + c < rank ? to_f32(A[(size_t)(j0 + c) * a.a_row + k_begin + k]) : 0.f; });
+        multiply(w, acc, depth, x, [&](int r) { return (named >> r & 1u) != 0; }, A, [&](int r) { return j0 + r < rank; });
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const long t = t0 + r4 + r;
-            if (adapter_of(a, t) != i) continue;
-            float* h = a.h + ((size_t)part * a.T + t) * a.R;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (j0 + c4 + j < rank) h[j0 + c4 + j] = acc[r][j];
+            for (int j = 0; j < 4; ++j) w.sums[r4 + r][c + 16 * j] = acc[r][j];
+        __syncthreads();
+        if (a.parts > 1) cluster_meet();
+        for (int e = part * kThreads + tid; e < kRows * kCols; e += a.parts * kThreads) {
+            const int r = e / kCols, j = e % kCols;
+            if (!(named >> r & 1u) || j0 + j >= rank) continue;
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(&w.sums[r][j]);
+            float got[kMostParts], total = 0.f;
+#pragma unroll
+            for (int p = 0; p < kMostParts; ++p) if (p < a.parts) got[p] = a.parts > 1 ? remote(at, p) : w.sums[r][j];
+#pragma unroll
+            for (int p = 0; p < kMostParts; ++p) if (p < a.parts) total += got[p];
+            a.h[(t0 + r) * a.R + j0 + j] = total;
         }
+        if (a.parts > 1) cluster_meet();                   // (the sums have been read)
     }
 }
 
-// grid: (row tiles, feature tiles)
+// grid: (row tiles, feature tiles, slots)
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adapter_expand_kernel(AdapterArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs a) {
     pdl_wait();
-    __shared__ Tiles s;
+    __shared__ __align__(16) Work w;
     const long t0 = (long)blockIdx.x * kRows;
-    const int n0 = blockIdx.y * kCols, tid = threadIdx.x;
+    const int n0 = blockIdx.y * kCols, slot = blockIdx.z, tid = threadIdx.x;
     const int mine = adapter_of(a, t0 + (tid & 31));
-    const int r4 = (tid >> 4) * 4, c4 = (tid & 15) * 4;
-    float sum[4][4] = {};
-    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i)) {
-        const int rank = rank_of(a, i);
-        const T* B = (const T*)a.B + (size_t)i * a.b_adapter;
-        const float scale = a.scales ? a.scales[i] : 1.f;
-        float acc[4][4] = {};
-        multiply(s, acc, rank,
-                 [&](int r, int j) {
-                     float h = 0.f;
-                     if (adapter_of(a, t0 + r) == i)
-                         for (int p = 0; p < a.parts; ++p) h += a.h[((size_t)p * a.T + t0 + r) * a.R + j];
-                     return h * scale;
-                 },
-                 [&](int c, int j) { return n0 + c < a.N ? to_f32(B[(size_t)(n0 + c) * a.b_row + j]) : 0.f; });
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (adapter_of(a, t0 + r4 + r) == i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum[r][j] = acc[r][j];
-    }
+    const int r4 = (tid >> 4) * 4, c = tid & 15;
+    unsigned ours = slot == 0 ? __ballot_sync(0xffffffffu, mine < 0) : 0u;       // the rows that this CTA writes
+    int turn = 0;
+    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i), ++turn)
+        if (turn % a.slots == slot) ours |= __ballot_sync(0xffffffffu, mine == i);
     const T* y = (const T*)a.y;
     T* out = (T*)a.out;
+    float sum[4][4] = {};                                  // y first: on its way while the short sums and B come
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((ours >> (r4 + r) & 1u) && t0 + r4 + r < a.T && n0 + c + 16 * j < a.N) sum[r][j] = to_f32(y[(t0 + r4 + r) * a.ldy + n0 + c + 16 * j]);
+    turn = 0;
+    for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i), ++turn) {
+        if (turn % a.slots != slot) continue;
+        const int rank = rank_of(a, i);
+        const unsigned named = __ballot_sync(0xffffffffu, mine == i);
+        const float scale = a.scales ? a.scales[i] : 1.f;
+        Operand<float> h{a.h + t0 * a.R, a.R, false};
+        h.wide = lies_wide(h.at, a.R, rank);
+        Operand<T> B{(const T*)a.B + (size_t)i * a.b_adapter + (size_t)n0 * a.b_row, a.b_row, false};
+        B.wide = lies_wide(B.at, a.b_row, rank);
+        float acc[4][4] = {};
+        multiply(w, acc, rank, h, [&](int r) { return (named >> r & 1u) != 0; }, B, [&](int r) { return n0 + r < a.N; });
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (named >> (r4 + r) & 1u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[r][j] += acc[r][j] * scale;
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const long t = t0 + r4 + r;
-        if (t >= a.T) continue;
+        if (t >= a.T || !(ours >> (r4 + r) & 1u)) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int n = n0 + c4 + j;
-            if (n < a.N) out[t * a.ldo + n] = from_f32<T>(to_f32(y[t * a.ldy + n]) + sum[r][j]);
+            const int n = n0 + c + 16 * j;
+            if (n < a.N) out[t * a.ldo + n] = from_f32<T>(sum[r][j]);
         }
     }
 }
@@ -116,33 +202,43 @@ __global__ void __launch_bounds__(kThreads) adapter_expand_kernel(AdapterArgs a)
 template <typename T>
 int launch_general(const AdapterArgs& a, cudaStream_t s) {
     const unsigned tiles = (unsigned)((a.T + kRows - 1) / kRows);
-    int rc = launch_pdl(adapter_shrink_kernel<T>, dim3(tiles, a.parts, a.R > 0 ? (a.R + kCols - 1) / kCols : 1), dim3(kThreads), 0, s, a);
-    if (rc == 0) rc = launch_pdl(adapter_expand_kernel<T>, dim3(tiles, (a.N + kCols - 1) / kCols), dim3(kThreads), 0, s, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles, a.parts, (a.R > 0 ? (a.R + kCols - 1) / kCols : 1) * a.slots); cfg.blockDim = dim3(kThreads); cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1; attr[1].val.clusterDim.y = (unsigned)a.parts; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    int rc = (int)cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<T>, a);
+    if (rc == 0) rc = launch_pdl(adapter_expand_kernel<T>, dim3(tiles, (a.N + kCols - 1) / kCols, a.slots), dim3(kThreads), 0, s, a);
     return rc != 0 ? rc : launch_status();
 }
 }  // namespace
 
-// How many parts K is cut into: enough CTAs for the SMs, each with 64 values of K at least.
-extern "C" int lb_adapter_parts(long T, int K, int R) {
+// How many parts K is cut into, the CTAs of a cluster: enough for the SMs, each with 64 values of K at least.
+static int parts_of(long T, int K, int R) {
     const long tiles = (T + kRows - 1) / kRows * (R > 0 ? (R + kCols - 1) / kCols : 1);
-    const long most = K / 64 < 1 ? 1 : K / 64, want = tiles > 0 ? (296 + tiles - 1) / tiles : 1;
-    return (int)(want < 1 ? 1 : want > most ? most : want > 32 ? 32 : want);
+    int parts = 1;
+    while (parts < kMostParts && tiles * parts < 296 && K / (2 * parts) >= 64) parts *= 2;
+    return parts;
 }
 
 // From so many rows on a call goes to the tiles' kernel.
 constexpr long kTileRows = 384;
 
-// h: float32 scratch [parts, T, R].  Strides in elements; columns lie side by side.  out may be y.
+// h: float32 scratch [T, R].  Strides in elements; columns lie side by side.  out may be y.
 // (h: float32, or ranks over 256.)  marks: int32 scratch, one per 128 rows; error: the device's error word.
 extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row,
                                const void* B, long b_adapter, long b_row, const int* index, const float* scales, const int* ranks,
-                               void* out, long ldo, float* h, int* marks, int* error, int parts, long T, int K, int N, int R, int adapters, int dtype,
+                               void* out, long ldo, float* h, int* marks, int* error, long T, int K, int N, int R, int adapters, int dtype,
                                void* stream) {
     if (T <= 0 || N <= 0) return kOk;
-    if (K < 0 || R < 0 || adapters < 0 || parts < 1) return kBadSize;
+    if (K < 0 || R < 0 || adapters < 0) return kBadSize;
+    const int parts = parts_of(T, K, R);
     if (T > 0x7fffffffL - 1024 || N > 0x3fffffff) return kTooLarge;
     AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, h, T, K, N, R, adapters,
-                  parts, (K + parts - 1) / parts};
+                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, T <= 512 ? 8 : 2};      // (a prompt's tiles name one adapter or two)
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == kF32) return launch_general<float>(a, s);

@@ -211,14 +211,12 @@ namespace serving {
 typedef int (*SplitsFn)(const void*, long, const void*, const void*, long, int, int, int, int, int, int, long, long, int);
 typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, const int*, long, int, int, const int*, const int*, const int*,
                            const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, float, int*, int, void*);
-typedef int (*PartsFn)(long, int, int);
 typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
-                          const int*, void*, long, float*, int*, int*, int, long, int, int, int, int, int, void*);
+                          const int*, void*, long, float*, int*, int*, long, int, int, int, int, int, void*);
 typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
                        const float*, const float*, const int*, const int*, const float*, int, const int*, long, int, const int*, void*);
 SplitsFn splits_fn;
 AttentionFn attention_fn;
-PartsFn parts_fn;
 AdaptersFn adapters_fn;
 RulesFn rules_fn;
 
@@ -300,12 +298,10 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int code = dtype_code(*y);
         const at::Tensor out = at::detail::empty_strided_cuda({rows, features}, {features, 1}, y->scalar_type(), y->device());
         at::Tensor scratch;
-        int parts = 1;
         float* h = nullptr;
         int* marks = nullptr;
         if (code == 0 || rank > 256) {
-            parts = parts_fn(rows, (int)width, (int)rank);
-            scratch = at::detail::empty_strided_cuda({parts * rows * rank}, {1}, at::kFloat, y->device());
+            scratch = at::detail::empty_strided_cuda({rows * rank}, {1}, at::kFloat, y->device());
             h = (float*)scratch.data_ptr();
         } else if (rows >= 384) {
             scratch = at::detail::empty_strided_cuda({(rows + 127) / 128}, {1}, at::kInt, y->device());
@@ -313,7 +309,7 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         const int rc = adapters_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
                                    b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features, h, marks,
-                                   error_words[device], parts, rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
+                                   error_words[device], rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
         return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
     });
 }
@@ -367,12 +363,11 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // the launchers' addresses
 PyObject* launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 5) { PyErr_SetString(PyExc_TypeError, "five addresses"); return nullptr; }
+    if (n != 4) { PyErr_SetString(PyExc_TypeError, "four addresses"); return nullptr; }
     splits_fn = (SplitsFn)PyLong_AsVoidPtr(args[0]);
     attention_fn = (AttentionFn)PyLong_AsVoidPtr(args[1]);
-    parts_fn = (PartsFn)PyLong_AsVoidPtr(args[2]);
-    adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[3]);
-    rules_fn = (RulesFn)PyLong_AsVoidPtr(args[4]);
+    adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[2]);
+    rules_fn = (RulesFn)PyLong_AsVoidPtr(args[3]);
     return none();
 }
 }  // namespace serving

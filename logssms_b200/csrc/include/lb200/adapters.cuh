@@ -12,9 +12,9 @@ struct AdapterArgs {
     const int* index;                                   // a row's adapter; outside of [0, adapters): none
     const float* scales; const int* ranks;              // per adapter; null: 1, R
     void* out; long ldo;
-    float* h;                                           // [parts, T, R]
+    float* h;                                           // [T, R]
     long T;
-    int K, N, R, adapters, parts, part_k;
+    int K, N, R, adapters, parts, part_k, slots;
 };
 
 // The smallest adapter behind `prev` that any of the warp's rows names (INT_MAX: none).

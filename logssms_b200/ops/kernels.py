@@ -461,7 +461,7 @@ def _serving_calls():
         binding = build.load_binding("host_calls")
         at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
         binding.serving_launchers(at("attention_shared", "lb_attention_shared_splits"), at("attention_shared", "lb_attention_shared"),
-                                  at("adapters", "lb_adapter_parts"), at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"))
+                                  at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"))
         _serving_binding = binding
     return _serving_binding
 
@@ -2995,17 +2995,16 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     _apart(out, x, "out and x")
     if rows == 0 or features == 0:
         return out
-    parts, h, marks = 1, None, None
+    h = marks = None
     if y.dtype == torch.float32 or rank > 256:             # two kernels, with the short sums between them
-        parts = _fn("adapters", "lb_adapter_parts", [c_long, c_int, c_int])(rows, width, rank)
-        h = torch.empty(max(1, parts * rows * rank), dtype=torch.float32, device=here)
+        h = torch.empty(max(1, rows * rank), dtype=torch.float32, device=here)
     elif rows >= 384:                                      # tiles of 128 rows, and what they leave to the rows' kernel
         marks = torch.empty((rows + 127) // 128, dtype=torch.int32, device=here)
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_long, c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
+             c_long, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
              _ptr(ranks), _ptr(out), ldo, _ptr(h), _ptr(marks),
-             _serving_error_word(here, "add_adapters"), parts, rows, width, features, rank, n, code, _stream()), "add_adapters",
+             _serving_error_word(here, "add_adapters"), rows, width, features, rank, n, code, _stream()), "add_adapters",
            f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None and marks is None else 2)
     return out
