@@ -14,8 +14,8 @@
 using namespace lb200;
 
 namespace {
-constexpr int kThreads = 512;
-constexpr int kUnroll = 4;                              // 16-byte pieces of the row in flight per thread
+constexpr int kThreads = 256;
+constexpr int kUnroll = 8;                              // 16-byte pieces of the row in flight per thread
 
 struct RuleArgs {
     const float* logits; long ld_in;
@@ -30,11 +30,12 @@ struct RuleArgs {
     int rows, V, slice, slices;
 };
 
-// Counters of a slice.  The highest bit says "seen", the others count answers.
+// Counters of a slice.  The highest bit says "seen", the others count answers.  The prompt's ids come first and are plain stores (all
+// of the same value); only answers need atomic additions.
 struct Half {
     typedef unsigned short Raw;
     static constexpr unsigned kSeen = 0x8000u;
-    static __device__ __forceinline__ void seen(unsigned* c, int i) { atomicOr(c + (i >> 1), kSeen << ((i & 1) * 16)); }
+    static __device__ __forceinline__ void seen(unsigned* c, int i) { reinterpret_cast<Raw*>(c)[i] = (Raw)kSeen; }
     static __device__ __forceinline__ void answered(unsigned* c, int i) { atomicAdd(c + (i >> 1), 1u << ((i & 1) * 16)); }
     static __device__ __forceinline__ unsigned get(const unsigned* c, int i) { return reinterpret_cast<const Raw*>(c)[i]; }
     static __device__ __forceinline__ bool any4(const unsigned* c, int i) {
@@ -45,7 +46,7 @@ struct Half {
 struct Whole {
     typedef unsigned Raw;
     static constexpr unsigned kSeen = 0x80000000u;
-    static __device__ __forceinline__ void seen(unsigned* c, int i) { atomicOr(c + i, kSeen); }
+    static __device__ __forceinline__ void seen(unsigned* c, int i) { c[i] = kSeen; }
     static __device__ __forceinline__ void answered(unsigned* c, int i) { atomicAdd(c + i, 1u); }
     static __device__ __forceinline__ unsigned get(const unsigned* c, int i) { return c[i]; }
     static __device__ __forceinline__ bool any4(const unsigned* c, int i) {
@@ -65,22 +66,43 @@ __device__ __forceinline__ float penalised(float l, unsigned c, float rep, float
 
 // VEC: the row's logits and outputs lie alike within 16 bytes, and are read and written in pieces of 16.
 template <typename C, bool VEC>
-__global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) logit_rules_kernel(RuleArgs a) {
     pdl_wait();
     extern __shared__ unsigned smem[];
     __shared__ int twice;                               // a token has several biases
-    unsigned* counts = smem;                            // the slice's, then up to 3 of the tokens in front of it
+    unsigned* counts = smem;                            // of up to 3 tokens in front (places 0 .. 3), then the slice's, from place 4 on
     const int words = a.slice / (4 / (int)sizeof(typename C::Raw));
-    unsigned* biased = smem + words + 4;                // a bit per token, in the same order
+    unsigned* biased = smem + words + 4;                // a bit per place
     const int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices, tid = threadIdx.x;
     const float* in = a.logits + (size_t)row * a.ld_in;
     float* out = a.out + (size_t)row * a.ld_out;
     // the first `skew` tokens lie in front of a 16-byte boundary; slice 0 has them as well
     const int skew = VEC ? min((int)((16 - ((uintptr_t)in & 15)) & 15) >> 2, a.V) : 0;
-    const int first = skew + part * a.slice;            // counters: token - first (those in front of slice 0: at its end)
+    const int first = skew + part * a.slice;            // the token at place 4
     const int last = min(first + a.slice, a.V);
-    const bool has_front = part == 0 && skew > 0;
     const int n = last - first;                         // (0 or less: only a front)
+    const int lowest = part == 0 ? 0 : first;           // this CTA's tokens: lowest .. last - 1, or the front alone
+    const unsigned span = (unsigned)max(max(last, part == 0 ? skew : 0) - lowest, 0);
+
+    // the first pieces are on their way while the history is counted
+    const int pieces = VEC && n > 0 ? n >> 2 : 0;
+    const float4* iv = reinterpret_cast<const float4*>(in + first);
+    float4 l[kUnroll];
+    unsigned words_of[kUnroll];                         // the mask's word of a piece's first token
+    const unsigned* mask = nullptr;
+    if (a.allowed != nullptr) {
+        const int m = a.allowed_row ? a.allowed_row[row] : row;
+        if (m >= 0 && m < a.n_masks) mask = a.allowed + (size_t)m * a.ld_allowed;
+    }
+    auto fetch = [&](int p0) {                          // (nothing here uses what is loaded: a warp would wait for it)
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) if (p0 + u * kThreads < pieces) l[u] = iv[p0 + u * kThreads];
+        if (mask != nullptr) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) if (p0 + u * kThreads < pieces) words_of[u] = mask[(first + 4 * (p0 + u * kThreads)) >> 5];
+        }
+    };
+    if (VEC) fetch(tid);
 
     const float rep = a.repetition ? a.repetition[row] : 1.f;
     const float freq = a.frequency ? a.frequency[row] : 0.f, pres = a.presence ? a.presence[row] : 0.f;
@@ -92,11 +114,6 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
         b0 = min(max(a.bias_start[row], 0), a.n_biases);
         b1 = min(max(a.bias_start[row + 1], b0), a.n_biases);
     }
-    const unsigned* mask = nullptr;
-    if (a.allowed != nullptr) {
-        const int m = a.allowed_row ? a.allowed_row[row] : row;
-        if (m >= 0 && m < a.n_masks) mask = a.allowed + (size_t)m * a.ld_allowed;
-    }
 
     // ------------------------------------------------------------ what the row has seen, within the slice
     if (length > 0) {
@@ -104,22 +121,26 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
         __syncthreads();
         const int prompt = a.prompt_lengths ? min(max(a.prompt_lengths[row], 0), length) : 0;
         const int* h = a.history + (size_t)slot * a.ld_history;
-        auto add = [&](int id, int at) {
-            int i = id - first;
-            if (i < 0 && has_front && id >= 0) i = a.slice + id;        // a front token: behind the slice's counters (at most 3)
-            else if (i >= n || i < 0) return;
-            if (at < prompt) C::seen(counts, i); else C::answered(counts, i);
+        auto each = [&](int from, int to, auto add) {       // of the ids from .. to - 1 those that are this CTA's, four pieces of 16 bytes on their way
+            const int lead = min((int)((16 - ((uintptr_t)(h + from) & 15)) & 15) >> 2, to - from), quads = (to - from - lead) >> 2;
+            auto one = [&](int id) { if ((unsigned)(id - lowest) < span) add(id - first + 4); };
+            const int4* hv = reinterpret_cast<const int4*>(h + from + lead);
+            for (int i0 = tid; i0 < quads; i0 += 4 * kThreads) {
+                int4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = i0 + u * kThreads < quads ? hv[i0 + u * kThreads] : make_int4(-1, -1, -1, -1);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) { one(v[u].x); one(v[u].y); one(v[u].z); one(v[u].w); }
+            }
+            if (tid < lead) one(h[from + tid]);
+            const int rest = from + lead + 4 * quads + tid;
+            if (rest < to) one(h[rest]);
         };
-        const int lead = min((int)((16 - ((uintptr_t)h & 15)) & 15) >> 2, length), pieces = (length - lead) >> 2;
-        if (tid < lead) add(h[tid], tid);
-        const int4* hv = reinterpret_cast<const int4*>(h + lead);
-        for (int i = tid; i < pieces; i += kThreads) {
-            const int4 v = hv[i];
-            const int at = lead + 4 * i;
-            add(v.x, at); add(v.y, at + 1); add(v.z, at + 2); add(v.w, at + 3);
+        if (prompt > 0) {
+            each(0, prompt, [&](int i) { C::seen(counts, i); });
+            __syncthreads();
         }
-        const int rest = lead + 4 * pieces + tid;
-        if (rest < length) add(h[rest], rest);
+        if (length > prompt) each(prompt, length, [&](int i) { C::answered(counts, i); });
         __syncthreads();
     }
 
@@ -129,31 +150,27 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
         if (length > 0) l = penalised<C>(l, C::get(counts, i), rep, freq, pres);
         return allowed(token) ? l : -INFINITY;
     };
-    if (has_front && tid < skew) out[tid] = edited(in[tid], tid, a.slice + tid);
+    if (part == 0 && tid < skew) out[tid] = edited(in[tid], tid, tid - skew + 4);
     int done = 0;
     if (VEC) {
-        const int pieces = n > 0 ? n >> 2 : 0;
-        const float4* iv = reinterpret_cast<const float4*>(in + first);
         float4* ov = reinterpret_cast<float4*>(out + first);
         for (int p0 = tid; p0 < pieces; p0 += kThreads * kUnroll) {
-            float4 l[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) if (p0 + u * kThreads < pieces) l[u] = iv[p0 + u * kThreads];
+            if (p0 != tid) fetch(p0);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int p = p0 + u * kThreads;
                 if (p >= pieces) break;
                 const int i = 4 * p;
-                if (length > 0 && C::any4(counts, i)) {
-                    l[u].x = penalised<C>(l[u].x, C::get(counts, i), rep, freq, pres);
-                    l[u].y = penalised<C>(l[u].y, C::get(counts, i + 1), rep, freq, pres);
-                    l[u].z = penalised<C>(l[u].z, C::get(counts, i + 2), rep, freq, pres);
-                    l[u].w = penalised<C>(l[u].w, C::get(counts, i + 3), rep, freq, pres);
+                if (length > 0 && C::any4(counts, i + 4)) {
+                    l[u].x = penalised<C>(l[u].x, C::get(counts, i + 4), rep, freq, pres);
+                    l[u].y = penalised<C>(l[u].y, C::get(counts, i + 5), rep, freq, pres);
+                    l[u].z = penalised<C>(l[u].z, C::get(counts, i + 6), rep, freq, pres);
+                    l[u].w = penalised<C>(l[u].w, C::get(counts, i + 7), rep, freq, pres);
                 }
                 if (mask != nullptr) {
                     const int token = first + i, bit = token & 31;
-                    unsigned bits = mask[token >> 5] >> bit;
-                    if (bit > 28) bits |= mask[(token >> 5) + 1] << (32 - bit);         // (a word more: its last token is below V)
+                    unsigned bits = words_of[u] >> bit;
+                    if (skew != 0 && bit > 28) bits |= mask[(token >> 5) + 1] << (32 - bit);        // (a word more: its last token is below V)
                     if (!(bits & 1u)) l[u].x = -INFINITY;
                     if (!(bits & 2u)) l[u].y = -INFINITY;
                     if (!(bits & 4u)) l[u].z = -INFINITY;
@@ -165,13 +182,13 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
         done = pieces * 4;
     }
     for (int i0 = done + tid; i0 < n; i0 += kThreads * kUnroll) {
-        float l[kUnroll];
+        float one[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) if (i0 + u * kThreads < n) l[u] = in[first + i0 + u * kThreads];
+        for (int u = 0; u < kUnroll; ++u) if (i0 + u * kThreads < n) one[u] = in[first + i0 + u * kThreads];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int i = i0 + u * kThreads;
-            if (i < n) out[first + i] = edited(l[u], first + i, i);
+            if (i < n) out[first + i] = edited(one[u], first + i, i + 4);
         }
     }
     if (b1 <= b0) return;
@@ -182,10 +199,7 @@ __global__ void __launch_bounds__(kThreads) logit_rules_kernel(RuleArgs a) {
     for (int i = tid; i < a.slice / 32 + 1; i += kThreads) biased[i] = 0u;
     if (tid == 0) twice = 0;
     __syncthreads();                                    // (also: the slice's outputs are there for all threads)
-    auto place = [&](int id) {                          // bit of a token of this CTA, or -1
-        if (id >= first && id < last) return id - first;
-        return has_front && id >= 0 && id < skew ? a.slice + id : -1;
-    };
+    auto place = [&](int id) { return (unsigned)(id - lowest) < span ? id - first + 4 : -1; };      // of a token of this CTA
     for (int j = b0 + tid; j < b1; j += kThreads) {
         const int i = place(a.bias_ids[j]);
         if (i >= 0 && (atomicOr(biased + (i >> 5), 1u << (i & 31)) >> (i & 31) & 1u)) twice = 1;
@@ -241,7 +255,7 @@ extern "C" int lb_logit_rules(const float* logits, long ld_in, float* out, long 
                allowed_row, rows, V, 0, 0};
     const bool half = capacity <= 0x7fff;               // the count of a 16-bit counter ends there
     // slices as long as the counters may be, shorter where rows are few, so that the GPU is full
-    int slice = half ? 32768 : 16384;
+    int slice = half ? 16384 : 8192;
     while (slice > 2048 && (long)rows * ((V + slice - 1) / slice) < 296) slice >>= 1;
     a.slice = slice;
     a.slices = (V + slice - 1) / slice;
