@@ -38,10 +38,11 @@ struct Half {
     static __device__ __forceinline__ void seen(unsigned* c, int i) { reinterpret_cast<Raw*>(c)[i] = (Raw)kSeen; }
     static __device__ __forceinline__ void answered(unsigned* c, int i) { atomicAdd(c + (i >> 1), 1u << ((i & 1) * 16)); }
     static __device__ __forceinline__ unsigned get(const unsigned* c, int i) { return reinterpret_cast<const Raw*>(c)[i]; }
-    static __device__ __forceinline__ bool any4(const unsigned* c, int i) {
+    static __device__ __forceinline__ uint4 get4(const unsigned* c, int i) {
         const uint2 v = *reinterpret_cast<const uint2*>(c + (i >> 1));
-        return (v.x | v.y) != 0;
+        return make_uint4(v.x & 0xffffu, v.x >> 16, v.y & 0xffffu, v.y >> 16);
     }
+    static __device__ __forceinline__ float as_float(unsigned n) { return __uint_as_float(0x4b000000u | n) - 8388608.f; }      // (below 2^23)
 };
 struct Whole {
     typedef unsigned Raw;
@@ -49,19 +50,22 @@ struct Whole {
     static __device__ __forceinline__ void seen(unsigned* c, int i) { c[i] = kSeen; }
     static __device__ __forceinline__ void answered(unsigned* c, int i) { atomicAdd(c + i, 1u); }
     static __device__ __forceinline__ unsigned get(const unsigned* c, int i) { return c[i]; }
-    static __device__ __forceinline__ bool any4(const unsigned* c, int i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(c + i);
-        return (v.x | v.y | v.z | v.w) != 0;
-    }
+    static __device__ __forceinline__ uint4 get4(const unsigned* c, int i) { return *reinterpret_cast<const uint4*>(c + i); }
+    static __device__ __forceinline__ float as_float(unsigned n) { return (float)n; }
 };
 
+// A row's penalties; `inverse`: 1 / repetition.
+struct Penalties { float repetition, inverse, frequency, presence; };
+
+// Without branches or a division: where a warp meets a token that was seen, all its tokens go through this.  The quotient is the
+// product with the inverse, corrected by its remainder (where there is one: not for infinities).
 template <typename C>
-__device__ __forceinline__ float penalised(float l, unsigned c, float rep, float freq, float pres) {
-    if (c == 0) return l;
-    l = l > 0.f ? l / rep : l * rep;
+__device__ __forceinline__ float penalised(float l, unsigned c, const Penalties& p) {
+    const float q = l * p.inverse, rest = fmaf(-q, p.repetition, l);
+    const float quotient = fabsf(rest) < INFINITY ? fmaf(rest, p.inverse, q) : q;
     const unsigned n = c & (C::kSeen - 1u);
-    if (n != 0) l = l - freq * (float)n - pres;
-    return l;
+    const float less = n != 0 ? fmaf(p.frequency, C::as_float(n), p.presence) : 0.f;
+    return c != 0 ? (l > 0.f ? quotient : l * p.repetition) - less : l;
 }
 
 // VEC: the row's logits and outputs lie alike within 16 bytes, and are read and written in pieces of 16.
@@ -106,6 +110,7 @@ __global__ void __launch_bounds__(kThreads, 4) logit_rules_kernel(RuleArgs a) {
 
     const float rep = a.repetition ? a.repetition[row] : 1.f;
     const float freq = a.frequency ? a.frequency[row] : 0.f, pres = a.presence ? a.presence[row] : 0.f;
+    const Penalties pen{rep, 1.f / rep, freq, pres};
     const int slot = a.slots ? a.slots[row] : row;
     const bool counted = a.history != nullptr && slot >= 0 && slot < a.n_slots && !(rep == 1.f && freq == 0.f && pres == 0.f);
     const int length = counted ? min(max(a.lengths[row], 0), a.capacity) : 0;
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 4) logit_rules_kernel(RuleArgs a) {
     // ------------------------------------------------------------ the slice
     auto allowed = [&](int token) { return mask == nullptr || ((mask[token >> 5] >> (token & 31)) & 1u) != 0; };
     auto edited = [&](float l, int token, int i) {
-        if (length > 0) l = penalised<C>(l, C::get(counts, i), rep, freq, pres);
+        if (length > 0) l = penalised<C>(l, C::get(counts, i), pen);
         return allowed(token) ? l : -INFINITY;
     };
     if (part == 0 && tid < skew) out[tid] = edited(in[tid], tid, tid - skew + 4);
@@ -161,11 +166,14 @@ __global__ void __launch_bounds__(kThreads, 4) logit_rules_kernel(RuleArgs a) {
                 const int p = p0 + u * kThreads;
                 if (p >= pieces) break;
                 const int i = 4 * p;
-                if (length > 0 && C::any4(counts, i + 4)) {
-                    l[u].x = penalised<C>(l[u].x, C::get(counts, i + 4), rep, freq, pres);
-                    l[u].y = penalised<C>(l[u].y, C::get(counts, i + 5), rep, freq, pres);
-                    l[u].z = penalised<C>(l[u].z, C::get(counts, i + 6), rep, freq, pres);
-                    l[u].w = penalised<C>(l[u].w, C::get(counts, i + 7), rep, freq, pres);
+                if (length > 0) {
+                    const uint4 c = C::get4(counts, i + 4);
+                    if ((c.x | c.y | c.z | c.w) != 0) {
+                        l[u].x = penalised<C>(l[u].x, c.x, pen);
+                        l[u].y = penalised<C>(l[u].y, c.y, pen);
+                        l[u].z = penalised<C>(l[u].z, c.z, pen);
+                        l[u].w = penalised<C>(l[u].w, c.w, pen);
+                    }
                 }
                 if (mask != nullptr) {
                     const int token = first + i, bit = token & 31;
