@@ -8,7 +8,7 @@
 // product of the short sums with B beside it, and the rows of y that name the adapter get its product added in place, from where TMA
 // stores them.  Rows of one adapter never see another's product: it is made for all 128 rows and kept by those that name it.
 //
-// 12 warps: TMA loads, products, one that clears what lies behind an adapter's rank in B (0 x NaN would be NaN), TMA stores, and two
+// 12 warps: TMA loads of x and y, products, loads of B (and zeros behind an adapter's rank: 0 x NaN would be NaN), TMA stores, and two
 // groups of 128 threads, a thread per row, which take the tiles of features in turn.
 //
 // A tile whose rows name more adapters than that (decoding rows in front of a prompt) is marked, and left to the rows' kernel.
@@ -27,14 +27,15 @@ constexpr uint32_t kXTile = kRows * 128, kYTile = 2 * kRows * 128;
 
 // RB: blocks of 64 ranks
 template <int RB> struct Shape {
-    static constexpr int kY = RB == 1 ? 3 : 2, kB = RB == 1 ? 3 : 2;             // tiles of y and B on their way or at work
+    // Tiles of y and of B on their way or at work.  Three of y held 4.5 TB/s, five 5.4: a tile is on its way, at work, or being
+    // stored for a microsecond or two each.
+    static constexpr int kY = RB == 1 ? 5 : 3, kB = 2;
     static constexpr uint32_t kBTile = RB * kCols * 128, kH = RB * kRows * 128;  // bytes; of the short sums' values (remainders the same)
     static constexpr uint32_t kSums = kRows * (RB * 64 + 4) * 4;                 // this CTA's sums, float32
-    static constexpr uint32_t kRings = kY * kYTile + kB * kBTile;
-    // short sums | y ring | B ring, and this CTA's sums behind them or (two blocks) over the rings, which are filled afterwards then
-    static constexpr bool kOver = RB == 2;
-    static constexpr uint32_t kWork = 2 * kH + (kOver ? (kRings > kSums ? kRings : kSums) : kRings + kSums);
-    static constexpr uint32_t kSmem = kWork + 1024;
+    // short sums | y ring | B ring; the first product's ring and this CTA's sums lie over both, which are filled afterwards
+    static constexpr uint32_t kRings = kY * kYTile + kB * kBTile, kWork = 2 * kH + kRings;
+    static_assert(kSums <= kRings, "sums over the rings");
+    static constexpr uint32_t kSmem = kWork + 1024 + 128; // ... | barriers, the rows' scales and ranks
     static constexpr int kMostStages = 8;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -85,7 +86,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     uint8_t* h_s = base;                                  // values: blocks of 64 ranks, [128][128 B]; then remainders
     uint8_t* y_s = h_s + 2 * Sh::kH;
     uint8_t* b_s = y_s + Sh::kY * kYTile;
-    float* sums = reinterpret_cast<float*>(Sh::kOver ? y_s : b_s + Sh::kB * Sh::kBTile);
+    float* sums = reinterpret_cast<float*>(y_s);
     uint8_t* ring = y_s;                                  // the first product's: x tile, then the adapters' A tiles
     uint64_t* bars = reinterpret_cast<uint64_t*>(base + Sh::kWork);
     uint64_t* x_full = bars;                              // [kMostStages]
@@ -102,6 +103,8 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     int* list = reinterpret_cast<int*>(d_empty + 4);      // the adapters, their ranks
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(list + 2 * kMost);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* row_scale = reinterpret_cast<float*>(tmem_slot + 2);        // [128]
+    unsigned char* row_ranks = reinterpret_cast<unsigned char*>(row_scale + kRows);     // [128]: 0 without an adapter
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ta.parts), tile = (int)(blockIdx.x / (unsigned)ta.parts);
     const long t0 = (long)tile * kRows;
@@ -203,6 +206,10 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     int place = -1;
     if (own >= 0)
         for (int q = 0; q < count; ++q) if (list[q] == own) place = q;
+    if (warp >= kFirstAdder && group == 1) {
+        row_scale[r] = own >= 0 && a.scales ? a.scales[own] : 1.f;
+        row_ranks[r] = (unsigned char)(own >= 0 ? rank_of(a, own) : 0);
+    }
     if (warp >= kFirstAdder && group == 0 && count > 0) {
         float* to = sums + r * (RB * 64 + 4);
         const bool ok = k_n <= 0 || wait(low_ready, 0, 5, 0);
@@ -231,18 +238,17 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const uint32_t from = smem_u32(sums), to = smem_u32(h_s);
         for (int i = threadIdx.x - 32 * kFirstAdder; i < kRows / ta.parts * pieces; i += 256) {
             const int row = rank * (kRows / ta.parts) + i / pieces, j = 4 * (i % pieces);
-            const int its = adapter_of(a, t0 + row);
+            const int ranks = row_ranks[row];
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (its >= 0) {
+            if (j < ranks) {
                 const uint32_t at = from + 4 * (row * (RB * 64 + 4) + j);
                 float4 got[8];
 #pragma unroll
                 for (int p = 0; p < 8; ++p) if (p < ta.parts) got[p] = remote4(ta.parts > 1 ? at_rank(at, p) : at);
 #pragma unroll
                 for (int p = 0; p < 8; ++p) if (p < ta.parts) { v.x += got[p].x; v.y += got[p].y; v.z += got[p].z; v.w += got[p].w; }
-                const float scale = a.scales ? a.scales[its] : 1.f;
-                const int ranks = rank_of(a, its);
-                v.x = j < ranks ? v.x * scale : 0.f;
+                const float scale = row_scale[row];
+                v.x *= scale;
                 v.y = j + 1 < ranks ? v.y * scale : 0.f;
                 v.z = j + 2 < ranks ? v.z * scale : 0.f;
                 v.w = j + 3 < ranks ? v.w * scale : 0.f;
@@ -268,7 +274,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     // ------------------------------------------------------------ this CTA's tiles of features
     const int steps = mine * max(count, 1);                // (tile, adapter) by (tile, adapter)
     if (warp == 0) {
-        int y_done = 0, b_done = 0;
+        int y_asked = 0;
         for (int i = 0; i < mine && !*failed; ++i) {
             const int n0 = (rank + i * ta.parts) * kCols, s = i % Sh::kY;
             if (i >= Sh::kY && !wait(y_empty + s, ((i / Sh::kY) - 1) & 1, 6, i)) break;
@@ -278,22 +284,10 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 tma_load_2d(y_s + s * kYTile + kRows * 128, &map_y, y_full + s, n0 + 64, (int)t0);
             }
             __syncwarp();
-            y_done = i + 1;
-            for (int q = 0; q < count; ++q) {
-                const int u = i * count + q, sb = u % Sh::kB;
-                if (u >= Sh::kB && !wait(b_empty + sb, ((u / Sh::kB) - 1) & 1, 7, u)) break;
-                if (elect_one()) {
-                    mbar_expect_tx(b_full + sb, Sh::kBTile);
-#pragma unroll
-                    for (int blk = 0; blk < RB; ++blk) tma_load_3d(b_s + sb * Sh::kBTile + blk * (kCols * 128), &map_b, b_full + sb, blk * 64, n0, list[q]);
-                }
-                __syncwarp();
-                b_done = u + 1;
-            }
+            y_asked = i + 1;
         }
         if (*failed) {                                     // let the copies already under way land before the CTA leaves
-            for (int i = max(0, y_done - Sh::kY); i < y_done; ++i) mbar_wait(y_full + i % Sh::kY, (i / Sh::kY) & 1);
-            for (int u = max(0, b_done - Sh::kB); u < b_done; ++u) mbar_wait(b_full + u % Sh::kB, (u / Sh::kB) & 1);
+            for (int i = max(0, y_asked - Sh::kY); i < y_asked; ++i) mbar_wait(y_full + i % Sh::kY, (i / Sh::kY) & 1);
         }
     } else if (warp == 1 && count > 0) {
         constexpr uint32_t idesc = umma_idesc(kRows, kCols);
@@ -319,9 +313,25 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             __syncwarp();
         }
     } else if (warp == 2 && count > 0) {
-        for (int u = 0; u < steps; ++u) {
+        int b_asked = 0;
+        auto ask = [&](int u) -> bool {                    // B of step u
+            const int i = u / count, q = u - i * count, sb = u % Sh::kB, n0 = (rank + i * ta.parts) * kCols;
+            if (u >= Sh::kB && !wait(b_empty + sb, ((u / Sh::kB) - 1) & 1, 7, u)) return false;
+            if (elect_one()) {
+                mbar_expect_tx(b_full + sb, Sh::kBTile);
+#pragma unroll
+                for (int blk = 0; blk < RB; ++blk) tma_load_3d(b_s + sb * Sh::kBTile + blk * (kCols * 128), &map_b, b_full + sb, blk * 64, n0, list[q]);
+            }
+            __syncwarp();
+            b_asked = u + 1;
+            return true;
+        };
+        bool ok = steps == 0 || ask(0);
+        for (int u = 0; u < steps && ok; ++u) {
+            if (u + 1 < steps && !ask(u + 1)) break;
             const int q = u % count, sb = u % Sh::kB, ranks = list[kMost + q], end = (ranks + 15) / 16 * 16;
-            if (!wait(b_full + sb, (u / Sh::kB) & 1, 10, u)) break;
+            ok = wait(b_full + sb, (u / Sh::kB) & 1, 10, u);
+            if (!ok) break;
             if (ranks < a.R && ranks < end) {              // (columns behind R are zeros already)
                 uint8_t* b = b_s + sb * Sh::kBTile + (ranks >> 6) * (kCols * 128);
                 for (int f = lane; f < kCols; f += 32)
@@ -332,6 +342,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             __syncwarp();
             if (lane == 0) mbar_arrive(b_clear + sb);
         }
+        if (*failed) for (int u = max(0, b_asked - Sh::kB); u < b_asked; ++u) mbar_wait(b_full + u % Sh::kB, (u / Sh::kB) & 1);
     } else if (warp == 3) {
         // One store may still be reading its tile while the next one's sums are made; with two tiles in all it is waited for at once.
         constexpr int kBehind = Sh::kY > 2 ? 1 : 0;
