@@ -230,7 +230,7 @@ Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_pref
     double least = 1e30;
     for (int two = 0; two < 2; ++two) {
         const long rows = two ? 256 : 128, tiles = ((tokens * G + rows - 1) / rows + (groups - 1) / 2) * Hkv;
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 3; ++k) {
             const int ranks = 1 << k;
             const long room = k == 0 ? 148 : k == 1 ? 148 : k == 2 ? 132 : 120;
             long clusters = room / (tiles * ranks);

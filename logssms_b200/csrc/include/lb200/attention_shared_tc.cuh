@@ -29,6 +29,8 @@ constexpr int kFirstSoftmaxWarp = 3;
 constexpr int kThreads = 32 * (kFirstSoftmaxWarp + 8);
 constexpr float kTau = 8.f;                               // log2 of the growth of a row's maximum that O is rescaled for
 
+constexpr int kMostRanks = 4;                             // CTAs of a cluster
+
 template <int HD, bool TWO> struct Shape {
     static constexpr int kBlocks = HD / 64;
     // tiles of K and of V on their way or at work: a tile's copy takes about as long as the softmax of two
@@ -39,7 +41,9 @@ template <int HD, bool TWO> struct Shape {
     static constexpr uint32_t kGroupCols = 128 + HD;      // per group: S (then P) of even tiles, of odd tiles, O from 128
     static constexpr uint32_t kResult = 2 * kQ * HD * 4;  // both groups' O at the end, over Q and the rings
     static constexpr uint32_t kTiles = kQBytes * (TWO ? 2 : 1) + (kK + kV) * kTileBytes;
-    static constexpr uint32_t kEnd = kResult + 2 * kQ * 8; // with their rows' (maximum, sum)
+    // ... with their rows' (maximum, sum), and of this CTA's part of the rows the results' weights and where they go
+    static constexpr int kSources = kMostRanks * (TWO ? 1 : 2);
+    static constexpr uint32_t kEnd = kResult + 2 * kQ * 8 + kRows * (kSources * 4 + 8);
     static constexpr uint32_t kWork = kTiles > kEnd ? kTiles : kEnd;
     static constexpr uint32_t kSmem = kWork + 512;
     static_assert(2 * kGroupCols <= 512, "tensor memory");
@@ -83,6 +87,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint8_t* k_s = q_s + Sh::kQBytes * (TWO ? 2 : 1);     // stages of K: blocks of [64][128 B]
     uint8_t* v_s = k_s + kK * kTileBytes;
     float2* ml_s = reinterpret_cast<float2*>(base + Sh::kResult);      // at the end: (maximum, sum) of both groups' rows
+    constexpr int kMostSources = Sh::kSources;
+    long* slots = reinterpret_cast<long*>(ml_s + 2 * kQ);
+    float* weights = reinterpret_cast<float*>(slots + Sh::kRows);
     uint64_t* k_full = reinterpret_cast<uint64_t*>(base + Sh::kWork);
     uint64_t* k_empty = k_full + kK;
     uint64_t* v_full = k_empty + kK;
@@ -205,57 +212,48 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     } else if (warp < kFirstSoftmaxWarp) {
         const int g = warp - 1, step = TWO ? 1 : 2, from = TWO ? 0 : g;
         if (g < active) {                                  // (whole warps: see elect_one)
-            constexpr uint32_t idesc_s = umma_idesc(kQ, kKV), idesc_o = idesc_s | kBMnMajor;
-            const uint64_t qdesc = umma_desc(q_s + (TWO ? g * Sh::kQBytes : 0)), kdesc0 = umma_desc(k_s), vdesc0 = umma_desc(v_s);
+            constexpr uint32_t idesc_s = umma_idesc(kQ, kKV), idesc_o = umma_idesc(kQ, HD) | kBMnMajor;
+            const uint64_t qdesc = umma_desc(q_s + (TWO ? g * Sh::kQBytes : 0)), kdesc0 = umma_desc(k_s), vdesc0 = umma_desc_mn(v_s, Sh::kKVBlock);
             const uint32_t cols = tmem + g * kGroupCols;
             bool ok = true;
-            auto issue_s = [&](int i, int t) -> bool {     // S of tile i, the group's tile number t, into its S buffer t & 1
-                const int s = i % kK;
-                if (!__all_sync(0xffffffffu, mbar_spin(k_full + s, (i / kK) & 1))) {
-                    if (lane == 0) report(a.error, 2, i);
-                    *failed = 1;
-                    return false;
-                }
-                fence_after_sync();
-                if (elect_one()) {
-                    const uint64_t kdesc = kdesc0 + (uint64_t)(s * (kTileBytes >> 4));
-                    const uint32_t d = cols + (t & 1) * 64;
+            auto loaded = [&](uint64_t* full, int stages, int i) { return mbar_spin(full + i % stages, (i / stages) & 1); };
+            auto issue_s = [&](int i, int t) {             // S of tile i, the group's tile number t, into its S buffer t & 1
+                const uint64_t kdesc = kdesc0 + (uint64_t)((i % kK) * (kTileBytes >> 4));
+                const uint32_t d = cols + (t & 1) * 64;
 #pragma unroll
-                    for (int blk = 0; blk < kBlocks; ++blk)
+                for (int blk = 0; blk < kBlocks; ++blk)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_bf16(d, qdesc + blk * (Sh::kQBlock >> 4) + 2 * k, kdesc + blk * (Sh::kKVBlock >> 4) + 2 * k, idesc_s, (blk | k) != 0);
-                    umma_commit(s_ready + 2 * g + (t & 1));
-                    umma_commit(k_empty + s);
-                }
-                __syncwarp();
-                return true;
+                    for (int k = 0; k < 4; ++k)
+                        umma_bf16(d, qdesc + blk * (Sh::kQBlock >> 4) + 2 * k, kdesc + blk * (Sh::kKVBlock >> 4) + 2 * k, idesc_s, (blk | k) != 0);
+                umma_commit(s_ready + 2 * g + (t & 1));
+                umma_commit(k_empty + i % kK);
             };
-            if (from < n_kt) ok = issue_s(from, 0);
-            if (ok && from + step < n_kt) ok = issue_s(from + step, 1);
+            for (int t = 0; t < 2 && ok; ++t) {
+                const int i = from + t * step;
+                if (i >= n_kt) break;
+                ok = __all_sync(0xffffffffu, loaded(k_full, kK, i));
+                if (!ok) { if (lane == 0) report(a.error, 2, i); *failed = 1; break; }
+                fence_after_sync();
+                if (elect_one()) issue_s(i, t);
+                __syncwarp();
+            }
             for (int i = from, t = 0; i < n_kt && ok && !*failed; i += step, ++t) {
-                const int s = i % kV;
-                // V of the tile is there, and P
-                if (!__all_sync(0xffffffffu, mbar_spin(v_full + s, (i / kV) & 1) && mbar_spin(p_ready + 2 * g + (t & 1), (t >> 1) & 1))) {
-                    if (lane == 0) report(a.error, 3, i);
-                    *failed = 1;
-                    break;
-                }
+                // V of the tile is there, K of the tile after the next, and P, which is waited for last: then all of it goes out at once
+                const int later = i + 2 * step;
+                const bool fine = loaded(v_full, kV, i) && (later >= n_kt || loaded(k_full, kK, later)) && mbar_spin(p_ready + 2 * g + (t & 1), (t >> 1) & 1);
+                if (!__all_sync(0xffffffffu, fine)) { if (lane == 0) report(a.error, 3, i); *failed = 1; break; }
                 fence_after_sync();
                 if (elect_one()) {
-                    const uint64_t vdesc = vdesc0 + (uint64_t)(s * (kTileBytes >> 4));
+                    const uint64_t vdesc = vdesc0 + (uint64_t)((i % kV) * (kTileBytes >> 4));
                     const uint32_t p = cols + (t & 1) * 64;
 #pragma unroll
-                    for (int blk = 0; blk < kBlocks; ++blk)
-#pragma unroll
-                        for (int k = 0; k < kKV / 16; ++k)
-                            umma_bf16_tmem_a(cols + 128 + blk * 64, p + 8 * k, vdesc + blk * (Sh::kKVBlock >> 4) + (uint64_t)(2048 >> 4) * k, idesc_o,
-                                             (t > 0 || k != 0) ? 1u : 0u);
+                    for (int k = 0; k < kKV / 16; ++k)     // all dims in one product: one of 64 columns takes as long as one of 128
+                        umma_bf16_tmem_a(cols + 128, p + 8 * k, vdesc + (uint64_t)(2048 >> 4) * k, idesc_o, (t > 0 || k != 0) ? 1u : 0u);
                     umma_commit(o_ready + 2 * g + (t & 1));
-                    umma_commit(v_empty + s);
+                    umma_commit(v_empty + i % kV);
+                    if (later < n_kt) issue_s(later, t + 2);
                 }
                 __syncwarp();
-                if (i + 2 * step < n_kt) ok = issue_s(i + 2 * step, t + 2);
             }
         }
     } else {
@@ -376,43 +374,62 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     __syncthreads();
     if (warp == 1) tmem_free<512>(tmem);
     if (ranks > 1) cluster_meet();
-    // This CTA's part of the rows: a warp per row adds up the cluster's results of it, 16 bytes a lane.
+    // This CTA's part of the rows, rank, rank + ranks, ...: a thread per row puts together the results' weights, then a warp takes a row
+    // at a time, 16 bytes a lane, with all results of two rows on their way.
     {
         constexpr int kPieces = HD / 4, kSources = TWO ? 1 : 2;
         const uint32_t here = smem_u32(base), ml_here = smem_u32(ml_s), rank = ranks > 1 ? cluster_rank() : 0u;
-        const int splits = a.prefix_splits + a.own_splits, sources = ranks * kSources;
-        for (int r = (int)rank + ranks * warp; r < rows; r += ranks * (kThreads / 32)) {
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (lane < sources) {
-                const uint32_t at = ml_here + 8 * (r + (lane % kSources) * kQ);
-                ml = ranks > 1 ? remote2(at_rank(at, lane / kSources)) : *reinterpret_cast<const float2*>(ml_s + r + (lane % kSources) * kQ);
-            }
-            const float m = warp_max(ml.x), ref = m == -INFINITY ? 0.f : m;
-            const float f = exp2f(ml.x - ref);
-            const float l = warp_sum(ml.y * f);
-            const int token = (int)((row0 + r) / G), head = (int)((row0 + r) % G);
-            const size_t slot = ((size_t)(first + token) * a.Hq + kvh * G + head) * splits + range / ranks;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            const uint32_t piece = here + 16 * (uint32_t)(r * kPieces + (lane ^ (r & (kPieces - 1) & 31)));      // (128 rows on: the same place)
-            for (int s0 = 0; s0 < sources; s0 += 8) {      // eight on their way
-                float4 v[8];
-                float w[8];
+        const int splits = a.prefix_splits + a.own_splits, sources = ranks * kSources, ours = (rows - (int)rank + ranks - 1) / ranks;
+        if ((int)threadIdx.x < ours) {
+            const int r = (int)rank + ranks * (int)threadIdx.x, at = (int)row0 + r, token = at / G;
+            float2 ml[kMostSources];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    w[u] = s0 + u < sources ? __shfl_sync(0xffffffffu, f, s0 + u) : 0.f;
-                    v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (w[u] != 0.f && lane < kPieces) {   // (a range without keys left nothing)
-                        const uint32_t at = piece + ((s0 + u) % kSources) * (kQ * kPieces * 16);
-                        v[u] = remote4(ranks > 1 ? at_rank(at, (s0 + u) / kSources) : at);
+            for (int s = 0; s < kMostSources; ++s)
+                if (s < sources) ml[s] = remote2(ranks > 1 ? at_rank(ml_here + 8 * (r + (s % kSources) * kQ), s / kSources) : ml_here + 8 * (r + (s % kSources) * kQ));
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int s = 0; s < kMostSources; ++s) if (s < sources) m = fmaxf(m, ml[s].x);
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int s = 0; s < kMostSources; ++s)
+                if (s < sources) {
+                    const float f = exp2f(ml[s].x - ref);
+                    l += ml[s].y * f;
+                    weights[threadIdx.x * kMostSources + s] = f;
+                }
+            const long slot = ((long)(first + token) * a.Hq + kvh * G + at - token * G) * splits + range / ranks;
+            slots[threadIdx.x] = slot;
+            *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(m, l);
+        }
+        __syncthreads();
+        for (int n0 = warp; n0 < ours; n0 += 2 * (kThreads / 32)) {
+            float4 v[2][kMostSources];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = n0 + h * (kThreads / 32), r = (int)rank + ranks * n;
+                const uint32_t piece = here + 16 * (uint32_t)(r * kPieces + (lane ^ (r & (kPieces - 1) & 31)));      // (128 rows on: the same place)
+#pragma unroll
+                for (int s = 0; s < kMostSources; ++s) {
+                    v[h][s] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (n < ours && s < sources && lane < kPieces && weights[n * kMostSources + s] != 0.f) {         // (a range without keys left nothing)
+                        const uint32_t at = piece + (s % kSources) * (kQ * kPieces * 16);
+                        v[h][s] = remote4(ranks > 1 ? at_rank(at, s / kSources) : at);
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    o.x = fmaf(v[u].x, w[u], o.x); o.y = fmaf(v[u].y, w[u], o.y); o.z = fmaf(v[u].z, w[u], o.z); o.w = fmaf(v[u].w, w[u], o.w);
-                }
             }
-            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(m, l);
-            if (lane < kPieces) *reinterpret_cast<float4*>(a.part_o + slot * HD + 4 * lane) = o;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = n0 + h * (kThreads / 32);
+                if (n >= ours || lane >= kPieces) continue;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int s = 0; s < kMostSources; ++s)
+                    if (s < sources) {
+                        const float w = weights[n * kMostSources + s];
+                        o.x = fmaf(v[h][s].x, w, o.x); o.y = fmaf(v[h][s].y, w, o.y); o.z = fmaf(v[h][s].z, w, o.z); o.w = fmaf(v[h][s].w, w, o.w);
+                    }
+                *reinterpret_cast<float4*>(a.part_o + slots[n] * HD + 4 * lane) = o;
+            }
         }
     }
     if (ranks > 1) cluster_meet();                         // nobody leaves while another CTA reads its results

@@ -53,6 +53,10 @@ __device__ __forceinline__ uint64_t umma_desc(const void* tile) {
     d |= (uint64_t)2 << 61;                               // 128-byte swizzle
     return d;
 }
+// of an MN-major operand with more than 64 values of m or n: the blocks of 64 lie `block` bytes apart
+__device__ __forceinline__ uint64_t umma_desc_mn(const void* tile, uint32_t block) {
+    return (umma_desc(tile) & ~((uint64_t)0x3FFF << 16)) | (uint64_t)(block >> 4) << 16;
+}
 // float32 accumulator, bfloat16 operands, both K-major; `kBMnMajor` added: the B operand is MN-major
 __host__ __device__ constexpr uint32_t umma_idesc(int M, int N) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
