@@ -221,28 +221,35 @@ bool tc_ok(const SharedArgs& a, int dtype) {
            (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
 }
 // How the prefix's work is laid out on the tensor cores: rows of a tile, CTAs of a cluster, clusters for a tile's keys.
-struct Layout { bool two; int ranks, clusters; };
-Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_prefix) {
-    // us: a tile of 64 keys takes 0.85 with 256 rows and 0.6 where the groups share the tiles out; a CTA's beginning and end
-    // 5; a row of partial results is written and read at 4 TB/s.  As many CTAs at once as the GPU holds in clusters of that size.
+struct Layout { bool two; int ranks, clusters; double us; };
+Layout best_layout(long tokens, int G, int Hkv, int hd, int groups, long max_prefix, long most_ctas) {
+    // us: a tile of 64 keys takes 1.1 with 256 rows and 0.6 where the groups share the tiles out; a CTA's beginning and end 8; a row of
+    // partial results is written and read at 4 TB/s.  As many CTAs at once as the GPU holds in clusters of that size.
     const long kt = max_prefix > 0 ? (max_prefix + 63) / 64 : 1;
-    Layout best{false, 1, 1};
-    double least = 1e30;
+    Layout best{false, 1, 1, 1e30};
     for (int two = 0; two < 2; ++two) {
         const long rows = two ? 256 : 128, tiles = ((tokens * G + rows - 1) / rows + (groups - 1) / 2) * Hkv;
         for (int k = 0; k < 3; ++k) {
             const int ranks = 1 << k;
-            const long room = k == 0 ? 148 : k == 1 ? 148 : k == 2 ? 132 : 120;
+            const long held = k == 2 ? 132 : 148, room = held < most_ctas ? held : most_ctas;
             long clusters = room / (tiles * ranks);
             if (clusters > (kt + ranks - 1) / ranks) clusters = (kt + ranks - 1) / ranks;
             if (clusters < 1) clusters = 1;
             if (clusters > 64) clusters = 64;
             const long per = (kt + clusters * ranks - 1) / (clusters * ranks), waves = (tiles * ranks * clusters + room - 1) / room;
-            const double us = waves * (5.0 + per * (two ? 0.85 : 0.6)) + clusters * tokens * G * Hkv * hd * 8e-6 / 4.0 + 0.2 * k;
-            if (us < least) { least = us; best = {two != 0, ranks, (int)clusters}; }
+            const double us = waves * (8.0 + per * (two ? 1.1 : 0.6)) + clusters * tokens * G * Hkv * hd * 8e-6 / 4.0 + 0.3 * k;
+            if (us < best.us) best = {two != 0, ranks, (int)clusters, us};
         }
     }
     return best;
+}
+// The own keys' kernel runs beside this one, on what it leaves: it gets SMs of its own, half as many as its share of the work says
+// (it is bound by memory).  256 requests, 32,768 + 2,048 keys: 144 CTAs of the prefix's take 118 us in all, 96 take 108.
+Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_prefix, long max_own) {
+    const Layout all = best_layout(tokens, G, Hkv, hd, groups, max_prefix, 148);
+    const double own = 4.0 + tokens * Hkv * hd * 4e-6 * (max_own > 0 ? max_own : 0) / 2 / 4.7;
+    const long room = (long)(148 * all.us / (all.us + 0.5 * own));
+    return best_layout(tokens, G, Hkv, hd, groups, max_prefix, room < 74 ? 74 : room);
 }
 
 int launch_tc(const SharedArgs& a, const Layout& y, cudaStream_t stream) {
@@ -282,7 +289,7 @@ extern "C" int lb_attention_shared_splits(const void* q, long q_stride, const vo
         const long most = keys / least < 1 ? 1 : keys / least, want = (ctas + n - 1) / n;
         return (int)(want > most ? (most > 64 ? 64 : most) : want > 64 ? 64 : want);
     };
-    const int prefix = tc ? layout_for(tokens, G, Hkv, hd, groups, max_prefix).clusters : cut(592, tiles, max_prefix, 64);
+    const int prefix = tc ? layout_for(tokens, G, Hkv, hd, groups, max_prefix, max_own).clusters : cut(592, tiles, max_prefix, 64);
     return prefix << 16 | cut(tc ? 2368 : 592, items, max_own, tc ? 256 : 64);
 }
 
@@ -293,7 +300,7 @@ extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_c
                                    const int* block_table, long bt_stride, int bt_cols, int requests, const int* token_req,
                                    const int* positions, const int* group_start, const int* prefix_lens, int groups, float* part_o,
                                    float* part_ml, long pages, int tokens, int Hq, int Hkv, int hd, int page_size, int prefix_splits,
-                                   int own_splits, long max_prefix, float scale, int* error, int dtype,
+                                   int own_splits, long max_prefix, long max_own, float scale, int* error, int dtype,
                                    void* stream) {
     if (tokens <= 0 || groups <= 0) return kOk;
     if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || hd <= 0 || hd % 8 != 0 || hd > 256 || page_size <= 0 || prefix_splits < 1 || own_splits < 1) return kBadSize;
@@ -306,7 +313,7 @@ extern "C" int lb_attention_shared(const void* q, long q_stride, const void* k_c
     if ((long)tokens * ((G + kRows - 1) / kRows) > 0x7fffffffL || tiles > 0x7fffffffL) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     int rc = kBadDType;
-    Layout y = layout_for(tokens, G, Hkv, hd, groups, max_prefix);
+    const Layout y = layout_for(tokens, G, Hkv, hd, groups, max_prefix, max_own);
     LB_DISPATCH_DTYPE(dtype, rc = tc_ok(a, dtype) ? launch_tc(a, y, s) : launch_general<T>(a, tiles, s);
                       if (rc == 0) rc = launch_pdl(shared_merge_kernel<T>, dim3((unsigned)(((long)tokens * Hq + 7) / 8)), dim3(256), 0, s, a));
     return rc != 0 ? rc : launch_status();

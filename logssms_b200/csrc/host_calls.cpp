@@ -210,7 +210,7 @@ PyObject* swiglu(PyObject*, PyObject* const* args, Py_ssize_t n) {
 namespace serving {
 typedef int (*SplitsFn)(const void*, long, const void*, const void*, long, int, int, int, int, int, int, long, long, int);
 typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, const int*, long, int, int, const int*, const int*, const int*,
-                           const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, float, int*, int, void*);
+                           const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, long, float, int*, int, void*);
 typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
                           const int*, void*, long, float*, int*, int*, long, int, int, int, int, int, void*);
 typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
@@ -275,7 +275,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         float* part_o = (float*)parts.data_ptr();
         const int rc = attention_fn(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), out.data_ptr(), (const int*)bt.data_ptr(), bt.stride(0),
                                     (int)bt.size(1), (int)bt.size(0), data<int>(t[4]), data<int>(t[5]), data<int>(t[6]), data<int>(t[7]), (int)groups,
-                                    part_o, part_o + rows * hd, pages, (int)tokens, (int)Hq, (int)Hkv, (int)hd, (int)page, sp, so, max_prefix,
+                                    part_o, part_o + rows * hd, pages, (int)tokens, (int)Hq, (int)Hkv, (int)hd, (int)page, sp, so, max_prefix, max_context - max_prefix,
                                     (float)scale, error_words[device], code, stream_of(device));
         return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
     });

@@ -14,7 +14,7 @@ namespace lb200 {
 namespace shared_own {
 using namespace tc;
 typedef __nv_bfloat16 bf16;
-constexpr int kWarps = 2, kThreads = 32 * kWarps, kKeys = 16, kStages = 3, kRows = 16;
+constexpr int kWarps = 2, kThreads = 32 * kWarps, kKeys = 16, kStages = 3, kRows = 16, kLeast = 256;
 constexpr float kTau = 8.f;                               // log2 of the growth of a row's maximum that sums are scaled for
 
 // A tile: blocks of 64 columns, [16 keys][128 bytes]; 16-byte piece c of key r lies at c ^ (r & 7).
@@ -80,7 +80,8 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int from = 0, to = 0;                                 // from: a multiple of 16; keys below `begin` are left out
     if (grouped && end > begin) {
         const int first = begin / kKeys * kKeys;
-        const int per = ((end - first + a.own_splits - 1) / a.own_splits + kKeys * kWarps - 1) / (kKeys * kWarps) * (kKeys * kWarps);
+        // (no range is shorter than kLeast: a CTA's beginning and end take as long as 200 keys)
+        const int per = max(((end - first + a.own_splits - 1) / a.own_splits + kKeys * kWarps - 1) / (kKeys * kWarps) * (kKeys * kWarps), kLeast);
         from = (int)min((long)first + (long)split * per, (long)end);
         to = (int)min((long)from + per, (long)end);
     }

@@ -158,7 +158,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     // (whole warps: see elect_one)
     auto load = [&](int i, int row, int stages, uint8_t* ring, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int role) -> bool {
         const int s = i % stages;
-        if (i >= stages && !__all_sync(0xffffffffu, mbar_spin(empty + s, ((i / stages) - 1) & 1))) {
+        if (i >= stages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / stages) - 1) & 1))) {
             if (lane == 0) report(a.error, role, i);
             *failed = 1;
             return false;
@@ -297,49 +297,65 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 if (id < 0 || id >= a.pages) seen = 0;
             }
             const bool whole = __all_sync(0xffffffffu, j0 + kKV <= seen);
-            uint32_t sc[64];                               // the row's scores
-            tmem_get64(lane_addr + (t & 1) * 64, sc);
-            if (!whole) {
+            uint32_t sc[64], pk[32];                       // the row's scores, its weights
+            float mx4[4], sum[4];                          // (four chains each: two warps a scheduler hide no latency)
+            // the weights relative to `ref`, and the scores' maximum on the way
+            auto weigh = [&](float ref) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) if (j0 + c >= seen) sc[c] = 0xff800000u;
-            }
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};       // (four chains: two warps a scheduler hide no latency)
+                for (int e = 0; e < 4; ++e) { mx4[e] = -INFINITY; sum[e] = 0.f; }
 #pragma unroll
-            for (int c = 0; c < 64; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], fmaxf(__uint_as_float(sc[c + e]), __uint_as_float(sc[c + 4 + e])));
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
-            const bool grow = mx > m_used + kTau;
-            if (__any_sync(0xffffffffu, grow)) {
-                float factor = 1.f;
-                if (grow) { factor = exp2f(m_used - mx); m_used = mx; l *= factor; }
-                if (t > 0) {
-                    if (!wait_pv(t - 1, 6, i)) { ok = false; break; }
-                    fence_after_sync();
-#pragma unroll 1
-                    for (int piece = 0; piece < HD / 8; ++piece) {
-                        uint32_t ov[8];
-                        tmem_get8(lane_addr + 128 + piece * 8, ov);
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * factor);
-                        tmem_st8(lane_addr + 128 + piece * 8, ov);
-                    }
-                    tmem_st_wait();
+                for (int c = 0; c < 64; c += 2) {
+                    const float x0 = __uint_as_float(sc[c]), x1 = __uint_as_float(sc[c + 1]);
+                    const float e0 = ex2_approx(fmaf(x0, a.scale_log2, -ref)), e1 = ex2_approx(fmaf(x1, a.scale_log2, -ref));
+                    mx4[(c >> 1) & 3] = fmaxf(mx4[(c >> 1) & 3], fmaxf(x0, x1));
+                    __nv_bfloat162 pr = __floats2bfloat162_rn(e0, e1);
+                    const uint32_t w = *reinterpret_cast<uint32_t*>(&pr);
+                    pk[c >> 1] = w;
+                    // the row sum takes the weights as the product will see them, rounded
+                    sum[(c >> 1) & 1] += __uint_as_float(w << 16);
+                    sum[2 + ((c >> 1) & 1)] += __uint_as_float(w & 0xffff0000u);
                 }
+            };
+            auto top = [&] { return fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2; };
+            tmem_get64(lane_addr + (t & 1) * 64, sc);
+            // Mostly no row's maximum grows by more than 2^kTau: the weights are made without waiting for it, and again where it does.
+            bool again = !whole || __any_sync(0xffffffffu, m_used == -INFINITY);
+            if (!again) {
+                weigh(m_used);
+                again = __any_sync(0xffffffffu, top() > m_used + kTau);
+                if (again) tmem_get64(lane_addr + (t & 1) * 64, sc);
             }
-            const float ref = m_used == -INFINITY ? 0.f : m_used;
-            float sum[4] = {};
-            uint32_t pk[32];
+            if (again) {
+                if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-                const float e0 = ex2_approx(fmaf(__uint_as_float(sc[c]), a.scale_log2, -ref));
-                const float e1 = ex2_approx(fmaf(__uint_as_float(sc[c + 1]), a.scale_log2, -ref));
-                __nv_bfloat162 pr = __floats2bfloat162_rn(e0, e1);
-                const uint32_t w = *reinterpret_cast<uint32_t*>(&pr);
-                pk[c >> 1] = w;
-                // the row sum takes the weights as the product will see them, rounded
-                sum[(c >> 1) & 1] += __uint_as_float(w << 16);
-                sum[2 + ((c >> 1) & 1)] += __uint_as_float(w & 0xffff0000u);
+                    for (int c = 0; c < 64; ++c) if (j0 + c >= seen) sc[c] = 0xff800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx4[e] = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 64; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(mx4[e], fmaxf(__uint_as_float(sc[c + e]), __uint_as_float(sc[c + 4 + e])));
+                const float mx = top();
+                const bool grow = mx > m_used + kTau;
+                if (__any_sync(0xffffffffu, grow)) {
+                    float factor = 1.f;
+                    if (grow) { factor = exp2f(m_used - mx); m_used = mx; l *= factor; }
+                    if (t > 0) {
+                        if (!wait_pv(t - 1, 6, i)) { ok = false; break; }
+                        fence_after_sync();
+#pragma unroll 1
+                        for (int piece = 0; piece < HD / 8; ++piece) {
+                            uint32_t ov[8];
+                            tmem_get8(lane_addr + 128 + piece * 8, ov);
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * factor);
+                            tmem_st8(lane_addr + 128 + piece * 8, ov);
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                weigh(m_used == -INFINITY ? 0.f : m_used);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_st32(lane_addr + (t & 1) * 64, pk);

@@ -544,10 +544,11 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     part_ml = torch.empty(tokens * Hq * (sp + so) * 2, dtype=torch.float32, device=q.device)
     f = _fn("attention_shared", "lb_attention_shared",
             [c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-             c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_float, c_void_p, c_int, c_void_p])
+             c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_float, c_void_p, c_int, c_void_p])
     _check(f(_ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(block_table), block_table.stride(0),
              block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(prefix_lens), groups,
-             _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, int(max_prefix), scale,
+             _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, int(max_prefix),
+             int(max_context) - int(max_prefix), scale,
              _serving_error_word(q.device, "attention_decode_shared"), code, _stream()), "attention_decode_shared", launches=3)
     return out
 
