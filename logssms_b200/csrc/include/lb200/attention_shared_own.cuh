@@ -58,7 +58,10 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     // for this one, behind both.  (If all waited, they would keep their places on the SMs until then.)
     const bool last = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
 
-    // the queries as A operands: rows lane / 4 and + 8, columns 2 (lane % 4) and + 8 of each step
+    const int request = a.token_req[t], position = a.positions[t];
+    int begin = 0;
+    const bool grouped = prefix_of(a, t, &begin);
+    // (behind the loads on whose answers the first tile waits) the queries as A operands: rows lane / 4 and + 8, columns 2 (lane % 4) and + 8 of each step
     uint32_t qa[kK][4];
     {
         const bf16* q = (const bf16*)a.q + (size_t)t * a.q_stride + (size_t)(kvh * G + h0) * HD + 2 * (lane & 3);
@@ -72,9 +75,6 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         }
     }
-    const int request = a.token_req[t], position = a.positions[t];
-    int begin = 0;
-    const bool grouped = prefix_of(a, t, &begin);
     const bool known = request >= 0 && request < a.requests;
     const int end = known ? (int)min((long)position + 1, (long)a.bt_cols * a.page_size) : 0;
     int from = 0, to = 0;                                 // from: a multiple of 16; keys below `begin` are left out
@@ -96,26 +96,28 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         return;
     }
     const int* bt = a.block_table + (long)request * a.bt_stride;
-    const int n_tiles = ((to - from + kKeys - 1) / kKeys + kWarps - 1 - warp) / kWarps;       // of this warp: the i-th begins at ...
+    const int n_tiles = (to - from + kKeys - 1) / kKeys;
+    const int mine = (n_tiles + kWarps - 1 - warp) / kWarps;               // of this warp: tiles warp, warp + kWarps, ...
     auto tile_at = [&](int i) { return from + (i * kWarps + warp) * kKeys; };
-    auto page_at = [&](int i) -> int { return i < n_tiles ? bt[tile_at(i) / a.page_size] : -1; };
+    // where the next tile that is asked for lies: its place in the table and within the page
+    int entry = tile_at(0) / a.page_size, offset = tile_at(0) - entry * a.page_size;
+    int next = mine > 0 ? bt[entry] : -1;
 
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kWarps * Sh::kRing) + warp * kStages;
     uint8_t* ring = smem + warp * Sh::kRing;
-    int next = page_at(0);
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(full + s, 1);
         mbar_fence_init();
     }
     __syncwarp();
     uint32_t there = 0;                                   // a bit per tile on its way: its page is there
-    // tile i into stage s (a page that is not there: rows behind the pool, which read as zeros)
-    auto fetch = [&](int i, int s, int ahead, int page) {
-        if (i >= n_tiles) return;
-        const bool ok = page >= 0 && page < a.pages;
+    // tile i into stage s (a page that is not there: rows behind the pool, which read as zeros).  Whole warps: see elect_one.
+    auto fetch = [&](int i, int s, int ahead) {
+        if (i >= mine) return;
+        const bool ok = next >= 0 && next < a.pages;
         there |= (uint32_t)ok << ahead;
-        if (lane == 0) {
-            const int row = (int)((ok ? (long)page : a.pages) * a.page_size + tile_at(i) % a.page_size);
+        const int row = (ok ? next : (int)a.pages) * a.page_size + offset;
+        if (elect_one()) {
             mbar_expect_tx(full + s, Sh::kStage);
 #pragma unroll
             for (int b = 0; b < Sh::kBlocks; ++b) {
@@ -123,13 +125,13 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                 tma_load_2d(ring + s * Sh::kStage + Sh::kTile + b * Sh::kBlock, &map_v, full + s, kvh * HD + b * 64, row);
             }
         }
+        __syncwarp();
+        offset += kKeys * kWarps;                          // (a page holds a multiple of 64 keys)
+        if (offset >= a.page_size) { offset -= a.page_size; ++entry; }
+        next = i + 1 < mine ? bt[entry] : -1;
     };
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        const int page = next;
-        next = page_at(s + 1);
-        fetch(s, s, s, page);
-    }
+    for (int s = 0; s < kStages - 1; ++s) fetch(s, s, s);
 
     float acc[2 * kK][4];                                 // 8 columns each
 #pragma unroll
@@ -140,13 +142,10 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int s = 0, i = 0;
     uint32_t phase = 0;
     bool good = true;
-    for (; i < n_tiles; ++i) {
-        {
-            const int page = next, to_stage = s == 0 ? kStages - 1 : s - 1;       // (stage of tile i + kStages - 1)
-            next = page_at(i + kStages);
-            fetch(i + kStages - 1, to_stage, kStages - 1, page);
-        }
-        good = __all_sync(0xffffffffu, mbar_wait(full + s, phase));
+    for (; i < mine; ++i) {
+        fetch(i + kStages - 1, s == 0 ? kStages - 1 : s - 1, kStages - 1);
+        good = mbar_test(full + s, phase) || mbar_wait(full + s, phase);
+        good = __all_sync(0xffffffffu, good);
         if (!good) break;
         const uint32_t k_at = smem_u32(ring) + s * Sh::kStage, v_at = k_at + Sh::kTile;
         float sc4[2][2][4] = {};                          // [keys 0..7 / 8..15][even and odd steps]
@@ -223,7 +222,7 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
     if (!good) {                                          // a copy that did not land: the row's result means nothing
         if (lane == 0) report(a.error, i);
-        for (int x = i; x < min(i + kStages, n_tiles); ++x) mbar_wait(full + x % kStages, (x / kStages) & 1);
+        for (int x = i; x < min(i + kStages, mine); ++x) mbar_wait(full + x % kStages, (x / kStages) & 1);
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
     }
