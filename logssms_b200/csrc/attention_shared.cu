@@ -6,7 +6,10 @@
 // a third kernel puts the ranges of a row together:
 //   m = max m_s,  out = sum o_s 2^(m_s - m) / sum l_s 2^(m_s - m)
 //
-// This file: the general form, for float32, any page size and head sizes in steps of 8 up to 256, and the merge.
+// This file: the general form, for float32, any page size and head sizes in steps of 8 up to 256, and the merge.  Its products are
+// float32 fused multiply-adds on tiles of 16 rows x 32 keys in shared memory (about as many shared-memory reads as multiply-adds to
+// feed them); the next tile's keys and values come by asynchronous copies while one is worked on, so that a short range costs its
+// latency once.  (Loads into registers between two barriers: 23 requests with prefixes of 800 to 1,500 keys took 89 us, this way 38.)
 #include "lb200/common.cuh"
 #include "lb200/attention_shared.h"
 #include "lb200/attention_shared_own.cuh"
@@ -16,19 +19,40 @@ using namespace lb200;
 namespace {
 constexpr int kThreads = 128, kRows = 16, kKeys = 32;
 
-struct Items { int head_tiles; long prefix_tiles; };
+__device__ __forceinline__ float4 get4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 get4(const __nv_bfloat16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+__device__ __forceinline__ void copy16(void* to, const void* from, bool there) {             // zeros where nothing is there
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
+// Shared memory: queries float32 [kRows][hd + 4], then two stages of K and V as they are [kKeys][hd + 16 bytes], then weights.
+template <typename T> struct Lay {
+    int ld_q, ld;                                         // numbers from row to row
+    size_t k, stage, p, all;                              // bytes: where K of stage 0 begins, a stage, the weights, the whole
+    __host__ __device__ explicit Lay(int hd) {
+        ld_q = hd + 4;
+        ld = hd + 16 / (int)sizeof(T);
+        k = (size_t)kRows * ld_q * 4;
+        stage = 2 * (size_t)kKeys * ld * sizeof(T);
+        p = k + 2 * stage;
+        all = p + kRows * (kKeys + 1) * 4;
+    }
+};
 
 // One CTA: 16 rows (token, query head of one key/value head) x a range of keys.
 //   prefix: grid (tiles of the groups' rows, kv heads, ranges); own: grid (tokens x tiles of a token's heads, kv heads, ranges)
 template <typename T, bool PREFIX>
 __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, int head_tiles) {
     pdl_wait();
-    extern __shared__ float smem[];
-    const int hd = a.hd, ld = hd + 4, tid = threadIdx.x;
-    float* q_s = smem;                                   // [kRows][ld]
-    float* k_s = q_s + kRows * ld;                       // [kKeys][ld]
-    float* v_s = k_s + kKeys * ld;
-    float* p_s = v_s + kKeys * ld;                       // [kRows][kKeys + 1]
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long place[2][kKeys];                      // of a tile's keys: the row in the pool, or -1
+    const int hd = a.hd, tid = threadIdx.x;
+    const Lay<T> lay(hd);
+    float* q_s = reinterpret_cast<float*>(smem);
+    float* p_s = reinterpret_cast<float*>(smem + lay.p);
     const int G = a.Hq / a.Hkv, kvh = blockIdx.y, split = blockIdx.z;
     int first, rows, request, begin, end;                // the rows: token first + (row0 + r) / G, head kvh * G + (row0 + r) % G
     long row0;
@@ -52,65 +76,87 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     const int per = end > begin ? (((end - begin + splits - 1) / splits) + kKeys - 1) / kKeys * kKeys : 0;
     const int from = (int)min((long)begin + (long)split * per, (long)max(end, begin)), to = (int)min((long)from + per, (long)max(end, begin));
     const int* bt = a.block_table + (long)(known ? request : 0) * a.bt_stride;
+    const T* kc = (const T*)a.k_cache + (size_t)kvh * hd;
+    const T* vc = (const T*)a.v_cache + (size_t)kvh * hd;
+    const size_t key_stride = (size_t)a.Hkv * hd;
 
-    const T* q = (const T*)a.q;
-    for (int i = tid; i < kRows * hd; i += kThreads) {
-        const int r = i / hd, d = i % hd;
-        float v = 0.f;
-        if (r < rows) {
-            const long at = row0 + r;
-            v = to_f32(q[(first + at / G) * a.q_stride + (kvh * G + at % G) * hd + d]) * a.scale_log2;
+    auto find = [&](int j0, int s) {                      // threads 0 .. 31: where the keys of the tile at j0 lie
+        if (tid < kKeys) {
+            long at = -1;
+            if (j0 + tid < to) {
+                const long page = bt[(j0 + tid) / a.page_size];
+                if (page >= 0 && page < a.pages) at = page * a.page_size + (j0 + tid) % a.page_size;
+            }
+            place[s][tid] = at;
         }
-        q_s[r * ld + d] = v;
+    };
+    auto fetch = [&](int s) {                             // the tile whose places are there
+        T* k_s = reinterpret_cast<T*>(smem + lay.k + s * lay.stage);
+        T* v_s = k_s + kKeys * lay.ld;
+        constexpr int kEach = 16 / (int)sizeof(T);
+        const int pieces = hd / kEach;
+        for (int i = tid; i < kKeys * pieces; i += kThreads) {
+            const int key = i / pieces, d = (i - key * pieces) * kEach;
+            const long at = place[s][key];
+            const size_t off = at >= 0 ? (size_t)at * key_stride + d : 0;
+            copy16(k_s + key * lay.ld + d, kc + off, at >= 0);
+            copy16(v_s + key * lay.ld + d, vc + off, at >= 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    find(from, 0);
+    __syncthreads();
+    if (from < to) fetch(0);
+    find(from + kKeys, 1);
+    const T* q = (const T*)a.q;
+    for (int i = tid; i < kRows * (hd >> 2); i += kThreads) {
+        const int r = i / (hd >> 2), d = (i % (hd >> 2)) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows) {
+            const int at = (int)row0 + r, token = at / G;
+            const T* src = q + (first + token) * a.q_stride + (kvh * G + at - token * G) * hd + d;         // (any alignment)
+            v = make_float4(to_f32(src[0]) * a.scale_log2, to_f32(src[1]) * a.scale_log2, to_f32(src[2]) * a.scale_log2, to_f32(src[3]) * a.scale_log2);
+        }
+        *reinterpret_cast<float4*>(q_s + r * lay.ld_q + d) = v;
     }
     const int r = tid >> 3, c = tid & 7;                 // this thread's row; its keys c + 8 i, its columns 4 c + 32 i
-    const long at = row0 + r;
-    const int token = r < rows ? (int)(first + at / G) : first;
+    const int at = (int)row0 + r;
+    const int token = r < rows ? first + at / G : first;
     const int limit = r < rows ? a.positions[token] + 1 : 0;
     float m = -INFINITY, l = 0.f;
     float4 acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const T* kc = (const T*)a.k_cache;
-    const T* vc = (const T*)a.v_cache;
-    for (int j0 = from; j0 < to; j0 += kKeys) {
+    int s_now = 0;
+    for (int j0 = from; j0 < to; j0 += kKeys, s_now ^= 1) {
         const int n = min(kKeys, to - j0);
-        __syncthreads();
-        // a page outside of the pool has no keys: its scores are left out below (p_s takes the mark in its last column)
-        for (int i = tid; i < kKeys * (hd >> 2); i += kThreads) {
-            const int key = i / (hd >> 2), d = (i % (hd >> 2)) * 4;
-            float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
-            bool there = key < n;
-            if (there) {
-                const int j = j0 + key;
-                const long page = bt[j / a.page_size];
-                there = page >= 0 && page < a.pages;
-                if (there) {
-                    const size_t base = (((size_t)page * a.page_size + j % a.page_size) * a.Hkv + kvh) * hd + d;
-                    kv = make_float4(to_f32(kc[base]), to_f32(kc[base + 1]), to_f32(kc[base + 2]), to_f32(kc[base + 3]));
-                    vv = make_float4(to_f32(vc[base]), to_f32(vc[base + 1]), to_f32(vc[base + 2]), to_f32(vc[base + 3]));
-                }
-            }
-            if (d == 0) k_s[key * ld + hd] = there ? 1.f : 0.f;
-            *reinterpret_cast<float4*>(k_s + key * ld + d) = kv;
-            *reinterpret_cast<float4*>(v_s + key * ld + d) = vv;
+        __syncthreads();                                  // the next tile's places are there, the other stage is done with
+        const bool more = j0 + kKeys < to;
+        if (more) {
+            fetch(s_now ^ 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
-        __syncthreads();
+        const bool there[4] = {place[s_now][c] >= 0, place[s_now][c + 8] >= 0, place[s_now][c + 16] >= 0, place[s_now][c + 24] >= 0};
+        __syncthreads();                                  // the tile is there for all
+        find(j0 + 2 * kKeys, s_now);
+        const T* k_s = reinterpret_cast<const T*>(smem + lay.k + s_now * lay.stage);
+        const T* v_s = k_s + kKeys * lay.ld;
         float s[4] = {};
 #pragma unroll 4
         for (int d = 0; d < hd; d += 4) {
-            const float4 u = *reinterpret_cast<const float4*>(q_s + r * ld + d);
+            const float4 u = *reinterpret_cast<const float4*>(q_s + r * lay.ld_q + d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float4 w = *reinterpret_cast<const float4*>(k_s + (c + 8 * i) * ld + d);
+                const float4 w = get4(k_s + (c + 8 * i) * lay.ld + d);
                 s[i] = fmaf(u.x, w.x, fmaf(u.y, w.y, fmaf(u.z, w.z, fmaf(u.w, w.w, s[i]))));
             }
         }
         float mx = m;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool there = c + 8 * i < n && j0 + c + 8 * i < limit && k_s[(c + 8 * i) * ld + hd] != 0.f;
-            if (!there) s[i] = -INFINITY;
+            if (!(there[i] && j0 + c + 8 * i < limit)) s[i] = -INFINITY;         // (no place: behind the range, or a page that is not there)
             mx = fmaxf(mx, s[i]);
         }
 #pragma unroll
@@ -136,7 +182,7 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
             for (int i = 0; i < 8; ++i) {
                 const int d = 4 * c + 32 * i;
                 if (d < hd) {
-                    const float4 w = *reinterpret_cast<const float4*>(v_s + key * ld + d);
+                    const float4 w = get4(v_s + key * lay.ld + d);
                     acc[i].x = fmaf(p, w.x, acc[i].x); acc[i].y = fmaf(p, w.y, acc[i].y);
                     acc[i].z = fmaf(p, w.z, acc[i].z); acc[i].w = fmaf(p, w.w, acc[i].w);
                 }
@@ -263,8 +309,8 @@ int launch_tc(const SharedArgs& a, const Layout& y, cudaStream_t stream) {
 template <typename T>
 int launch_general(const SharedArgs& a, long prefix_tiles, cudaStream_t stream) {
     static SharedLimits limits[2];
-    const int G = a.Hq / a.Hkv, head_tiles = (G + kRows - 1) / kRows, ld = a.hd + 4;
-    const size_t smem = (size_t)((kRows + 2 * kKeys) * ld + kRows * (kKeys + 1)) * sizeof(float);
+    const int G = a.Hq / a.Hkv, head_tiles = (G + kRows - 1) / kRows;
+    const size_t smem = Lay<T>(a.hd).all;
     int rc = ensure_dynamic_smem(shared_general_kernel<T, true>, smem, limits[0]);
     if (rc == 0) rc = ensure_dynamic_smem(shared_general_kernel<T, false>, smem, limits[1]);
     if (rc == 0 && prefix_tiles > 0)
