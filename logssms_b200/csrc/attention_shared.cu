@@ -10,6 +10,7 @@
 // float32 fused multiply-adds on tiles of 16 rows x 32 keys in shared memory (about as many shared-memory reads as multiply-adds to
 // feed them); the next tile's keys and values come by asynchronous copies while one is worked on, so that a short range costs its
 // latency once.  (Loads into registers between two barriers: 23 requests with prefixes of 800 to 1,500 keys took 89 us, this way 38.)
+#include <type_traits>
 #include "lb200/common.cuh"
 #include "lb200/attention_shared.h"
 #include "lb200/attention_shared_own.cuh"
@@ -46,7 +47,11 @@ template <typename T> struct Lay {
 //   prefix: grid (tiles of the groups' rows, kv heads, ranges); own: grid (tokens x tiles of a token's heads, kv heads, ranges)
 template <typename T, bool PREFIX>
 __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, int head_tiles) {
-    pdl_wait();
+    // The own keys' launch runs beside the prefix's, of which it needs nothing; its last CTA waits for it, so that the merge, which
+    // waits for this launch, comes behind both.
+    const bool last = !PREFIX && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
+    if (PREFIX) { pdl_wait(); pdl_trigger(); }
+    if (last) pdl_wait();
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long place[2][kKeys];                      // of a tile's keys: the row in the pool, or -1
     const int hd = a.hd, tid = threadIdx.x;
@@ -139,7 +144,8 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         const bool there[4] = {place[s_now][c] >= 0, place[s_now][c + 8] >= 0, place[s_now][c + 16] >= 0, place[s_now][c + 24] >= 0};
-        __syncthreads();                                  // the tile is there for all
+        // the tile is there for all; and does every row see all of its keys?
+        const bool clean = __syncthreads_and(r >= rows || (there[0] && there[1] && there[2] && there[3] && j0 + kKeys <= limit));
         find(j0 + 2 * kKeys, s_now);
         const T* k_s = reinterpret_cast<const T*>(smem + lay.k + s_now * lay.stage);
         const T* v_s = k_s + kKeys * lay.ld;
@@ -175,7 +181,22 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) { acc[i].x *= factor; acc[i].y *= factor; acc[i].z *= factor; acc[i].w *= factor; }
-        for (int key = 0; key < n; ++key) {
+        if (clean) {
+#pragma unroll 4
+            for (int key = 0; key < kKeys; ++key) {
+                const float p = p_s[r * (kKeys + 1) + key];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int d = 4 * c + 32 * i;
+                    if (d < hd) {
+                        const float4 w = get4(v_s + key * lay.ld + d);
+                        acc[i].x = fmaf(p, w.x, acc[i].x); acc[i].y = fmaf(p, w.y, acc[i].y);
+                        acc[i].z = fmaf(p, w.z, acc[i].z); acc[i].w = fmaf(p, w.w, acc[i].w);
+                    }
+                }
+            }
+        }
+        for (int key = 0; key < n && !clean; ++key) {
             const float p = p_s[r * (kKeys + 1) + key];
             if (p == 0.f) continue;                      // (a masked key's value may be anything)
 #pragma unroll
@@ -263,7 +284,7 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
 
 // Do the tensor-core forms take the call?  (Else: the general form.)
 bool tc_ok(const SharedArgs& a, int dtype) {
-    return dtype == kBF16 && (a.hd == 64 || a.hd == 128) && a.page_size % 64 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
+    return dtype == kBF16 && (a.hd == 64 || a.hd == 96 || a.hd == 128) && a.page_size % 16 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
            (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
 }
 // How the prefix's work is laid out on the tensor cores: rows of a tile, CTAs of a cluster, clusters for a tile's keys.
@@ -299,11 +320,12 @@ Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_pref
 }
 
 int launch_tc(const SharedArgs& a, const Layout& y, cudaStream_t stream) {
-    int rc;
-    if (a.hd == 64) rc = y.two ? shared_tc::launch_prefix<64, true>(a, y.ranks, stream) : shared_tc::launch_prefix<64, false>(a, y.ranks, stream);
-    else rc = y.two ? shared_tc::launch_prefix<128, true>(a, y.ranks, stream) : shared_tc::launch_prefix<128, false>(a, y.ranks, stream);
-    if (rc == 0) rc = a.hd == 64 ? shared_own::launch_own<64>(a, stream) : shared_own::launch_own<128>(a, stream);
-    return rc;
+    auto both = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        const int rc = y.two ? shared_tc::launch_prefix<HD, true>(a, y.ranks, stream) : shared_tc::launch_prefix<HD, false>(a, y.ranks, stream);
+        return rc != 0 ? rc : shared_own::launch_own<HD>(a, stream);
+    };
+    return a.hd == 64 ? both(std::integral_constant<int, 64>()) : a.hd == 96 ? both(std::integral_constant<int, 96>()) : both(std::integral_constant<int, 128>());
 }
 
 template <typename T>

@@ -1,4 +1,4 @@
-// A token's own keys (behind the shared prefix): bfloat16, heads of 64 or 128, pages of a multiple of 64 keys.
+// A token's own keys (behind the shared prefix): bfloat16, heads of 64, 96 or 128, pages of a multiple of 16 keys.
 //
 // Bound by reading the keys and values once: 16 query heads of a key/value head are the rows of m16n8k16 products, which is all the
 // arithmetic needs (the tile of 128 rows that tcgen05 wants would be an eighth full, and its scores would go through tensor memory).
@@ -19,7 +19,7 @@ constexpr float kTau = 8.f;                               // log2 of the growth 
 
 // A tile: blocks of 64 columns, [16 keys][128 bytes]; 16-byte piece c of key r lies at c ^ (r & 7).
 template <int HD> struct Shape {
-    static constexpr int kBlocks = HD / 64;
+    static constexpr int kBlocks = (HD + 63) / 64;
     static constexpr uint32_t kBlock = kKeys * 128, kTile = kBlocks * kBlock, kStage = 2 * kTile, kRing = kStages * kStage;
     static constexpr uint32_t kResult = kWarps * kRows * (HD + 2) * 4;         // at the end, over the rings
     static constexpr uint32_t kSmem = kWarps * kRing + 64;
@@ -126,8 +126,8 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             }
         }
         __syncwarp();
-        offset += kKeys * kWarps;                          // (a page holds a multiple of 64 keys)
-        if (offset >= a.page_size) { offset -= a.page_size; ++entry; }
+        offset += kKeys * kWarps;
+        while (offset >= a.page_size) { offset -= a.page_size; ++entry; }
         next = i + 1 < mine ? bt[entry] : -1;
     };
 #pragma unroll

@@ -1,5 +1,5 @@
-// The prefix's part of attention over a shared prefix on the 5th-generation tensor cores: bfloat16, heads of 64 or 128, pages of a
-// multiple of 64 keys.  The products, the softmax threads and the lazily followed maximum are those of the prompt kernel
+// The prefix's part of attention over a shared prefix on the 5th-generation tensor cores: bfloat16, heads of 64, 96 or 128, pages of a
+// multiple of 16 keys.  The products, the softmax threads and the lazily followed maximum are those of the prompt kernel
 // (attention_prefill_tc.cu); what differs is whose rows meet: the rows of a tile are (token, head) pairs of one group, gathered into
 // shared memory by the threads (TMA has no box for them), and every row sees the same keys.
 //
@@ -32,14 +32,15 @@ constexpr float kTau = 8.f;                               // log2 of the growth 
 constexpr int kMostRanks = 4;                             // CTAs of a cluster
 
 template <int HD, bool TWO> struct Shape {
-    static constexpr int kBlocks = HD / 64;
+    static constexpr int kBlocks = (HD + 63) / 64;        // of 64 columns (heads of 96: the second one is half used)
+    static constexpr int kPitch = HD == 64 ? 16 : 32;     // pieces of 16 bytes from row to row of a result
     // tiles of K and of V on their way or at work: a tile's copy takes about as long as the softmax of two
     static constexpr int kK = (TWO ? 3 : 4) * (HD == 64 ? 2 : 1), kV = kK + (HD == 64 ? 2 : 1);
     static constexpr int kRows = TWO ? 256 : 128;
     static constexpr uint32_t kQBlock = kQ * 128, kKVBlock = kKV * 128;
     static constexpr uint32_t kQBytes = kQBlock * kBlocks, kTileBytes = kKVBlock * kBlocks;
     static constexpr uint32_t kGroupCols = 128 + HD;      // per group: S (then P) of even tiles, of odd tiles, O from 128
-    static constexpr uint32_t kResult = 2 * kQ * HD * 4;  // both groups' O at the end, over Q and the rings
+    static constexpr uint32_t kResult = 2 * kQ * kPitch * 16;   // both groups' O at the end, over Q and the rings
     static constexpr uint32_t kTiles = kQBytes * (TWO ? 2 : 1) + (kK + kV) * kTileBytes;
     // ... with their rows' (maximum, sum), and of this CTA's part of the rows the results' weights and where they go
     static constexpr int kSources = kMostRanks * (TWO ? 1 : 2);
@@ -76,7 +77,7 @@ __device__ __forceinline__ float2 remote2(uint32_t addr) {
 // grid: (tiles x kv heads) x ranges of keys; `ranks` ranges, which follow one another, are a cluster and one of a row's results
 template <int HD, bool TWO>
 __global__ void __maxnreg__(120)
-shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, SharedArgs a, int ranks) {
+shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, SharedArgs a, int ranks, int box) {
     pdl_wait();
     pdl_trigger();                                        // the own parts need nothing of this kernel's
     typedef Shape<HD, TWO> Sh;
@@ -150,12 +151,14 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         }
     }
     int k_issued = 0, v_issued = 0;
-    // a page that is not there: rows behind the pool, which read as zeros (its scores are left out below)
+    // Where the keys of a tile lie, kept by the lanes: lane n has the row of its keys n * box .. (a box of keys lies within a page).  A
+    // page that is not there: rows behind the pool, which read as zeros (its scores are left out below).  (Whole warps: see elect_one.)
+    const int boxes = kKV / box;
     auto row_of = [&](int i) -> int {
-        const int j0 = (kt_begin + i) * kKV, page = j0 / a.page_size, id = bt[page];
-        return (int)((id >= 0 && id < a.pages ? (long)id : a.pages) * a.page_size + (j0 - page * a.page_size));
+        const int j = (kt_begin + i) * kKV + min(lane, boxes - 1) * box, page = j / a.page_size;
+        const int id = page < a.bt_cols ? bt[page] : -1;
+        return (int)((id >= 0 && id < a.pages ? (long)id : a.pages) * a.page_size + (j - page * a.page_size));
     };
-    // (whole warps: see elect_one)
     auto load = [&](int i, int row, int stages, uint8_t* ring, const CUtensorMap* map, uint64_t* full, uint64_t* empty, int role) -> bool {
         const int s = i % stages;
         if (i >= stages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / stages) - 1) & 1))) {
@@ -163,13 +166,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             *failed = 1;
             return false;
         }
-        if (elect_one()) {
-            mbar_expect_tx(full + s, kTileBytes);
-#pragma unroll
-            for (int blk = 0; blk < kBlocks; ++blk)
-                tma_load_2d(ring + s * kTileBytes + blk * Sh::kKVBlock, map, full + s, kvh * HD + blk * 64, row);
-        }
+        if (elect_one()) mbar_expect_tx(full + s, kTileBytes);
         __syncwarp();
+        for (int n = 0; n < boxes; ++n) {
+            const int y = __shfl_sync(0xffffffffu, row, n);
+            if (elect_one()) {
+#pragma unroll
+                for (int blk = 0; blk < kBlocks; ++blk)
+                    tma_load_2d(ring + s * kTileBytes + blk * Sh::kKVBlock + n * box * 128, map, full + s, kvh * HD + blk * 64, y);
+            }
+            __syncwarp();
+        }
         return true;
     };
     int first_row = 0;
@@ -223,7 +230,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
                 for (int blk = 0; blk < kBlocks; ++blk)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < (HD - 64 * blk >= 64 ? 4 : (HD - 64 * blk) / 16); ++k)
                         umma_bf16(d, qdesc + blk * (Sh::kQBlock >> 4) + 2 * k, kdesc + blk * (Sh::kKVBlock >> 4) + 2 * k, idesc_s, (blk | k) != 0);
                 umma_commit(s_ready + 2 * g + (t & 1));
                 umma_commit(k_empty + i % kK);
@@ -291,12 +298,14 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                     *reinterpret_cast<uint4*>(v_tile + blk * Sh::kKVBlock + (first_bad + y / 8) * 128 + (y % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
-            int seen = limit;                              // keys of the tile that the row sees: those in front of `seen`
-            if (any_bad) {
-                const int id = bt[j0 / a.page_size];
-                if (id < 0 || id >= a.pages) seen = 0;
-            }
-            const bool whole = __all_sync(0xffffffffu, j0 + kKV <= seen);
+            const int seen = limit;                        // keys of the tile that the row sees: those in front of `seen` ...
+            uint64_t lost = 0;                             // ... that are not on a page that is not there
+            if (any_bad)
+                for (int c = 0; c < kKV; c += 16) {
+                    const int page = (j0 + c) / a.page_size, id = page < a.bt_cols ? bt[page] : -1;
+                    if (id < 0 || id >= a.pages) lost |= (uint64_t)0xffff << c;
+                }
+            const bool whole = __all_sync(0xffffffffu, j0 + kKV <= seen && lost == 0);
             uint32_t sc[64], pk[32];                       // the row's scores, its weights
             float mx4[4], sum[4];                          // (four chains each: two warps a scheduler hide no latency)
             // the weights relative to `ref`, and the scores' maximum on the way
@@ -328,7 +337,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             if (again) {
                 if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) if (j0 + c >= seen) sc[c] = 0xff800000u;
+                    for (int c = 0; c < 64; ++c) if (j0 + c >= seen || (lost >> c & 1u)) sc[c] = 0xff800000u;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx4[e] = -INFINITY;
@@ -370,9 +379,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const bool have = ok && done > 0;
         if (l != l) m_used = 0.f;                          // (a NaN among the scores: the range counts, and makes the row NaN)
         asm volatile("bar.sync 1, 256;" ::: "memory");     // every product has read Q and the rings: the results lie over them
-        // a row of O: pieces of 16 bytes, piece c at c ^ (row % pieces)
-        constexpr int kPieces = HD / 4;
-        float4* mine = reinterpret_cast<float4*>(base) + (size_t)(grp * kQ + lr) * kPieces;
+        // a row of O: pieces of 16 bytes, piece c at c ^ (row % kPitch)
+        constexpr int kPitch = Sh::kPitch;
+        float4* mine = reinterpret_cast<float4*>(base) + (size_t)(grp * kQ + lr) * kPitch;
         ml_s[grp * kQ + lr] = have ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
         if (have) {
 #pragma unroll 1
@@ -381,7 +390,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
                 tmem_ld32(lane_addr + 128 + piece * 32, ov);
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    mine[(piece * 8 + c) ^ (lr & (kPieces - 1) & 31)] =
+                    mine[(piece * 8 + c) ^ (lr & (kPitch - 1))] =
                         make_float4(__uint_as_float(ov[4 * c]), __uint_as_float(ov[4 * c + 1]), __uint_as_float(ov[4 * c + 2]), __uint_as_float(ov[4 * c + 3]));
             }
         }
@@ -393,7 +402,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     // This CTA's part of the rows, rank, rank + ranks, ...: a thread per row puts together the results' weights, then a warp takes a row
     // at a time, 16 bytes a lane, with all results of two rows on their way.
     {
-        constexpr int kPieces = HD / 4, kSources = TWO ? 1 : 2;
+        constexpr int kPieces = HD / 4, kPitch = Sh::kPitch, kSources = TWO ? 1 : 2;
         const uint32_t here = smem_u32(base), ml_here = smem_u32(ml_s), rank = ranks > 1 ? cluster_rank() : 0u;
         const int splits = a.prefix_splits + a.own_splits, sources = ranks * kSources, ours = (rows - (int)rank + ranks - 1) / ranks;
         if ((int)threadIdx.x < ours) {
@@ -423,12 +432,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int n = n0 + h * (kThreads / 32), r = (int)rank + ranks * n;
-                const uint32_t piece = here + 16 * (uint32_t)(r * kPieces + (lane ^ (r & (kPieces - 1) & 31)));      // (128 rows on: the same place)
+                const uint32_t piece = here + 16 * (uint32_t)(r * kPitch + (lane ^ (r & (kPitch - 1))));      // (128 rows on: the same place)
 #pragma unroll
                 for (int s = 0; s < kMostSources; ++s) {
                     v[h][s] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (n < ours && s < sources && lane < kPieces && weights[n * kMostSources + s] != 0.f) {         // (a range without keys left nothing)
-                        const uint32_t at = piece + (s % kSources) * (kQ * kPieces * 16);
+                        const uint32_t at = piece + (s % kSources) * (kQ * kPitch * 16);
                         v[h][s] = remote4(ranks > 1 ? at_rank(at, s / kSources) : at);
                     }
                 }
@@ -459,8 +468,9 @@ inline int launch_prefix(const SharedArgs& a, int ranks, cudaStream_t stream) {
     const long grid = tiles * a.Hkv * a.prefix_splits * ranks;
     if (grid > 0x7fffffffL) return kTooLarge;
     CUtensorMap map_k, map_v;
-    int rc = make_tile_map(&map_k, a.k_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, kKV);
-    if (rc == 0) rc = make_tile_map(&map_v, a.v_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, kKV);
+    const int box = a.page_size % 64 == 0 ? 64 : a.page_size % 32 == 0 ? 32 : 16;          // keys that one copy brings
+    int rc = make_tile_map(&map_k, a.k_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, box);
+    if (rc == 0) rc = make_tile_map(&map_v, a.v_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, box);
     static SharedLimits limits;
     if (rc == 0) rc = ensure_dynamic_smem(shared_prefix_kernel<HD, TWO>, Sh::kSmem, limits);
     if (rc == 0) rc = whole_carveout(shared_prefix_kernel<HD, TWO>);
@@ -473,7 +483,7 @@ inline int launch_prefix(const SharedArgs& a, int ranks, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)ranks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, shared_prefix_kernel<HD, TWO>, map_k, map_v, a, ranks);
+    return (int)cudaLaunchKernelEx(&cfg, shared_prefix_kernel<HD, TWO>, map_k, map_v, a, ranks, box);
 }
 
 }  // namespace shared_tc
