@@ -7,9 +7,9 @@
 //   m = max m_s,  out = sum o_s 2^(m_s - m) / sum l_s 2^(m_s - m)
 //
 // This file: the general form, for float32, any page size and head sizes in steps of 8 up to 256, and the merge.  Its products are
-// float32 fused multiply-adds on tiles of 16 rows x 32 keys in shared memory (about as many shared-memory reads as multiply-adds to
-// feed them); the next tile's keys and values come by asynchronous copies while one is worked on, so that a short range costs its
-// latency once.  (Loads into registers between two barriers: 23 requests with prefixes of 800 to 1,500 keys took 89 us, this way 38.)
+// float32 fused multiply-adds on tiles of 16 rows x 32 keys in shared memory, bound by its reads (16 bytes a lane are four of its
+// cycles, also where lanes read the same): so a thread makes 4 x 4 scores of a quarter of the columns, which the four warps add up,
+// and 4 rows x 4 columns of the output.  The next tile's keys and values come by asynchronous copies while one is worked on.
 #include <type_traits>
 #include "lb200/common.cuh"
 #include "lb200/attention_shared.h"
@@ -29,17 +29,19 @@ __device__ __forceinline__ void copy16(void* to, const void* from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-// Shared memory: queries float32 [kRows][hd + 4], then two stages of K and V as they are [kKeys][hd + 16 bytes], then weights.
+// Shared memory: queries float32 [kRows][hd + 4], two stages of K and V as they are [kKeys][hd + 16 bytes], the warps' scores
+// [4][kRows][kKeys + 1], the weights [kKeys][kRows + 4], the rows' factors.
 template <typename T> struct Lay {
     int ld_q, ld;                                         // numbers from row to row
-    size_t k, stage, p, all;                              // bytes: where K of stage 0 begins, a stage, the weights, the whole
+    size_t k, stage, s, p, all;                           // bytes: where K of stage 0 begins, a stage, the scores, the weights, the whole
     __host__ __device__ explicit Lay(int hd) {
         ld_q = hd + 4;
         ld = hd + 16 / (int)sizeof(T);
         k = (size_t)kRows * ld_q * 4;
         stage = 2 * (size_t)kKeys * ld * sizeof(T);
-        p = k + 2 * stage;
-        all = p + kRows * (kKeys + 1) * 4;
+        s = k + 2 * stage;
+        p = s + (4 * kRows * (kKeys + 1) * 4 + 15) / 16 * 16;
+        all = p + (kKeys * (kRows + 4) + kRows) * 4;
     }
 };
 
@@ -57,7 +59,9 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     const int hd = a.hd, tid = threadIdx.x;
     const Lay<T> lay(hd);
     float* q_s = reinterpret_cast<float*>(smem);
+    float* s_s = reinterpret_cast<float*>(smem + lay.s);
     float* p_s = reinterpret_cast<float*>(smem + lay.p);
+    float* factors = p_s + kKeys * (kRows + 4);
     const int G = a.Hq / a.Hkv, kvh = blockIdx.y, split = blockIdx.z;
     int first, rows, request, begin, end;                // the rows: token first + (row0 + r) / G, head kvh * G + (row0 + r) % G
     long row0;
@@ -124,14 +128,16 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         }
         *reinterpret_cast<float4*>(q_s + r * lay.ld_q + d) = v;
     }
-    const int r = tid >> 3, c = tid & 7;                 // this thread's row; its keys c + 8 i, its columns 4 c + 32 i
+    const int r = tid >> 3, c = tid & 7;                 // this thread's row of the softmax, its keys c + 8 i
+    const int warp = tid >> 5, lane = tid & 31, rg = lane >> 3, kg = lane & 7;         // of the scores: rows 4 rg + i, keys kg + 8 j
+    const int o4 = (tid >> 5) * 4, col = (tid & 31) * 4; // of the output: rows o4 + i, columns col and 128 on
     const int at = (int)row0 + r;
     const int token = r < rows ? first + at / G : first;
     const int limit = r < rows ? a.positions[token] + 1 : 0;
     float m = -INFINITY, l = 0.f;
-    float4 acc[8];
+    float4 acc[2][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < 8; ++i) acc[i >> 2][i & 3] = make_float4(0.f, 0.f, 0.f, 0.f);
     int s_now = 0;
     for (int j0 = from; j0 < to; j0 += kKeys, s_now ^= 1) {
         const int n = min(kKeys, to - j0);
@@ -149,15 +155,32 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         find(j0 + 2 * kKeys, s_now);
         const T* k_s = reinterpret_cast<const T*>(smem + lay.k + s_now * lay.stage);
         const T* v_s = k_s + kKeys * lay.ld;
-        float s[4] = {};
-#pragma unroll 4
-        for (int d = 0; d < hd; d += 4) {
-            const float4 u = *reinterpret_cast<const float4*>(q_s + r * lay.ld_q + d);
+        {
+            float part[4][4] = {};
+#pragma unroll 2
+            for (int d = 4 * warp; d < hd; d += 16) {
+                float4 u[4], w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 w = get4(k_s + (c + 8 * i) * lay.ld + d);
-                s[i] = fmaf(u.x, w.x, fmaf(u.y, w.y, fmaf(u.z, w.z, fmaf(u.w, w.w, s[i]))));
+                for (int i = 0; i < 4; ++i) u[i] = *reinterpret_cast<const float4*>(q_s + (4 * rg + i) * lay.ld_q + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = get4(k_s + (kg + 8 * i) * lay.ld + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        part[i][j] = fmaf(u[i].x, w[j].x, fmaf(u[i].y, w[j].y, fmaf(u[i].z, w[j].z, fmaf(u[i].w, w[j].w, part[i][j]))));
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s_s[(warp * kRows + 4 * rg + i) * (kKeys + 1) + kg + 8 * j] = part[i][j];
+        }
+        __syncthreads();
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* at_s = s_s + r * (kKeys + 1) + c + 8 * i;
+            s[i] = (at_s[0] + at_s[kRows * (kKeys + 1)]) + (at_s[2 * kRows * (kKeys + 1)] + at_s[3 * kRows * (kKeys + 1)]);
         }
         float mx = m;
 #pragma unroll
@@ -173,54 +196,60 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float p = exp2f(s[i] - ref);
-            p_s[r * (kKeys + 1) + c + 8 * i] = p;
+            p_s[(c + 8 * i) * (kRows + 4) + r] = p;
             sum += p;
         }
         l = l * factor + sum;
         m = mx;
-        __syncwarp();
+        if (c == 0) factors[r] = factor;
+        __syncthreads();
+        if (col < hd) {
+            const float4 f = *reinterpret_cast<const float4*>(factors + o4);
+            const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { acc[i].x *= factor; acc[i].y *= factor; acc[i].z *= factor; acc[i].w *= factor; }
-        if (clean) {
-#pragma unroll 4
-            for (int key = 0; key < kKeys; ++key) {
-                const float p = p_s[r * (kKeys + 1) + key];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = 4 * c + 32 * i;
-                    if (d < hd) {
-                        const float4 w = get4(v_s + key * lay.ld + d);
-                        acc[i].x = fmaf(p, w.x, acc[i].x); acc[i].y = fmaf(p, w.y, acc[i].y);
-                        acc[i].z = fmaf(p, w.z, acc[i].z); acc[i].w = fmaf(p, w.w, acc[i].w);
+                for (int i = 0; i < 4; ++i) { acc[h][i].x *= fs[i]; acc[h][i].y *= fs[i]; acc[h][i].z *= fs[i]; acc[h][i].w *= fs[i]; }
+            auto add = [&](int key, auto guarded) {
+                const float4 p4 = *reinterpret_cast<const float4*>(p_s + key * (kRows + 4) + o4);
+                const float ps[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (col + 128 * h >= hd) break;
+                    const float4 w = get4(v_s + key * lay.ld + col + 128 * h);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (guarded.value && ps[i] == 0.f) continue;             // (a masked key's value may be anything)
+                        acc[h][i].x = fmaf(ps[i], w.x, acc[h][i].x); acc[h][i].y = fmaf(ps[i], w.y, acc[h][i].y);
+                        acc[h][i].z = fmaf(ps[i], w.z, acc[h][i].z); acc[h][i].w = fmaf(ps[i], w.w, acc[h][i].w);
                     }
                 }
+            };
+            if (clean) {
+#pragma unroll 4
+                for (int key = 0; key < kKeys; ++key) add(key, std::false_type());
+            } else {
+                for (int key = 0; key < n; ++key) add(key, std::true_type());
             }
         }
-        for (int key = 0; key < n && !clean; ++key) {
-            const float p = p_s[r * (kKeys + 1) + key];
-            if (p == 0.f) continue;                      // (a masked key's value may be anything)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = 4 * c + 32 * i;
-                if (d < hd) {
-                    const float4 w = get4(v_s + key * lay.ld + d);
-                    acc[i].x = fmaf(p, w.x, acc[i].x); acc[i].y = fmaf(p, w.y, acc[i].y);
-                    acc[i].z = fmaf(p, w.z, acc[i].z); acc[i].w = fmaf(p, w.w, acc[i].w);
-                }
-            }
-        }
-        __syncwarp();
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (r >= rows) return;
-    if (l != l) m = 0.f;                                 // (a NaN among the scores: the range counts, and makes the row NaN)
-    const size_t slot = ((size_t)token * a.Hq + kvh * G + at % G) * (a.prefix_splits + a.own_splits) + (PREFIX ? split : a.prefix_splits + split);
-    if (c == 0) { a.part_ml[2 * slot] = m; a.part_ml[2 * slot + 1] = l; }
+    const int results = a.prefix_splits + a.own_splits, result = PREFIX ? split : a.prefix_splits + split;
+    if (r < rows && c == 0) {
+        if (l != l) m = 0.f;                             // (a NaN among the scores: the range counts, and makes the row NaN)
+        const size_t slot = ((size_t)token * a.Hq + kvh * G + at % G) * results + result;
+        a.part_ml[2 * slot] = m;
+        a.part_ml[2 * slot + 1] = l;
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = 4 * c + 32 * i;
-        if (d < hd) *reinterpret_cast<float4*>(a.part_o + slot * hd + d) = acc[i];
+    for (int i = 0; i < 4; ++i) {
+        if (o4 + i >= rows) break;
+        const int its = (int)row0 + o4 + i, of = its / G;
+        const size_t slot = ((size_t)(first + of) * a.Hq + kvh * G + its - of * G) * results + result;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (col + 128 * h < hd) *reinterpret_cast<float4*>(a.part_o + slot * hd + col + 128 * h) = acc[h][i];
     }
 }
 
