@@ -2991,9 +2991,10 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
         out = torch.empty((rows, features), dtype=y.dtype, device=here)
     else:
         _need(out.shape == y.shape and out.dtype == y.dtype, "out must match y")
+        _rows_out(out, "out")
         _same_place(out, y, "out")
-    ldo = _rows_out(out, "out")
-    _apart(out, x, "out and x")
+        _apart(out, x, "out and x")
+    ldo = out.stride(0)
     if rows == 0 or features == 0:
         return out
     h = marks = None

@@ -92,8 +92,9 @@ def edit_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, le
         out = torch.empty((rows, V), dtype=torch.float32, device=here)
     else:
         K._need(out.shape == logits.shape and out.dtype == torch.float32, "out must match the logits")
+        K._rows_out(out, "out")
         K._same_place(out, logits, "out")
-    ld_out = K._rows_out(out, "out")
+    ld_out = out.stride(0)
     if rows == 0 or V == 0:
         return out
     f = K._fn("logit_rules", "lb_logit_rules",

@@ -54,7 +54,8 @@ def test_decoding_rows_in_any_order_some_without_an_adapter(dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,width,features,rank", [(700, 256, 384, 16), (1500, 192, 136, 64), (1025, 512, 128, 40), (640, 72, 1000, 8)])
+@pytest.mark.parametrize("rows,width,features,rank", [(700, 256, 384, 16), (1500, 192, 136, 64), (1025, 512, 128, 40), (640, 72, 1000, 8),
+                                                      (600, 200, 264, 128), (700, 250, 333, 13), (900, 328, 1032, 72), (520, 64, 128, 200)])
 def test_prompts_one_behind_the_other(dtype, rows, width, features, rank):
     """Portions whose ends lie within tiles, one of a single token, one without an adapter."""
     cuts = [0, rows // 5, rows // 5 + 1, rows // 2 + 3, rows - 130, rows]
@@ -163,3 +164,39 @@ def test_empty_sizes(dtype):
     assert check(make(4, 16, 24, 0, 8, dtype, [0, 1, 0, -1])).shape == (4, 24)
     assert check(make(0, 16, 24, 2, 8, dtype, [])).shape == (0, 24)
     assert check(make(4, 16, 0, 2, 8, dtype, [0, 1, 0, -1])).shape == (4, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ranks_past_what_the_tensor_core_forms_take(dtype):
+    check(make(6, 96, 80, 3, 300, dtype, [0, 1, 2, -1, 1, 0]))
+    check(make(450, 64, 40, 2, 264, dtype, [0] * 200 + [1] * 250))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_keep_their_sign(dtype):
+    """A short sum that is infinite has no remainder to add: y becomes that infinity and no NaN."""
+    for rows in (3, 400):
+        s = make(rows, 64, 48, 1, 16, dtype, [0] * rows)
+        s["x"][1] = 0.0
+        s["x"][1, 0] = float("inf")
+        s["a"][0, :, 0], s["b"][0] = 1.0, s["b"][0].abs() + 0.5
+        s["scales"][0] = 1.0
+        got = K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"], s["scales"])
+        assert bool((got[1] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [5, 500])
+def test_the_binding_and_the_ordinary_way_are_the_same_call(dtype, rows):
+    s = make(rows, 256, 136, 4, 16, dtype, [t % 5 - 1 for t in range(rows)])
+    got = K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"], s["scales"])
+    again = K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"], s["scales"], out=torch.empty_like(s["y"]))
+    assert torch.equal(got, again)
+
+
+def test_without_scales_and_ranks_and_a_single_adapter():
+    for rows in (2, 400):
+        s = make(rows, 64, 64, 1, 8, torch.bfloat16, [0] * rows)
+        s["scales"].fill_(1.0)
+        got = check(s)
+        assert torch.equal(got, K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"]))

@@ -31,6 +31,7 @@ def listed(biases):
 def agree(got, want, size):
     """Equal infinities and NaN; the others within six roundings of 32 bits of what was added."""
     want = want.to(got.device)
+    want = torch.where(want.float().isinf(), want.float().double(), want)          # (past 32 bits' largest number: that infinity)
     fine = want.isfinite()
     assert torch.equal(got.isfinite(), fine) and torch.equal(got.isnan(), want.isnan())
     assert torch.equal(got[~fine & ~want.isnan()].double(), want[~fine & ~want.isnan()])
@@ -188,3 +189,20 @@ def test_nothing_to_do_copies_and_empty_calls_return():
     assert torch.equal(got, logits) and got.data_ptr() != logits.data_ptr()
     assert edit(logits[:0]).shape == (0, 50)
     assert edit(torch.zeros((2, 0), device="cuda")).shape == (2, 0)
+
+
+def test_the_binding_and_the_ordinary_way_are_the_same_call():
+    logits, kw = draw(5, 4099, 300)
+    more = listed([[(1, 2.0)], [], [(3, -1.0), (3, 5.0)], [], []])
+    got = edit(logits, **kw, **more)
+    assert torch.equal(got, edit(logits, **kw, **more, out=torch.empty_like(logits)))
+
+
+def test_extreme_penalties():
+    """Quotients by the inverse and its remainder: numbers of every size, infinities, zero, a repetition of zero and infinity."""
+    l = torch.tensor([[1e-30, 3e38, -3e38, float("inf"), float("-inf"), 0.0, -0.0, 1.0, 7.0, 1e30]] * 4, device="cuda")
+    history = torch.arange(10, dtype=torch.int32, device="cuda").expand(4, 10).contiguous()
+    for rep in ([1.3, 0.7, 3.0, 1e3], [1e-3, 1e10, 7.0, 0.9]):
+        check(l, history=history, lengths=ints([10] * 4), prompt_lengths=ints([10] * 4), repetition=floats(rep))
+    got = edit(l, history=history, lengths=ints([10] * 4), repetition=floats([0.0, float("inf"), float("nan"), 1.0]))
+    assert float(got[0, 7]) == float("inf") and float(got[1, 7]) == 0.0 and bool(got[2].isnan().all()) and torch.equal(got[3], l[3])

@@ -75,7 +75,9 @@ def check(s, **kw):
 
 FORMS = [(8, 2, 64, 64, torch.bfloat16), (6, 2, 128, 64, torch.bfloat16), (12, 2, 128, 128, torch.bfloat16), (4, 4, 64, 16, torch.bfloat16),
          (16, 1, 96, 64, torch.bfloat16), (20, 1, 128, 64, torch.bfloat16), (3, 1, 8, 5, torch.bfloat16), (4, 2, 256, 32, torch.bfloat16),
-         (8, 2, 64, 64, torch.float32), (6, 2, 128, 48, torch.float32), (5, 1, 24, 7, torch.float32), (2, 1, 256, 64, torch.float32)]
+         (8, 2, 64, 64, torch.float32), (6, 2, 128, 48, torch.float32), (5, 1, 24, 7, torch.float32), (2, 1, 256, 64, torch.float32),
+         (16, 1, 96, 16, torch.bfloat16), (6, 2, 128, 16, torch.bfloat16), (4, 2, 96, 48, torch.bfloat16), (8, 2, 64, 32, torch.bfloat16),
+         (34, 2, 128, 64, torch.bfloat16), (6, 2, 128, 24, torch.bfloat16)]
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", FORMS)
@@ -87,13 +89,13 @@ def test_groups_of_every_kind(heads, kv_heads, hd, page, dtype):
     check(make([(64, [0, 0, 9])], heads, kv_heads, hd, page, dtype))            # tokens that stand on the prefix's last key
 
 
-@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", FORMS[:6] + FORMS[8:9])
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", FORMS[:6] + FORMS[8:9] + FORMS[12:16])
 @pytest.mark.parametrize("requests", [9, 40, 90])
 def test_more_rows_than_a_tile(heads, kv_heads, hd, page, dtype, requests):
     check(make([(700, [1 + (i * 37) % 150 for i in range(requests)])], heads, kv_heads, hd, page, dtype))
 
 
-@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", FORMS[:3] + FORMS[8:9])
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", FORMS[:3] + FORMS[8:9] + FORMS[12:14])
 def test_a_long_prefix(heads, kv_heads, hd, page, dtype):
     check(make([(5000, [10, 3000, 1, 77])], heads, kv_heads, hd, page, dtype))
     check(make([(5000, [10, 300]), (2500, [4] * 11)], heads, kv_heads, hd, page, dtype, q_size=4.0))
@@ -139,7 +141,7 @@ def test_rows_of_no_group_are_left_alone(heads, kv_heads, hd, page, dtype):
     assert bool((call(s, out=torch.full_like(s["q"], 3.0)) == 3).all())
 
 
-@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[2], FORMS[4], FORMS[8]])
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[2], FORMS[4], FORMS[8], FORMS[13]])
 def test_what_is_not_there_has_no_keys(heads, kv_heads, hd, page, dtype):
     """A request that the table does not have, positions past the table's columns, pages outside of the pool: the keys that are
     there are what counts."""
@@ -212,3 +214,35 @@ def test_row_strides_streams_and_graphs(heads, kv_heads, hd, page, dtype):
     graph.replay()
     torch.cuda.synchronize()
     assert bool(((out.float() - check(s).float()).abs() <= 2.0 ** -6).all())
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[2], FORMS[8], FORMS[13]])
+def test_one_page_of_the_prefix_is_not_there(heads, kv_heads, hd, page, dtype):
+    """Keys of a page outside of the pool are left out, its neighbours within a tile are not."""
+    s = make([(5 * page, [3, 70])], heads, kv_heads, hd, page, dtype, stale=0.0)
+    s["block_table"][:, 2] = s["k_cache"].shape[0]
+    got = call(s)
+    # the same without that page: a table that skips it, positions a page earlier
+    t = {**s, "block_table": torch.cat([s["block_table"][:, :2], s["block_table"][:, 3:]], 1).contiguous(),
+         "positions": s["positions"] - page, "prefix_lens": s["prefix_lens"] - page}
+    want, size, reach = shared_attention(*(t[n].cpu() for n in ("q", "k_cache", "v_cache", "block_table", "token_req", "positions")), hd ** -0.5)
+    assert bool(((got.cpu().double() - want).abs() <= shared_attention_error(want, size, reach, hd, dtype)).all())
+    K().check_kernel_errors()
+
+
+@pytest.mark.parametrize("groups", [33, 70])
+def test_many_groups(groups):
+    """More groups than a warp has lanes, some of them empty."""
+    heads, kv_heads, hd, page, dtype = FORMS[0]
+    check(make([((37 * i) % 150, [1 + (i + r) % 5 for r in range(i % 3)]) for i in range(groups)], heads, kv_heads, hd, page, dtype))
+
+
+def test_the_binding_and_the_ordinary_way_are_the_same_call():
+    k = K()
+    for heads, kv_heads, hd, page, dtype in (FORMS[0], FORMS[8]):
+        s = make([(300, [1, 5, 64, 200]), (0, [7])], heads, kv_heads, hd, page, dtype)
+        launched = k.launch_count
+        got = call(s)
+        assert k.launch_count == launched + 3
+        again = call(s, out=torch.empty_like(s["q"]))                             # (an output of the caller's goes the ordinary way)
+        assert torch.equal(again, got) and k.launch_count == launched + 6
