@@ -55,7 +55,8 @@ def test_decoding_rows_in_any_order_some_without_an_adapter(dtype, rows):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,width,features,rank", [(700, 256, 384, 16), (1500, 192, 136, 64), (1025, 512, 128, 40), (640, 72, 1000, 8),
-                                                      (600, 200, 264, 128), (700, 250, 333, 13), (900, 328, 1032, 72), (520, 64, 128, 200)])
+                                                      (600, 200, 264, 128), (700, 250, 333, 13), (900, 328, 1032, 72), (520, 64, 128, 200),
+                                                      (1100, 131, 1001, 96), (400, 65, 129, 64), (2100, 1003, 515, 5)])
 def test_prompts_one_behind_the_other(dtype, rows, width, features, rank):
     """Portions whose ends lie within tiles, one of a single token, one without an adapter."""
     cuts = [0, rows // 5, rows // 5 + 1, rows // 2 + 3, rows - 130, rows]
