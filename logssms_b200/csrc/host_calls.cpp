@@ -260,6 +260,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         long max_prefix, max_context;
         if (!number(&scale, args[8]) || !whole(&max_prefix, args[9]) || !whole(&max_context, args[10])) return none();
         const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &bt = *t[3];
+        if (!((float)scale > 0.f && (float)scale < INFINITY) || (((uintptr_t)k.data_ptr() | (uintptr_t)v.data_ptr()) & 15) != 0) return none();
         if (q.dim() != 3 || k.dim() != 4 || dtype_code(q) < 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return none();
         const int64_t tokens = q.size(0), Hq = q.size(1), hd = q.size(2), pages = k.size(0), page = k.size(1), Hkv = k.size(2), groups = t[7]->numel();
         if (tokens < 1 || groups < 1 || hd < 8 || hd > 256 || hd % 8 != 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || pages < 1 || page < 1 || tokens > kFits || Hq > 65535

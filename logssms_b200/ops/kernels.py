@@ -497,8 +497,8 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     are of requests whose first prefix_lens[g] keys are the same (0: nothing in common); these are read through the table row of the
     group's first token, and what lies behind them through each token's own.  A request's row may name the same pages or copies of
     them.  A group's tokens may stand inside of the prefix, belong to any requests and be several of one request.  Rows of no group
-    are left as they are (in `out`; otherwise unwritten).  A row without keys (position -1; a request or pages that are not there)
-    becomes zeros.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right too.
+    are left as they are (in `out`; otherwise unwritten).  A token whose request is not there sees the prefix alone, keys on pages
+    that are not there count for nobody, and a row without keys (position -1) becomes zeros.  Keys and values that a row does not see may be anything.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right too.
 
     bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits.  `check_kernel_errors()`
     reports a kernel whose internal wait gave up."""
@@ -529,9 +529,14 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         _need(t is None or t.device == q.device, f"{n} must be on q's device")
     _need(token_req.shape == (tokens,) == positions.shape, "one entry of token_req and positions per token")
     _need(prefix_lens.dim() == 1 and group_start.shape == (prefix_lens.numel() + 1,), "group_start must have one entry more than prefix_lens")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((tokens, Hq, hd), dtype=q.dtype, device=q.device)
     _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out must be a contiguous tensor like q")
+    _need((out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0, "the caches and out must begin at a multiple of 16 bytes")
+    if given:
+        _same_place(out, q, "out")
+    _need(0.0 < ctypes.c_float(scale).value < float("inf"), f"the scale must be a positive number of 32 bits, got {scale}")
     groups = prefix_lens.numel()
     if tokens == 0 or groups == 0:
         return out
@@ -2964,7 +2969,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if out is None and not PROFILER.enabled:
         got = (_serving_binding or _serving_calls()).adapters(y, x, a, b, index, scales, ranks)
         if got is not None:
-            return _serving_done(got, "add_adapters", 2 if y.shape[0] >= 384 or y.dtype is torch.float32 else 1)
+            return _serving_done(got, "add_adapters", 2 if y.shape[0] >= 384 or a.shape[1] > 256 or y.dtype is torch.float32 else 1)
     _cuda(y, x, a, b, index, scales, ranks, out)
     ldy, ldx = _rows_of(y, "y"), _rows_of(x, "x")
     rows, features = y.shape

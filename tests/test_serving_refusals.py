@@ -39,11 +39,11 @@ def refused(call, words):
 
 
 # --------------------------------------------------------------------------- attention over a shared prefix
-def attention(**change):
+def attention(scale=0.125, **change):
     a = {"q": on(4, 8, 64, dtype=torch.bfloat16), "k_cache": on(10, 64, 2, 64, dtype=torch.bfloat16), "v_cache": on(10, 64, 2, 64, dtype=torch.bfloat16),
          "block_table": i32(3, 5), "token_req": i32(4), "positions": i32(4), "group_start": i32(3), "prefix_lens": i32(2), **change}
     kw = {k: a.pop(k) for k in ("out",) if k in a}
-    return K.attention_decode_shared(*a.values(), 0.125, max_prefix=64, max_context=128, **kw)
+    return K.attention_decode_shared(*a.values(), scale, max_prefix=64, max_context=128, **kw)
 
 
 def test_attention_in_order_reaches_the_launcher():
@@ -76,6 +76,19 @@ def test_attention_refuses(change, words):
     if words == "CUDA tensors only":
         change = {"q": lambda: on(4, 8, 64, dtype=torch.bfloat16, device="cpu")}
     refused(lambda: attention(**{k: v() for k, v in change.items()}), words)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e39, 1e-60])
+def test_attention_refuses_scales_that_are_no_positive_numbers(scale):
+    refused(lambda: attention(scale=scale), "scale must be a positive number")
+
+
+@pytest.mark.parametrize("which", ["k_cache", "v_cache", "out"])
+def test_attention_refuses_places_between_16_bytes(which):
+    shape = (4, 8, 64) if which == "out" else (10, 64, 2, 64)
+    n = shape[0] * shape[1] * shape[2] * (shape[3] if len(shape) > 3 else 1)
+    for off in (1, 4):
+        refused(lambda: attention(**{which: on(n + 8, dtype=torch.bfloat16)[off:off + n].view(shape)}), "multiple of 16 bytes")
 
 
 def test_attention_of_another_device_than_the_current_one(monkeypatch):
