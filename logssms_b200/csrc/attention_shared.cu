@@ -75,9 +75,10 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         first = blockIdx.x / head_tiles;
         row0 = (long)(blockIdx.x % head_tiles) * kRows;
         rows = (int)min((long)kRows, (long)G - row0);
-        if (!prefix_of(a, first, &begin)) return;
+        int group_first;
+        if (!prefix_of(a, first, &begin, &group_first)) return;
         request = a.token_req[first];
-        end = a.positions[first] + 1;
+        end = keys_of(a, first);
     }
     const bool known = request >= 0 && request < a.requests;
     end = known ? (int)min((long)end, (long)a.bt_cols * a.page_size) : begin;
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     const int o4 = (tid >> 5) * 4, col = (tid & 31) * 4; // of the output: rows o4 + i, columns col and 128 on
     const int at = (int)row0 + r;
     const int token = r < rows ? first + at / G : first;
-    const int limit = r < rows ? a.positions[token] + 1 : 0;
+    const int limit = r < rows ? keys_of(a, token) : 0;
     float m = -INFINITY, l = 0.f;
     float4 acc[2][4];
 #pragma unroll
@@ -261,14 +262,65 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
+// A row that stands within the prefix and came out as no number.  The tensor cores multiply the values of all of a tile's keys, those
+// that the row does not see by zero, and zero times an infinity is NaN: so once more, key by key, over those that it sees.  A warp.
 template <typename T>
-__global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
+__device__ __noinline__ void again(const SharedArgs& a, int t, int head, int first, int keys) {
+    const int lane = threadIdx.x & 31, pieces = a.hd >> 2, request = a.token_req[first];
+    const T* q = (const T*)a.q + (long)t * a.q_stride + (long)head * a.hd;
+    const size_t column = (size_t)(head / (a.Hq / a.Hkv)) * a.hd;
+    float4 qv[2], o[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        qv[h] = o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane + 32 * h < pieces) {
+            const T* src = q + 4 * (lane + 32 * h);                              // (any alignment)
+            qv[h] = make_float4(to_f32(src[0]), to_f32(src[1]), to_f32(src[2]), to_f32(src[3]));
+        }
+    }
+    float m = -INFINITY, l = 0.f;
+    if (request < 0 || request >= a.requests) keys = 0;
+    keys = (int)min((long)keys, (long)a.bt_cols * a.page_size);
+    for (int j = 0; j < keys; ++j) {
+        const long page = a.block_table[(long)request * a.bt_stride + j / a.page_size];
+        if (page < 0 || page >= a.pages) continue;
+        const size_t at = (size_t)(page * a.page_size + j % a.page_size) * a.Hkv * a.hd + column;
+        float score = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (lane + 32 * h < pieces) {
+                const float4 k = get4((const T*)a.k_cache + at + 4 * (lane + 32 * h));
+                score = fmaf(qv[h].x, k.x, fmaf(qv[h].y, k.y, fmaf(qv[h].z, k.z, fmaf(qv[h].w, k.w, score))));
+            }
+        score = warp_sum(score) * a.scale_log2;
+        const float top = fmaxf(m, score), ref = top == -INFINITY ? 0.f : top, before = exp2f(m - ref), w = exp2f(score - ref);
+        m = top;
+        l = l * before + w;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (lane + 32 * h < pieces) {
+                const float4 v = w != 0.f ? get4((const T*)a.v_cache + at + 4 * (lane + 32 * h)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                o[h].x = fmaf(o[h].x, before, w * v.x); o[h].y = fmaf(o[h].y, before, w * v.y);
+                o[h].z = fmaf(o[h].z, before, w * v.z); o[h].w = fmaf(o[h].w, before, w * v.w);
+            }
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (lane + 32 * h < pieces)
+            store4((T*)a.out + ((size_t)t * a.Hq + head) * a.hd + 4 * (lane + 32 * h), make_float4(o[h].x * inv, o[h].y * inv, o[h].z * inv, o[h].w * inv));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 4) shared_merge_kernel(const __grid_constant__ SharedArgs a) {
     pdl_wait();
     const long item = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (item >= (long)a.tokens * a.Hq) return;
-    int prefix;
-    if (!prefix_of(a, (int)(item / a.Hq), &prefix)) return;         // rows of no group are left as they are
+    const int t = (int)(item / a.Hq);
+    int prefix, first;
+    if (!prefix_of(a, t, &prefix, &first)) return;                  // rows of no group are left as they are
+    const int keys = keys_of(a, t);
     const int splits = a.prefix_splits + a.own_splits;
     const int s0 = prefix > 0 ? 0 : a.prefix_splits;     // without a prefix nobody wrote its ranges
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (size_t)item * splits;
@@ -305,6 +357,10 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(SharedArgs a) {
         }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;          // a row that saw no key: zeros
+    if (keys < prefix) {
+        const float all = (o[0].x + o[0].y) + (o[0].z + o[0].w) + ((o[1].x + o[1].y) + (o[1].z + o[1].w));
+        if (__any_sync(0xffffffffu, !(fabsf(all) < INFINITY))) return again<T>(a, t, (int)(item % a.Hq), first, keys);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         if (lane + 32 * h < pieces)

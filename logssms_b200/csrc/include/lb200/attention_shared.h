@@ -71,9 +71,12 @@ __device__ __forceinline__ bool find_tile(const SharedArgs& a, long target, int 
     return false;
 }
 
-// The shared prefix of a token's group; false: the token is of no group.  Called by whole warps: up to 32 groups are looked through
-// at once, more by halves.
-__device__ __forceinline__ bool prefix_of(const SharedArgs& a, int t, int* prefix) {
+// How many keys a token sees: those up to its position.
+__device__ __forceinline__ int keys_of(const SharedArgs& a, int t) { return min(a.positions[t], 0x7ffffffe) + 1; }
+
+// The shared prefix of a token's group and the group's first token; false: the token is of no group.  Called by whole warps: up to 32
+// groups are looked through at once, more by halves.
+__device__ __forceinline__ bool prefix_of(const SharedArgs& a, int t, int* prefix, int* first) {
     if (a.groups <= 32) {
         const int lane = threadIdx.x & 31;
         int from = 0, to = 0, p = 0;
@@ -81,6 +84,7 @@ __device__ __forceinline__ bool prefix_of(const SharedArgs& a, int t, int* prefi
         const unsigned hit = __ballot_sync(0xffffffffu, t >= from && t < to);
         if (hit == 0) return false;
         *prefix = max(__shfl_sync(0xffffffffu, p, __ffs(hit) - 1), 0);
+        *first = max(__shfl_sync(0xffffffffu, from, __ffs(hit) - 1), 0);
         return true;
     }
     int lo = 0, hi = a.groups;                           // the last group that starts at or in front of t
@@ -90,6 +94,7 @@ __device__ __forceinline__ bool prefix_of(const SharedArgs& a, int t, int* prefi
     }
     if (lo == 0 || t >= a.group_start[lo]) return false;
     *prefix = max(a.prefix_lens[lo - 1], 0);
+    *first = max(a.group_start[lo - 1], 0);
     return true;
 }
 

@@ -59,8 +59,8 @@ shared_own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const bool last = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
 
     const int request = a.token_req[t], position = a.positions[t];
-    int begin = 0;
-    const bool grouped = prefix_of(a, t, &begin);
+    int begin = 0, first_token;
+    const bool grouped = prefix_of(a, t, &begin, &first_token);
     // (behind the loads on whose answers the first tile waits) the queries as A operands: rows lane / 4 and + 8, columns 2 (lane % 4) and + 8 of each step
     uint32_t qa[kK][4];
     {

@@ -269,7 +269,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         const int r = (TWO ? grp * kQ : 0) + lr;           // and row of the tile
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + grp * kGroupCols;
         // the keys that the row sees: those in front of the prefix's end, and of its own position's
-        const int limit = r < rows ? min(prefix, a.positions[first + (int)((row0 + r) / G)] + 1) : prefix;
+        const int limit = r < rows ? min(prefix, keys_of(a, first + (int)((row0 + r) / G))) : prefix;
         const int step = TWO ? 1 : 2, from = TWO ? 0 : grp;
         float m_used = -INFINITY, l = 0.f;
         uint64_t* o_bar = o_ready + 2 * grp;

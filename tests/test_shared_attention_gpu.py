@@ -110,6 +110,41 @@ def test_several_tokens_of_a_request_and_tokens_inside_the_prefix(heads, kv_head
     assert bool((got[2] == 0).all())
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[2], FORMS[4], FORMS[6], FORMS[8], FORMS[13]])
+@pytest.mark.parametrize("stale", [float("nan"), float("inf")])
+def test_what_a_row_does_not_see_may_be_anything(heads, kv_heads, hd, page, dtype, stale):
+    """Tokens inside of the prefix: keys and values behind all of them; behind some of them (those that see it are no numbers)."""
+    s = make([(200, [4, 60, 130]), (150, [9])], heads, kv_heads, hd, page, dtype, stale=0.0, q_size=2.0)
+    s["positions"].copy_(ints([17, 99, 98, 158]))
+    want = check(s)
+    row = s["block_table"][0].long()
+    for j in range(100, 200):
+        s["k_cache"][row[j // page], j % page] = stale
+        s["v_cache"][row[j // page], j % page] = stale
+    got = call(s)
+    scale_of_values = float(s["v_cache"][s["v_cache"].isfinite()].abs().max())
+    close = (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -16) * scale_of_values   # weights in bfloat16 or in 32 bits: 2^-8 of the values, twice
+    assert bool(((got.float() - want.float()).abs() <= close).all())
+    s["v_cache"][row[99 // page], 99 % page] = stale                            # token 1 sees this one
+    again = call(s)
+    assert not bool(again[1].isfinite().any())
+    keep = [0, 2, 3]
+    assert bool(((again[keep].float() - want[keep].float()).abs() <= close).all())
+    K().check_kernel_errors()
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[8]])
+def test_positions_at_the_end_of_32_bits(heads, kv_heads, hd, page, dtype):
+    """A position behind everything sees all that its table has."""
+    s = make([(page, [2 * page, page])], heads, kv_heads, hd, page, dtype, stale=0.0)
+    s["block_table"] = s["block_table"][:, :2].contiguous()
+    s["positions"].copy_(ints([2 * page - 1, 2 * page - 1]))
+    want = check(s)
+    s["positions"].fill_(0x7fffffff)
+    assert torch.equal(call(s, max_context=3 * page), call(s, max_context=3 * page))
+    assert bool(((call(s, max_context=2 * page).float() - want.float()).abs() <= 2.0 ** -6).all())
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd,page,dtype", [FORMS[0], FORMS[2], FORMS[4], FORMS[8]])
 def test_cutting_up_changes_no_result(heads, kv_heads, hd, page, dtype):
     s = make([(1500, [5, 900, 40])], heads, kv_heads, hd, page, dtype)
