@@ -48,12 +48,11 @@ template <typename T> struct Lay {
 // One CTA: 16 rows (token, query head of one key/value head) x a range of keys.
 //   prefix: grid (tiles of the groups' rows, kv heads, ranges); own: grid (tokens x tiles of a token's heads, kv heads, ranges)
 template <typename T, bool PREFIX>
-__global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, int head_tiles) {
-    // The own keys' launch runs beside the prefix's, of which it needs nothing; its last CTA waits for it, so that the merge, which
-    // waits for this launch, comes behind both.
+__global__ void __launch_bounds__(kThreads, 4) shared_general_kernel(SharedArgs a, int head_tiles) {
+    // The own keys' launch runs beside the prefix's, of which it needs nothing; its last CTA waits for it at its end, so that the merge,
+    // which waits for this launch, comes behind both.
     const bool last = !PREFIX && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1;
     if (PREFIX) { pdl_wait(); pdl_trigger(); }
-    if (last) pdl_wait();
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long place[2][kKeys];                      // of a tile's keys: the row in the pool, or -1
     const int hd = a.hd, tid = threadIdx.x;
@@ -76,7 +75,10 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         row0 = (long)(blockIdx.x % head_tiles) * kRows;
         rows = (int)min((long)kRows, (long)G - row0);
         int group_first;
-        if (!prefix_of(a, first, &begin, &group_first)) return;
+        if (!prefix_of(a, first, &begin, &group_first)) {
+            if (last) pdl_wait();
+            return;
+        }
         request = a.token_req[first];
         end = keys_of(a, first);
     }
@@ -114,20 +116,19 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    find(from, 0);
-    __syncthreads();
-    if (from < to) fetch(0);
-    find(from + kKeys, 1);
+    // the queries and positions are on their way while the places of the first keys are looked up
+    constexpr int kQ = kRows * (256 / 4) / kThreads;
     const T* q = (const T*)a.q;
-    for (int i = tid; i < kRows * (hd >> 2); i += kThreads) {
-        const int r = i / (hd >> 2), d = (i % (hd >> 2)) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    T qv[kQ][4];
+#pragma unroll
+    for (int n = 0; n < kQ; ++n) {
+        const int i = tid + n * kThreads, r = i / (hd >> 2), d = (i - r * (hd >> 2)) * 4;
         if (r < rows) {
             const int at = (int)row0 + r, token = at / G;
             const T* src = q + (first + token) * a.q_stride + (kvh * G + at - token * G) * hd + d;         // (any alignment)
-            v = make_float4(to_f32(src[0]) * a.scale_log2, to_f32(src[1]) * a.scale_log2, to_f32(src[2]) * a.scale_log2, to_f32(src[3]) * a.scale_log2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qv[n][e] = src[e];
         }
-        *reinterpret_cast<float4*>(q_s + r * lay.ld_q + d) = v;
     }
     const int r = tid >> 3, c = tid & 7;                 // this thread's row of the softmax, its keys c + 8 i
     const int warp = tid >> 5, lane = tid & 31, rg = lane >> 3, kg = lane & 7;         // of the scores: rows 4 rg + i, keys kg + 8 j
@@ -135,6 +136,18 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
     const int at = (int)row0 + r;
     const int token = r < rows ? first + at / G : first;
     const int limit = r < rows ? keys_of(a, token) : 0;
+    find(from, 0);
+    __syncthreads();
+    if (from < to) fetch(0);
+    find(from + kKeys, 1);
+#pragma unroll
+    for (int n = 0; n < kQ; ++n) {
+        const int i = tid + n * kThreads, r = i / (hd >> 2), d = (i - r * (hd >> 2)) * 4;
+        if (r >= kRows) break;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows) v = make_float4(to_f32(qv[n][0]) * a.scale_log2, to_f32(qv[n][1]) * a.scale_log2, to_f32(qv[n][2]) * a.scale_log2, to_f32(qv[n][3]) * a.scale_log2);
+        *reinterpret_cast<float4*>(q_s + r * lay.ld_q + d) = v;
+    }
     float m = -INFINITY, l = 0.f;
     float4 acc[2][4];
 #pragma unroll
@@ -252,6 +265,7 @@ __global__ void __launch_bounds__(kThreads) shared_general_kernel(SharedArgs a, 
         for (int h = 0; h < 2; ++h)
             if (col + 128 * h < hd) *reinterpret_cast<float4*>(a.part_o + slot * hd + col + 128 * h) = acc[h][i];
     }
+    if (last) pdl_wait();
 }
 
 // One warp per (token, head): the ranges' weights first, a lane each, then their rows, 16 bytes a lane and several on their way.
@@ -442,7 +456,14 @@ extern "C" int lb_attention_shared_splits(const void* q, long q_stride, const vo
         const long most = keys / least < 1 ? 1 : keys / least, want = (ctas + n - 1) / n;
         return (int)(want > most ? (most > 64 ? 64 : most) : want > 64 ? 64 : want);
     };
-    const int prefix = tc ? layout_for(tokens, G, Hkv, hd, groups, max_prefix, max_own).clusters : cut(592, tiles, max_prefix, 64);
+    // The general form's prefix: no more CTAs than are at work at once, two an SM (float32, 64 requests of 12 heads of 128, 8,192 keys: 6
+    // ranges 217 us, 7 of which some wait for a place 303, 13 255).  The own keys' are shorter and take what is left.
+    auto whole_wave = [&] {
+        const size_t smem = dtype == kBF16 ? Lay<__nv_bfloat16>(hd).all : Lay<float>(hd).all;
+        const long n = 148 * (smem <= 113 * 1024 ? 2 : 1) / tiles, most = max_prefix / 64;
+        return (int)(n > 64 && most > 64 ? 64 : n < most ? (n < 1 ? 1 : n) : most < 1 ? 1 : most);
+    };
+    const int prefix = tc ? layout_for(tokens, G, Hkv, hd, groups, max_prefix, max_own).clusters : whole_wave();
     return prefix << 16 | cut(tc ? 2368 : 592, items, max_own, tc ? 256 : 64);
 }
 
