@@ -7,6 +7,7 @@
 // a tile's rows name are shared out to some CTAs ("slots"), each of which makes a pass for each of its own.  In `shrink` the
 // CTAs of a cluster have a part of K each and add their sums up in their order; `expand` multiplies by the scale and adds to y: one
 // rounding, of the output.
+#include <algorithm>
 #include "lb200/common.cuh"
 #include "lb200/adapters.cuh"
 #include "lb200/adapters_rows.cuh"
@@ -66,23 +67,25 @@ __device__ __forceinline__ void fill(float (&to)[ROWS][kLd], const Operand<T>& o
         }
     }
 }
-// acc[i][j] += row r4 + i of P times row c + 16 j of Q, over `depth` values; rows that are not there are zeros
-template <typename TP, typename TQ, typename FP, typename FQ>
-__device__ __forceinline__ void multiply(Work& w, float (&acc)[4][4], int depth, const Operand<TP>& p, FP p_there, const Operand<TQ>& q, FQ q_there) {
+// acc[i][j] += row r4 + i of P times row c + 16 j of Q, over `depth` values; rows that are not there are zeros.  `p_ready` comes
+// before P is read, and behind what is asked for of Q at once.
+template <typename TP, typename TQ, typename FP, typename FQ, typename Ready>
+__device__ __forceinline__ void multiply(Work& w, float (&acc)[4][4], int depth, const Operand<TP>& p, FP p_there, const Operand<TQ>& q, FQ q_there, Ready p_ready) {
     const int r4 = (threadIdx.x >> 4) * 4, c = threadIdx.x & 15, chunks = (depth + kChunk - 1) / kChunk;
-    auto fetch = [&](int n) {
-        if (n < chunks) {
-            fill(w.stage[n % kStages].p, p, n * kChunk, depth, p_there);
-            fill(w.stage[n % kStages].q, q, n * kChunk, depth, q_there);
-        }
+    auto fetch_q = [&](int n) { if (n < chunks) fill(w.stage[n % kStages].q, q, n * kChunk, depth, q_there); };
+    auto fetch_p = [&](int n) {
+        if (n < chunks) fill(w.stage[n % kStages].p, p, n * kChunk, depth, p_there);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     __syncthreads();                                       // (what was there has been read)
-    for (int n = 0; n < kStages - 1; ++n) fetch(n);
+    for (int n = 0; n < kStages - 1; ++n) fetch_q(n);
+    p_ready();
+    for (int n = 0; n < kStages - 1; ++n) fetch_p(n);
     for (int n = 0; n < chunks; ++n) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncthreads();
-        fetch(n + kStages - 1);
+        fetch_q(n + kStages - 1);
+        fetch_p(n + kStages - 1);
         const auto& s = w.stage[n % kStages];
 #pragma unroll
         for (int k = 0; k < kChunk; k += 4) {
@@ -109,6 +112,7 @@ template <typename T> __device__ __forceinline__ bool lies_wide(const T* p, long
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs a) {
     pdl_wait();
+    pdl_trigger();                                         // `expand` asks for what it does not have from here
     __shared__ __align__(16) Work w;
     const long t0 = (long)blockIdx.x * kRows;
     const int part = blockIdx.y, j0 = (int)(blockIdx.z / a.slots) * kCols, slot = blockIdx.z % a.slots, tid = threadIdx.x;
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs
         Operand<T> A{(const T*)a.A + (size_t)i * a.a_adapter + (size_t)j0 * a.a_row + k_begin, a.a_row, false};
         A.wide = lies_wide(A.at, a.a_row, depth);
         float acc[4][4] = {};
-        multiply(w, acc, depth, x, [&](int r) { return (named >> r & 1u) != 0; }, A, [&](int r) { return j0 + r < rank; });
+        multiply(w, acc, depth, x, [&](int r) { return (named >> r & 1u) != 0; }, A, [&](int r) { return j0 + r < rank; }, [] {});
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs
 // grid: (row tiles, feature tiles, slots)
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs a) {
-    pdl_wait();
+    // (what `shrink` does not make, index, y and B, is there since that kernel has begun)
     __shared__ __align__(16) Work w;
     const long t0 = (long)blockIdx.x * kRows;
     const int n0 = blockIdx.y * kCols, slot = blockIdx.z, tid = threadIdx.x;
@@ -180,13 +184,14 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs
         Operand<T> B{(const T*)a.B + (size_t)i * a.b_adapter + (size_t)n0 * a.b_row, a.b_row, false};
         B.wide = lies_wide(B.at, a.b_row, rank);
         float acc[4][4] = {};
-        multiply(w, acc, rank, h, [&](int r) { return (named >> r & 1u) != 0; }, B, [&](int r) { return n0 + r < a.N; });
+        multiply(w, acc, rank, h, [&](int r) { return (named >> r & 1u) != 0; }, B, [&](int r) { return n0 + r < a.N; }, [] { pdl_wait(); });
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (named >> (r4 + r) & 1u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sum[r][j] += acc[r][j] * scale;
     }
+    pdl_wait();                                            // (this kernel ends behind `shrink`, with or without work)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const long t = t0 + r4 + r;
@@ -238,7 +243,7 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     const int parts = parts_of(T, K, R);
     if (T > 0x7fffffffL - 1024 || N > 0x3fffffff) return kTooLarge;
     AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, h, T, K, N, R, adapters,
-                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, T <= 512 ? 8 : 2};      // (a prompt's tiles name one adapter or two)
+                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? 8 : 2))};      // (a prompt's tiles name one adapter or two)
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == kF32) return launch_general<float>(a, s);

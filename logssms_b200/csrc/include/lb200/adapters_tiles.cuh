@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(kThreads)
 adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, TileArgs ta) {
     pdl_wait();
+    pdl_trigger();                                         // (the rows' kernel finds its places as CTAs of this one end)
     typedef Shape<RB> Sh;
     const AdapterArgs& a = ta.a;
     extern __shared__ __align__(1024) uint8_t base[];      // (the swizzle goes by the address)
