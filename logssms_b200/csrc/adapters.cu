@@ -10,6 +10,7 @@
 #include <algorithm>
 #include "lb200/common.cuh"
 #include "lb200/adapters.cuh"
+#include "lb200/adapters_order.cuh"
 #include "lb200/adapters_rows.cuh"
 #include "lb200/adapters_tiles.cuh"
 using namespace lb200;
@@ -36,6 +37,7 @@ union Work {
 };
 template <typename T> struct Operand {
     const T* at; long ld;                                 // row r at `at + r * ld`
+    const int* rows;                                      // ... or at `at + rows[r] * ld` (shared memory; null: as they come)
     bool wide;                                            // 16 bytes at a time: rows lie so, and the depth is a multiple of 4
 };
 __device__ __forceinline__ void put(float* to, const float* from, bool there) {
@@ -56,14 +58,14 @@ __device__ __forceinline__ void fill(float (&to)[ROWS][kLd], const Operand<T>& o
         for (int n = 0; n < ROWS * kChunk / 4 / kThreads; ++n) {
             const int i = threadIdx.x + n * kThreads, r = i / (kChunk / 4), k = i % (kChunk / 4) * 4;
             const bool ok = there(r) && k0 + k < depth;
-            put4(&to[r][k], o.at + (ok ? (long)r * o.ld + k0 + k : 0), ok);
+            put4(&to[r][k], o.at + (ok ? (long)(o.rows != nullptr ? o.rows[r] : r) * o.ld + k0 + k : 0), ok);
         }
     } else {
 #pragma unroll 8
         for (int n = 0; n < ROWS * kChunk / kThreads; ++n) {
             const int i = threadIdx.x + n * kThreads, r = i / kChunk, k = i % kChunk;
             const bool ok = there(r) && k0 + k < depth;
-            put(&to[r][k], o.at + (ok ? (long)r * o.ld + k0 + k : 0), ok);
+            put(&to[r][k], o.at + (ok ? (long)(o.rows != nullptr ? o.rows[r] : r) * o.ld + k0 + k : 0), ok);
         }
     }
 }
@@ -108,18 +110,34 @@ template <typename T> __device__ __forceinline__ bool lies_wide(const T* p, long
     return sizeof(T) == 4 && ((uintptr_t)p & 15) == 0 && ld % 4 == 0 && depth % 4 == 0;
 }
 
+// The CTA's rows: places first .. first + rows - 1 (none: 0 rows).
+struct TileOfRows {
+    long first;
+    int rows;
+    __device__ explicit TileOfRows(const AdapterArgs& a) : first((long)blockIdx.x * kRows), rows((int)min((long)kRows, a.T - first)) {
+        if (a.order == nullptr) return;
+        const int4 its = (int)blockIdx.x < *a.n_tiles ? a.tiles[blockIdx.x] : make_int4(0, 0, 0, 0);
+        first = its.y;
+        rows = its.z;
+    }
+};
+
 // grid: (row tiles, parts of K, rank tiles x slots); a cluster: the parts
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs a) {
     pdl_wait();
     pdl_trigger();                                         // `expand` asks for what it does not have from here
     __shared__ __align__(16) Work w;
-    const long t0 = (long)blockIdx.x * kRows;
+    const TileOfRows tile(a);
+    if (tile.rows <= 0) return;                            // (the whole cluster)
+    const long t0 = tile.first;
+    __shared__ int rows_s[kRows];                          // the tile's rows
+    if (threadIdx.x < kRows) rows_s[threadIdx.x] = (int)threadIdx.x < tile.rows ? (int)row_at(a, t0 + threadIdx.x) : 0;
     const int part = blockIdx.y, j0 = (int)(blockIdx.z / a.slots) * kCols, slot = blockIdx.z % a.slots, tid = threadIdx.x;
     const int k_begin = min(part * a.part_k, a.K), depth = min(a.part_k, a.K - k_begin);
-    const int mine = adapter_of(a, t0 + (tid & 31));
+    const int mine = (tid & 31) < tile.rows ? adapter_of(a, t0 + (tid & 31)) : -1;
     const int r4 = (tid >> 4) * 4, c = tid & 15;
-    Operand<T> x{(const T*)a.x + t0 * a.ldx + k_begin, a.ldx, false};
+    Operand<T> x{(const T*)a.x + k_begin, a.ldx, rows_s, false};
     x.wide = lies_wide(x.at, a.ldx, depth);
     int turn = 0;
     for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i), ++turn) {
@@ -127,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_shrink_kernel(AdapterArgs
         const int rank = rank_of(a, i);
         if (j0 >= rank) continue;
         const unsigned named = __ballot_sync(0xffffffffu, mine == i);            // (bit r: row r)
-        Operand<T> A{(const T*)a.A + (size_t)i * a.a_adapter + (size_t)j0 * a.a_row + k_begin, a.a_row, false};
+        Operand<T> A{(const T*)a.A + (size_t)i * a.a_adapter + (size_t)j0 * a.a_row + k_begin, a.a_row, nullptr, false};
         A.wide = lies_wide(A.at, a.a_row, depth);
         float acc[4][4] = {};
         multiply(w, acc, depth, x, [&](int r) { return (named >> r & 1u) != 0; }, A, [&](int r) { return j0 + r < rank; }, [] {});
@@ -157,9 +175,18 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs a) {
     // (what `shrink` does not make, index, y and B, is there since that kernel has begun)
     __shared__ __align__(16) Work w;
-    const long t0 = (long)blockIdx.x * kRows;
+    const TileOfRows tile(a);
+    if (tile.rows <= 0) {
+        pdl_wait();
+        return;
+    }
+    const long t0 = tile.first;
     const int n0 = blockIdx.y * kCols, slot = blockIdx.z, tid = threadIdx.x;
-    const int mine = adapter_of(a, t0 + (tid & 31));
+    const int mine = (tid & 31) < tile.rows ? adapter_of(a, t0 + (tid & 31)) : -1;
+    const int its_row = (tid & 31) < tile.rows ? (int)row_at(a, t0 + (tid & 31)) : 0;
+    long row[4];                                           // this thread's
+#pragma unroll
+    for (int r = 0; r < 4; ++r) row[r] = __shfl_sync(0xffffffffu, its_row, (tid >> 4) * 4 + r);
     const int r4 = (tid >> 4) * 4, c = tid & 15;
     unsigned ours = slot == 0 ? __ballot_sync(0xffffffffu, mine < 0) : 0u;       // the rows that this CTA writes
     int turn = 0;
@@ -172,16 +199,16 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs
     for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if ((ours >> (r4 + r) & 1u) && t0 + r4 + r < a.T && n0 + c + 16 * j < a.N) sum[r][j] = to_f32(y[(t0 + r4 + r) * a.ldy + n0 + c + 16 * j]);
+            if ((ours >> (r4 + r) & 1u) && r4 + r < tile.rows && n0 + c + 16 * j < a.N) sum[r][j] = to_f32(y[row[r] * a.ldy + n0 + c + 16 * j]);
     turn = 0;
     for (int i = next_adapter(mine, -1); i != kNoAdapter; i = next_adapter(mine, i), ++turn) {
         if (turn % a.slots != slot) continue;
         const int rank = rank_of(a, i);
         const unsigned named = __ballot_sync(0xffffffffu, mine == i);
         const float scale = a.scales ? a.scales[i] : 1.f;
-        Operand<float> h{a.h + t0 * a.R, a.R, false};
+        Operand<float> h{a.h + t0 * a.R, a.R, nullptr, false};
         h.wide = lies_wide(h.at, a.R, rank);
-        Operand<T> B{(const T*)a.B + (size_t)i * a.b_adapter + (size_t)n0 * a.b_row, a.b_row, false};
+        Operand<T> B{(const T*)a.B + (size_t)i * a.b_adapter + (size_t)n0 * a.b_row, a.b_row, nullptr, false};
         B.wide = lies_wide(B.at, a.b_row, rank);
         float acc[4][4] = {};
         multiply(w, acc, rank, h, [&](int r) { return (named >> r & 1u) != 0; }, B, [&](int r) { return n0 + r < a.N; }, [] { pdl_wait(); });
@@ -194,19 +221,18 @@ __global__ void __launch_bounds__(kThreads, 5) adapter_expand_kernel(AdapterArgs
     pdl_wait();                                            // (this kernel ends behind `shrink`, with or without work)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const long t = t0 + r4 + r;
-        if (t >= a.T || !(ours >> (r4 + r) & 1u)) continue;
+        if (r4 + r >= tile.rows || !(ours >> (r4 + r) & 1u)) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int n = n0 + c + 16 * j;
-            if (n < a.N) out[t * a.ldo + n] = from_f32<T>(sum[r][j]);
+            if (n < a.N) out[row[r] * a.ldo + n] = from_f32<T>(sum[r][j]);
         }
     }
 }
 
 template <typename T>
 int launch_general(const AdapterArgs& a, cudaStream_t s) {
-    const unsigned tiles = (unsigned)((a.T + kRows - 1) / kRows);
+    const unsigned tiles = (unsigned)(a.order == nullptr ? (a.T + kRows - 1) / kRows : adapter_order::most_tiles(a.T, a.adapters, kRows));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles, a.parts, (a.R > 0 ? (a.R + kCols - 1) / kCols : 1) * a.slots); cfg.blockDim = dim3(kThreads); cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -229,27 +255,42 @@ static int parts_of(long T, int K, int R) {
     return parts;
 }
 
-// From so many rows on a call goes to the tiles' kernel.
-constexpr long kTileRows = 384;
+// From so many rows on a call in bfloat16 goes to the tiles' kernel, and, where its rows may name several adapters, in their order.
+constexpr long kTileRows = 384, kOrderRows = 64;
+static bool two_kernels(int R, int dtype) { return dtype != kBF16 || R > adapter_rows::kMostRanks; }
+static bool in_order(long T, int R, int adapters, int dtype) {
+    return adapters > 1 && adapters <= adapter_order::kMostAdapters && T >= (two_kernels(R, dtype) ? kOrderRows : kTileRows);
+}
+static long words_of_h(long T, int R, int dtype) { return two_kernels(R, dtype) ? (T * R + 3) / 4 * 4 : 0; }
 
-// h: float32 scratch [T, R].  Strides in elements; columns lie side by side.  out may be y.
-// (h: float32, or ranks over 256.)  marks: int32 scratch, one per 128 rows; error: the device's error word.
+// Scratch that a call needs, in pieces of 256 bytes: the short sums [T, R] of the form with two kernels, the rows' order.
+extern "C" int lb_adapters_scratch(long T, int R, int adapters, int dtype) {
+    return T <= 0 ? 0 : (int)((words_of_h(T, R, dtype) + (in_order(T, R, adapters, dtype) ? adapter_order::words(T, adapters, adapter_rows::kRows) : 0) + 63) / 64);
+}
+
+// Strides in elements; columns lie side by side.  out may be y.  error: the device's error word.
 extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row,
                                const void* B, long b_adapter, long b_row, const int* index, const float* scales, const int* ranks,
-                               void* out, long ldo, float* h, int* marks, int* error, long T, int K, int N, int R, int adapters, int dtype,
+                               void* out, long ldo, void* scratch, int* error, long T, int K, int N, int R, int adapters, int dtype,
                                void* stream) {
     if (T <= 0 || N <= 0) return kOk;
     if (K < 0 || R < 0 || adapters < 0) return kBadSize;
     const int parts = parts_of(T, K, R);
     if (T > 0x7fffffffL - 1024 || N > 0x3fffffff) return kTooLarge;
-    AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, h, T, K, N, R, adapters,
-                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? 8 : 2))};      // (a prompt's tiles name one adapter or two)
+    if (dtype != kF32 && dtype != kBF16) return kBadDType;
+    float* h = (float*)scratch;
+    int* plan = in_order(T, R, adapters, dtype) ? (int*)scratch + words_of_h(T, R, dtype) : nullptr;
+    AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, h, nullptr, nullptr, nullptr, T, K, N, R, adapters,
+                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? 8 : 2))};      // (tiles of more rows name one adapter or two)
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
+    if (dtype == kBF16 && R <= adapter_rows::kMostRanks && T >= kTileRows && adapters <= adapter_order::kMostAdapters && adapter_tiles::takes(a))
+        return adapter_tiles::launch(a, plan, error, s);
+    if (plan != nullptr) {
+        const int rc = adapter_order::launch(a, plan, two_kernels(R, dtype) ? kRows : adapter_rows::kRows, -1, s);
+        if (rc != 0) return rc;
+        a.slots = 1;                                       // (one adapter in a tile)
+    }
     if (dtype == kF32) return launch_general<float>(a, s);
-    if (dtype != kBF16) return kBadDType;
-    if (R > adapter_rows::kMostRanks) return launch_general<__nv_bfloat16>(a, s);
-    if (T < kTileRows || marks == nullptr || !adapter_tiles::takes(a)) return adapter_rows::launch(a, nullptr, s);
-    const int rc = adapter_tiles::launch(a, marks, error, s);
-    return rc != 0 ? rc : adapter_rows::launch(a, marks, s);       // what was left to it, if anything
+    return R > adapter_rows::kMostRanks ? launch_general<__nv_bfloat16>(a, s) : adapter_rows::launch(a, s);
 }

@@ -212,12 +212,14 @@ typedef int (*SplitsFn)(const void*, long, const void*, const void*, long, int, 
 typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, const int*, long, int, int, const int*, const int*, const int*,
                            const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, long, float, int*, int, void*);
 typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
-                          const int*, void*, long, float*, int*, int*, long, int, int, int, int, int, void*);
+                          const int*, void*, long, void*, int*, long, int, int, int, int, int, void*);
+typedef int (*ScratchFn)(long, int, int, int);
 typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
                        const float*, const float*, const int*, const int*, const float*, int, const int*, long, int, const int*, void*);
 SplitsFn splits_fn;
 AttentionFn attention_fn;
 AdaptersFn adapters_fn;
+ScratchFn scratch_fn;
 RulesFn rules_fn;
 
 
@@ -282,7 +284,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-// (y, x, a, b, index, scales | None, ranks | None) -> (out, kernels)
+// (y, x, a, b, index, scales | None, ranks | None) -> out
 PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const int device = (int)c10::cuda::current_device();
@@ -299,18 +301,11 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int code = dtype_code(*y);
         const at::Tensor out = at::detail::empty_strided_cuda({rows, features}, {features, 1}, y->scalar_type(), y->device());
         at::Tensor scratch;
-        float* h = nullptr;
-        int* marks = nullptr;
-        if (code == 0 || rank > 256) {
-            scratch = at::detail::empty_strided_cuda({rows * rank}, {1}, at::kFloat, y->device());
-            h = (float*)scratch.data_ptr();
-        } else if (rows >= 384) {
-            scratch = at::detail::empty_strided_cuda({(rows + 127) / 128}, {1}, at::kInt, y->device());
-            marks = (int*)scratch.data_ptr();
-        }
+        const int64_t pieces = scratch_fn(rows, (int)rank, (int)count, code);
+        if (pieces > 0) scratch = at::detail::empty_strided_cuda({64 * pieces}, {1}, at::kInt, y->device());
         const int rc = adapters_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
-                                   b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features, h, marks,
-                                   error_words[device], rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
+                                   b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features,
+                                   pieces > 0 ? scratch.data_ptr() : nullptr, error_words[device], rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
         return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
     });
 }
@@ -364,11 +359,12 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // the launchers' addresses
 PyObject* launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 4) { PyErr_SetString(PyExc_TypeError, "four addresses"); return nullptr; }
+    if (n != 5) { PyErr_SetString(PyExc_TypeError, "five addresses"); return nullptr; }
     splits_fn = (SplitsFn)PyLong_AsVoidPtr(args[0]);
     attention_fn = (AttentionFn)PyLong_AsVoidPtr(args[1]);
     adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[2]);
     rules_fn = (RulesFn)PyLong_AsVoidPtr(args[3]);
+    scratch_fn = (ScratchFn)PyLong_AsVoidPtr(args[4]);
     return none();
 }
 }  // namespace serving

@@ -12,7 +12,9 @@ struct AdapterArgs {
     const int* index;                                   // a row's adapter; outside of [0, adapters): none
     const float* scales; const int* ranks;              // per adapter; null: 1, R
     void* out; long ldo;
-    float* h;                                           // [T, R]
+    float* h;                                           // [T, R], by the places of the rows
+    // the rows in the order of their adapters, by tiles of one adapter each (null: as they come): see adapters_order.cuh
+    const int* order; const int4* tiles; const int* n_tiles;
     long T;
     int K, N, R, adapters, parts, part_k, slots;
 };
@@ -21,9 +23,11 @@ struct AdapterArgs {
 constexpr int kNoAdapter = 0x7fffffff;
 __device__ __forceinline__ int next_adapter(int mine, int prev) { return __reduce_min_sync(0xffffffffu, mine > prev ? mine : kNoAdapter); }
 
+// The row at place t.
+__device__ __forceinline__ long row_at(const AdapterArgs& a, long t) { return a.order != nullptr ? a.order[t] : t; }
 __device__ __forceinline__ int adapter_of(const AdapterArgs& a, long t) {
     if (t >= a.T) return -1;
-    const int i = a.index[t];
+    const int i = a.index[row_at(a, t)];
     return i >= 0 && i < a.adapters ? i : -1;
 }
 __device__ __forceinline__ int rank_of(const AdapterArgs& a, int i) { return a.ranks ? min(max(a.ranks[i], 0), a.R) : a.R; }

@@ -13,6 +13,7 @@
 // alone would be off by as much as the output's own rounding.
 #pragma once
 #include "lb200/adapters.cuh"
+#include "lb200/adapters_order.cuh"
 #include "lb200/common.cuh"
 
 namespace lb200 {
@@ -52,10 +53,10 @@ __device__ __forceinline__ void hand(uint32_t at, uint32_t rank, float v) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// The rows t0 .. t0 + rows_per - 1.  MT: 16 MT ranks at a time.  XV: rows of x and A lie on 16 bytes and K is a multiple of 8;
+// The rows at places t0 .. t0 + rows - 1.  MT: 16 MT ranks at a time.  XV: rows of x and A lie on 16 bytes and K is a multiple of 8;
 // BV: rows of B on 8 bytes, R a multiple of 4.
 template <int MT, bool XV, bool BV>
-__device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int rows_per, int parts) {
+__device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int rows, int parts) {
     constexpr int kRanks = 16 * MT;
     constexpr int kUnits = MT == 4 ? 1 : 2;                // units of K, or of features, on their way (twice as many features)
     __shared__ float part[kWarps][kRanks][kRows];         // the warps' sums of some ranks
@@ -63,8 +64,7 @@ __device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int
     extern __shared__ float handed[];                     // [parts][ranks][kRows]: the CTAs' sums
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, c = lane & 3;
     const int rank = (int)(blockIdx.x % (unsigned)parts), padded = (a.R + 15) / 16 * 16;
-    const int rows = (int)min((long)rows_per, a.T - t0);
-    const bf16* x = (const bf16*)a.x + (t0 + min(n, rows - 1)) * a.ldx;          // row n of the columns
+    const bf16* x = (const bf16*)a.x + row_at(a, t0 + min(n, rows - 1)) * a.ldx; // row n of the columns
     const bf16* y = (const bf16*)a.y;
     bf16* out = (bf16*)a.out;
     // this CTA's part of K, in units of 32, and of the features, in units of 16
@@ -78,7 +78,7 @@ __device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int
     for (int i = next_adapter(own, -1); i != kNoAdapter; i = next_adapter(own, i)) { if (own == i) place = adapters; ++adapters; }
     if (adapters == 0) {                                   // (the same in all warps and CTAs of the cluster)
         for (int i = n_from * 16 + threadIdx.x; i < min(n_to * 16, a.N); i += kThreads)
-            for (int r = 0; r < rows; ++r) out[(t0 + r) * a.ldo + i] = y[(t0 + r) * a.ldy + i];
+            for (int r = 0; r < rows; ++r) { const long t = row_at(a, t0 + r); out[t * a.ldo + i] = y[t * a.ldy + i]; }
         return;
     }
     cluster_arrive();                                      // this CTA is there
@@ -142,6 +142,7 @@ __device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int
     constexpr int kAhead = 2 * kUnits;
     const int own0 = __shfl_sync(0xffffffffu, own, 2 * c), own1 = __shfl_sync(0xffffffffu, own, 2 * c + 1);
     const bool write0 = 2 * c < rows && (own0 >= 0 ? own0 == i : ours == 0), write1 = 2 * c + 1 < rows && (own1 >= 0 ? own1 == i : ours == 0);
+    const long row0 = row_at(a, t0 + min(2 * c, rows - 1)), row1 = row_at(a, t0 + min(2 * c + 1, rows - 1));
     const bf16* B = (const bf16*)a.B + (size_t)max(i, 0) * a.b_adapter;
     uint32_t bv[kAhead][MT][2][2];
     auto features = [&](int u, int j0) {                   // ranks j0 .. of the features of units u, u + teams, ...
@@ -163,7 +164,7 @@ __device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
-                if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N) yv[h][e] = y[(t0 + 2 * c + (e & 1)) * a.ldy + f];
+                if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N) yv[h][e] = y[(e & 1 ? row1 : row0) * a.ldy + f];
             }
     };
     const int u0 = n_from + team;
@@ -236,46 +237,35 @@ __device__ __forceinline__ void block_of_rows(const AdapterArgs& a, long t0, int
             for (int e = 0; e < 4; ++e) {
                 const int f = 16 * (u + h * teams) + n + (e >> 1) * 8;
                 if ((e & 1 ? write1 : write0) && u + h * teams < n_to && f < a.N)
-                    out[(t0 + 2 * c + (e & 1)) * a.ldo + f] = (e & 1 ? own1 : own0) >= 0 ? __float2bfloat16_rn(__bfloat162float(yv[h][e]) + sum[h][e]) : yv[h][e];
+                    out[(e & 1 ? row1 : row0) * a.ldo + f] = (e & 1 ? own1 : own0) >= 0 ? __float2bfloat16_rn(__bfloat162float(yv[h][e]) + sum[h][e]) : yv[h][e];
             }
     }
 }
 
-// grid: clusters, each with rows_per rows; or (MARKED) which go through the blocks of rows_per rows of the marked tiles of 128.
-// (A CTA is past the first barrier of a block only when all are done with the one before.)
-template <int MT, bool XV, bool BV, bool MARKED>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel(AdapterArgs a, int rows_per, int parts, const int* marks, int tiles) {
+// grid: clusters, each with rows_per rows, or with a tile of rows in order
+template <int MT, bool XV, bool BV>
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 3 : 2) adapter_rows_kernel(AdapterArgs a, int rows_per, int parts) {
     pdl_wait();
-    const int cluster = (int)(blockIdx.x / (unsigned)parts), clusters = (int)(gridDim.x / (unsigned)parts);
-    if constexpr (!MARKED) {
-        block_of_rows<MT, XV, BV>(a, (long)cluster * rows_per, rows_per, parts);
-        return;
-    }
-    const int lane = threadIdx.x & 31, blocks = 128 / rows_per;
-    int turn = cluster;                                    // of the blocks of all marked tiles, this cluster's are cluster, + clusters, ...
-    for (int base = 0; base < tiles; base += 32) {
-        unsigned marked = __ballot_sync(0xffffffffu, base + lane < tiles && marks[base + lane] != 0);
-        for (; marked != 0; marked &= marked - 1, turn -= blocks) {
-            const long first = (long)(base + __ffs(marked) - 1) * 128;
-            for (; turn < blocks; turn += clusters) {
-                const long t0 = first + (long)turn * rows_per;
-                if (t0 < a.T) block_of_rows<MT, XV, BV>(a, t0, rows_per, parts);
-            }
-        }
+    const long cluster = blockIdx.x / (unsigned)parts, t0 = cluster * rows_per;
+    if (a.order == nullptr) {
+        block_of_rows<MT, XV, BV>(a, t0, (int)min((long)rows_per, a.T - t0), parts);
+    } else if (cluster < *a.n_tiles) {
+        const int4 its = a.tiles[cluster];
+        block_of_rows<MT, XV, BV>(a, its.y, its.z, parts);
     }
 }
 
-template <int MT, bool XV, bool BV, bool MARKED>
-inline int launch_as(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
+template <int MT, bool XV, bool BV>
+inline int launch_as(const AdapterArgs& a, cudaStream_t stream) {
     // About 64 clusters while there are rows for them; of 8 CTAs where all of them are on an SM at once, else of 4.
     int rows_per = 1;
     while (rows_per < kRows && a.T > 64 * rows_per) rows_per *= 2;
-    const long clusters = MARKED ? 64 : (a.T + rows_per - 1) / rows_per;
-    const int parts = clusters <= 40 ? 8 : 4, tiles = MARKED ? (int)((a.T + 127) / 128) : 0;
+    const long clusters = a.order == nullptr ? (a.T + rows_per - 1) / rows_per : adapter_order::most_tiles(a.T, a.adapters, kRows);
+    const int parts = clusters <= 40 ? 8 : 4;
     if (clusters * parts > 0x7fffffffL) return kTooLarge;
     const size_t smem = (size_t)parts * ((a.R + 15) / 16 * 16) * kRows * sizeof(float);
     static SharedLimits limits;
-    int rc = ensure_dynamic_smem(adapter_rows_kernel<MT, XV, BV, MARKED>, smem + 25 * 1024, limits);        // (with what it has besides)
+    int rc = ensure_dynamic_smem(adapter_rows_kernel<MT, XV, BV>, smem + 25 * 1024, limits);        // (with what it has besides)
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
@@ -285,24 +275,18 @@ inline int launch_as(const AdapterArgs& a, const int* marks, cudaStream_t stream
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV, MARKED>, a, rows_per, parts, marks, tiles);
-}
-template <bool XV, bool BV, bool MARKED>
-inline int launch_ranks(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
-    return a.R <= 16 ? launch_as<1, XV, BV, MARKED>(a, marks, stream) : a.R <= 32 ? launch_as<2, XV, BV, MARKED>(a, marks, stream)
-                                                                                  : launch_as<4, XV, BV, MARKED>(a, marks, stream);
+    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV>, a, rows_per, parts);
 }
 template <bool XV, bool BV>
-inline int launch_loads(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
-    return marks != nullptr ? launch_ranks<XV, BV, true>(a, marks, stream) : launch_ranks<XV, BV, false>(a, marks, stream);
+inline int launch_ranks(const AdapterArgs& a, cudaStream_t stream) {
+    return a.R <= 16 ? launch_as<1, XV, BV>(a, stream) : a.R <= 32 ? launch_as<2, XV, BV>(a, stream) : launch_as<4, XV, BV>(a, stream);
 }
 
-// `marks` (null: all rows): which tiles of 128 rows are meant.
-inline int launch(const AdapterArgs& a, const int* marks, cudaStream_t stream) {
+inline int launch(const AdapterArgs& a, cudaStream_t stream) {
     const bool xv = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.A & 15) == 0 && a.ldx % 8 == 0 && a.a_row % 8 == 0 && a.a_adapter % 8 == 0 && a.K % 8 == 0;
     const bool bv = ((uintptr_t)a.B & 7) == 0 && a.b_row % 4 == 0 && a.b_adapter % 4 == 0 && a.R % 4 == 0;
-    const int rc = xv ? bv ? launch_loads<true, true>(a, marks, stream) : launch_loads<true, false>(a, marks, stream)
-                      : bv ? launch_loads<false, true>(a, marks, stream) : launch_loads<false, false>(a, marks, stream);
+    const int rc = xv ? bv ? launch_ranks<true, true>(a, stream) : launch_ranks<true, false>(a, stream)
+                      : bv ? launch_ranks<false, true>(a, stream) : launch_ranks<false, false>(a, stream);
     return rc != 0 ? rc : launch_status();
 }
 

@@ -11,9 +11,13 @@
 // 12 warps: TMA loads of x and y, products, loads of B (and zeros behind an adapter's rank: 0 x NaN would be NaN), TMA stores, and two
 // groups of 128 threads, a thread per row, which take the tiles of features in turn.
 //
-// A tile whose rows name more adapters than that (decoding rows in front of a prompt) is marked, and left to the rows' kernel.
+// A tile whose rows name more adapters than that (decoding rows in front of a prompt, a batch in any order) is left to others: the
+// rows of all such tiles are put in the order of their adapters (adapters_order.cuh), and the grid's last clusters take them by tiles of
+// one adapter each, whose rows TMA gathers and scatters four at a time.  A tile's last four may hold its last row several times; the
+// rows behind them hold anything, which nothing of the others' depends on.
 #pragma once
 #include "lb200/adapters.cuh"
+#include "lb200/adapters_order.cuh"
 #include "lb200/common.cuh"
 #include "lb200/tcgen05.cuh"
 
@@ -35,15 +39,15 @@ template <int RB> struct Shape {
     // short sums | y ring | B ring; the first product's ring and this CTA's sums lie over both, which are filled afterwards
     static constexpr uint32_t kRings = kY * kYTile + kB * kBTile, kWork = 2 * kH + kRings;
     static_assert(kSums <= kRings, "sums over the rings");
-    static constexpr uint32_t kSmem = kWork + 1024 + 128; // ... | barriers, the rows' scales and ranks
+    static constexpr uint32_t kSmem = kWork + 1024 + 640; // ... | barriers, the rows' scales, ranks and places
     static constexpr int kMostStages = 8;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 struct TileArgs {
     AdapterArgs a;
-    int* marks;                                           // per tile: 1, left to the rows' kernel
-    int parts, padded;                                    // CTAs of a cluster; ranks, filled up to a multiple of 16
+    int straight;                                         // tiles of rows as they come
+    int parts, padded, limit;                             // CTAs of a cluster; ranks, filled up to a multiple of 16; adapters of such a tile
     int* error;
 };
 
@@ -74,13 +78,22 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
-// grid: tiles x parts; a cluster: a tile's parts
+// four rows each
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int x, const int4& rows) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w) : "memory");
+}
+__device__ __forceinline__ void tma_scatter4(const CUtensorMap* map, const void* src, int x, const int4& rows) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile::scatter4.bulk_group [%0, {%1, %2, %3, %4, %5}], [%6];"
+                 ::"l"(map), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(smem_u32(src)) : "memory");
+}
+
+// grid: (tiles of rows as they come, then tiles of rows in order) x parts; a cluster: a tile's parts
 template <int RB>
 __global__ void __launch_bounds__(kThreads)
 adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, TileArgs ta) {
-    pdl_wait();
-    pdl_trigger();                                         // (the rows' kernel finds its places as CTAs of this one end)
+                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_x1,
+                     const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_out1, TileArgs ta) {
     typedef Shape<RB> Sh;
     const AdapterArgs& a = ta.a;
     extern __shared__ __align__(1024) uint8_t base[];      // (the swizzle goes by the address)
@@ -106,16 +119,28 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* row_scale = reinterpret_cast<float*>(tmem_slot + 2);        // [128]
     unsigned char* row_ranks = reinterpret_cast<unsigned char*>(row_scale + kRows);     // [128]: 0 without an adapter
+    int4* fours = reinterpret_cast<int4*>(base + Sh::kWork + 1152);              // the rows of a tile in order, four by four
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)(blockIdx.x % (unsigned)ta.parts), tile = (int)(blockIdx.x / (unsigned)ta.parts);
     const long t0 = (long)tile * kRows;
 
     // ------------------------------------------------------------ who is in the tile (all warps alike)
-    int count = 0, who[kMost] = {};
-    {
+    int count = 0, who[kMost] = {}, n_fours = 0;           // n_fours > 0: the tile's rows are gathered
+    // (the kernel in front, which puts rows in order, has waited for all others before this one began)
+    auto straight_adapter = [&](long t) { const int i = t < a.T ? a.index[t] : -1; return i >= 0 && i < a.adapters ? i : -1; };
+    if (a.order == nullptr || tile >= ta.straight) pdl_wait();
+    if (tile >= ta.straight) {
+        const int at = tile - ta.straight;
+        if (at >= *a.n_tiles) return;                      // (the whole cluster)
+        const int4 its = a.tiles[at];
+        count = its.x >= 0 ? 1 : 0;
+        who[0] = its.x;
+        n_fours = (its.z + 3) / 4;
+        if (threadIdx.x < 4 * n_fours) reinterpret_cast<int*>(fours)[threadIdx.x] = a.order[its.y + min((int)threadIdx.x, its.z - 1)];
+    } else {
         int own[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) own[q] = adapter_of(a, t0 + 32 * q + lane);
+        for (int q = 0; q < 4; ++q) own[q] = straight_adapter(t0 + 32 * q + lane);
         int prev = -1;
         while (true) {
             int best = kNoAdapter;
@@ -126,18 +151,13 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
             for (int q = 0; q < kMost; ++q) if (q == count) who[q] = best;
             prev = best;
-            if (++count > kMost) break;
+            if (++count > ta.limit) return;                // (the whole cluster: these rows are put in order)
         }
     }
-    if (count > kMost || count * ta.padded > 256) {        // (the whole cluster)
-        if (rank == 0 && threadIdx.x == 0) ta.marks[tile] = 1;
-        return;
-    }
-    if (rank == 0 && threadIdx.x == 0) ta.marks[tile] = 0;
     const int n_tiles = (a.N + kCols - 1) / kCols, mine = n_tiles > rank ? (n_tiles - rank + ta.parts - 1) / ta.parts : 0;      // tiles rank, rank + parts, ...
     const int k_tiles = count > 0 ? (a.K + 63) / 64 : 0, k_per = (k_tiles + ta.parts - 1) / ta.parts;
     const int k_from = min(rank * k_per, k_tiles), k_n = min(k_per, k_tiles - k_from);
-    const uint32_t a_tile = ta.padded * 128, stage = kXTile + count * a_tile;    // (A tiles: multiples of 2,048 bytes)
+    const uint32_t a_tile = ta.padded * 128, stage = kXTile + count * a_tile, x_bytes = n_fours > 0 ? n_fours * 512 : kXTile;    // (A tiles: multiples of 2,048 bytes)
     const int stages = min((int)((Sh::kWork - 2 * Sh::kH) / stage), Sh::kMostStages);
 
     if (threadIdx.x == 0) {
@@ -171,8 +191,9 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (i >= stages && !wait(x_empty + s, ((i / stages) - 1) & 1, 1, i)) break;
             if (elect_one()) {
                 uint8_t* at = ring + s * stage;
-                mbar_expect_tx(x_full + s, stage);
-                tma_load_2d(at, &map_x, x_full + s, (k_from + i) * 64, (int)t0);
+                mbar_expect_tx(x_full + s, x_bytes + count * a_tile);
+                if (n_fours == 0) tma_load_2d(at, &map_x, x_full + s, (k_from + i) * 64, (int)t0);
+                for (int f = 0; f < n_fours; ++f) tma_gather4(at + f * 512, &map_x1, x_full + s, (k_from + i) * 64, fours[f]);
                 for (int q = 0; q < count; ++q) tma_load_3d(at + kXTile + q * a_tile, &map_a, x_full + s, (k_from + i) * 64, 0, list[q]);
             }
             __syncwarp();
@@ -203,7 +224,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     }
     const int group = (warp - kFirstAdder) >> 2, r = (warp & 3) * 32 + lane;     // of an adder: its row is its lane of tensor memory
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int own = warp >= kFirstAdder ? adapter_of(a, t0 + r) : -1;
+    const int own = warp < kFirstAdder ? -1 : n_fours == 0 ? straight_adapter(t0 + r) : r < 4 * n_fours ? who[0] : -1;
     int place = -1;
     if (own >= 0)
         for (int q = 0; q < count; ++q) if (list[q] == own) place = q;
@@ -280,9 +301,17 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             const int n0 = (rank + i * ta.parts) * kCols, s = i % Sh::kY;
             if (i >= Sh::kY && !wait(y_empty + s, ((i / Sh::kY) - 1) & 1, 6, i)) break;
             if (elect_one()) {
-                mbar_expect_tx(y_full + s, kYTile);
-                tma_load_2d(y_s + s * kYTile, &map_y, y_full + s, n0, (int)t0);
-                tma_load_2d(y_s + s * kYTile + kRows * 128, &map_y, y_full + s, n0 + 64, (int)t0);
+                const bool both = n_fours == 0 || n0 + 64 < a.N;
+                mbar_expect_tx(y_full + s, both ? 2 * x_bytes : x_bytes);
+                if (n_fours == 0) {
+                    tma_load_2d(y_s + s * kYTile, &map_y, y_full + s, n0, (int)t0);
+                    tma_load_2d(y_s + s * kYTile + kRows * 128, &map_y, y_full + s, n0 + 64, (int)t0);
+                }
+                for (int f = 0; f < n_fours; ++f) {
+                    const int4 rows = fours[f];
+                    tma_gather4(y_s + s * kYTile + f * 512, &map_y1, y_full + s, n0, rows);
+                    if (both) tma_gather4(y_s + s * kYTile + kRows * 128 + f * 512, &map_y1, y_full + s, n0 + 64, rows);
+                }
             }
             __syncwarp();
             y_asked = i + 1;
@@ -351,8 +380,15 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             const int s = i % Sh::kY, n0 = (rank + i * ta.parts) * kCols;
             if (!wait(y_done + s, (i / Sh::kY) & 1, 13, i)) break;
             if (lane == 0) {                               // (the same thread every time: it waits for its own stores)
-                tma_store_2d(&map_out, y_s + s * kYTile, n0, (int)t0);
-                if (n0 + 64 < a.N) tma_store_2d(&map_out, y_s + s * kYTile + kRows * 128, n0 + 64, (int)t0);
+                if (n_fours == 0) {
+                    tma_store_2d(&map_out, y_s + s * kYTile, n0, (int)t0);
+                    if (n0 + 64 < a.N) tma_store_2d(&map_out, y_s + s * kYTile + kRows * 128, n0 + 64, (int)t0);
+                }
+                for (int f = 0; f < n_fours; ++f) {
+                    const int4 rows = fours[f];
+                    tma_scatter4(&map_out1, y_s + s * kYTile + f * 512, n0, rows);
+                    if (n0 + 64 < a.N) tma_scatter4(&map_out1, y_s + s * kYTile + kRows * 128 + f * 512, n0 + 64, rows);
+                }
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBehind) : "memory");
                 if (i >= kBehind) mbar_arrive(y_empty + (i - kBehind) % Sh::kY);
@@ -439,34 +475,41 @@ inline bool takes(const AdapterArgs& a) {
 }
 
 template <int RB>
-inline int launch_as(const TileArgs& ta, int tiles, cudaStream_t stream) {
+inline int launch_as(const TileArgs& ta, long clusters, cudaStream_t stream) {
     const AdapterArgs& a = ta.a;
-    CUtensorMap map_x, map_a, map_b, map_y, map_out;
+    CUtensorMap map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1;
     int rc = make_tile_map(&map_x, a.x, a.T, a.K, a.ldx, kRows);
     if (rc == 0) rc = make_tile_map_3d(&map_a, a.A, a.adapters, a.R, a.K, a.adapters > 1 ? a.a_adapter : a.a_row * a.R, a.a_row, ta.padded);
     if (rc == 0) rc = make_tile_map_3d(&map_b, a.B, a.adapters, a.N, a.R, a.adapters > 1 ? a.b_adapter : a.b_row * a.N, a.b_row, kCols);
     if (rc == 0) rc = make_tile_map(&map_y, a.y, a.T, a.N, a.ldy, kRows);
     if (rc == 0) rc = make_tile_map(&map_out, a.out, a.T, a.N, a.ldo, kRows);
+    if (rc == 0) rc = make_tile_map(&map_x1, a.x, a.T, a.K, a.ldx, 1);                     // (a row at a time, four by four)
+    if (rc == 0) rc = make_tile_map(&map_y1, a.y, a.T, a.N, a.ldy, 1);
+    if (rc == 0) rc = make_tile_map(&map_out1, a.out, a.T, a.N, a.ldo, 1);
     static SharedLimits limits;
     if (rc == 0) rc = ensure_dynamic_smem(adapter_tiles_kernel<RB>, Shape<RB>::kSmem, limits);
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * ta.parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Shape<RB>::kSmem; cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(clusters * ta.parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Shape<RB>::kSmem; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)ta.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB>, map_x, map_a, map_b, map_y, map_out, ta);
+    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB>, map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1, ta);
 }
 
-inline int launch(const AdapterArgs& a, int* marks, int* error, cudaStream_t stream) {
-    const long tiles = (a.T + kRows - 1) / kRows;
-    const int parts = tiles <= 18 ? 8 : tiles <= 37 ? 4 : tiles <= 74 ? 2 : 1;
-    if (tiles * parts > 0x7fffffffL) return kTooLarge;
-    const TileArgs ta{a, marks, parts, (a.R + 15) / 16 * 16, error};
-    const int rc = a.R <= 64 ? launch_as<1>(ta, (int)tiles, stream) : launch_as<2>(ta, (int)tiles, stream);
+// `plan` (null: there is one adapter): scratch for the rows in order.
+inline int launch(AdapterArgs a, int* plan, int* error, cudaStream_t stream) {
+    const long tiles = (a.T + kRows - 1) / kRows, most = plan != nullptr ? adapter_order::most_tiles(a.T, a.adapters, kRows) : 0;
+    const int parts = tiles <= 18 ? 8 : tiles <= 37 ? 4 : tiles <= 74 ? 2 : 1, padded = (a.R + 15) / 16 * 16;
+    const int limit = 256 / padded < kMost ? 256 / padded : kMost;
+    if ((tiles + most) * parts > 0x7fffffffL) return kTooLarge;
+    int rc = plan != nullptr ? adapter_order::launch(a, plan, kRows, limit, stream) : 0;
+    if (rc != 0) return rc;
+    const TileArgs ta{a, (int)tiles, parts, padded, limit, error};
+    rc = a.R <= 64 ? launch_as<1>(ta, tiles + most, stream) : launch_as<2>(ta, tiles + most, stream);
     return rc != 0 ? rc : launch_status();
 }
 

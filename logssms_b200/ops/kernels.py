@@ -461,7 +461,8 @@ def _serving_calls():
         binding = build.load_binding("host_calls")
         at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
         binding.serving_launchers(at("attention_shared", "lb_attention_shared_splits"), at("attention_shared", "lb_attention_shared"),
-                                  at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"))
+                                  at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"),
+                                  at("adapters", "lb_adapters_scratch"))
         _serving_binding = binding
     return _serving_binding
 
@@ -2954,6 +2955,12 @@ def _rows_out(t: torch.Tensor, name: str) -> int:
     return ld
 
 
+def _adapter_launches(rows: int, rank: int, adapters: int, code: int) -> int:
+    """As in `lb_add_adapters`: one kernel, or two in float32 and for long ranks; one more where the rows are put in order."""
+    two = code == _DTYPE_CODE[torch.float32] or rank > 256
+    return 1 + two + (1 < adapters <= 4096 and rows >= (64 if two else 384))
+
+
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
                  scales: torch.Tensor | None = None, *, ranks: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -2969,7 +2976,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if out is None and not PROFILER.enabled:
         got = (_serving_binding or _serving_calls()).adapters(y, x, a, b, index, scales, ranks)
         if got is not None:
-            return _serving_done(got, "add_adapters", 2 if y.shape[0] >= 384 or a.shape[1] > 256 or y.dtype is torch.float32 else 1)
+            return _serving_done(got, "add_adapters", _adapter_launches(y.shape[0], a.shape[1], a.shape[0], _DTYPE_CODE[y.dtype]))
     _cuda(y, x, a, b, index, scales, ranks, out)
     ldy, ldx = _rows_of(y, "y"), _rows_of(x, "x")
     rows, features = y.shape
@@ -3002,16 +3009,13 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     ldo = out.stride(0)
     if rows == 0 or features == 0:
         return out
-    h = marks = None
-    if y.dtype == torch.float32 or rank > 256:             # two kernels, with the short sums between them
-        h = torch.empty(max(1, rows * rank), dtype=torch.float32, device=here)
-    elif rows >= 384:                                      # tiles of 128 rows, and what they leave to the rows' kernel
-        marks = torch.empty((rows + 127) // 128, dtype=torch.int32, device=here)
+    pieces = _fn("adapters", "lb_adapters_scratch", [c_long, c_int, c_int, c_int])(rows, rank, n, code)
+    scratch = torch.empty(64 * pieces, dtype=torch.int32, device=here) if pieces > 0 else None
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_long, c_void_p, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
+             c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
     _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
-             _ptr(ranks), _ptr(out), ldo, _ptr(h), _ptr(marks),
+             _ptr(ranks), _ptr(out), ldo, _ptr(scratch),
              _serving_error_word(here, "add_adapters"), rows, width, features, rank, n, code, _stream()), "add_adapters",
-           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=1 if h is None and marks is None else 2)
+           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=_adapter_launches(rows, rank, n, code))
     return out

@@ -201,3 +201,35 @@ def test_without_scales_and_ranks_and_a_single_adapter():
         s["scales"].fill_(1.0)
         got = check(s)
         assert torch.equal(got, K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,features,n,rank", [(64, 96, 72, 7, 16), (390, 256, 200, 9, 16), (777, 131, 97, 30, 24), (1500, 264, 328, 5, 64),
+                                                        (900, 328, 130, 700, 40), (1300, 128, 264, 8, 128), (400, 64, 80, 5000, 8), (500, 72, 66, 6, 260)])
+def test_many_rows_in_any_order(dtype, rows, width, features, n, rank):
+    """Rows in random order; the same in two captures of a graph; a part of a wider matrix, in place; the same bits every time."""
+    g = torch.Generator().manual_seed(rows)
+    index = torch.randint(-1, n, (rows,), generator=g).tolist()
+    if rows == 1500:
+        index[256:640] = [3] * 384                                       # some rows as they come in between
+    s = make(rows, width, features, n, rank, dtype, index)
+    ranks = torch.randint(0, rank + 1, (n,), generator=g).to(torch.int32).cuda()
+    want = check(s, ranks)
+    call = lambda out=None: K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"], s["scales"], ranks=ranks, out=out)       # noqa: E731
+    assert torch.equal(call(), want)
+    wide = torch.full((rows, features + 24), 7.0, dtype=dtype, device="cuda")
+    base = s["y"]
+    s["y"] = wide[:, 8:8 + features]
+    s["y"].copy_(base)
+    call(s["y"])
+    assert torch.equal(s["y"], want) or bool(((s["y"].double() - want.double()).abs() <= 2.0 ** -7 * (1 + want.double().abs())).all())
+    assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 8 + features:] == 7).all())
+    s["y"] = base
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(base)
+    with torch.cuda.graph(graph):
+        call(out)
+    graph.replay()
+    assert torch.equal(out, want)
+    s["index"].copy_(s["index"].flip(0))
+    graph.replay()
+    assert torch.equal(out, check(s, ranks))
