@@ -263,9 +263,20 @@ static bool in_order(long T, int R, int adapters, int dtype) {
 }
 static long words_of_h(long T, int R, int dtype) { return two_kernels(R, dtype) ? (T * R + 3) / 4 * 4 : 0; }
 
-// Scratch that a call needs, in pieces of 256 bytes: the short sums [T, R] of the form with two kernels, the rows' order.
-extern "C" int lb_adapters_scratch(long T, int R, int adapters, int dtype) {
-    return T <= 0 ? 0 : (int)((words_of_h(T, R, dtype) + (in_order(T, R, adapters, dtype) ? adapter_order::words(T, adapters, adapter_rows::kRows) : 0) + 63) / 64);
+static bool to_tiles(const AdapterArgs& a, int dtype) {
+    return dtype == kBF16 && a.T >= kTileRows && a.adapters <= adapter_order::kMostAdapters && adapter_tiles::takes(a);
+}
+static long words_of_copies(const AdapterArgs& a, int dtype) { return to_tiles(a, dtype) ? adapter_tiles::words_of_copies(a, adapter_tiles::lying(a)) : 0; }
+
+// Scratch that a call needs, in pieces of 256 bytes: copies of what does not lie on 16 bytes, the short sums [T, R] of the form with two
+// kernels, the rows' order.
+extern "C" int lb_adapters_scratch(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row, const void* B,
+                                   long b_adapter, long b_row, const void* out, long ldo, long T, int K, int N, int R, int adapters, int dtype) {
+    if (T <= 0 || N <= 0) return 0;
+    AdapterArgs a{};
+    a.y = y; a.ldy = ldy; a.out = const_cast<void*>(out); a.ldo = ldo; a.x = x; a.ldx = ldx; a.A = A; a.a_adapter = a_adapter; a.a_row = a_row; a.B = B; a.b_adapter = b_adapter; a.b_row = b_row;
+    a.T = T; a.K = K; a.N = N; a.R = R; a.adapters = adapters;
+    return (int)((words_of_copies(a, dtype) + words_of_h(T, R, dtype) + (in_order(T, R, adapters, dtype) ? adapter_order::words(T, adapters, adapter_rows::kRows) : 0) + 63) / 64);
 }
 
 // Strides in elements; columns lie side by side.  out may be y.  error: the device's error word.
@@ -278,14 +289,14 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     const int parts = parts_of(T, K, R);
     if (T > 0x7fffffffL - 1024 || N > 0x3fffffff) return kTooLarge;
     if (dtype != kF32 && dtype != kBF16) return kBadDType;
-    float* h = (float*)scratch;
-    int* plan = in_order(T, R, adapters, dtype) ? (int*)scratch + words_of_h(T, R, dtype) : nullptr;
-    AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, h, nullptr, nullptr, nullptr, T, K, N, R, adapters,
+    AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, nullptr, nullptr, nullptr, nullptr, T, K, N, R, adapters,
                   parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? 8 : 2))};      // (tiles of more rows name one adapter or two)
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == kBF16 && R <= adapter_rows::kMostRanks && T >= kTileRows && adapters <= adapter_order::kMostAdapters && adapter_tiles::takes(a))
-        return adapter_tiles::launch(a, plan, error, s);
+    int* words = (int*)scratch + words_of_copies(a, dtype);
+    a.h = (float*)words;
+    int* plan = in_order(T, R, adapters, dtype) ? words + words_of_h(T, R, dtype) : nullptr;
+    if (to_tiles(a, dtype)) return adapter_tiles::launch(a, (__nv_bfloat16*)scratch, plan, error, s);
     if (plan != nullptr) {
         const int rc = adapter_order::launch(a, plan, two_kernels(R, dtype) ? kRows : adapter_rows::kRows, -1, s);
         if (rc != 0) return rc;

@@ -213,7 +213,8 @@ typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, c
                            const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, long, float, int*, int, void*);
 typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
                           const int*, void*, long, void*, int*, long, int, int, int, int, int, void*);
-typedef int (*ScratchFn)(long, int, int, int);
+typedef int (*ScratchFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const void*, long, long, int, int, int, int,
+                         int);
 typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
                        const float*, const float*, const int*, const int*, const float*, int, const int*, long, int, const int*, void*);
 SplitsFn splits_fn;
@@ -301,7 +302,8 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int code = dtype_code(*y);
         const at::Tensor out = at::detail::empty_strided_cuda({rows, features}, {features, 1}, y->scalar_type(), y->device());
         at::Tensor scratch;
-        const int64_t pieces = scratch_fn(rows, (int)rank, (int)count, code);
+        const int64_t pieces = scratch_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
+                                          b->stride(0), b->stride(1), out.data_ptr(), features, rows, (int)width, (int)features, (int)rank, (int)count, code);
         if (pieces > 0) scratch = at::detail::empty_strided_cuda({64 * pieces}, {1}, at::kInt, y->device());
         const int rc = adapters_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
                                    b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features,

@@ -15,8 +15,16 @@
 // rows of all such tiles are put in the order of their adapters (adapters_order.cuh), and the grid's last clusters take them by tiles of
 // one adapter each, whose rows TMA gathers and scatters four at a time.  A tile's last four may hold its last row several times; the
 // rows behind them hold anything, which nothing of the others' depends on.
+//
+// PLAIN: the rows of y or of the output do not lie at multiples of 16 bytes (an odd number of features).  Every eighth row does, or lies
+// as far behind one: eight tensors, 8 columns more than a tile's, hold all rows.  Gathered rows come one by one, by copies of the pieces
+// of 16 bytes that have any of a row's columns.  The products, turned round in shared memory, are added by whole warps row by row and
+// stored 2 bytes a lane.  8,000 x 12,001, rank 61: PLAIN_US us; rows copied one by one, both ways 660 and in alone 333 (a copy costs about
+// as much as sixteen rows of a tensor's box); y read 2 bytes a lane 860 (beside 227 KB of shared memory little of the L1 is left, and few
+// such reads are on their way).  Such a tile has one adapter at most.  x, A and B that do not lie so are copied first (adapters_lay.cuh).
 #pragma once
 #include "lb200/adapters.cuh"
+#include "lb200/adapters_lay.cuh"
 #include "lb200/adapters_order.cuh"
 #include "lb200/common.cuh"
 #include "lb200/tcgen05.cuh"
@@ -28,6 +36,10 @@ typedef __nv_bfloat16 bf16;
 constexpr int kRows = 128, kCols = 128, kMost = 4;        // rows and features of a tile, adapters
 constexpr int kFirstAdder = 4, kThreads = 32 * (kFirstAdder + 8);
 constexpr uint32_t kXTile = kRows * 128, kYTile = 2 * kRows * 128;
+constexpr int kPlainY = 3;                                // PLAIN: tiles of y on their way or at work
+constexpr uint32_t kPlainPitch = kCols * 2 + 16, kPlainTile = kRows * kPlainPitch;
+struct Eighths { CUtensorMap map[8]; };                   // rows e, e + 8, ... of y, from the 16-byte boundary at or in front of row e on
+__device__ __forceinline__ int plain_slot(int row) { return (row & 7) * 16 + (row >> 3); }
 
 // RB: blocks of 64 ranks
 template <int RB> struct Shape {
@@ -89,12 +101,14 @@ __device__ __forceinline__ void tma_scatter4(const CUtensorMap* map, const void*
 }
 
 // grid: (tiles of rows as they come, then tiles of rows in order) x parts; a cluster: a tile's parts
-template <int RB>
+template <int RB, bool PLAIN>
 __global__ void __launch_bounds__(kThreads)
 adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_x1,
-                     const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_out1, TileArgs ta) {
+                     const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_out1,
+                     const __grid_constant__ Eighths eighths, TileArgs ta) {
     typedef Shape<RB> Sh;
+    static_assert(!PLAIN || kPlainY * kPlainTile + 8 * 32 * 33 * 4 <= Sh::kY * kYTile, "the tiles of y and the turned products");
     const AdapterArgs& a = ta.a;
     extern __shared__ __align__(1024) uint8_t base[];      // (the swizzle goes by the address)
     uint8_t* h_s = base;                                  // values: blocks of 64 ranks, [128][128 B]; then remainders
@@ -125,7 +139,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const long t0 = (long)tile * kRows;
 
     // ------------------------------------------------------------ who is in the tile (all warps alike)
-    int count = 0, who[kMost] = {}, n_fours = 0;           // n_fours > 0: the tile's rows are gathered
+    int count = 0, who[kMost] = {}, n_fours = 0, n_rows = 0;           // n_fours > 0: the tile's rows are gathered
     // (the kernel in front, which puts rows in order, has waited for all others before this one began)
     auto straight_adapter = [&](long t) { const int i = t < a.T ? a.index[t] : -1; return i >= 0 && i < a.adapters ? i : -1; };
     if (a.order == nullptr || tile >= ta.straight) pdl_wait();
@@ -135,8 +149,9 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const int4 its = a.tiles[at];
         count = its.x >= 0 ? 1 : 0;
         who[0] = its.x;
-        n_fours = (its.z + 3) / 4;
-        if (threadIdx.x < 4 * n_fours) reinterpret_cast<int*>(fours)[threadIdx.x] = a.order[its.y + min((int)threadIdx.x, its.z - 1)];
+        n_rows = its.z;
+        n_fours = (n_rows + 3) / 4;
+        if (threadIdx.x < 4 * n_fours) reinterpret_cast<int*>(fours)[threadIdx.x] = a.order[its.y + min((int)threadIdx.x, n_rows - 1)];
     } else {
         int own[4];
 #pragma unroll
@@ -164,7 +179,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int s = 0; s < Sh::kMostStages; ++s) { mbar_init(x_full + s, 1); mbar_init(x_empty + s, 1); }
         mbar_init(low_ready, 1);
         for (int s = 0; s < Sh::kB; ++s) { mbar_init(b_full + s, 1); mbar_init(b_clear + s, 1); mbar_init(b_empty + s, 1); }
-        for (int s = 0; s < Sh::kY; ++s) { mbar_init(y_full + s, 1); mbar_init(y_empty + s, 1); mbar_init(y_done + s, 128); }
+        for (int s = 0; s < Sh::kY; ++s) { mbar_init(y_full + s, 1); mbar_init(y_empty + s, PLAIN ? 128 : 1); mbar_init(y_done + s, 128); }
         for (int s = 0; s < 4; ++s) { mbar_init(d_full + s, 1); mbar_init(d_empty + s, 128); }
         for (int q = 0; q < kMost; ++q) { list[q] = who[q]; list[kMost + q] = q < count ? rank_of(a, who[q]) : 0; }
         *failed = 0;
@@ -295,7 +310,45 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 
     // ------------------------------------------------------------ this CTA's tiles of features
     const int steps = mine * max(count, 1);                // (tile, adapter) by (tile, adapter)
-    if (warp == 0) {
+    if (PLAIN && warp == 0) {
+        int y_asked = 0;
+        for (int i = 0; i < mine && !*failed; ++i) {
+            const int n0 = (rank + i * ta.parts) * kCols, s = i % kPlainY, bytes = 2 * min(kCols, a.N - n0);
+            if (i >= kPlainY && !wait(y_empty + s, ((i / kPlainY) - 1) & 1, 6, i)) break;
+            if (n_fours == 0) {                            // eight tensors of every eighth row, whose rows are 16 ldy bytes apart
+                if (elect_one()) {
+                    mbar_expect_tx(y_full + s, kPlainTile);
+                    for (int e = 0; e < 8; ++e) tma_load_2d(y_s + s * kPlainTile + e * (16 * kPlainPitch), &eighths.map[e], y_full + s, n0, (int)(t0 >> 3));
+                }
+            } else {
+                uintptr_t from[4];
+                uint32_t length[4], all = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {              // the pieces of 16 bytes that have any of the row's columns
+                    const int r = 32 * q + lane;
+                    const uintptr_t at = (uintptr_t)((const bf16*)a.y + (long)(r < n_rows ? reinterpret_cast<int*>(fours)[r] : 0) * a.ldy + n0);
+                    from[q] = at & ~(uintptr_t)15;
+                    length[q] = r < n_rows ? (uint32_t)(((at + bytes + 15) & ~(uintptr_t)15) - from[q]) : 0u;
+                    all += length[q];
+                }
+                all = __reduce_add_sync(0xffffffffu, all);
+                if (lane == 0) mbar_expect_tx(y_full + s, all);
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (length[q] != 0)
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                     ::"r"(smem_u32(y_s + s * kPlainTile + plain_slot(32 * q + lane) * kPlainPitch)), "l"(from[q]), "r"(length[q]), "r"(smem_u32(y_full + s)) : "memory");
+            }
+            __syncwarp();
+            y_asked = i + 1;
+        }
+        if (*failed) {
+            for (int i = max(0, y_asked - kPlainY); i < y_asked; ++i) mbar_wait(y_full + i % kPlainY, (i / kPlainY) & 1);
+        }
+    } else if (PLAIN && warp == 3) {
+        // (the adders store)
+    } else if (warp == 0) {
         int y_asked = 0;
         for (int i = 0; i < mine && !*failed; ++i) {
             const int n0 = (rank + i * ta.parts) * kCols, s = i % Sh::kY;
@@ -396,6 +449,45 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             __syncwarp();
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else if (PLAIN && warp >= kFirstAdder) {
+        float* turned = reinterpret_cast<float*>(y_s + kPlainY * kPlainTile) + (warp - kFirstAdder) * (32 * 33);     // of this warp: [32 rows][32 features + 1]
+        const long own_row = n_fours == 0 ? (t0 + r < a.T ? t0 + r : -1) : r < n_rows ? (long)reinterpret_cast<int*>(fours)[r] : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, own_row >= 0), named = __ballot_sync(0xffffffffu, place >= 0 && list[kMost] > 0);
+        const int own_off = (int)((uintptr_t)((const bf16*)a.y + max(own_row, 0L) * a.ldy) & 15);        // (n0 is a multiple of 8)
+        bool ok = true;
+        for (int i = group; i < mine && ok; i += 2) {
+            const int n0 = (rank + i * ta.parts) * kCols, v = i >> 1, d = 2 * group + (v & 1), s = i % kPlainY;
+            ok = wait(y_full + s, (i / kPlainY) & 1, 11, i) && (count == 0 || wait(d_full + d, (v >> 1) & 1, 12, i));
+            if (!ok) break;
+            fence_after_sync();
+            const uint8_t* tile_s = y_s + s * kPlainTile;
+#pragma unroll 1
+            for (int piece = 0; piece < kCols / 32; ++piece) {
+                const int c = piece * 32 + lane;
+                if (named != 0) {
+                    uint32_t acc[32];
+                    tmem_ld32(lane_addr + d * kCols + piece * 32, acc);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = __uint_as_float(acc[k]);
+                    __syncwarp();
+                }
+#pragma unroll 8
+                for (int k = 0; k < 32; ++k) {
+                    const int off = __shfl_sync(0xffffffffu, own_off, k);
+                    const long row = __shfl_sync(0xffffffffu, (int)own_row, k);
+                    unsigned short w = *reinterpret_cast<const unsigned short*>(tile_s + plain_slot((warp & 3) * 32 + k) * kPlainPitch + off + 2 * c);
+                    const float sum = __uint_as_float((uint32_t)w << 16) + turned[k * 33 + lane];
+                    if (named >> k & 1u) w = __bfloat16_as_ushort(__float2bfloat16_rn(sum));
+                    if ((there >> k & 1u) && n0 + c < a.N) reinterpret_cast<unsigned short*>(a.out)[row * a.ldo + n0 + c] = w;
+                }
+                __syncwarp();
+            }
+            if (count > 0) {
+                fence_before_sync();
+                mbar_arrive(d_empty + d);
+            }
+            mbar_arrive(y_empty + s);
+        }
     } else if (warp >= kFirstAdder) {
         bool ok = true;
         for (int i = group; i < mine && ok; i += 2) {
@@ -466,28 +558,66 @@ inline int make_tile_map_3d(CUtensorMap* map, const void* ptr, long layers, long
     return 0;
 }
 
-// Does the kernel take the call (apart from its number of rows)?
-inline bool takes(const AdapterArgs& a) {
-    auto lies = [](const void* p, long stride) { return ((uintptr_t)p & 15) == 0 && stride % 8 == 0; };
-    return a.R > 0 && a.R <= 128 && a.K > 0 && a.adapters > 0 && lies(a.x, a.ldx) && lies(a.y, a.ldy) && lies(a.out, a.ldo) && lies(a.A, a.a_row) &&
-           a.a_adapter % 8 == 0 && lies(a.B, a.b_row) && a.b_adapter % 8 == 0 && a.ldx >= a.K && a.ldy >= a.N && a.ldo >= a.N && a.a_row >= a.K &&
-           a.b_row >= a.R && (a.adapters == 1 || (a.a_adapter > 0 && a.b_adapter > 0));
+// Rows of bfloat16 that lie alike within 16 bytes, from the boundary at or in front of the first one on: boxes of kCols + 8 columns x 16
+// rows, as they lie.  (What comes with them from in front of a row is of the 16 bytes that hold its first column.)
+inline int make_eighth(CUtensorMap* map, const void* ptr, long rows, long width, long row_stride) {
+    EncodeTiled enc = tensor_map_encoder();
+    if (enc == nullptr) return (int)cudaErrorNotSupported;
+    const uintptr_t at = (uintptr_t)ptr, base = at & ~(uintptr_t)15;
+    const cuuint64_t dims[2] = {(cuuint64_t)width + (at - base) / 2, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)row_stride * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)kCols + 8, 16u};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, reinterpret_cast<void*>(base), dims, strides, box, elem,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 
-template <int RB>
+// What TMA can fetch and store as it lies.
+struct Lying { bool x, A, B, y; };
+inline Lying lying(const AdapterArgs& a) {
+    auto lies = [](const void* p, long stride, long width) { return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && stride >= width; };
+    auto layers = [&](long stride) { return a.adapters == 1 || (stride > 0 && stride % 8 == 0); };
+    return {lies(a.x, a.ldx, a.K), lies(a.A, a.a_row, a.K) && layers(a.a_adapter), lies(a.B, a.b_row, a.R) && layers(a.b_adapter),
+            lies(a.y, a.ldy, a.N) && lies(a.out, a.ldo, a.N)};
+}
+inline int pitch_of(int width) { return (width + 7) / 8 * 8; }
+// Words of 4 bytes that the copies take.
+inline long words_of_copies(const AdapterArgs& a, const Lying& l) {
+    return ((l.x ? 0 : a.T * pitch_of(a.K)) + (l.A ? 0 : (long)a.adapters * a.R * pitch_of(a.K)) + (l.B ? 0 : (long)a.adapters * a.N * pitch_of(a.R))) / 2;
+}
+// Does the kernel take the call (apart from its number of rows)?  Adapters are not copied for a few rows each: the rows' kernel reads
+// an adapter for every 8 rows of it, at about the same rate as a copy is read and written.
+inline bool takes(const AdapterArgs& a) {
+    if (!(a.R > 0 && a.R <= 128 && a.K > 0 && a.adapters > 0)) return false;
+    const Lying l = lying(a);
+    if (!l.y && !(a.R <= 64 && a.ldy >= a.N)) return false;                    // (PLAIN)
+    const long most = 1L << 33;                            // (values of a copy: the copying kernel counts pieces of 16 bytes in 32 bits)
+    return ((l.A && l.B) || a.T >= 16L * a.adapters) && a.T * pitch_of(a.K) < most && (long)a.adapters * a.R * pitch_of(a.K) < most &&
+           (long)a.adapters * a.N * pitch_of(a.R) < most;
+}
+
+template <int RB, bool PLAIN>
 inline int launch_as(const TileArgs& ta, long clusters, cudaStream_t stream) {
     const AdapterArgs& a = ta.a;
     CUtensorMap map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1;
     int rc = make_tile_map(&map_x, a.x, a.T, a.K, a.ldx, kRows);
     if (rc == 0) rc = make_tile_map_3d(&map_a, a.A, a.adapters, a.R, a.K, a.adapters > 1 ? a.a_adapter : a.a_row * a.R, a.a_row, ta.padded);
     if (rc == 0) rc = make_tile_map_3d(&map_b, a.B, a.adapters, a.N, a.R, a.adapters > 1 ? a.b_adapter : a.b_row * a.N, a.b_row, kCols);
-    if (rc == 0) rc = make_tile_map(&map_y, a.y, a.T, a.N, a.ldy, kRows);
-    if (rc == 0) rc = make_tile_map(&map_out, a.out, a.T, a.N, a.ldo, kRows);
     if (rc == 0) rc = make_tile_map(&map_x1, a.x, a.T, a.K, a.ldx, 1);                     // (a row at a time, four by four)
-    if (rc == 0) rc = make_tile_map(&map_y1, a.y, a.T, a.N, a.ldy, 1);
-    if (rc == 0) rc = make_tile_map(&map_out1, a.out, a.T, a.N, a.ldo, 1);
+    Eighths eighths{};
+    if (PLAIN) {
+        map_y = map_out = map_y1 = map_out1 = map_x;       // (not used)
+        for (int e = 0; e < 8 && rc == 0; ++e) rc = make_eighth(&eighths.map[e], (const bf16*)a.y + e * a.ldy, (a.T - e + 7) / 8, a.N, 8 * a.ldy);
+    } else {
+        if (rc == 0) rc = make_tile_map(&map_y, a.y, a.T, a.N, a.ldy, kRows);
+        if (rc == 0) rc = make_tile_map(&map_out, a.out, a.T, a.N, a.ldo, kRows);
+        if (rc == 0) rc = make_tile_map(&map_y1, a.y, a.T, a.N, a.ldy, 1);
+        if (rc == 0) rc = make_tile_map(&map_out1, a.out, a.T, a.N, a.ldo, 1);
+    }
     static SharedLimits limits;
-    if (rc == 0) rc = ensure_dynamic_smem(adapter_tiles_kernel<RB>, Shape<RB>::kSmem, limits);
+    if (rc == 0) rc = ensure_dynamic_smem(adapter_tiles_kernel<RB, PLAIN>, Shape<RB>::kSmem, limits);
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * ta.parts)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Shape<RB>::kSmem; cfg.stream = stream;
@@ -497,19 +627,41 @@ inline int launch_as(const TileArgs& ta, long clusters, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)ta.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB>, map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1, ta);
+    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB, PLAIN>, map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1, eighths, ta);
 }
 
-// `plan` (null: there is one adapter): scratch for the rows in order.
-inline int launch(AdapterArgs a, int* plan, int* error, cudaStream_t stream) {
+// `copies`: scratch for what does not lie as TMA wants it; `plan` (null: there is one adapter): for the rows in order.
+inline int launch(AdapterArgs a, bf16* copies, int* plan, int* error, cudaStream_t stream) {
     const long tiles = (a.T + kRows - 1) / kRows, most = plan != nullptr ? adapter_order::most_tiles(a.T, a.adapters, kRows) : 0;
     const int parts = tiles <= 18 ? 8 : tiles <= 37 ? 4 : tiles <= 74 ? 2 : 1, padded = (a.R + 15) / 16 * 16;
-    const int limit = 256 / padded < kMost ? 256 / padded : kMost;
+    const Lying l = lying(a);
+    const int limit = !l.y ? 1 : 256 / padded < kMost ? 256 / padded : kMost;
     if ((tiles + most) * parts > 0x7fffffffL) return kTooLarge;
-    int rc = plan != nullptr ? adapter_order::launch(a, plan, kRows, limit, stream) : 0;
+    int rc = 0;
+    if (!l.x || !l.A || !l.B) {
+        adapter_lay::Pieces pieces{};
+        const int pk = pitch_of(a.K), pr = pitch_of(a.R);
+        if (!l.x) {
+            pieces.p[0] = {(const bf16*)a.x, copies, (unsigned)a.T, (unsigned)a.T, a.K, pk, 0, a.ldx};
+            a.x = copies; a.ldx = pk;
+            copies += a.T * pk;
+        }
+        if (!l.A) {
+            pieces.p[1] = {(const bf16*)a.A, copies, (unsigned)a.R, (unsigned)a.R * a.adapters, a.K, pk, a.a_adapter, a.a_row};
+            a.A = copies; a.a_row = pk; a.a_adapter = (long)a.R * pk;
+            copies += (long)a.adapters * a.R * pk;
+        }
+        if (!l.B) {
+            pieces.p[2] = {(const bf16*)a.B, copies, (unsigned)a.N, (unsigned)a.N * a.adapters, a.R, pr, a.b_adapter, a.b_row};
+            a.B = copies; a.b_row = pr; a.b_adapter = (long)a.N * pr;
+        }
+        rc = adapter_lay::launch(pieces, stream);
+    }
+    if (rc == 0 && plan != nullptr) rc = adapter_order::launch(a, plan, kRows, limit, stream);
     if (rc != 0) return rc;
     const TileArgs ta{a, (int)tiles, parts, padded, limit, error};
-    rc = a.R <= 64 ? launch_as<1>(ta, tiles + most, stream) : launch_as<2>(ta, tiles + most, stream);
+    const long all = tiles + most;
+    rc = !l.y ? launch_as<1, true>(ta, all, stream) : a.R <= 64 ? launch_as<1, false>(ta, all, stream) : launch_as<2, false>(ta, all, stream);
     return rc != 0 ? rc : launch_status();
 }
 

@@ -2956,7 +2956,8 @@ def _rows_out(t: torch.Tensor, name: str) -> int:
 
 
 def _adapter_launches(rows: int, rank: int, adapters: int, code: int) -> int:
-    """As in `lb_add_adapters`: one kernel, or two in float32 and for long ranks; one more where the rows are put in order."""
+    """As in `lb_add_adapters`: one kernel, or two in float32 and for long ranks; one more where the rows are put in order.  (A copy of
+    what does not lie on 16 bytes is not counted.)"""
     two = code == _DTYPE_CODE[torch.float32] or rank > 256
     return 1 + two + (1 < adapters <= 4096 and rows >= (64 if two else 384))
 
@@ -3009,7 +3010,11 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     ldo = out.stride(0)
     if rows == 0 or features == 0:
         return out
-    pieces = _fn("adapters", "lb_adapters_scratch", [c_long, c_int, c_int, c_int])(rows, rank, n, code)
+    f = _fn("adapters", "lb_adapters_scratch",
+            [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_int, c_int, c_int,
+             c_int, c_int])
+    pieces = f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(out), ldo, rows, width,
+               features, rank, n, code)
     scratch = torch.empty(64 * pieces, dtype=torch.int32, device=here) if pieces > 0 else None
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
