@@ -19,10 +19,11 @@
 // PLAIN: the rows of y or of the output do not lie at multiples of 16 bytes (an odd number of features).  Every eighth row does, or lies
 // as far behind one: eight tensors, 8 columns more than a tile's, hold all rows.  Gathered rows come one by one, by copies of the pieces
 // of 16 bytes that have any of a row's columns.  The products, turned round in shared memory, are added by whole warps row by row and
-// stored 2 bytes a lane.  8,000 x 12,001, rank 61: PLAIN_US us; rows copied one by one, both ways 660 and in alone 333 (a copy costs about
+// stored 2 bytes a lane.  8,000 x 12,001, rank 61: 220 us for the tiles; rows copied one by one, both ways 660 and in alone 333 (a copy costs about
 // as much as sixteen rows of a tensor's box); y read 2 bytes a lane 860 (beside 227 KB of shared memory little of the L1 is left, and few
-// such reads are on their way).  Such a tile has one adapter at most.  x, A and B that do not lie so are copied first (adapters_lay.cuh).
+// such reads are on their way).  Such a tile has two adapters at most.  x, A and B that do not lie so are copied first (adapters_lay.cuh).
 #pragma once
+#include <type_traits>
 #include "lb200/adapters.cuh"
 #include "lb200/adapters_lay.cuh"
 #include "lb200/adapters_order.cuh"
@@ -38,6 +39,7 @@ constexpr int kFirstAdder = 4, kThreads = 32 * (kFirstAdder + 8);
 constexpr uint32_t kXTile = kRows * 128, kYTile = 2 * kRows * 128;
 constexpr int kPlainY = 3;                                // PLAIN: tiles of y on their way or at work
 constexpr uint32_t kPlainPitch = kCols * 2 + 16, kPlainTile = kRows * kPlainPitch;
+constexpr int kTurned = 36;                               // numbers from row to row of the turned products (16 bytes at a time hit all banks once)
 struct Eighths { CUtensorMap map[8]; };                   // rows e, e + 8, ... of y, from the 16-byte boundary at or in front of row e on
 __device__ __forceinline__ int plain_slot(int row) { return (row & 7) * 16 + (row >> 3); }
 
@@ -108,7 +110,7 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                      const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_out1,
                      const __grid_constant__ Eighths eighths, TileArgs ta) {
     typedef Shape<RB> Sh;
-    static_assert(!PLAIN || kPlainY * kPlainTile + 8 * 32 * 33 * 4 <= Sh::kY * kYTile, "the tiles of y and the turned products");
+    static_assert(!PLAIN || kPlainY * kPlainTile + 8 * 32 * kTurned * 4 <= Sh::kY * kYTile, "the tiles of y and the turned products");
     const AdapterArgs& a = ta.a;
     extern __shared__ __align__(1024) uint8_t base[];      // (the swizzle goes by the address)
     uint8_t* h_s = base;                                  // values: blocks of 64 ranks, [128][128 B]; then remainders
@@ -450,41 +452,70 @@ adapter_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (PLAIN && warp >= kFirstAdder) {
-        float* turned = reinterpret_cast<float*>(y_s + kPlainY * kPlainTile) + (warp - kFirstAdder) * (32 * 33);     // of this warp: [32 rows][32 features + 1]
+        float* turned = reinterpret_cast<float*>(y_s + kPlainY * kPlainTile) + (warp - kFirstAdder) * (32 * kTurned);      // of this warp: [32 rows][32 features]
         const long own_row = n_fours == 0 ? (t0 + r < a.T ? t0 + r : -1) : r < n_rows ? (long)reinterpret_cast<int*>(fours)[r] : -1;
-        const unsigned there = __ballot_sync(0xffffffffu, own_row >= 0), named = __ballot_sync(0xffffffffu, place >= 0 && list[kMost] > 0);
+        const unsigned named = __ballot_sync(0xffffffffu, place >= 0 && list[kMost + max(place, 0)] > 0);
         const int own_off = (int)((uintptr_t)((const bf16*)a.y + max(own_row, 0L) * a.ldy) & 15);        // (n0 is a multiple of 8)
+        int off8[8];                                       // rows as they come: every eighth lies alike
+#pragma unroll
+        for (int k = 0; k < 8; ++k) off8[k] = __shfl_sync(0xffffffffu, own_off, k);
+        const int first_there = (warp & 3) * 32, rows_there = (int)min(32L, a.T - t0 - first_there);
+        // (shuffles and shared memory are what this loop is bound by)
+        auto add = [&](auto straight, int col, const uint8_t* tile_s) {
+            unsigned short* out = reinterpret_cast<unsigned short*>(a.out) + col + (straight.value ? (t0 + first_there) * a.ldo : 0L);
+#pragma unroll 1
+            for (int k0 = 0; k0 < 32; k0 += 16) {          // (all reads in front of the first store, which they may not pass)
+                const uint8_t* from = tile_s + (first_there + k0) / 8 * kPlainPitch + 2 * (col & (kCols - 1));
+                uint32_t w[16];
+                float sum[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int off = straight.value ? off8[k & 7] : __shfl_sync(0xffffffffu, own_off, k0 + k);
+                    w[k] = *reinterpret_cast<const unsigned short*>(from + plain_slot(k) * kPlainPitch + off);
+                    sum[k] = turned[(k0 + k) * kTurned + lane];
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const uint32_t added = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(w[k] << 16) + sum[k]));
+                    const long row = straight.value ? (k0 + k < rows_there ? k0 + k : -1) : (long)__shfl_sync(0xffffffffu, (int)own_row, k0 + k);
+                    if (col < a.N && row >= 0) out[row * a.ldo] = (unsigned short)(named >> (k0 + k) & 1u ? added : w[k]);
+                }
+            }
+        };
         bool ok = true;
         for (int i = group; i < mine && ok; i += 2) {
-            const int n0 = (rank + i * ta.parts) * kCols, v = i >> 1, d = 2 * group + (v & 1), s = i % kPlainY;
-            ok = wait(y_full + s, (i / kPlainY) & 1, 11, i) && (count == 0 || wait(d_full + d, (v >> 1) & 1, 12, i));
+            const int n0 = (rank + i * ta.parts) * kCols, s = i % kPlainY;
+            const int v = (i >> 1) * count, d = 2 * group + (v & 1);             // the first adapter's step and accumulator; a second one's: the other
+            ok = wait(y_full + s, (i / kPlainY) & 1, 11, i) && (count == 0 || wait(d_full + d, (v >> 1) & 1, 12, i)) &&
+                 (count <= 1 || wait(d_full + d + 1, (v >> 1) & 1, 12, i));
             if (!ok) break;
             fence_after_sync();
             const uint8_t* tile_s = y_s + s * kPlainTile;
 #pragma unroll 1
             for (int piece = 0; piece < kCols / 32; ++piece) {
-                const int c = piece * 32 + lane;
                 if (named != 0) {
                     uint32_t acc[32];
                     tmem_ld32(lane_addr + d * kCols + piece * 32, acc);
+                    if (count > 1) {
+                        uint32_t other[32];
+                        tmem_ld32(lane_addr + (d + 1) * kCols + piece * 32, other);
+                        if (place == 1) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = __uint_as_float(acc[k]);
+                            for (int k = 0; k < 32; ++k) acc[k] = other[k];
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4*>(turned + lane * kTurned + k) = make_uint4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
                     __syncwarp();
                 }
-#pragma unroll 8
-                for (int k = 0; k < 32; ++k) {
-                    const int off = __shfl_sync(0xffffffffu, own_off, k);
-                    const long row = __shfl_sync(0xffffffffu, (int)own_row, k);
-                    unsigned short w = *reinterpret_cast<const unsigned short*>(tile_s + plain_slot((warp & 3) * 32 + k) * kPlainPitch + off + 2 * c);
-                    const float sum = __uint_as_float((uint32_t)w << 16) + turned[k * 33 + lane];
-                    if (named >> k & 1u) w = __bfloat16_as_ushort(__float2bfloat16_rn(sum));
-                    if ((there >> k & 1u) && n0 + c < a.N) reinterpret_cast<unsigned short*>(a.out)[row * a.ldo + n0 + c] = w;
-                }
+                if (n_fours == 0) add(std::true_type(), n0 + piece * 32 + lane, tile_s);
+                else add(std::false_type(), n0 + piece * 32 + lane, tile_s);
                 __syncwarp();
             }
             if (count > 0) {
                 fence_before_sync();
                 mbar_arrive(d_empty + d);
+                if (count > 1) mbar_arrive(d_empty + d + 1);
             }
             mbar_arrive(y_empty + s);
         }
@@ -635,7 +666,7 @@ inline int launch(AdapterArgs a, bf16* copies, int* plan, int* error, cudaStream
     const long tiles = (a.T + kRows - 1) / kRows, most = plan != nullptr ? adapter_order::most_tiles(a.T, a.adapters, kRows) : 0;
     const int parts = tiles <= 18 ? 8 : tiles <= 37 ? 4 : tiles <= 74 ? 2 : 1, padded = (a.R + 15) / 16 * 16;
     const Lying l = lying(a);
-    const int limit = !l.y ? 1 : 256 / padded < kMost ? 256 / padded : kMost;
+    const int limit = !l.y ? 2 : 256 / padded < kMost ? 256 / padded : kMost;
     if ((tiles + most) * parts > 0x7fffffffL) return kTooLarge;
     int rc = 0;
     if (!l.x || !l.A || !l.B) {
