@@ -3,8 +3,9 @@
 // x [T, K], y and out [T, N], A [adapters, R, K], B [adapters, N, R], an adapter's rank up to R.
 //
 // bfloat16: adapters_rows.cuh (decoding rows, any order of adapters) and adapters_tiles.cuh (prompts).  This file: the float32
-// form (and that of ranks over 256), and the choice between them.  Tiles of 32 rows, products in float32 registers; the adapters that
-// a tile's rows name are shared out to some CTAs ("slots"), each of which makes a pass for each of its own.  In `shrink` the
+// form (and that of ranks over 256), and the choice between them.  Tiles of 32 rows, products in float32 registers; where many rows may
+// name several adapters they are put in order first (adapters_order.cuh), else the adapters that a tile's rows name are shared out to
+// some CTAs ("slots"), each of which makes a pass for each of its own.  In `shrink` the
 // CTAs of a cluster have a part of K each and add their sums up in their order; `expand` multiplies by the scale and adds to y: one
 // rounding, of the output.
 #include <algorithm>
@@ -255,11 +256,16 @@ static int parts_of(long T, int K, int R) {
     return parts;
 }
 
-// From so many rows on a call in bfloat16 goes to the tiles' kernel, and, where its rows may name several adapters, in their order.
+// From so many rows on a call in bfloat16 goes to the tiles' kernel (384 rows of 40 adapters, 2,048 -> 4,096, rank 16: 49 us there, 44 in
+// the rows' kernel; 600 of 4 adapters 18 and 36), and, where its rows may name several adapters, in their order.  The form with two
+// kernels takes rows in order from fewer on: 63 rows of 64 adapters 55 us, 84 as they come, 32 of 32 34 and 56; a few rows of few adapters
+// lose the 3 us that putting them in order takes (32 of 4: 17, 14).
 constexpr long kTileRows = 384, kOrderRows = 64;
+constexpr int kMostSlots = 8;
 static bool two_kernels(int R, int dtype) { return dtype != kBF16 || R > adapter_rows::kMostRanks; }
 static bool in_order(long T, int R, int adapters, int dtype) {
-    return adapters > 1 && adapters <= adapter_order::kMostAdapters && T >= (two_kernels(R, dtype) ? kOrderRows : kTileRows);
+    if (adapters <= 1 || adapters > adapter_order::kMostAdapters) return false;
+    return T >= (!two_kernels(R, dtype) ? kTileRows : adapters > kMostSlots ? kMostSlots + 1 : kOrderRows);
 }
 static long words_of_h(long T, int R, int dtype) { return two_kernels(R, dtype) ? (T * R + 3) / 4 * 4 : 0; }
 
@@ -290,7 +296,7 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     if (T > 0x7fffffffL - 1024 || N > 0x3fffffff) return kTooLarge;
     if (dtype != kF32 && dtype != kBF16) return kBadDType;
     AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, nullptr, nullptr, nullptr, nullptr, T, K, N, R, adapters,
-                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? 8 : 2))};      // (tiles of more rows name one adapter or two)
+                  parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? kMostSlots : 2))};      // (tiles of more rows name one adapter or two)
     if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     int* words = (int*)scratch + words_of_copies(a, dtype);

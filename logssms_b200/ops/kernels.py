@@ -2959,7 +2959,7 @@ def _adapter_launches(rows: int, rank: int, adapters: int, code: int) -> int:
     """As in `lb_add_adapters`: one kernel, or two in float32 and for long ranks; one more where the rows are put in order.  (A copy of
     what does not lie on 16 bytes is not counted.)"""
     two = code == _DTYPE_CODE[torch.float32] or rank > 256
-    return 1 + two + (1 < adapters <= 4096 and rows >= (64 if two else 384))
+    return 1 + two + (1 < adapters <= 4096 and rows >= (384 if not two else 9 if adapters > 8 else 64))
 
 
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,

@@ -233,3 +233,18 @@ def test_many_rows_in_any_order(dtype, rows, width, features, n, rank):
     s["index"].copy_(s["index"].flip(0))
     graph.replay()
     assert torch.equal(out, check(s, ranks))
+
+
+def test_launches_are_counted_as_they_are():
+    from torch.profiler import ProfilerActivity, profile
+    for rows, n, rank, dtype in ((4, 3, 8, torch.bfloat16), (400, 3, 8, torch.bfloat16), (400, 1, 8, torch.bfloat16), (70, 3, 8, torch.float32),
+                                 (12, 9, 8, torch.float32), (12, 8, 8, torch.float32), (5, 2, 264, torch.bfloat16)):
+        s = make(rows, 64, 64, n, rank, dtype, [t % n for t in range(rows)])
+        call = lambda: K().add_adapters(s["y"], s["x"], s["a"], s["b"], s["index"], s["scales"])         # noqa: E731
+        call()
+        before = K().launch_count
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            call()
+            torch.cuda.synchronize()
+        ran = sum(e.count for e in p.key_averages() if "adapter_" in e.key)
+        assert K().launch_count - before == ran
