@@ -10,6 +10,7 @@
 // float32 fused multiply-adds on tiles of 16 rows x 32 keys in shared memory, bound by its reads (16 bytes a lane are four of its
 // cycles, also where lanes read the same): so a thread makes 4 x 4 scores of a quarter of the columns, which the four warps add up,
 // and 4 rows x 4 columns of the output.  The next tile's keys and values come by asynchronous copies while one is worked on.
+// 64 requests of 12 heads of 128 (2 of keys), 8,192 + 512 keys, float32: 217 us, 15 TFLOP/s; 46 tokens in 5 groups, 1,531 + 203 keys: 35.
 #include <type_traits>
 #include "lb200/common.cuh"
 #include "lb200/attention_shared.h"

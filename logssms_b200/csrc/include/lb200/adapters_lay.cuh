@@ -1,6 +1,6 @@
 // Operands of the adapters' tile kernel whose rows do not lie at multiples of 16 bytes, which TMA cannot fetch, copied to where they
 // do, zeros behind their ends.  Bound by memory: 4 bytes read and written a value; x, the longest, is small beside y and the output
-// (8,000 rows, 4,001 -> 12,001: see adapters.cu).
+// (8,000 rows, 4,001 -> 12,001: 37 us of 295).
 #pragma once
 #include "lb200/adapters.cuh"
 #include "lb200/common.cuh"

@@ -1,6 +1,7 @@
 // Adapters of prompts, bfloat16, on the 5th-generation tensor cores: tiles of 128 rows, one launch.
 //
-// Bound by reading x and y and writing the output once: the products are a tenth of that.  A cluster of 1 to 8 CTAs (as many as make
+// Bound by reading x and y and writing the output once: the products are a tenth of that.  8,192 rows, 4,096 -> 12,288, 8 adapters of
+// rank 64: 100 us, 4.9 TB/s (74 us at the copy rate).  A cluster of 1 to 8 CTAs (as many as make
 // about as many CTAs as there are SMs) has a tile.  Each CTA multiplies its part of K (x and A by TMA, 64 columns a stage, one product
 // for each adapter that the tile's rows name, at most four: their A tiles lie side by side as one B operand); the CTAs' sums meet in
 // distributed shared memory, each CTA adding up a part of the rows and handing them, times the scale and as two bfloat16 numbers
@@ -14,7 +15,8 @@
 // A tile whose rows name more adapters than that (decoding rows in front of a prompt, a batch in any order) is left to others: the
 // rows of all such tiles are put in the order of their adapters (adapters_order.cuh), and the grid's last clusters take them by tiles of
 // one adapter each, whose rows TMA gathers and scatters four at a time.  A tile's last four may hold its last row several times; the
-// rows behind them hold anything, which nothing of the others' depends on.
+// rows behind them hold anything, which nothing of the others' depends on.  8,000 rows in random order: 264 us with 8 adapters, 378 with
+// 60 (row by row 2,892 and 3,407).
 //
 // PLAIN: the rows of y or of the output do not lie at multiples of 16 bytes (an odd number of features).  Every eighth row does, or lies
 // as far behind one: eight tensors, 8 columns more than a tile's, hold all rows.  Gathered rows come one by one, by copies of the pieces
