@@ -282,7 +282,8 @@ extern "C" int lb_adapters_scratch(const void* y, long ldy, const void* x, long 
     AdapterArgs a{};
     a.y = y; a.ldy = ldy; a.out = const_cast<void*>(out); a.ldo = ldo; a.x = x; a.ldx = ldx; a.A = A; a.a_adapter = a_adapter; a.a_row = a_row; a.B = B; a.b_adapter = b_adapter; a.b_row = b_row;
     a.T = T; a.K = K; a.N = N; a.R = R; a.adapters = adapters;
-    return (int)((words_of_copies(a, dtype) + words_of_h(T, R, dtype) + (in_order(T, R, adapters, dtype) ? adapter_order::words(T, adapters, adapter_rows::kRows) : 0) + 63) / 64);
+    const long pieces = (words_of_copies(a, dtype) + words_of_h(T, R, dtype) + (in_order(T, R, adapters, dtype) ? adapter_order::words(T, adapters, adapter_rows::kRows) : 0) + 63) / 64;
+    return (int)std::min(pieces, 0x7fffffffL);             // (so much is not to be had)
 }
 
 // Strides in elements; columns lie side by side.  out may be y.  error: the device's error word.

@@ -194,3 +194,16 @@ def test_overlaps():
     for b in (At(1004, (4, 8), (8, 1)), At(1000, (4, 8), (9, 1)), At(900, (4, 8), (8, 1))):
         refused(lambda b=b: K._same_place(a, b, "out"), "must not share memory")
         refused(lambda b=b: K._apart(a, b, "out and x"), "must not share memory")
+
+
+def test_scratch_of_adapters_never_wraps_round():
+    """More than 2^31 pieces of 256 bytes are asked for as the most there are (which nobody has), not as a few."""
+    import ctypes
+
+    from logssms_b200.ops import build
+    f = build.load("adapters").lb_adapters_scratch
+    p, n, i = ctypes.c_void_p, ctypes.c_long, ctypes.c_int
+    f.argtypes = [p, n, p, n, p, n, n, p, n, n, p, n, n, i, i, i, i, i]
+    pieces = lambda rows, rank, count, code: f(0, 64, 0, 64, 0, 64 * rank, 64, 0, 64 * rank, rank, 0, 64, rows, 64, 64, rank, count, code)      # noqa: E731
+    assert pieces(100, 8, 1, 0) == 4 * 100 * 8 // 256 + 1 and pieces(100, 8, 3, 1) == 0
+    assert pieces(1 << 24, 1 << 24, 1, 0) == pieces(1 << 30, 1 << 29, 1, 0) == 0x7fffffff
