@@ -411,7 +411,7 @@ Layout best_layout(long tokens, int G, int Hkv, int hd, int groups, long max_pre
     return best;
 }
 // The own keys' kernel runs beside this one, on what it leaves: it gets SMs of its own, half as many as its share of the work says
-// (it is bound by memory).  256 requests, 32,768 + 2,048 keys: 144 CTAs of the prefix's take 118 us in all, 96 take 108.
+// (it is bound by memory).  256 requests, 32,768 + 2,048 keys, from a graph: 144 CTAs of the prefix's take 112 us in all, 96 take 97, 80 take 119.
 Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_prefix, long max_own) {
     const Layout all = best_layout(tokens, G, Hkv, hd, groups, max_prefix, 148);
     const double own = 4.0 + tokens * Hkv * hd * 4e-6 * (max_own > 0 ? max_own : 0) / 2 / 4.7;
