@@ -21,14 +21,14 @@ struct SharedArgs {
 };
 
 // An SM on which the kernel runs has all of its shared memory as such (and CTAs of another kernel find room beside it), on each
-// device by itself.
+// device by itself.  `carveout` is a static of the calling launcher, one per kernel instantiation.
 template <typename Kernel>
-inline int whole_carveout(Kernel kernel) {
-    static AskedOnce done;
+inline int whole_carveout(Kernel kernel, DoneOnce& carveout) {
     int device = 0;
-    const int rc = (int)cudaGetDevice(&device);
-    if (rc != 0) return rc;
-    return done.get(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
+    int rc = (int)cudaGetDevice(&device);
+    if (rc == 0) rc = carveout.run(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
+    if (rc != 0) (void)cudaGetLastError();
+    return rc;
 }
 
 // At most so many tiles of `per_tile` rows hold `rows` rows of `groups` groups, none of them empty.  (No more: a CTA that finds no tile

@@ -280,11 +280,12 @@ template <int HD>
 inline int launch_own(const SharedArgs& a, cudaStream_t stream) {
     const int head_tiles = (a.Hq / a.Hkv + kRows - 1) / kRows;
     static SharedLimits limits;
+    static DoneOnce carveout;
     CUtensorMap map_k, map_v;
     int rc = make_tile_map(&map_k, a.k_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, kKeys);
     if (rc == 0) rc = make_tile_map(&map_v, a.v_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, kKeys);
     if (rc == 0) rc = ensure_dynamic_smem(shared_own_kernel<HD>, Shape<HD>::kSmem, limits);
-    if (rc == 0) rc = whole_carveout(shared_own_kernel<HD>);
+    if (rc == 0) rc = whole_carveout(shared_own_kernel<HD>, carveout);
     if (rc == 0) rc = launch_pdl(shared_own_kernel<HD>, dim3((unsigned)(a.tokens * head_tiles), a.Hkv, a.own_splits), dim3(kThreads), Shape<HD>::kSmem, stream, map_k, map_v, a, head_tiles);
     return rc;
 }

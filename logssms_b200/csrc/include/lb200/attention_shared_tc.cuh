@@ -472,8 +472,9 @@ inline int launch_prefix(const SharedArgs& a, int ranks, cudaStream_t stream) {
     int rc = make_tile_map(&map_k, a.k_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, box);
     if (rc == 0) rc = make_tile_map(&map_v, a.v_cache, a.pages * a.page_size, (long)a.Hkv * HD, (long)a.Hkv * HD, box);
     static SharedLimits limits;
+    static DoneOnce carveout;
     if (rc == 0) rc = ensure_dynamic_smem(shared_prefix_kernel<HD, TWO>, Sh::kSmem, limits);
-    if (rc == 0) rc = whole_carveout(shared_prefix_kernel<HD, TWO>);
+    if (rc == 0) rc = whole_carveout(shared_prefix_kernel<HD, TWO>, carveout);
     if (rc != 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = Sh::kSmem; cfg.stream = stream;

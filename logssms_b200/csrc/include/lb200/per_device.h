@@ -36,4 +36,19 @@ struct AskedOnce {
     }
 };
 
+// A setting that a launcher makes once for its kernel.  One per kernel: a static beside the launch, as with SharedLimits (kernels of one
+// type, which the instantiations of a template are, must not share it).
+struct DoneOnce {
+    std::atomic<bool> done[kRememberedDevices] = {};
+    // `set()` returns an error code; its success is remembered, its failure is not
+    template <typename Set>
+    int run(int device, Set set) {
+        const bool known = device >= 0 && device < kRememberedDevices;
+        if (known && done[device].load(std::memory_order_relaxed)) return 0;
+        const int rc = set();
+        if (rc == 0 && known) done[device].store(true, std::memory_order_relaxed);
+        return rc;
+    }
+};
+
 }  // namespace lb200
