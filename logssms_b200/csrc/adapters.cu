@@ -242,7 +242,7 @@ int launch_general(const AdapterArgs& a, cudaStream_t s) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = 1; attr[1].val.clusterDim.y = (unsigned)a.parts; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    int rc = (int)cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<T>, a);
+    int rc = launched(cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<T>, a));
     if (rc == 0) rc = launch_pdl(adapter_expand_kernel<T>, dim3(tiles, (a.N + kCols - 1) / kCols, a.slots), dim3(kThreads), 0, s, a);
     return rc != 0 ? rc : launch_status();
 }

@@ -859,7 +859,7 @@ int launch_mma_form(const FusedArgs& a, int tokens, cudaStream_t s, const CUtens
         }
         if (fits) {
             cfg.numAttrs = tokens <= kPdlMaxRows ? 2 : 1;
-            return (int)cudaLaunchKernelEx(&cfg, attn_decode_mma_kernel<HDT, NS, true, TMA, KT>, a, map_k, map_v);
+            return launched(cudaLaunchKernelEx(&cfg, attn_decode_mma_kernel<HDT, NS, true, TMA, KT>, a, map_k, map_v));
         }
     }
     static size_t have_plain = 0;

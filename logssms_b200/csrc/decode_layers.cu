@@ -1155,7 +1155,7 @@ int launch_states(Launch& p, cudaStream_t stream) {
     attr[0].val.cooperative = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
     int rc = (int)cudaMemsetAsync(p.s.barrier, 0, sizeof(unsigned) * (32 + (size_t)p.s.M * p.s.Hkv), stream);
-    if (rc == 0) rc = (int)cudaLaunchKernelEx(&cfg, decode_layers_kernel<ROWS, HD, ST, NP>, p);
+    if (rc == 0) rc = launched(cudaLaunchKernelEx(&cfg, decode_layers_kernel<ROWS, HD, ST, NP>, p));
     return rc != 0 ? rc : launch_status();
 }
 template <int HD, typename ST, int NP>

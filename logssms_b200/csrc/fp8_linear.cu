@@ -484,7 +484,7 @@ int launch(const Operands& o, Args a, int sms, cudaStream_t s) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)a.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = a.split > 1 ? 2 : 1;
-    rc = (int)cudaLaunchKernelEx(&cfg, fp8_linear_kernel<kSwap, NR, kSwiglu>, map_w0, map_w1, map_x, a);
+    rc = launched(cudaLaunchKernelEx(&cfg, fp8_linear_kernel<kSwap, NR, kSwiglu>, map_w0, map_w1, map_x, a));
     return rc != 0 ? rc : launch_status();
 }
 
@@ -527,7 +527,7 @@ struct PairLaunch {
     // (one pair for a tile: tile0 is 0)
     int run(const CUtensorMap& map_w0, const CUtensorMap& map_w1, const CUtensorMap& map_x, Args a, int tile0, int tiles) {
         a.tile0 = tile0; a.tiles = tiles;
-        if (rc == 0) rc = (int)cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged, kParts>, map_w0, map_w1, map_x, a);
+        if (rc == 0) rc = launched(cudaLaunchKernelEx(&cfg, fp8_pair_kernel<kSwiglu, kRagged, kParts>, map_w0, map_w1, map_x, a));
         return rc != 0 ? rc : launch_status();
     }
     // clusters that are at work at one time (a group of neighbouring SMs holds whole clusters only: 15 of eight CTAs, 33 of four)

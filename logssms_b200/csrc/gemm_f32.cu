@@ -273,7 +273,7 @@ int launch_tile(const float* A, long lda, const float* W, const float* bias, flo
     attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = parts;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, tile_f32_kernel<MI, ALIGNED>, A, lda, W, bias, C, ldc, M, N, K, out_scale);
+    return launched(cudaLaunchKernelEx(&cfg, tile_f32_kernel<MI, ALIGNED>, A, lda, W, bias, C, ldc, M, N, K, out_scale));
 }
 }  // namespace
 

@@ -348,8 +348,8 @@ extern "C" int lb_gemm_f32_tc(const float* A, long lda, const float* W, const fl
         cudaLaunchConfig_t cfg = launch_config(attr, parts[i]);
         cfg.gridDim = listed ? dim3((unsigned)count[i], 1, parts[i]) : dim3((unsigned)tiles_n, (unsigned)tiles_m, parts[i]);
         cfg.stream = (cudaStream_t)stream;
-        rc = (int)cudaLaunchKernelEx(&cfg, listed ? gemm_f32_tc_kernel<true> : gemm_f32_tc_kernel<false>, A, lda, W, bias, C, ldc, M, N, K,
-                                     out_scale, i == 0 ? 0 : (int)count[0], error);
+        rc = launched(cudaLaunchKernelEx(&cfg, listed ? gemm_f32_tc_kernel<true> : gemm_f32_tc_kernel<false>, A, lda, W, bias, C, ldc, M, N, K,
+                                         out_scale, i == 0 ? 0 : (int)count[0], error));
     }
     return rc != 0 ? rc : launch_status();
 }

@@ -277,7 +277,7 @@ inline int launch_as(const AdapterArgs& a, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV>, a, rows_per, parts);
+    return launched(cudaLaunchKernelEx(&cfg, adapter_rows_kernel<MT, XV, BV>, a, rows_per, parts));
 }
 template <bool XV, bool BV>
 inline int launch_ranks(const AdapterArgs& a, cudaStream_t stream) {

@@ -660,7 +660,7 @@ inline int launch_as(const TileArgs& ta, long clusters, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)ta.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB, PLAIN>, map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1, eighths, ta);
+    return launched(cudaLaunchKernelEx(&cfg, adapter_tiles_kernel<RB, PLAIN>, map_x, map_a, map_b, map_y, map_out, map_x1, map_y1, map_out1, eighths, ta));
 }
 
 // `copies`: scratch for what does not lie as TMA wants it; `plan` (null: there is one adapter): for the rows in order.

@@ -484,7 +484,7 @@ inline int launch_prefix(const SharedArgs& a, int ranks, cudaStream_t stream) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)ranks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, shared_prefix_kernel<HD, TWO>, map_k, map_v, a, ranks, box);
+    return launched(cudaLaunchKernelEx(&cfg, shared_prefix_kernel<HD, TWO>, map_k, map_v, a, ranks, box));
 }
 
 }  // namespace shared_tc

@@ -76,6 +76,12 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 inline int launch_status() { return (int)cudaGetLastError(); }
+// What a launch answered.  An error is taken back from the runtime as well, where the next call's `launch_status` would find it and
+// refuse that call.
+inline int launched(cudaError_t rc) {
+    if (rc != cudaSuccess) (void)cudaGetLastError();
+    return (int)rc;
+}
 
 // Raise a kernel's dynamic shared-memory limit, once per size: the attribute call costs the host tens of microseconds,
 // which a step that is launched kernel by kernel pays at every launch otherwise.  `have` is a static of the calling
@@ -108,7 +114,7 @@ inline int launch_pdl_if(bool allow, void (*kernel)(KArgs...), dim3 grid, dim3 b
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = allow ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    return launched(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
 }
 template <typename... KArgs, typename... Args>
 inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {

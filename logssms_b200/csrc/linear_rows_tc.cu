@@ -350,7 +350,7 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs a, int t
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = (unsigned)a.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = a.split > 1 ? 2 : 1;
-    const int rc = (int)cudaLaunchKernelEx(&cfg, linear_rows_tc_kernel<NR, EPI>, map_w, map_x, a);
+    const int rc = launched(cudaLaunchKernelEx(&cfg, linear_rows_tc_kernel<NR, EPI>, map_w, map_x, a));
     return rc != 0 ? rc : launch_status();
 }
 
