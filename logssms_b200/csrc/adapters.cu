@@ -298,16 +298,17 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     if (dtype != kF32 && dtype != kBF16) return kBadDType;
     AdapterArgs a{y, ldy, x, ldx, A, a_adapter, a_row, B, b_adapter, b_row, index, scales, ranks, out, ldo, nullptr, nullptr, nullptr, nullptr, T, K, N, R, adapters,
                   parts, ((K + parts - 1) / parts + 31) / 32 * 32, std::max(1, std::min(adapters, T <= 512 ? kMostSlots : 2))};      // (tiles of more rows name one adapter or two)
-    if ((N + kCols - 1) / kCols > 65535) return kTooLarge;
+    const bool ordered = in_order(T, R, adapters, dtype);
+    if (ordered) a.slots = 1;                              // (one adapter in a tile)
+    if ((N + kCols - 1) / kCols > 65535 || (two_kernels(R, dtype) && ((long)R + kCols - 1) / kCols * a.slots > 65535)) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
     int* words = (int*)scratch + words_of_copies(a, dtype);
     a.h = (float*)words;
-    int* plan = in_order(T, R, adapters, dtype) ? words + words_of_h(T, R, dtype) : nullptr;
+    int* plan = ordered ? words + words_of_h(T, R, dtype) : nullptr;
     if (to_tiles(a, dtype)) return adapter_tiles::launch(a, (__nv_bfloat16*)scratch, plan, error, s);
     if (plan != nullptr) {
         const int rc = adapter_order::launch(a, plan, two_kernels(R, dtype) ? kRows : adapter_rows::kRows, -1, s);
         if (rc != 0) return rc;
-        a.slots = 1;                                       // (one adapter in a tile)
     }
     if (dtype == kF32) return launch_general<float>(a, s);
     return R > adapter_rows::kMostRanks ? launch_general<__nv_bfloat16>(a, s) : adapter_rows::launch(a, s);
