@@ -286,11 +286,12 @@ extern "C" int lb_adapters_scratch(const void* y, long ldy, const void* x, long 
     return (int)std::min(pieces, 0x7fffffffL);             // (so much is not to be had)
 }
 
-// Strides in elements; columns lie side by side.  out may be y.  error: the device's error word.
+// Strides in elements; columns lie side by side.  out may be y.  error: the device's error word.  launches: how many kernels it were.
 extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx, const void* A, long a_adapter, long a_row,
                                const void* B, long b_adapter, long b_row, const int* index, const float* scales, const int* ranks,
                                void* out, long ldo, void* scratch, int* error, long T, int K, int N, int R, int adapters, int dtype,
-                               void* stream) {
+                               int* launches, void* stream) {
+    *launches = 0;
     if (T <= 0 || N <= 0) return kOk;
     if (K < 0 || R < 0 || adapters < 0) return kBadSize;
     const int parts = parts_of(T, K, R);
@@ -302,10 +303,13 @@ extern "C" int lb_add_adapters(const void* y, long ldy, const void* x, long ldx,
     if (ordered) a.slots = 1;                              // (one adapter in a tile)
     if ((N + kCols - 1) / kCols > 65535 || (two_kernels(R, dtype) && ((long)R + kCols - 1) / kCols * a.slots > 65535)) return kTooLarge;
     const cudaStream_t s = (cudaStream_t)stream;
-    int* words = (int*)scratch + words_of_copies(a, dtype);
+    const long copies = words_of_copies(a, dtype);
+    const bool tiles = to_tiles(a, dtype);
+    *launches = (copies > 0) + ordered + (two_kernels(R, dtype) ? 2 : 1);
+    int* words = (int*)scratch + copies;
     a.h = (float*)words;
     int* plan = ordered ? words + words_of_h(T, R, dtype) : nullptr;
-    if (to_tiles(a, dtype)) return adapter_tiles::launch(a, (__nv_bfloat16*)scratch, plan, error, s);
+    if (tiles) return adapter_tiles::launch(a, (__nv_bfloat16*)scratch, plan, error, s);
     if (plan != nullptr) {
         const int rc = adapter_order::launch(a, plan, two_kernels(R, dtype) ? kRows : adapter_rows::kRows, -1, s);
         if (rc != 0) return rc;

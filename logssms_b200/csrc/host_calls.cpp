@@ -212,7 +212,7 @@ typedef int (*SplitsFn)(const void*, long, const void*, const void*, long, int, 
 typedef int (*AttentionFn)(const void*, long, const void*, const void*, void*, const int*, long, int, int, const int*, const int*, const int*,
                            const int*, int, float*, float*, long, int, int, int, int, int, int, int, long, long, float, int*, int, void*);
 typedef int (*AdaptersFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const int*, const float*,
-                          const int*, void*, long, void*, int*, long, int, int, int, int, int, void*);
+                          const int*, void*, long, void*, int*, long, int, int, int, int, int, int*, void*);
 typedef int (*ScratchFn)(const void*, long, const void*, long, const void*, long, long, const void*, long, long, const void*, long, long, int, int, int, int,
                          int);
 typedef int (*RulesFn)(const float*, long, float*, long, int, int, const int*, long, int, int, const int*, const int*, const int*, const float*,
@@ -285,7 +285,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-// (y, x, a, b, index, scales | None, ranks | None) -> out
+// (y, x, a, b, index, scales | None, ranks | None) -> (out, kernels launched)
 PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const int device = (int)c10::cuda::current_device();
@@ -305,10 +305,16 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t pieces = scratch_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
                                           b->stride(0), b->stride(1), out.data_ptr(), features, rows, (int)width, (int)features, (int)rank, (int)count, code);
         if (pieces > 0) scratch = at::detail::empty_strided_cuda({64 * pieces}, {1}, at::kInt, y->device());
+        int launches = 0;
         const int rc = adapters_fn(y->data_ptr(), y->stride(0), x->data_ptr(), x->stride(0), a->data_ptr(), a->stride(0), a->stride(1), b->data_ptr(),
                                    b->stride(0), b->stride(1), data<int>(index), data<float>(scales), data<int>(ranks), out.data_ptr(), features,
-                                   pieces > 0 ? scratch.data_ptr() : nullptr, error_words[device], rows, (int)width, (int)features, (int)rank, (int)count, code, stream_of(device));
-        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+                                   pieces > 0 ? scratch.data_ptr() : nullptr, error_words[device], rows, (int)width, (int)features, (int)rank, (int)count, code, &launches, stream_of(device));
+        if (rc != 0) return PyLong_FromLong(rc);
+        PyObject *po = THPVariable_Wrap(out), *pn = PyLong_FromLong(launches);
+        PyObject* r = po != nullptr && pn != nullptr ? PyTuple_Pack(2, po, pn) : nullptr;
+        Py_XDECREF(po);
+        Py_XDECREF(pn);
+        return r;
     });
 }
 

@@ -2955,13 +2955,6 @@ def _rows_out(t: torch.Tensor, name: str) -> int:
     return ld
 
 
-def _adapter_launches(rows: int, rank: int, adapters: int, code: int) -> int:
-    """As in `lb_add_adapters`: one kernel, or two in float32 and for long ranks; one more where the rows are put in order.  (A copy of
-    what does not lie on 16 bytes is not counted.)"""
-    two = code == _DTYPE_CODE[torch.float32] or rank > 256
-    return 1 + two + (1 < adapters <= 4096 and rows >= (384 if not two else 9 if adapters > 8 else 64))
-
-
 def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
                  scales: torch.Tensor | None = None, *, ranks: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
@@ -2977,7 +2970,8 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if out is None and not PROFILER.enabled:
         got = (_serving_binding or _serving_calls()).adapters(y, x, a, b, index, scales, ranks)
         if got is not None:
-            return _serving_done(got, "add_adapters", _adapter_launches(y.shape[0], a.shape[1], a.shape[0], _DTYPE_CODE[y.dtype]))
+            got, launches = got if type(got) is tuple else (got, 0)
+            return _serving_done(got, "add_adapters", launches)
     _cuda(y, x, a, b, index, scales, ranks, out)
     ldy, ldx = _rows_of(y, "y"), _rows_of(x, "x")
     rows, features = y.shape
@@ -3018,9 +3012,10 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     scratch = torch.empty(64 * pieces, dtype=torch.int32, device=here) if pieces > 0 else None
     f = _fn("adapters", "lb_add_adapters",
             [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p])
-    _check(f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
-             _ptr(ranks), _ptr(out), ldo, _ptr(scratch),
-             _serving_error_word(here, "add_adapters"), rows, width, features, rank, n, code, _stream()), "add_adapters",
-           f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=_adapter_launches(rows, rank, n, code))
+             c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
+    launches = c_int(0)
+    rc = f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
+           _ptr(ranks), _ptr(out), ldo, _ptr(scratch),
+           _serving_error_word(here, "add_adapters"), rows, width, features, rank, n, code, ctypes.byref(launches), _stream())
+    _check(rc, "add_adapters", f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=launches.value)
     return out
