@@ -33,14 +33,21 @@ class KernelError(RuntimeError):
     pass
 
 
-def _fn(lib: str, name: str, argtypes):
-    key = (lib, name)
-    f = _fn_cache.get(key)
+def _host_fn(lib: str, name: str, argtypes):
+    """A function of a library that launches nothing (what a launcher asks for first); `_fn` for launchers."""
+    f = _fn_cache.get((lib, name))
     if f is None:
         f = getattr(build.load(lib), name)
         f.argtypes = argtypes
         f.restype = c_int
-        _fn_cache[key] = f
+        _fn_cache[lib, name] = f
+    return f
+
+
+def _fn(lib: str, name: str, argtypes):
+    f = _fn_cache.get((lib, name))
+    if f is None:
+        f = _host_fn(lib, name, argtypes)
     if PROFILER.enabled:                  # opt-in: every launch between two events, summed per kernel class
         return lambda *args: PROFILER.timed(lib, name, lambda: f(*args))
     return f
@@ -541,8 +548,8 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     groups = prefix_lens.numel()
     if tokens == 0 or groups == 0:
         return out
-    f = _fn("attention_shared", "lb_attention_shared_splits",
-            [c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_int])
+    f = _host_fn("attention_shared", "lb_attention_shared_splits",
+                 [c_void_p, c_long, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_int])
     splits = f(_ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), pages, tokens, Hq, Hkv, hd, page_size, groups, int(max_prefix),
                int(max_context) - int(max_prefix), code)
     sp, so = splits >> 16, splits & 0xffff
@@ -3004,9 +3011,9 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     ldo = out.stride(0)
     if rows == 0 or features == 0:
         return out
-    f = _fn("adapters", "lb_adapters_scratch",
-            [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_int, c_int, c_int,
-             c_int, c_int])
+    f = _host_fn("adapters", "lb_adapters_scratch",
+                 [c_void_p, c_long, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_void_p, c_long, c_long, c_int, c_int, c_int,
+                  c_int, c_int])
     pieces = f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(out), ldo, rows, width,
                features, rank, n, code)
     scratch = torch.empty(64 * pieces, dtype=torch.int32, device=here) if pieces > 0 else None
