@@ -425,9 +425,9 @@ __global__ void __launch_bounds__(256, 4) shared_merge_kernel(const __grid_const
         if (lane + 32 * h < pieces) store4((T*)a.out + (size_t)item * a.hd + 4 * (lane + 32 * h), o[h]);
 }
 
-// Do the tensor-core forms take the call?  (Else: the general form.)
+// Do the tensor-core forms take the call?  (Else: the general form; TMA has no map of a pool without pages.)
 bool tc_ok(const SharedArgs& a, int dtype) {
-    return dtype == kBF16 && (a.hd == 64 || a.hd == 96 || a.hd == 128) && a.page_size % 16 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
+    return dtype == kBF16 && a.pages > 0 && (a.hd == 64 || a.hd == 96 || a.hd == 128) && a.page_size % 16 == 0 && (a.pages + 1) * a.page_size < 0x7fffffffL && a.q_stride % 8 == 0 &&
            (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0;
 }
 // How the prefix's work is laid out on the tensor cores: rows of a tile, CTAs of a cluster, clusters for a tile's keys.
