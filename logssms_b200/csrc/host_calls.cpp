@@ -365,14 +365,22 @@ PyObject* rules(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
-// the launchers' addresses
-PyObject* launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 5) { PyErr_SetString(PyExc_TypeError, "five addresses"); return nullptr; }
+// the launchers' addresses, each operator's by itself: its library is not loaded for the others'
+PyObject* attention_launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 2) { PyErr_SetString(PyExc_TypeError, "two addresses"); return nullptr; }
     splits_fn = (SplitsFn)PyLong_AsVoidPtr(args[0]);
     attention_fn = (AttentionFn)PyLong_AsVoidPtr(args[1]);
-    adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[2]);
-    rules_fn = (RulesFn)PyLong_AsVoidPtr(args[3]);
-    scratch_fn = (ScratchFn)PyLong_AsVoidPtr(args[4]);
+    return none();
+}
+PyObject* adapters_launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 2) { PyErr_SetString(PyExc_TypeError, "two addresses"); return nullptr; }
+    scratch_fn = (ScratchFn)PyLong_AsVoidPtr(args[0]);
+    adapters_fn = (AdaptersFn)PyLong_AsVoidPtr(args[1]);
+    return none();
+}
+PyObject* rules_launchers(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 1) { PyErr_SetString(PyExc_TypeError, "one address"); return nullptr; }
+    rules_fn = (RulesFn)PyLong_AsVoidPtr(args[0]);
     return none();
 }
 }  // namespace serving
@@ -398,7 +406,10 @@ PyMethodDef methods[] = {
     {"norm", (PyCFunction)(void*)norm, METH_FASTCALL, nullptr},         {"quantize", (PyCFunction)(void*)quantize, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},     {"swiglu", (PyCFunction)(void*)swiglu, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void*)serving::attention, METH_FASTCALL, nullptr}, {"adapters", (PyCFunction)(void*)serving::adapters, METH_FASTCALL, nullptr},
-    {"rules", (PyCFunction)(void*)serving::rules, METH_FASTCALL, nullptr}, {"serving_launchers", (PyCFunction)(void*)serving::launchers, METH_FASTCALL, nullptr},
+    {"rules", (PyCFunction)(void*)serving::rules, METH_FASTCALL, nullptr},
+    {"attention_launchers", (PyCFunction)(void*)serving::attention_launchers, METH_FASTCALL, nullptr},
+    {"adapters_launchers", (PyCFunction)(void*)serving::adapters_launchers, METH_FASTCALL, nullptr},
+    {"rules_launchers", (PyCFunction)(void*)serving::rules_launchers, METH_FASTCALL, nullptr},
     {"launchers", (PyCFunction)(void*)launchers, METH_FASTCALL, nullptr}, {"error_word", (PyCFunction)(void*)error_word, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

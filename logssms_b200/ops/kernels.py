@@ -458,29 +458,33 @@ def attention_decode_listed(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
 
 _serving_binding = None
+_SERVING_LAUNCHERS = {"attention": ("attention_shared", "lb_attention_shared_splits", "lb_attention_shared"),
+                      "adapters": ("adapters", "lb_adapters_scratch", "lb_add_adapters"), "rules": ("logit_rules", "lb_logit_rules")}
+_serving_known: set[str] = set()        # the operators whose launchers the binding has
 
 
-def _serving_calls():
+def _serving_calls(operator: str):
     """The binding that takes a call of the serving operators that is plainly in order straight to its launcher
-    (`csrc/host_calls.cpp`); it answers None to anything else, and the functions in Python take over."""
+    (`csrc/host_calls.cpp`), with the launchers of this operator (and of those before; no library is loaded for another operator's
+    sake); it answers None to anything else, and the functions in Python take over."""
     global _serving_binding
-    if _serving_binding is None:
-        binding = build.load_binding("host_calls")
-        at = lambda lib, name: ctypes.cast(getattr(build.load(lib), name), c_void_p).value     # noqa: E731
-        binding.serving_launchers(at("attention_shared", "lb_attention_shared_splits"), at("attention_shared", "lb_attention_shared"),
-                                  at("adapters", "lb_add_adapters"), at("logit_rules", "lb_logit_rules"),
-                                  at("adapters", "lb_adapters_scratch"))
-        _serving_binding = binding
-    return _serving_binding
+    binding = _serving_binding or build.load_binding("host_calls")
+    if operator not in _serving_known:
+        library, *names = _SERVING_LAUNCHERS[operator]
+        lib = build.load(library)
+        getattr(binding, f"{operator}_launchers")(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in names))
+        _serving_known.add(operator)
+    _serving_binding = binding
+    return binding
 
 
-def _serving_error_word(device: torch.device, name: str) -> int:
+def _serving_error_word(device: torch.device, operator: str, name: str) -> int:
     """Address of the device's error word, which the binding has from then on (until then it takes no call that needs it there)."""
     if device not in _gemm_error:
         # (made inside, it would lie in the graph's memory, and every replay would clear what was reported before)
         _need(not torch.cuda.is_current_stream_capturing(), f"the first {name} on a device must come before a capture")
     address = error_word(device).data_ptr()
-    _serving_calls().error_word(device.index, address)
+    _serving_calls(operator).error_word(device.index, address)
     return address
 
 
@@ -511,7 +515,7 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits.  `check_kernel_errors()`
     reports a kernel whose internal wait gave up."""
     if out is None and not PROFILER.enabled:
-        got = (_serving_binding or _serving_calls()).attention(q, k_cache, v_cache, block_table, token_req, positions, group_start,
+        got = (_serving_binding or _serving_calls("attention")).attention(q, k_cache, v_cache, block_table, token_req, positions, group_start,
                                                                prefix_lens, scale, max_prefix, max_context)
         if got is not None:
             return _serving_done(got, "attention_decode_shared", 3)
@@ -562,7 +566,7 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
              block_table.shape[1], block_table.shape[0], _ptr(token_req), _ptr(positions), _ptr(group_start), _ptr(prefix_lens), groups,
              _ptr(part_o), _ptr(part_ml), pages, tokens, Hq, Hkv, hd, page_size, sp, so, int(max_prefix),
              int(max_context) - int(max_prefix), scale,
-             _serving_error_word(q.device, "attention_decode_shared"), code, _stream()), "attention_decode_shared", launches=3)
+             _serving_error_word(q.device, "attention", "attention_decode_shared"), code, _stream()), "attention_decode_shared", launches=3)
     return out
 
 
@@ -2975,7 +2979,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     b[i] are its own (none: all of them); the others are not read as values.  `check_kernel_errors()` reports a kernel whose internal
     wait gave up."""
     if out is None and not PROFILER.enabled:
-        got = (_serving_binding or _serving_calls()).adapters(y, x, a, b, index, scales, ranks)
+        got = (_serving_binding or _serving_calls("adapters")).adapters(y, x, a, b, index, scales, ranks)
         if got is not None:
             got, launches = got if type(got) is tuple else (got, 0)
             return _serving_done(got, "add_adapters", launches)
@@ -3023,6 +3027,6 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     launches = c_int(0)
     rc = f(_ptr(y), ldy, _ptr(x), ldx, _ptr(a), a.stride(0), a.stride(1), _ptr(b), b.stride(0), b.stride(1), _ptr(index), _ptr(scales),
            _ptr(ranks), _ptr(out), ldo, _ptr(scratch),
-           _serving_error_word(here, "add_adapters"), rows, width, features, rank, n, code, ctypes.byref(launches), _stream())
+           _serving_error_word(here, "adapters", "add_adapters"), rows, width, features, rank, n, code, ctypes.byref(launches), _stream())
     _check(rc, "add_adapters", f"([{rows}, {width}] -> [{rows}, {features}], rank {rank})", launches=launches.value)
     return out

@@ -42,7 +42,7 @@ def edit_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, le
     names each row's mask; without, row i's is i; a row whose mask is none of these (-1) allows every token.  A mask that allows
     nothing leaves a row of -inf.  Row strides of `logits`, `history`, `allowed` and `out` are free."""
     if out is None and not K.PROFILER.enabled:
-        got = (K._serving_binding or K._serving_calls()).rules(logits, history, lengths, prompt_lengths, slots, repetition, frequency, presence,
+        got = (K._serving_binding or K._serving_calls("rules")).rules(logits, history, lengths, prompt_lengths, slots, repetition, frequency, presence,
                                                                bias_start, bias_ids, bias_values, allowed, allowed_row)
         if got is not None:
             return K._serving_done(got, "edit_logits", 1)
@@ -97,6 +97,7 @@ def edit_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, le
     ld_out = out.stride(0)
     if rows == 0 or V == 0:
         return out
+    K._serving_calls("rules")                    # (where another operator's call has loaded the binding)
     f = K._fn("logit_rules", "lb_logit_rules",
               [c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_long, c_int, c_void_p, c_void_p])
