@@ -1,5 +1,6 @@
 // Operands of the kernels for attention over a shared prefix (attention_shared.cu), and who belongs to which group.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "lb200/per_device.h"
 
@@ -29,6 +30,17 @@ inline int whole_carveout(Kernel kernel, DoneOnce& carveout) {
     if (rc == 0) rc = carveout.run(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); });
     if (rc != 0) (void)cudaGetLastError();
     return rc;
+}
+
+// Two weights of the softmax as bfloat16 operands: their first 8 bits, and what is cut off them, rounded; 2^-16 of a weight is lost.  What
+// is cut off is above zero wherever the weight is (2^-20 of the weight is added, which the rounding would hide): an infinite value must
+// not meet a zero or a number of the other sign.
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t& high, uint32_t& low) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    constexpr float kMore = 1.f + 0x1p-20f;
+    high = __byte_perm(a, b, 0x7632);
+    const __nv_bfloat162 rest = __floats2bfloat162_rn(fmaf(x, kMore, -__uint_as_float(a & 0xffff0000u)), fmaf(y, kMore, -__uint_as_float(b & 0xffff0000u)));
+    low = *reinterpret_cast<const uint32_t*>(&rest);
 }
 
 // At most so many tiles of `per_tile` rows hold `rows` rows of `groups` groups, none of them empty.  (No more: a CTA that finds no tile

@@ -502,18 +502,22 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             scale: float, *, max_prefix: int, max_context: int, out: torch.Tensor | None = None) -> torch.Tensor:
     """`attention_decode` for tokens whose requests begin with the same keys, which are read once for all of them.  The same q
     [tokens, Hq, hd] (rotated queries; the row stride is free), caches [pages, page_size, Hkv, hd] (every key and value, the tokens'
-    own included, is there already), block_table [requests, columns], token_req and positions (int32 per token), and the same result:
-    a token sees the keys 0 .. its position of its request.
+    own included, is there already), block_table [requests, columns], token_req and positions (int32 per token), and the same result
+    as without a `window`, which it has not: a token sees all keys 0 .. its position of its request.
 
     `group_start` (int32 [groups + 1], ascending) and `prefix_lens` (int32 [groups]): tokens group_start[g] .. group_start[g + 1] - 1
     are of requests whose first prefix_lens[g] keys are the same (0: nothing in common); these are read through the table row of the
     group's first token, and what lies behind them through each token's own.  A request's row may name the same pages or copies of
     them.  A group's tokens may stand inside of the prefix, belong to any requests and be several of one request.  Rows of no group
     are left as they are (in `out`; otherwise unwritten).  A token whose request is not there sees the prefix alone, keys on pages
-    that are not there count for nobody, and a row without keys (position -1) becomes zeros.  Keys and values that a row does not see may be anything.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right too.
+    that are not there count for nobody, and a row without keys (position -1) becomes zeros.  Keys and values that a row does not see
+    may be anything.  `max_prefix`, `max_context`: the longest prefix and context, by which the work is cut up; longer ones are right
+    too.
 
-    bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits.  `check_kernel_errors()`
-    reports a kernel whose internal wait gave up."""
+    bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits (on the tensor cores the
+    weights multiply the values as two bfloat16 numbers each, which leaves 2^-16 of them).  A column in which a token inside of the
+    prefix has become NaN, because of values that it does not see, is made once more, at 0.2 us a key that it sees.
+    `check_kernel_errors()` reports a kernel whose internal wait gave up."""
     if out is None and not PROFILER.enabled:
         got = (_serving_binding or _serving_calls("attention")).attention(q, k_cache, v_cache, block_table, token_req, positions, group_start,
                                                                prefix_lens, scale, max_prefix, max_context)
