@@ -22,11 +22,10 @@ namespace {
 constexpr int kThreads = 128, kRows = 16, kKeys = 32;
 
 __device__ __forceinline__ float4 get4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 four(const float4& v) { return v; }
-__device__ __forceinline__ float4 four(const uint2& v) {    // of bfloat16
+__device__ __forceinline__ float4 get4(const __nv_bfloat16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
-__device__ __forceinline__ float4 get4(const __nv_bfloat16* p) { return four(*reinterpret_cast<const uint2*>(p)); }
 __device__ __forceinline__ void copy16(void* to, const void* from, bool there) {             // zeros where nothing is there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
@@ -279,92 +278,55 @@ template <> __device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16*
 }
 
 // A row that stands within the prefix and has columns that are no numbers.  The tensor cores multiply the values of all of a tile's keys,
-// those that the row does not see by zero, and zero times an infinity is NaN: so those columns (of `had`, the row's result) once more
-// over the keys that the row sees.  A warp: 32 keys at a time, a lane each for the scores (16 bytes of a key a load), four or eight
-// columns a lane for the values.  It ends where every column in question has met a NaN that the row does see, so that only values that
-// nobody sees, and those that come late, cost a walk, 0.23 us a key (eight tokens
-// of 12 heads of 128 behind 19,000 keys 4.5 ms; an infinity that they see 0.04, as any call).
+// those that the row does not see by zero, and zero times an infinity is NaN: so those columns (of `result`, the row's, where each lane
+// finds what it has left there) once more, key by key, over the keys that the row sees.  A warp, four columns a lane.  It ends where every
+// such column has met a NaN that the row does see, so that only values that nobody sees, and those that come late, cost a walk: 0.8 us a
+// key.  It is kept as small as this for the sake of the calls that never come here: with 32 keys at a time (0.2 us a key) its registers
+// and its stack cost every call 1.5 us, and 4 behind a cold cache.
 template <typename T>
-__device__ __noinline__ void again(const SharedArgs& a, int t, int head, int first, int keys, const float4 (&had)[2]) {
-    typedef typename std::conditional<sizeof(T) == 2, uint2, float4>::type Raw;           // four numbers
-    constexpr int kAtOnce = 4, kFours = 4 / (int)sizeof(T);                      // loads of a lane on their way; fours of numbers in 16 bytes
+__device__ __noinline__ void again(const SharedArgs& a, int t, int head, int first, int keys, float4* result) {
     const int lane = threadIdx.x & 31, pieces = a.hd >> 2, request = a.token_req[first];
     const T* q = (const T*)a.q + (long)t * a.q_stride + (long)head * a.hd;
+    T* out = (T*)a.out + ((size_t)t * a.Hq + head) * a.hd;
     const size_t column = (size_t)(head / (a.Hq / a.Hkv)) * a.hd;
-    float4 qv[2], o[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        qv[h] = o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (lane + 32 * h < pieces) {
-            const T* src = q + 4 * (lane + 32 * h);                              // (any alignment)
-            qv[h] = make_float4(to_f32(src[0]), to_f32(src[1]), to_f32(src[2]), to_f32(src[3]));
-        }
-    }
-    float m = -INFINITY, l = 0.f;
     if (request < 0 || request >= a.requests) keys = 0;
     keys = (int)min((long)keys, (long)a.bt_cols * a.page_size);
-    auto open = [](float was, float is) { return was != was && is == is; };      // in question, and no NaN met so far
-    for (int j0 = 0; j0 < keys; j0 += 32) {
-        bool undecided = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            undecided = undecided || open(had[h].x, o[h].x) || open(had[h].y, o[h].y) || open(had[h].z, o[h].z) || open(had[h].w, o[h].w);
-        if (!__any_sync(0xffffffffu, undecided)) break;
-        long at = -1;                                     // this lane's key
-        if (j0 + lane < keys) {
-            const long page = a.block_table[(long)request * a.bt_stride + (j0 + lane) / a.page_size];
-            if (page >= 0 && page < a.pages) at = ((page * a.page_size + (j0 + lane) % a.page_size) * a.Hkv) * a.hd + (long)column;
-        }
-        float part[4] = {};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            for (int i0 = 32 * h; i0 < min(pieces, 32 * h + 32); i0 += kAtOnce * kFours) {          // (whole warps: the queries come from the lanes)
-                uint4 k[kAtOnce];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u)
-                    k[u] = at >= 0 && i0 + u * kFours < pieces ? *reinterpret_cast<const uint4*>((const T*)a.k_cache + at + 4 * (i0 + u * kFours)) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int u = 0; u < kAtOnce * kFours; ++u) {
-                    const float4 x = four(reinterpret_cast<const Raw*>(k)[u]);
-                    part[0] = fmaf(__shfl_sync(0xffffffffu, qv[h].x, (i0 + u) & 31), x.x, part[0]);
-                    part[1] = fmaf(__shfl_sync(0xffffffffu, qv[h].y, (i0 + u) & 31), x.y, part[1]);
-                    part[2] = fmaf(__shfl_sync(0xffffffffu, qv[h].z, (i0 + u) & 31), x.z, part[2]);
-                    part[3] = fmaf(__shfl_sync(0xffffffffu, qv[h].w, (i0 + u) & 31), x.w, part[3]);
-                }
+    const float4 nothing = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += 32) {              // (heads of up to 128: once)
+        const bool mine = p0 + lane < pieces;
+        const float4 had = mine ? result[p0 + lane] : nothing;
+        float4 o = nothing;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < keys; ++j) {
+            auto open = [](float was, float is) { return was != was && is == is; };         // in question, and no NaN met so far
+            if (!__any_sync(0xffffffffu, open(had.x, o.x) || open(had.y, o.y) || open(had.z, o.z) || open(had.w, o.w))) break;
+            const long page = a.block_table[(long)request * a.bt_stride + j / a.page_size];
+            if (page < 0 || page >= a.pages) continue;
+            const size_t at = (size_t)(page * a.page_size + j % a.page_size) * a.Hkv * a.hd + column;
+            float4 v = mine ? get4((const T*)a.v_cache + at + 4 * (p0 + lane)) : nothing;
+            float score = 0.f;
+#pragma unroll 1
+            for (int p = lane; p < pieces; p += 32) {
+                const float4 k = get4((const T*)a.k_cache + at + 4 * p);
+                const T* u = q + 4 * p;                   // (any alignment)
+                score = fmaf(to_f32(u[0]), k.x, fmaf(to_f32(u[1]), k.y, fmaf(to_f32(u[2]), k.z, fmaf(to_f32(u[3]), k.w, score))));
             }
-        const float score = at >= 0 ? ((part[0] + part[1]) + (part[2] + part[3])) * a.scale_log2 : -INFINITY;
-        const float top = fmaxf(m, warp_max(score)), ref = top == -INFINITY ? 0.f : top, before = exp2f(m - ref), w = exp2f(score - ref);
-        m = top;
-        l = l * before + warp_sum(w);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (32 * h >= pieces) break;
-            o[h].x *= before; o[h].y *= before; o[h].z *= before; o[h].w *= before;
-            for (int j = 0; j < 32; j += kAtOnce) {
-                Raw v[kAtOnce];
-                float its[kAtOnce];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    its[u] = __shfl_sync(0xffffffffu, w, j + u);
-                    const long place = __shfl_sync(0xffffffffu, at, j + u);
-                    v[u] = its[u] != 0.f && lane + 32 * h < pieces ? *reinterpret_cast<const Raw*>((const T*)a.v_cache + place + 4 * (lane + 32 * h)) : Raw{};
-                }
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    const float4 x = four(v[u]);
-                    o[h].x = fmaf(its[u], x.x, o[h].x); o[h].y = fmaf(its[u], x.y, o[h].y);
-                    o[h].z = fmaf(its[u], x.z, o[h].z); o[h].w = fmaf(its[u], x.w, o[h].w);
-                }
-            }
+            score = warp_sum(score) * a.scale_log2;
+            const float top = fmaxf(m, score), ref = top == -INFINITY ? 0.f : top, before = exp2f(m - ref), w = exp2f(score - ref);
+            m = top;
+            l = l * before + w;
+            if (w == 0.f) v = nothing;
+            o.x = fmaf(o.x, before, w * v.x); o.y = fmaf(o.y, before, w * v.y);
+            o.z = fmaf(o.z, before, w * v.z); o.w = fmaf(o.w, before, w * v.w);
         }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        auto pick = [&](float was, float is) { return was != was ? is * inv : was; };
+        // (out may be q, whose row is read for every piece: the results wait in their place until the last one)
+        if (mine) result[p0 + lane] = make_float4(pick(had.x, o.x), pick(had.y, o.y), pick(had.z, o.z), pick(had.w, o.w));
     }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    auto pick = [&](float was, float is) { return was != was ? is * inv : was; };
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (lane + 32 * h < pieces)
-            store4((T*)a.out + ((size_t)t * a.Hq + head) * a.hd + 4 * (lane + 32 * h),
-                   make_float4(pick(had[h].x, o[h].x), pick(had[h].y, o[h].y), pick(had[h].z, o[h].z), pick(had[h].w, o[h].w)));
+    for (int p = lane; p < pieces; p += 32) store4(out + 4 * p, result[p]);
 }
 
 template <typename T>
@@ -413,16 +375,20 @@ __global__ void __launch_bounds__(256, 4) shared_merge_kernel(const __grid_const
         }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;          // a row that saw no key: zeros
+    if (keys < prefix && l == l) {                       // (an infinity is one that the row sees, and so is what made its sum NaN)
+        const float all = (fabsf(o[0].x) + fabsf(o[0].y)) + (fabsf(o[0].z) + fabsf(o[0].w)) + ((fabsf(o[1].x) + fabsf(o[1].y)) + (fabsf(o[1].z) + fabsf(o[1].w)));
+        if (__any_sync(0xffffffffu, all != all)) {
+            float4* result = reinterpret_cast<float4*>(a.part_o) + (size_t)item * splits * pieces;       // (what lay there is in it)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) { o[h].x *= inv; o[h].y *= inv; o[h].z *= inv; o[h].w *= inv; }
-    // (an infinity is one that the row sees, and so is what made its sum NaN)
-    if (keys < prefix && l == l) {
-        const float all = fabsf(o[0].x) + fabsf(o[0].y) + fabsf(o[0].z) + fabsf(o[0].w) + (fabsf(o[1].x) + fabsf(o[1].y) + fabsf(o[1].z) + fabsf(o[1].w));
-        if (__any_sync(0xffffffffu, all != all)) return again<T>(a, t, (int)(item % a.Hq), first, keys, o);
+            for (int h = 0; h < 2; ++h)
+                if (lane + 32 * h < pieces) result[lane + 32 * h] = make_float4(o[h].x * inv, o[h].y * inv, o[h].z * inv, o[h].w * inv);
+            return again<T>(a, t, (int)(item % a.Hq), first, keys, result);
+        }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        if (lane + 32 * h < pieces) store4((T*)a.out + (size_t)item * a.hd + 4 * (lane + 32 * h), o[h]);
+        if (lane + 32 * h < pieces)
+            store4((T*)a.out + (size_t)item * a.hd + 4 * (lane + 32 * h), make_float4(o[h].x * inv, o[h].y * inv, o[h].z * inv, o[h].w * inv));
 }
 
 // Do the tensor-core forms take the call?  (Else: the general form; TMA has no map of a pool without pages.)

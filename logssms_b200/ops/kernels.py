@@ -516,7 +516,7 @@ def attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     bfloat16 or float32, heads in steps of 8 up to 256; sums, softmax and the joining of ranges in 32 bits (on the tensor cores the
     weights multiply the values as two bfloat16 numbers each, which leaves 2^-16 of them).  A column in which a token inside of the
-    prefix has become NaN, because of values that it does not see, is made once more, at 0.2 us a key that it sees.
+    prefix has become NaN, because of values that it does not see, is made once more, at 0.8 us a key that it sees.
     `check_kernel_errors()` reports a kernel whose internal wait gave up."""
     if out is None and not PROFILER.enabled:
         got = (_serving_binding or _serving_calls("attention")).attention(q, k_cache, v_cache, block_table, token_req, positions, group_start,
