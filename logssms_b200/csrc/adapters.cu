@@ -256,9 +256,10 @@ static int parts_of(long T, int K, int R) {
     return parts;
 }
 
-// From so many rows on a call in bfloat16 goes to the tiles' kernel (384 rows of 40 adapters, 2,048 -> 4,096, rank 16: 49 us there, 44
-// in the rows' kernel; 8,000 of 8 adapters in random order, 4,096 -> 12,288, rank 64: 264 and 2,892), and, where its rows may name several
-// adapters, in their order.  The form with two kernels takes rows in order from fewer on: 63 rows of 64 adapters 55 us, 84 as they come,
+// From so many rows on a call in bfloat16 goes to the tiles' kernel, and, where its rows may name several adapters, in their order.  Tiles
+// / rows' kernel, us, 2,048 -> 4,096, rank 16: 8 adapters in random order 27 / 44 at 384 rows, 35 / 56 at 768, 37 / 84 at 1,024; 40
+// adapters 51 / 45, 53 / 58, 56 / 97; portions of 8 adapters, whose order nobody knows beforehand, 29 / 12, 20 / 14, 16 / 22; 8,000 rows
+// of 8 adapters in random order, 4,096 -> 12,288, rank 64, 264 / 2,892.  The form with two kernels takes rows in order from fewer on: 63 rows of 64 adapters 55 us, 84 as they come,
 // 32 of 32 34 and 56; a few rows of few adapters would lose the 3 us that putting them in order takes (32 of 4: 17, 14).
 constexpr long kTileRows = 384, kOrderRows = 64;
 constexpr int kMostSlots = 8;

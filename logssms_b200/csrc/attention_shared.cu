@@ -399,8 +399,8 @@ bool tc_ok(const SharedArgs& a, int dtype) {
 // How the prefix's work is laid out on the tensor cores: rows of a tile, CTAs of a cluster, clusters for a tile's keys.
 struct Layout { bool two; int ranks, clusters; double us; };
 Layout best_layout(long tokens, int G, int Hkv, int hd, int groups, long max_prefix, long most_ctas) {
-    // us: a tile of 64 keys takes 1.1 with 256 rows and 0.6 where the groups share the tiles out; a CTA's beginning and end 8; a row of
-    // partial results is written and read at 4 TB/s.  As many CTAs at once as the GPU holds in clusters of that size.
+    // us: a tile of 64 keys takes 1.1 with 256 rows and 0.6 where the groups share the tiles out (a quarter more changes no call's time
+    // by more than the clock's noise); a CTA's beginning and end 8; a row of partial results is written and read at 4 TB/s.  As many CTAs at once as the GPU holds in clusters of that size.
     const long kt = max_prefix > 0 ? (max_prefix + 63) / 64 : 1;
     Layout best{false, 1, 1, 1e30};
     for (int two = 0; two < 2; ++two) {
@@ -420,7 +420,7 @@ Layout best_layout(long tokens, int G, int Hkv, int hd, int groups, long max_pre
     return best;
 }
 // The own keys' kernel runs beside this one, on what it leaves: it gets SMs of its own, half as many as its share of the work says
-// (it is bound by memory).  256 requests, 32,768 + 2,048 keys, from a graph: 144 CTAs of the prefix's take 112 us in all, 96 take 97, 80 take 119.
+// (it is bound by memory).  256 requests, 32,768 + 2,048 keys, from a graph: 144 CTAs of the prefix's take 121 us in all, 108 115, 96 109, 84 120.
 Layout layout_for(long tokens, int G, int Hkv, int hd, int groups, long max_prefix, long max_own) {
     const Layout all = best_layout(tokens, G, Hkv, hd, groups, max_prefix, 148);
     const double own = 4.0 + tokens * Hkv * hd * 4e-6 * (max_own > 0 ? max_own : 0) / 2 / 4.7;

@@ -10,8 +10,8 @@
 // traffic again): a history of some thousand ids is counted anew every step, in shared memory.  A CTA owns a slice of the
 // vocabulary, so that its counters fit; it reads the whole history (from L2) and counts what falls into its slice.  16-bit
 // counters where the history's capacity allows, which makes slices twice as long and the history be read half as often.
-// 256 rows of 130,048 with 16,384 ids each 62 us, 4.4 TB/s (42 us at the copy rate), of which half is the history; 64 rows with 4,096
-// ids, 300 biases and masks 16 (10).  A history shared by a cluster's CTAs, with remote atomics, took 109 us where this form took 80.
+// 256 rows of 130,048 with 16,384 ids each 62 us, 4.4 TB/s (42 us at the copy rate), 44 without a history; 64 rows with 4,096
+// ids, 300 biases and masks 20 (10).  A history shared by a cluster's CTAs, with remote atomics, took 109 us where this form took 80.
 #include "lb200/common.cuh"
 using namespace lb200;
 
